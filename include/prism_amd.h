@@ -382,6 +382,84 @@ PRISM_API int prism_mxfp4_gemm_ws(const uint8_t* aq, const uint8_t* as, int a_fm
 /* Bytes of work the split decode needs for an N x K projection; 0 for shapes it does not take. */
 PRISM_API int64_t prism_mxfp4_split_workspace_bytes(int64_t N, int64_t K);
 
+/* ------------------------------------------------------------------------------------- token mixers (serving) */
+/*
+ * The paged key-value cache of a full-attention layer: k_cache and v_cache [pages, page, HKV, D] (strides k_page, k_tok,
+ * k_head and v_page, v_tok, v_head in elements, unit stride in D) of bf16 or (e4m3 = 1) OCP e4m3; an e4m3 cache may have
+ * a scale per head (k_scale, v_scale fp32 [HKV], or null for 1): it holds x / scale clamped to +-448, nearest even, and
+ * stands for value * scale.  table int32 [sequences, cols] (row stride table_ld): token t of sequence s lies in row
+ * t % page of page table[s][t / page].  D 64, 128 or 256; page a power of two in 16 .. 65536; both caches 16-byte aligned
+ * with strides of whole 16-byte units, a token stride of at most 2^26 elements.
+ *
+ * prism_kv_append: token i < *n_rows, at position p = pos[i] of sequence s = seq[i] (seq null: i).  The first rot dims of
+ * q and k turn by rope [rope_rows, rot] (fp32, row stride ldr: row p holds rot / 2 cosines, then the sines), pairs
+ * (j, j + rot / 2), or (2 j, 2 j + 1) when adjacent = 1:
+ *   a' = RN(RN(a cos) - RN(b sin)), b' = RN(RN(b cos) + RN(a sin)), rounded to the stored type.
+ * q bf16 [T, HQ, D] -> q_out (which may be q; HQ = 0: no queries), k, v bf16 [T, HKV, D] -> the cache; row and head
+ * strides in elements.  A token with no place (a position negative, past the table or the rotations; a sequence or page
+ * out of range) is skipped.  rot = 0: no rotation.  Needs rot % 16 == 0, rot <= D, 16-byte aligned q, k, v, q_out and rope,
+ * strides % 8 == 0 (ldr % 4).  No counterpart among the reference's quantized linear ops; nor have the entries below.
+ */
+PRISM_API int prism_kv_append(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
+                              int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, uint16_t* q_out, int64_t ldo,
+                              int64_t ho_s, const float* rope, int64_t ldr, int64_t rope_rows, int64_t rot,
+                              int adjacent, const int32_t* pos, const int32_t* seq, void* k_cache, int64_t k_page,
+                              int64_t k_tok, int64_t k_head, void* v_cache, int64_t v_page, int64_t v_tok,
+                              int64_t v_head, int e4m3, const float* k_scale, const float* v_scale,
+                              const int32_t* table, int64_t table_ld, int64_t seqs, int64_t cols, int64_t pages,
+                              int64_t page, const int32_t* n_rows, int64_t T, int64_t HQ, int64_t HKV, int64_t D,
+                              void* stream);
+
+/*
+ * Attention of one new token per sequence over the cache: for i < *n_rows, out[i][h] = sum_t softmax_t(scale q[i][h] .
+ * k_t) v_t over tokens t of max(0, lens[i] - window) .. lens[i] - 1 (window 0: all), head h on cache head h / (HQ / HKV);
+ * no tokens: zeros.  lens counts past the table's capacity, cols page, are taken as that.  fp32 sums and softmax, the
+ * weights in two bf16 parts; parts of a sequence (the split depends on all lengths) are joined in a fixed order through
+ * `ws` (prism_kv_attend_workspace_bytes, no initial contents; 16-byte aligned; calls that overlap must not share it).
+ * Rows >= *n_rows are untouched.  Needs HQ % HKV == 0, T <= 65535, 16-byte aligned q with strides % 8, 8-byte aligned out
+ * with strides % 4, cols page < 2^31 - 65536.
+ */
+PRISM_API int prism_kv_attend(const uint16_t* q, int64_t ldq, int64_t hq_s, const void* k_cache, int64_t k_page,
+                              int64_t k_tok, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_tok,
+                              int64_t v_head, int e4m3, const float* k_scale, const float* v_scale,
+                              const int32_t* table, int64_t table_ld, int64_t cols, int64_t pages, int64_t page,
+                              const int32_t* lens, uint16_t* out, int64_t ldo, int64_t ho_s, const int32_t* n_rows,
+                              int64_t T, int64_t HQ, int64_t HKV, int64_t D, float scale, int64_t window, void* ws,
+                              int64_t ws_bytes, void* stream);
+/* Bytes of ws for T sequences; 0 where nothing is split (ws may be null). */
+PRISM_API int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t cols,
+                                                  int64_t page);
+
+/*
+ * The gated delta rule, per value head h with key head h / (HV / HK) and state S fp32 [DK, DV]:
+ *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q,
+ * k and q first divided by sqrt(|.|^2 + eps) when norm = 1, q times scale either way; fp32 sums throughout.
+ * q, k bf16 [T, HK, DK], v bf16 [T, HV, DV] (row and head strides in elements), g, beta fp32 [T, HV], out fp32
+ * [T, HV, DV]; state [nslots, HV, DK, DV] contiguous per slot, slot_stride elements apart, updated in place; slots int32:
+ * the state of each sequence (null: its number).  A sequence whose slot is out of range is skipped; two sequences must
+ * not share one.  Needs DK, DV in {64, 128}, HV % HK == 0, 16-byte aligned tensors, strides % 8 (out and state % 4).
+ *
+ * prism_delta_step: row i < *n_rows is one token of sequence i.
+ * prism_delta_prefill: sequence s is rows cu[s] .. cu[s + 1] - 1 (cu int32 [seqs + 1], non-decreasing within 0 .. T), in
+ * order.  ws: prism_delta_prefill_workspace_bytes (no initial contents, 16-byte aligned; calls that overlap must not
+ * share it), null where that is 0.
+ */
+PRISM_API int prism_delta_step(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
+                               int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, const float* g, int64_t ldg,
+                               const float* beta, int64_t ldb, float* state, int64_t slot_stride, int64_t nslots,
+                               const int32_t* slots, float* out, int64_t ldo, int64_t ho_s, const int32_t* n_rows,
+                               int64_t T, int64_t HK, int64_t HV, int64_t DK, int64_t DV, int norm, float scale,
+                               float eps, void* stream);
+PRISM_API int prism_delta_prefill(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
+                                  int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, const float* g,
+                                  int64_t ldg, const float* beta, int64_t ldb, float* state, int64_t slot_stride,
+                                  int64_t nslots, const int32_t* slots, float* out, int64_t ldo, int64_t ho_s,
+                                  const int32_t* cu, int64_t seqs, int64_t T, int64_t HK, int64_t HV, int64_t DK,
+                                  int64_t DV, int norm, float scale, float eps, void* ws, int64_t ws_bytes,
+                                  void* stream);
+PRISM_API int64_t prism_delta_prefill_workspace_bytes(int64_t T, int64_t seqs, int64_t HK, int64_t HV, int64_t DK,
+                                                      int64_t DV);
+
 /*
  * Peak probes (measurement tooling: the reference's bench/csrc/mma_peak.cu:14-70 and bench/csrc/l2_bw.cu:8 for
  * this GPU, no counterpart on the engine's path).  prism_probe_mfma launches `workgroups` workgroups of 4 waves,
