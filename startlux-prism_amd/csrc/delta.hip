@@ -145,6 +145,415 @@ static int launch_rec(const DeltaArgs& a, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? (int)PRISM_OK : (int)PRISM_ERR_LAUNCH;
 }
 
+// ---------------------------------------------------------------------------------------------------------- chunked form
+// Chunks of 64 tokens.  With G the running sum of g in the chunk, the chunk's updates solve a triangular system:
+//   A_ij = beta_i e^(G_i - G_j) k_i . k_j (j < i),  X = (I + A)^-1,  U = X diag(beta) (V - diag(e^G) K S)
+//   O = diag(e^G) Q S + P U,  P_ij = e^(G_i - G_j) q_i . k_j (j <= i);  S <- e^(G_63) S + K^T diag(e^(G_63 - G)) U
+// Only S runs from chunk to chunk, so two kernels: delta_prep computes X diag(beta) and P of all chunks at once,
+// delta_scan walks each sequence's chunks.  The normalisation is row scales (rk, rq), so K and Q stay the bf16 they are.
+//
+// The products run on the bf16 MFMA at fp32's precision: an fp32 operand is three bf16 (x = hi + mid + lo, 8 bits each,
+// by truncation, exact), three products against K or Q, six against another such triple (what is dropped is below
+// 2^-24 of the terms).  That is 5 and 2.7 times the fp32 MFMA's rate.
+//
+// Everything that delta_scan multiplies from the left (K, Q, K^T, X diag(beta), P) lies in the workspace as MFMA
+// fragments, 1 KB each in lane order.  Inside a product the order of the summed index is free: taking it as an
+// accumulator's rows lie (lane group g: 4 g + r of one 16-row tile, then 4 g + r of the next), the accumulators of one
+// product are the right operand of the next as they are, and a wave owns 16 columns of S for the whole sequence
+// without exchanging anything.
+constexpr int kC = 64;                                        // tokens per chunk
+constexpr int kFrag = 1024;                                   // bytes of a fragment: 64 lanes of 8 bf16
+constexpr int kTri = 6;                                       // fragments (i, s) of a lower triangle: 16-row tile i, 32 columns s <= i / 2
+__host__ __device__ constexpr int tri(int i, int s) { return i < 2 ? i : 2 * i - 2 + s; }
+__host__ __device__ constexpr int64_t rec_k(int DK) { return (int64_t)(4 * (DK / 32) * 2 + DK / 16 * 2) * kFrag; }   // K, Q, K^T
+constexpr int64_t kRecV = 2 * 3 * kTri * kFrag + 4 * kC * 4;  // X diag(beta), P; row factors of K S and Q S, of U; e^(G_63)
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma_f32(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Eight fp32 (x then y) as three bf16 fragments.
+struct Split {
+    v4u h, m, l;
+};
+__device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_hi(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ Split split8(v4f x, v4f y) {
+    Split s;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const float a = w < 2 ? x[2 * w] : y[2 * w - 4], b = w < 2 ? x[2 * w + 1] : y[2 * w - 3];
+        const float a1 = a - cut(a), b1 = b - cut(b);
+        s.h[w] = pack_hi(a, b);
+        s.m[w] = pack_hi(a1, b1);
+        s.l[w] = pack_hi(a1 - cut(a1), b1 - cut(b1));
+    }
+    return s;
+}
+
+// Chunk `id` of the workspace: sequence b's chunks start at id cu[b] / 64 + b, which leaves each sequence room for its
+// ceil(length / 64) whatever the lengths.  False: no chunk has that number.
+__device__ __forceinline__ bool find_chunk(const DeltaArgs& a, int id, int& first, int& count) {
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < a.seqs; b0 += 64) {
+        const int b = b0 + lane;
+        int f = 0, n = 0;
+        if (b < a.seqs) {
+            f = min(max(__ldg(a.cu + b), 0), a.rows);
+            n = max(min(max(__ldg(a.cu + b + 1), 0), a.rows) - f, 0);
+        }
+        const int at = id - (f / kC + b);
+        const bool hit = at >= 0 && (int64_t)at * kC < n;
+        const uint64_t m = __ballot(hit);
+        if (m) {
+            const int src = __builtin_ctzll(m), c = __shfl(at, src, kWave) * kC;
+            first = __shfl(f, src, kWave) + c;
+            count = min(__shfl(n, src, kWave) - c, kC);
+            return true;
+        }
+    }
+    return false;
+}
+
+// One wave per chunk (blockIdx.x) and value head (blockIdx.y).
+template <int DK>
+__global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, char* wv) {
+    constexpr int KS = DK / 32, LD = kC + 4;
+    __shared__ __align__(16) float x[kC * LD];                // A, then X, in place; before that, K's rows (bf16)
+    __shared__ double gsum[kC];
+    __shared__ float rkv[kC], rqv[kC], bev[kC];
+    static_assert(sizeof(x) >= kC * (DK + 2) * 2, "K's rows");
+    int first, count;
+    if (!find_chunk(a, blockIdx.x, first, count)) return;
+    const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
+    const int head = blockIdx.y, share = a.HV / a.HK, hk = head / share;
+    const bool copies = head % share == 0;                    // this key head's K, Q and K^T fragments are this wave's to write
+    char* rk = wk + ((int64_t)blockIdx.x * a.HK + hk) * rec_k(DK);
+    char* rv = wv + ((int64_t)blockIdx.x * a.HV + head) * kRecV;
+
+    // the chunk's gates, one token per lane, the sums in 64 bits: the differences G_i - G_j are then as exact as the g.
+    // Below -1e4 a decay is 0 either way, and sums stay finite (-inf minus -inf would not be a number)
+    {
+        const bool in = lane < count;
+        float gv = in ? a.g[(int64_t)(first + lane) * a.ldg + head] : 0.f;
+        gv = gv < -1e4f ? -1e4f : gv;
+        double s = gv;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double up = __shfl_up(s, o, kWave);
+            if (lane >= o) s += up;
+        }
+        gsum[lane] = s;
+        bev[lane] = in ? a.beta[(int64_t)(first + lane) * a.ldb + head] : 0.f;
+    }
+    // K's and Q's rows as fragments: tile i's row col, dims 32 s + 8 g .. + 7; rows past the chunk are zeros
+    v4u kf[4][KS], qf[4][KS];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool in = 16 * i + col < count;
+        const int64_t t = first + (in ? 16 * i + col : 0);
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const v4u kk = *reinterpret_cast<const v4u*>(a.k + t * a.ldk + hk * a.hk_s + 32 * s + 8 * g);
+            const v4u qq = *reinterpret_cast<const v4u*>(a.q + t * a.ldq + hk * a.hq_s + 32 * s + 8 * g);
+            kf[i][s] = in ? kk : v4u{0, 0, 0, 0};
+            qf[i][s] = in ? qq : v4u{0, 0, 0, 0};
+        }
+        float sk = 0.f, sq = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float k0 = __uint_as_float(kf[i][s][w] << 16), k1 = cut(__uint_as_float(kf[i][s][w]));
+                const float q0 = __uint_as_float(qf[i][s][w] << 16), q1 = cut(__uint_as_float(qf[i][s][w]));
+                sk = fmaf(k0, k0, fmaf(k1, k1, sk));
+                sq = fmaf(q0, q0, fmaf(q1, q1, sq));
+            }
+        sk += __shfl_xor(sk, 16, kWave);
+        sk += __shfl_xor(sk, 32, kWave);
+        sq += __shfl_xor(sq, 16, kWave);
+        sq += __shfl_xor(sq, 32, kWave);
+        if (g == 0) {
+            rkv[16 * i + col] = a.norm ? div_rn(1.f, sqrt_rn(sk + a.eps)) : 1.f;
+            rqv[16 * i + col] = (a.norm ? div_rn(1.f, sqrt_rn(sq + a.eps)) : 1.f) * a.scale;
+        }
+    }
+    if (copies) {
+        // K and Q: fragment (i, s), piece p (4 dims) of a row at lane 16 (p % 4) + row, half p / 4
+        uint16_t* rows = reinterpret_cast<uint16_t*>(x);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                char* fk = rk + (i * KS + s) * kFrag;
+                char* fq = fk + 4 * KS * kFrag;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int p = 2 * g + h, at = (16 * (p & 3) + col) * 16 + 8 * (p >> 2);
+                    *reinterpret_cast<v2u*>(fk + at) = v2u{kf[i][s][2 * h], kf[i][s][2 * h + 1]};
+                    *reinterpret_cast<v2u*>(fq + at) = v2u{qf[i][s][2 * h], qf[i][s][2 * h + 1]};
+                }
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    *reinterpret_cast<uint32_t*>(rows + (16 * i + col) * (DK + 2) + 32 * s + 8 * g + 2 * w) = kf[i][s][w];
+            }
+        __syncthreads();
+        // K^T: fragment (d, s), row 16 d + col, tokens 32 s + 4 g + j and 32 s + 16 + 4 g + j
+        char* ft = rk + 8 * KS * kFrag;
+#pragma unroll
+        for (int d = 0; d < DK / 16; d++)
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                uint32_t u[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) u[j] = rows[(32 * s + 16 * (j / 4) + 4 * g + j % 4) * (DK + 2) + 16 * d + col];
+                *reinterpret_cast<v4u*>(ft + (2 * d + s) * kFrag + lane * 16) =
+                    v4u{u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16)};
+            }
+    }
+    __syncthreads();
+
+    // k_i . k_j and q_i . k_j, tiles j <= i, transposed: a lane holds row i = col for columns 4 g + r, which is a
+    // fragment's order
+    v4f pt[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const double gi = gsum[16 * i + col];
+        const float ki = bev[16 * i + col] * rkv[16 * i + col], qi = rqv[16 * i + col];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            pt[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (j > i) continue;
+            v4f kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                kk = mfma_bf16(kf[j][s], kf[i][s], kk);
+                qk = mfma_bf16(kf[j][s], qf[i][s], qk);
+            }
+            v4f am;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int row = 16 * i + col, c = 16 * j + 4 * g + r;
+                const float f = expf((float)(gi - gsum[c])) * rkv[c];
+                am[r] = c < row ? f * ki * kk[r] : 0.f;
+                pt[i][j][r] = c <= row ? f * qi * qk[r] : 0.f;
+            }
+            *reinterpret_cast<v4f*>(x + (16 * i + col) * LD + 16 * j + 4 * g) = am;
+        }
+    }
+    char* pa = rv + 3 * kTri * kFrag;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int s = 0; s <= i / 2; s++) {
+            const Split p = split8(pt[i][2 * s], pt[i][2 * s + 1]);
+            char* f = pa + 3 * tri(i, s) * kFrag + lane * 16;
+            *reinterpret_cast<v4u*>(f) = p.h;
+            *reinterpret_cast<v4u*>(f + kFrag) = p.m;
+            *reinterpret_cast<v4u*>(f + 2 * kFrag) = p.l;
+        }
+    {
+        float* vec = reinterpret_cast<float*>(rv + 6 * kTri * kFrag);
+        const double gl = gsum[lane], gc = gsum[kC - 1];
+        const float e = expf((float)gl);
+        vec[lane] = e * rkv[lane];
+        vec[kC + lane] = e * rqv[lane];
+        vec[2 * kC + lane] = expf((float)(gc - gl)) * rkv[lane];
+        vec[3 * kC + lane] = expf((float)gc);
+    }
+    __syncthreads();
+
+    // the four diagonal blocks of I + A inverted at once by forward substitution, a column per lane
+    {
+        const float* d = x + 16 * g * LD + 16 * g;
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float s = i == col ? 1.f : 0.f;
+#pragma unroll
+            for (int j4 = 0; j4 < (i + 3) / 4; j4++) {
+                const v4f row = *reinterpret_cast<const v4f*>(d + i * LD + 4 * j4);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (4 * j4 + j < i) s = fmaf(-row[j], v[4 * j4 + j], s);
+            }
+            v[i] = s;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; i++) x[(16 * g + i) * LD + 16 * g + col] = v[i];
+    }
+    __syncthreads();
+    // the blocks below: X_ij = -X_ii sum_k A_ik X_kj, columns from the left, so that A_ij's place is free for X_ij
+#pragma unroll
+    for (int j = 0; j < 3; j++)
+#pragma unroll
+        for (int i = j + 1; i < 4; i++) {
+            v4f s = {0.f, 0.f, 0.f, 0.f}, y = s;
+#pragma unroll
+            for (int k = j; k < i; k++) {
+                const v4f am = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * k + 4 * g);
+#pragma unroll
+                for (int r = 0; r < 4; r++) s = mfma_f32(am[r], x[(16 * k + 4 * g + r) * LD + 16 * j + col], s);
+            }
+            const v4f xi = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * i + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++) y = mfma_f32(xi[r], s[r], y);
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[(16 * i + 4 * g + r) * LD + 16 * j + col] = -y[r];
+            __syncthreads();
+        }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int s = 0; s <= i / 2; s++) {
+            v4f h[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int c = 32 * s + 16 * e + 4 * g;
+                h[e] = v4f{0.f, 0.f, 0.f, 0.f};
+                if (2 * s + e <= i) {
+                    h[e] = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + c);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) h[e][r] *= bev[c + r];
+                }
+            }
+            const Split p = split8(h[0], h[1]);
+            char* f = rv + 3 * tri(i, s) * kFrag + lane * 16;
+            *reinterpret_cast<v4u*>(f) = p.h;
+            *reinterpret_cast<v4u*>(f + kFrag) = p.m;
+            *reinterpret_cast<v4u*>(f + 2 * kFrag) = p.l;
+        }
+}
+
+__device__ __forceinline__ v4u frag(const char* base, int i, int lane) {
+    return *reinterpret_cast<const v4u*>(base + i * kFrag + lane * 16);
+}
+// c + (three-part a)(three-part b), the small products first
+__device__ __forceinline__ v4f mfma_six(v4u ah, v4u am, v4u al, const Split& b, v4f c) {
+    c = mfma_bf16(al, b.h, c);
+    c = mfma_bf16(am, b.m, c);
+    c = mfma_bf16(ah, b.l, c);
+    c = mfma_bf16(am, b.h, c);
+    c = mfma_bf16(ah, b.m, c);
+    return mfma_bf16(ah, b.h, c);
+}
+__device__ __forceinline__ v4f mfma_three(v4u a, const Split& b, v4f c) {
+    c = mfma_bf16(a, b.l, c);
+    c = mfma_bf16(a, b.m, c);
+    return mfma_bf16(a, b.h, c);
+}
+
+// One wave per sequence, value head and 16 columns.
+template <int DK, int DV>
+__global__ __launch_bounds__(64, 1) void delta_scan_kernel(DeltaArgs a, const char* wk, const char* wv) {
+    constexpr int KS = DK / 32, DT = DK / 16, CT = DV / 16;
+    const int ct = blockIdx.x % CT, head = blockIdx.x / CT % a.HV, b = blockIdx.x / CT / a.HV;
+    int first, count, slot;
+    if (!delta_seq(a, b, first, count, slot)) return;
+    const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
+    const int hk = head / (a.HV / a.HK);
+    float* st = a.state + slot * a.lds_ + (int64_t)head * DK * DV + 16 * ct + col;
+    v4f s[DT];
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[d][r] = st[(16 * d + 4 * g + r) * DV];
+    const int base = first / kC + b;
+    for (int c = 0; c * kC < count; c++) {
+        const char* rk = wk + ((int64_t)(base + c) * a.HK + hk) * rec_k(DK);
+        const char* rv = wv + ((int64_t)(base + c) * a.HV + head) * kRecV;
+        const float* vec = reinterpret_cast<const float*>(rv + 6 * kTri * kFrag);
+        const int left = count - c * kC;
+        const uint16_t* v = a.v + (int64_t)(first + c * kC) * a.ldv + head * a.hv_s + 16 * ct + col;
+        Split sp[KS];
+#pragma unroll
+        for (int k = 0; k < KS; k++) sp[k] = split8(s[2 * k], s[2 * k + 1]);
+        v4f rr[4], o[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v4f ks = {0.f, 0.f, 0.f, 0.f}, qs = ks;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                ks = mfma_three(frag(rk, i * KS + k, lane), sp[k], ks);
+                qs = mfma_three(frag(rk, (4 + i) * KS + k, lane), sp[k], qs);
+            }
+            const v4f ek = *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
+            const v4f eq = *reinterpret_cast<const v4f*>(vec + kC + 16 * i + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int t = 16 * i + 4 * g + r;
+                const float vt = t < left ? bf16_to_f32(v[(int64_t)t * a.ldv]) : 0.f;
+                rr[i][r] = fmaf(-ek[r], ks[r], vt);
+                o[i][r] = eq[r] * qs[r];
+            }
+        }
+        v4f u[4];
+        {
+            const Split r0 = split8(rr[0], rr[1]), r1 = split8(rr[2], rr[3]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                u[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k <= i / 2; k++)
+                    u[i] = mfma_six(frag(rv, 3 * tri(i, k), lane), frag(rv, 3 * tri(i, k) + 1, lane),
+                                    frag(rv, 3 * tri(i, k) + 2, lane), k ? r1 : r0, u[i]);
+            }
+        }
+        {
+            const char* pa = rv + 3 * kTri * kFrag;
+            const Split u0 = split8(u[0], u[1]), u1 = split8(u[2], u[3]);
+            float* out = a.out + (int64_t)(first + c * kC) * a.ldo + head * a.ho_s + 16 * ct + col;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+#pragma unroll
+                for (int k = 0; k <= i / 2; k++)
+                    o[i] = mfma_six(frag(pa, 3 * tri(i, k), lane), frag(pa, 3 * tri(i, k) + 1, lane),
+                                    frag(pa, 3 * tri(i, k) + 2, lane), k ? u1 : u0, o[i]);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int t = 16 * i + 4 * g + r;
+                    if (t < left) out[(int64_t)t * a.ldo] = o[i][r];
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[i] *= *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
+        const Split u0 = split8(u[0], u[1]), u1 = split8(u[2], u[3]);
+        const float ec = vec[3 * kC];
+        const char* kt = rk + 8 * KS * kFrag;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            s[d] *= ec;
+            s[d] = mfma_three(frag(kt, 2 * d, lane), u0, s[d]);
+            s[d] = mfma_three(frag(kt, 2 * d + 1, lane), u1, s[d]);
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) st[(16 * d + 4 * g + r) * DV] = s[d][r];
+}
+
+static int64_t chunks(int64_t T, int64_t seqs) { return T / kC + seqs; }
+
+template <int DK, int DV>
+static int launch_chunks(const DeltaArgs& a, char* ws, hipStream_t st) {
+    const int64_t nc = chunks(a.rows, a.seqs), waves = (int64_t)a.seqs * a.HV * (DV / 16);
+    if (nc > INT32_MAX || a.HV > 65535 || waves > INT32_MAX) return PRISM_ERR_SHAPE;
+    char* wv = ws + nc * a.HK * rec_k(DK);
+    hipLaunchKernelGGL(delta_prep_kernel<DK>, dim3((unsigned)nc, (unsigned)a.HV), dim3(64), 0, st, a, ws, wv);
+    PRISM_LAUNCH_CHECK();
+    hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)waves), dim3(64), 0, st, a, ws, wv);
+    PRISM_LAUNCH_CHECK();
+    return PRISM_OK;
+}
+
 static int check(const DeltaArgs& a, int64_t rows, int64_t seqs, int64_t nslots, int64_t HK, int64_t HV, int64_t DK,
                  int64_t DV) {
     if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.state || !a.out || (a.norm != 0 && a.norm != 1)) return PRISM_ERR_ARG;
@@ -163,6 +572,14 @@ static int dispatch_rec(const DeltaArgs& a, int64_t DK, int64_t DV, hipStream_t 
     if (DK == 64) return DV == 64 ? launch_rec<64, 64>(a, st) : launch_rec<64, 128>(a, st);
     return DV == 64 ? launch_rec<128, 64>(a, st) : launch_rec<128, 128>(a, st);
 }
+
+static int dispatch_chunks(const DeltaArgs& a, int64_t DK, int64_t DV, char* ws, hipStream_t st) {
+    if (DK == 64) return DV == 64 ? launch_chunks<64, 64>(a, ws, st) : launch_chunks<64, 128>(a, ws, st);
+    return DV == 64 ? launch_chunks<128, 64>(a, ws, st) : launch_chunks<128, 128>(a, ws, st);
+}
+
+// A handful of rows go token by token.
+static bool by_token(int64_t T) { return T <= 16; }
 
 }  // namespace prism
 
@@ -195,11 +612,16 @@ extern "C" int prism_delta_prefill(const uint16_t* q, int64_t ldq, int64_t hq_s,
     const int rc = check(a, T, seqs, nslots, HK, HV, DK, DV);
     if (rc != PRISM_OK) return rc;
     if (!cu) return PRISM_ERR_ARG;
+    const int64_t need = prism_delta_prefill_workspace_bytes(T, seqs, HK, HV, DK, DV);
+    if (need > 0 && (!ws || ws_bytes < need)) return PRISM_ERR_ARG;
+    if (need > 0 && !PRISM_ALIGNED(ws, 16)) return PRISM_ERR_ALIGN;
     if (T == 0 || seqs == 0 || nslots == 0) return PRISM_OK;
-    return dispatch_rec(a, DK, DV, (hipStream_t)stream);
+    if (by_token(T)) return dispatch_rec(a, DK, DV, (hipStream_t)stream);
+    return dispatch_chunks(a, DK, DV, (char*)ws, (hipStream_t)stream);
 }
 
 extern "C" int64_t prism_delta_prefill_workspace_bytes(int64_t T, int64_t seqs, int64_t HK, int64_t HV, int64_t DK,
                                                        int64_t DV) {
-    return 0;
+    if (T < 1 || seqs < 1 || HK < 1 || HV < 1 || (DK != 64 && DK != 128) || by_token(T)) return 0;
+    return chunks(T, seqs) * (HK * rec_k((int)DK) + HV * kRecV);
 }

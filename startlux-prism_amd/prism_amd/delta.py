@@ -1,5 +1,5 @@
 """The gated delta rule of a linear-attention layer in serving: `step` for one new token per sequence (the recurrent
-form), `prefill` for whole prompts packed one after the other.
+form), `prefill` for whole prompts packed one after the other (chunks on the matrix cores).
 
 Per value head, with its state S fp32 [dk, dv], a = exp(g), key k and query q of key head h // (value heads / key heads):
 
