@@ -449,107 +449,187 @@ __device__ __forceinline__ v4f mfma_three(v4u a, const Split& b, v4f c) {
     return mfma_bf16(a, b.h, c);
 }
 
-// One wave per sequence, value head and 16 columns.
+// The fragments base + i KB, i < N, one load each.
+template <int N>
+__device__ __forceinline__ void load_frags(v4u (&f)[N], const char* base, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; i++) f[i] = frag(base, i, lane);
+}
+
+// A workgroup walks the chunks of one sequence and value head for 32 columns of the state, two waves to 16 columns: one
+// holds S and takes what the next chunk waits for (K S, U, K^T U), the other the chunk's output (Q S, P U).  They share S
+// and U through LDS, fp32 in the accumulators' order, a barrier for each; fragments come straight into registers, each
+// group for the next chunk right after its last use, so that a load has a whole chunk's time.
 template <int DK, int DV>
-__global__ __launch_bounds__(64, 1) void delta_scan_kernel(DeltaArgs a, const char* wk, const char* wv) {
-    constexpr int KS = DK / 32, DT = DK / 16, CT = DV / 16;
-    const int ct = blockIdx.x % CT, head = blockIdx.x / CT % a.HV, b = blockIdx.x / CT / a.HV;
+__global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, const char* wk, const char* wv, int keys) {
+    constexpr int KS = DK / 32, DT = DK / 16, CT = DV / 32;
+    __shared__ v4f sx[2][DT][64], ux[2][4][64];
+    // the workgroups of one key head, which read the same K and Q, on one XCD (workgroup i runs on XCD i % 8)
+    const int share = a.HV / a.HK, per = share * CT;
+    const int grp = blockIdx.x / (8 * per), key = 8 * grp + blockIdx.x % 8, m = blockIdx.x / 8 % per;
+    if (key >= keys) return;
+    const int b = key / a.HK, hk = key % a.HK, head = hk * share + m / CT;
     int first, count, slot;
     if (!delta_seq(a, b, first, count, slot)) return;
-    const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
-    const int hk = head / (a.HV / a.HK);
-    float* st = a.state + slot * a.lds_ + (int64_t)head * DK * DV + 16 * ct + col;
-    v4f s[DT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4, w = wave & 1;
+    const int c0 = 32 * (m % CT) + 16 * w + col;              // this lane's column
+    const int nc = (count + kC - 1) / kC, base = first / kC + b;
+    const char* rk = wk + ((int64_t)base * a.HK + hk) * rec_k(DK);
+    const char* rv = wv + ((int64_t)base * a.HV + head) * kRecV;
+    const int64_t rks = (int64_t)a.HK * rec_k(DK), rvs = (int64_t)a.HV * kRecV;
+    constexpr int kVec = 6 * kTri * kFrag;
+    if (wave < 2) {
+        float* st = a.state + slot * a.lds_ + (int64_t)head * DK * DV + c0;
+        v4f s[DT];
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) s[d][r] = st[(16 * d + 4 * g + r) * DV];
-    const int base = first / kC + b;
-    for (int c = 0; c * kC < count; c++) {
-        const char* rk = wk + ((int64_t)(base + c) * a.HK + hk) * rec_k(DK);
-        const char* rv = wv + ((int64_t)(base + c) * a.HV + head) * kRecV;
-        const float* vec = reinterpret_cast<const float*>(rv + 6 * kTri * kFrag);
-        const int left = count - c * kC;
-        const uint16_t* v = a.v + (int64_t)(first + c * kC) * a.ldv + head * a.hv_s + 16 * ct + col;
-        Split sp[KS];
+            for (int r = 0; r < 4; r++) s[d][r] = st[(16 * d + 4 * g + r) * DV];
+        v4u ka[4 * KS], ta[3 * kTri], kt[2 * DT];
+        v4f ek[4], ew[4];
+        uint16_t v[4][4];
+        float ec;
+        load_frags(ka, rk, lane);
+        load_frags(ta, rv, lane);
+        load_frags(kt, rk + 8 * KS * kFrag, lane);
+        const uint16_t* vp = a.v + (int64_t)first * a.ldv + head * a.hv_s + c0;
+        // rows past the chunk's end read its last row: their columns of X diag(beta) are zeros
+        auto load_v = [&](const uint16_t* p, int left) {
 #pragma unroll
-        for (int k = 0; k < KS; k++) sp[k] = split8(s[2 * k], s[2 * k + 1]);
-        v4f rr[4], o[4];
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v4f ks = {0.f, 0.f, 0.f, 0.f}, qs = ks;
+                for (int r = 0; r < 4; r++) v[i][r] = p[(int64_t)min(16 * i + 4 * g + r, left - 1) * a.ldv];
+        };
+        auto load_vec = [&](const char* r) {
+            const float* vec = reinterpret_cast<const float*>(r + kVec);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ek[i] = *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
+                ew[i] = *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
+            }
+            ec = vec[3 * kC];
+        };
+        load_v(vp, count);
+        load_vec(rv);
+#pragma unroll
+        for (int d = 0; d < DT; d++) sx[w][d][lane] = s[d];
+        lds_barrier();
+        for (int c = 0; c < nc; c++) {
+            const bool more = c + 1 < nc;                     // (past the last chunk it is read again)
+            rk += more ? rks : 0;
+            rv += more ? rvs : 0;
+            v4f ks[4], rr[4], u[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) ks[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                ks = mfma_three(frag(rk, i * KS + k, lane), sp[k], ks);
-                qs = mfma_three(frag(rk, (4 + i) * KS + k, lane), sp[k], qs);
-            }
-            const v4f ek = *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
-            const v4f eq = *reinterpret_cast<const v4f*>(vec + kC + 16 * i + 4 * g);
+                const Split sp = split8(s[2 * k], s[2 * k + 1]);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int t = 16 * i + 4 * g + r;
-                const float vt = t < left ? bf16_to_f32(v[(int64_t)t * a.ldv]) : 0.f;
-                rr[i][r] = fmaf(-ek[r], ks[r], vt);
-                o[i][r] = eq[r] * qs[r];
+                for (int i = 0; i < 4; i++) ks[i] = mfma_three(ka[i * KS + k], sp, ks[i]);
             }
-        }
-        v4f u[4];
-        {
+            load_frags(ka, rk, lane);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) rr[i][r] = fmaf(-ek[i][r], ks[i][r], bf16_to_f32(v[i][r]));
+            const int left = count - (c + more) * kC;
+            vp += more ? kC * a.ldv : 0;
+            load_v(vp, left);
             const Split r0 = split8(rr[0], rr[1]), r1 = split8(rr[2], rr[3]);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 u[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k <= i / 2; k++)
-                    u[i] = mfma_six(frag(rv, 3 * tri(i, k), lane), frag(rv, 3 * tri(i, k) + 1, lane),
-                                    frag(rv, 3 * tri(i, k) + 2, lane), k ? r1 : r0, u[i]);
+                    u[i] = mfma_six(ta[3 * tri(i, k)], ta[3 * tri(i, k) + 1], ta[3 * tri(i, k) + 2], k ? r1 : r0, u[i]);
             }
-        }
-        {
-            const char* pa = rv + 3 * kTri * kFrag;
-            const Split u0 = split8(u[0], u[1]), u1 = split8(u[2], u[3]);
-            float* out = a.out + (int64_t)(first + c * kC) * a.ldo + head * a.ho_s + 16 * ct + col;
+            load_frags(ta, rv, lane);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < 4; i++) ux[w][i][lane] = u[i];
+            lds_barrier();
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[i] *= ew[i];
+            const Split u0 = split8(u[0], u[1]), u1 = split8(u[2], u[3]);
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                s[d] *= ec;
+                s[d] = mfma_three(kt[2 * d], u0, s[d]);
+                s[d] = mfma_three(kt[2 * d + 1], u1, s[d]);
+            }
+            load_frags(kt, rk + 8 * KS * kFrag, lane);
+            load_vec(rv);
+#pragma unroll
+            for (int d = 0; d < DT; d++) sx[w][d][lane] = s[d];
+            lds_barrier();
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) st[(16 * d + 4 * g + r) * DV] = s[d][r];
+    } else {
+        v4u qa[4 * KS], pa[3 * kTri];
+        v4f eq[4];
+        auto load_vec = [&](const char* r) {
+            const float* vec = reinterpret_cast<const float*>(r + kVec);
+#pragma unroll
+            for (int i = 0; i < 4; i++) eq[i] = *reinterpret_cast<const v4f*>(vec + kC + 16 * i + 4 * g);
+        };
+        load_frags(qa, rk + 4 * KS * kFrag, lane);
+        load_frags(pa, rv + 3 * kTri * kFrag, lane);
+        load_vec(rv);
+        float* out = a.out + (int64_t)first * a.ldo + head * a.ho_s + c0;
+        lds_barrier();
+        for (int c = 0; c < nc; c++) {
+            const bool more = c + 1 < nc;
+            rk += more ? rks : 0;
+            rv += more ? rvs : 0;
+            v4f o[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const Split sp = split8(sx[w][2 * k][lane], sx[w][2 * k + 1][lane]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = mfma_three(qa[i * KS + k], sp, o[i]);
+            }
+            load_frags(qa, rk + 4 * KS * kFrag, lane);
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] *= eq[i];
+            load_vec(rv);
+            lds_barrier();
+            const Split u0 = split8(ux[w][0][lane], ux[w][1][lane]), u1 = split8(ux[w][2][lane], ux[w][3][lane]);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int k = 0; k <= i / 2; k++)
-                    o[i] = mfma_six(frag(pa, 3 * tri(i, k), lane), frag(pa, 3 * tri(i, k) + 1, lane),
-                                    frag(pa, 3 * tri(i, k) + 2, lane), k ? u1 : u0, o[i]);
+                    o[i] = mfma_six(pa[3 * tri(i, k)], pa[3 * tri(i, k) + 1], pa[3 * tri(i, k) + 2], k ? u1 : u0, o[i]);
+            load_frags(pa, rv + 3 * kTri * kFrag, lane);
+            const int left = count - c * kC;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int t = 16 * i + 4 * g + r;
                     if (t < left) out[(int64_t)t * a.ldo] = o[i][r];
                 }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) u[i] *= *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
-        const Split u0 = split8(u[0], u[1]), u1 = split8(u[2], u[3]);
-        const float ec = vec[3 * kC];
-        const char* kt = rk + 8 * KS * kFrag;
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-            s[d] *= ec;
-            s[d] = mfma_three(frag(kt, 2 * d, lane), u0, s[d]);
-            s[d] = mfma_three(frag(kt, 2 * d + 1, lane), u1, s[d]);
+            out += kC * a.ldo;
+            lds_barrier();
         }
     }
-#pragma unroll
-    for (int d = 0; d < DT; d++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) st[(16 * d + 4 * g + r) * DV] = s[d][r];
 }
 
 static int64_t chunks(int64_t T, int64_t seqs) { return T / kC + seqs; }
 
 template <int DK, int DV>
 static int launch_chunks(const DeltaArgs& a, char* ws, hipStream_t st) {
-    const int64_t nc = chunks(a.rows, a.seqs), waves = (int64_t)a.seqs * a.HV * (DV / 16);
-    if (nc > INT32_MAX || a.HV > 65535 || waves > INT32_MAX) return PRISM_ERR_SHAPE;
+    const int64_t nc = chunks(a.rows, a.seqs), keys = (int64_t)a.seqs * a.HK;
+    const int64_t wgs = (keys + 7) / 8 * 8 * (a.HV / a.HK) * (DV / 32);
+    if (nc > INT32_MAX || a.HV > 65535 || wgs > INT32_MAX) return PRISM_ERR_SHAPE;
     char* wv = ws + nc * a.HK * rec_k(DK);
     hipLaunchKernelGGL(delta_prep_kernel<DK>, dim3((unsigned)nc, (unsigned)a.HV), dim3(64), 0, st, a, ws, wv);
     PRISM_LAUNCH_CHECK();
-    hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)waves), dim3(64), 0, st, a, ws, wv);
+    hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)wgs), dim3(256), 0, st, a, ws, wv, (int)keys);
     PRISM_LAUNCH_CHECK();
     return PRISM_OK;
 }
