@@ -431,39 +431,18 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
         }
 }
 
-__device__ __forceinline__ v4u frag(const char* base, int i, int lane) {
-    return *reinterpret_cast<const v4u*>(base + i * kFrag + lane * 16);
-}
-// c + (three-part a)(three-part b), the small products first
-__device__ __forceinline__ v4f mfma_six(v4u ah, v4u am, v4u al, const Split& b, v4f c) {
-    c = mfma_bf16(al, b.h, c);
-    c = mfma_bf16(am, b.m, c);
-    c = mfma_bf16(ah, b.l, c);
-    c = mfma_bf16(am, b.h, c);
-    c = mfma_bf16(ah, b.m, c);
-    return mfma_bf16(ah, b.h, c);
-}
-__device__ __forceinline__ v4f mfma_three(v4u a, const Split& b, v4f c) {
-    c = mfma_bf16(a, b.l, c);
-    c = mfma_bf16(a, b.m, c);
-    return mfma_bf16(a, b.h, c);
-}
-
-// The fragments base + i KB, i < N, one load each.
-template <int N>
-__device__ __forceinline__ void load_frags(v4u (&f)[N], const char* base, int lane) {
-#pragma unroll
-    for (int i = 0; i < N; i++) f[i] = frag(base, i, lane);
-}
-
-// A workgroup walks the chunks of one sequence and value head for 32 columns of the state, two waves to 16 columns: one
-// holds S and takes what the next chunk waits for (K S, U, K^T U), the other the chunk's output (Q S, P U).  They share S
-// and U through LDS, fp32 in the accumulators' order, a barrier for each; fragments come straight into registers, each
-// group for the next chunk right after its last use, so that a load has a whole chunk's time.
+// A workgroup walks the chunks of one sequence and value head for 32 columns of the state: four waves to 16 columns, on
+// a SIMD each, two holding the halves of S's rows and taking what the next chunk waits for (K S, U, K^T U), two the
+// chunk's output (Q S, P U).  Products split over the summed index: a wave multiplies its half of S's rows, or its half
+// of U's tokens, and the halves' sums (fp32, always the same two added) meet in LDS.  Two barriers per chunk:
+//   state waves   K S, halves out | halves in, R, X R out | U in, S <- ..., S out, next K S
+//   output waves  (rest of the last chunk's output) S in, Q S | U in, P U, halves out
+// Fragments come straight into registers, each group for the next chunk right after its last use, so that a load has
+// about a whole chunk's time.
 template <int DK, int DV>
-__global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, const char* wk, const char* wv, int keys) {
-    constexpr int KS = DK / 32, DT = DK / 16, CT = DV / 32;
-    __shared__ v4f sx[2][DT][64], ux[2][4][64];
+__global__ __launch_bounds__(512, 1) void delta_scan_kernel(DeltaArgs a, const char* wk, const char* wv, int keys) {
+    constexpr int KS = DK / 32, DT = DK / 16, CT = DV / 32, KH = KS / 2, DH = DT / 2;
+    __shared__ v4f sx[2][DT][64], kx[2][4][64], ux[2][6][64], ox[2][4][64];
     // the workgroups of one key head, which read the same K and Q, on one XCD (workgroup i runs on XCD i % 8)
     const int share = a.HV / a.HK, per = share * CT;
     const int grp = blockIdx.x / (8 * per), key = 8 * grp + blockIdx.x % 8, m = blockIdx.x / 8 % per;
@@ -472,150 +451,229 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(DeltaArgs a, const c
     int first, count, slot;
     if (!delta_seq(a, b, first, count, slot)) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4, w = wave & 1;
+    const int col = lane & 15, g = lane >> 4, w = wave & 1, half = wave >> 1 & 1;
     const int c0 = 32 * (m % CT) + 16 * w + col;              // this lane's column
     const int nc = (count + kC - 1) / kC, base = first / kC + b;
-    const char* rk = wk + ((int64_t)base * a.HK + hk) * rec_k(DK);
-    const char* rv = wv + ((int64_t)base * a.HV + head) * kRecV;
+    const char* rk = wk + ((int64_t)base * a.HK + hk) * rec_k(DK) + lane * 16;
+    const char* rv = wv + ((int64_t)base * a.HV + head) * kRecV + lane * 16;
+    const float* vec = reinterpret_cast<const float*>(wv + ((int64_t)base * a.HV + head) * kRecV + 6 * kTri * kFrag);
     const int64_t rks = (int64_t)a.HK * rec_k(DK), rvs = (int64_t)a.HV * kRecV;
-    constexpr int kVec = 6 * kTri * kFrag;
-    if (wave < 2) {
+    // K or Q (4 token tiles, this half's k), X diag(beta) or P (token tiles from 2 half, columns half)
+    v4u fk[4][KH], ft[4][3];
+    auto load_rows = [&](const char* r) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int k = 0; k < KH; k++)
+                fk[i][k] = *reinterpret_cast<const v4u*>(r + (i * KS + half * KH + k) * kFrag);
+    };
+    auto load_tri = [&](const char* r) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (half && i < 2) continue;                      // (wave-uniform)
+#pragma unroll
+            for (int x = 0; x < 3; x++)
+                ft[i][x] = *reinterpret_cast<const v4u*>(r + (3 * (i < 2 ? i : 2 * i - 2 + half) + x) * kFrag);
+        }
+    };
+    if (wave < 4) {
         float* st = a.state + slot * a.lds_ + (int64_t)head * DK * DV + c0;
-        v4f s[DT];
+        v4f s[DH];
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DH; d++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[d][r] = st[(16 * d + 4 * g + r) * DV];
-        v4u ka[4 * KS], ta[3 * kTri], kt[2 * DT];
-        v4f ek[4], ew[4];
-        uint16_t v[4][4];
+            for (int r = 0; r < 4; r++) s[d][r] = st[(16 * (half * DH + d) + 4 * g + r) * DV];
+        v4u kt[DH][2];
+        v4f ek[2], ew[4];
+        uint32_t off[2][4];                                   // this half's tokens' values (bytes from the chunk's)
+        uint16_t v[2][4];
         float ec;
-        load_frags(ka, rk, lane);
-        load_frags(ta, rv, lane);
-        load_frags(kt, rk + 8 * KS * kFrag, lane);
-        const uint16_t* vp = a.v + (int64_t)first * a.ldv + head * a.hv_s + c0;
-        // rows past the chunk's end read its last row: their columns of X diag(beta) are zeros
-        auto load_v = [&](const uint16_t* p, int left) {
+        const char* vp = reinterpret_cast<const char*>(a.v + (int64_t)first * a.ldv + head * a.hv_s + c0);
+        auto load_kt = [&](const char* r) {
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int d = 0; d < DH; d++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) v[i][r] = p[(int64_t)min(16 * i + 4 * g + r, left - 1) * a.ldv];
+                for (int x = 0; x < 2; x++)
+                    kt[d][x] = *reinterpret_cast<const v4u*>(r + (8 * KS + 2 * (half * DH + d) + x) * kFrag);
         };
-        auto load_vec = [&](const char* r) {
-            const float* vec = reinterpret_cast<const float*>(r + kVec);
+        // rows past the chunk's end read its last row: their columns of X diag(beta) are zeros
+        auto offsets = [&](int left) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                ek[i] = *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
-                ew[i] = *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
-            }
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    off[i][r] = 2u * (uint32_t)a.ldv * (uint32_t)min(32 * half + 16 * i + 4 * g + r, left - 1);
+        };
+        auto load_v = [&] {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[i][r] = *reinterpret_cast<const uint16_t*>(vp + off[i][r]);
+        };
+        auto load_vec = [&] {
+#pragma unroll
+            for (int i = 0; i < 2; i++) ek[i] = *reinterpret_cast<const v4f*>(vec + 32 * half + 16 * i + 4 * g);
+#pragma unroll
+            for (int i = 0; i < 4; i++) ew[i] = *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
             ec = vec[3 * kC];
         };
-        load_v(vp, count);
-        load_vec(rv);
+        load_rows(rk);
+        load_tri(rv);
+        load_kt(rk);
+        offsets(count);
+        load_v();
+        load_vec();
 #pragma unroll
-        for (int d = 0; d < DT; d++) sx[w][d][lane] = s[d];
-        lds_barrier();
+        for (int d = 0; d < DH; d++) sx[w][half * DH + d][lane] = s[d];
         for (int c = 0; c < nc; c++) {
             const bool more = c + 1 < nc;                     // (past the last chunk it is read again)
             rk += more ? rks : 0;
             rv += more ? rvs : 0;
-            v4f ks[4], rr[4], u[4];
+            vec += more ? rvs / 4 : 0;
+            v4f ks[4], u[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) ks[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
+            for (int k = 0; k < KH; k++) {
                 const Split sp = split8(s[2 * k], s[2 * k + 1]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) ks[i] = mfma_three(ka[i * KS + k], sp, ks[i]);
+                for (int i = 0; i < 4; i++) ks[i] = mfma_bf16(fk[i][k], sp.l, ks[i]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) ks[i] = mfma_bf16(fk[i][k], sp.m, ks[i]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) ks[i] = mfma_bf16(fk[i][k], sp.h, ks[i]);
             }
-            load_frags(ka, rk, lane);
+            load_rows(rk);
+            // the other half's tokens' sums out, this half's in
+            v4f mine[2];
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) rr[i][r] = fmaf(-ek[i][r], ks[i][r], bf16_to_f32(v[i][r]));
-            const int left = count - (c + more) * kC;
-            vp += more ? kC * a.ldv : 0;
-            load_v(vp, left);
-            const Split r0 = split8(rr[0], rr[1]), r1 = split8(rr[2], rr[3]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                u[i] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k <= i / 2; k++)
-                    u[i] = mfma_six(ta[3 * tri(i, k)], ta[3 * tri(i, k) + 1], ta[3 * tri(i, k) + 2], k ? r1 : r0, u[i]);
+            for (int i = 0; i < 2; i++) {
+                kx[w][2 - 2 * half + i][lane] = half ? ks[i] : ks[2 + i];
+                mine[i] = half ? ks[2 + i] : ks[i];
             }
-            load_frags(ta, rv, lane);
-#pragma unroll
-            for (int i = 0; i < 4; i++) ux[w][i][lane] = u[i];
             lds_barrier();
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                mine[i] += kx[w][2 * half + i][lane];
+#pragma unroll
+                for (int r = 0; r < 4; r++) mine[i][r] = fmaf(-ek[i][r], mine[i][r], bf16_to_f32(v[i][r]));
+            }
+            if (more) {
+                vp += 2 * kC * a.ldv;
+                if (count - (c + 1) * kC < kC) offsets(count - (c + 1) * kC);
+            }
+            load_v();
+            const Split rs = split8(mine[0], mine[1]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#define TRI(X, Y)                                                            \
+    if (!half) {                                                             \
+        u[0] = mfma_bf16(ft[0][X], rs.Y, u[0]);                              \
+        u[1] = mfma_bf16(ft[1][X], rs.Y, u[1]);                              \
+    }                                                                        \
+    u[2] = mfma_bf16(ft[2][X], rs.Y, u[2]);                                  \
+    u[3] = mfma_bf16(ft[3][X], rs.Y, u[3]);
+            TRI(2, h) TRI(1, m) TRI(0, l) TRI(1, h) TRI(0, m) TRI(0, h)
+            load_tri(rv);
+            if (!half) {
+                ux[w][0][lane] = u[0];
+                ux[w][1][lane] = u[1];
+            }
+            ux[w][2 + 2 * half][lane] = u[2];
+            ux[w][3 + 2 * half][lane] = u[3];
+            lds_barrier();
+            u[0] = ux[w][0][lane];
+            u[1] = ux[w][1][lane];
+            u[2] = ux[w][2][lane] + ux[w][4][lane];
+            u[3] = ux[w][3][lane] + ux[w][5][lane];
 #pragma unroll
             for (int i = 0; i < 4; i++) u[i] *= ew[i];
             const Split u0 = split8(u[0], u[1]), u1 = split8(u[2], u[3]);
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                s[d] *= ec;
-                s[d] = mfma_three(kt[2 * d], u0, s[d]);
-                s[d] = mfma_three(kt[2 * d + 1], u1, s[d]);
-            }
-            load_frags(kt, rk + 8 * KS * kFrag, lane);
-            load_vec(rv);
+            for (int d = 0; d < DH; d++) s[d] *= ec;
+#define COL(X, U)                                                            \
+    _Pragma("unroll") for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d][X], U, s[d]);
+            COL(0, u0.l) COL(0, u0.m) COL(0, u0.h) COL(1, u1.l) COL(1, u1.m) COL(1, u1.h)
+#undef COL
+            load_kt(rk);
+            load_vec();
 #pragma unroll
-            for (int d = 0; d < DT; d++) sx[w][d][lane] = s[d];
-            lds_barrier();
+            for (int d = 0; d < DH; d++) sx[w][half * DH + d][lane] = s[d];
         }
 #pragma unroll
-        for (int d = 0; d < DT; d++)
+        for (int d = 0; d < DH; d++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) st[(16 * d + 4 * g + r) * DV] = s[d][r];
-    } else {
-        v4u qa[4 * KS], pa[3 * kTri];
-        v4f eq[4];
-        auto load_vec = [&](const char* r) {
-            const float* vec = reinterpret_cast<const float*>(r + kVec);
-#pragma unroll
-            for (int i = 0; i < 4; i++) eq[i] = *reinterpret_cast<const v4f*>(vec + kC + 16 * i + 4 * g);
-        };
-        load_frags(qa, rk + 4 * KS * kFrag, lane);
-        load_frags(pa, rv + 3 * kTri * kFrag, lane);
-        load_vec(rv);
-        float* out = a.out + (int64_t)first * a.ldo + head * a.ho_s + c0;
+            for (int r = 0; r < 4; r++) st[(16 * (half * DH + d) + 4 * g + r) * DV] = s[d][r];
         lds_barrier();
+    } else {
+        v4f eq[4], o[4];
+        rk += 4 * KS * kFrag;
+        rv += 3 * kTri * kFrag;
+        vec += kC;
+        auto load_vec = [&] {
+#pragma unroll
+            for (int i = 0; i < 4; i++) eq[i] = *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
+        };
+        load_rows(rk);
+        load_tri(rv);
+        load_vec();
+        float* out = a.out + (int64_t)first * a.ldo + head * a.ho_s + c0;
+        v4f mine[2];
+        // the last chunk's sums of this half's tokens, joined and stored; `left` rows of it are there
+        auto finish = [&](int left) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const v4f x = mine[i] + ox[w][2 * half + i][lane];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int t = 32 * half + 16 * i + 4 * g + r;
+                    if (left >= kC || t < left) out[(int64_t)t * a.ldo] = x[r];
+                }
+            }
+            out += kC * a.ldo;
+        };
         for (int c = 0; c < nc; c++) {
             const bool more = c + 1 < nc;
             rk += more ? rks : 0;
             rv += more ? rvs : 0;
-            v4f o[4];
+            vec += more ? rvs / 4 : 0;
+            lds_barrier();
+            if (c) finish(kC);
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const Split sp = split8(sx[w][2 * k][lane], sx[w][2 * k + 1][lane]);
+            for (int k = 0; k < KH; k++) {
+                const Split sp = split8(sx[w][half * DH + 2 * k][lane], sx[w][half * DH + 2 * k + 1][lane]);
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = mfma_three(qa[i * KS + k], sp, o[i]);
+                for (int i = 0; i < 4; i++) o[i] = mfma_bf16(fk[i][k], sp.l, o[i]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = mfma_bf16(fk[i][k], sp.m, o[i]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] = mfma_bf16(fk[i][k], sp.h, o[i]);
             }
-            load_frags(qa, rk + 4 * KS * kFrag, lane);
+            load_rows(rk);
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] *= eq[i];
-            load_vec(rv);
+            load_vec();
             lds_barrier();
-            const Split u0 = split8(ux[w][0][lane], ux[w][1][lane]), u1 = split8(ux[w][2][lane], ux[w][3][lane]);
+            v4f x = ux[w][2 * half][lane], y = ux[w][2 * half + 1][lane];
+            if (half) {
+                x += ux[w][4][lane];
+                y += ux[w][5][lane];
+            }
+            const Split rs = split8(x, y);
+            v4f(&u)[4] = o;
+            TRI(2, h) TRI(1, m) TRI(0, l) TRI(1, h) TRI(0, m) TRI(0, h)
+#undef TRI
+            load_tri(rv);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int k = 0; k <= i / 2; k++)
-                    o[i] = mfma_six(pa[3 * tri(i, k)], pa[3 * tri(i, k) + 1], pa[3 * tri(i, k) + 2], k ? u1 : u0, o[i]);
-            load_frags(pa, rv + 3 * kTri * kFrag, lane);
-            const int left = count - c * kC;
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int t = 16 * i + 4 * g + r;
-                    if (t < left) out[(int64_t)t * a.ldo] = o[i][r];
-                }
-            out += kC * a.ldo;
-            lds_barrier();
+            for (int i = 0; i < 2; i++) {
+                ox[w][2 - 2 * half + i][lane] = half ? o[i] : o[2 + i];
+                mine[i] = half ? o[2 + i] : o[i];
+            }
         }
+        lds_barrier();
+        finish(count - (nc - 1) * kC);
     }
 }
 
@@ -626,10 +684,11 @@ static int launch_chunks(const DeltaArgs& a, char* ws, hipStream_t st) {
     const int64_t nc = chunks(a.rows, a.seqs), keys = (int64_t)a.seqs * a.HK;
     const int64_t wgs = (keys + 7) / 8 * 8 * (a.HV / a.HK) * (DV / 32);
     if (nc > INT32_MAX || a.HV > 65535 || wgs > INT32_MAX) return PRISM_ERR_SHAPE;
+    if (a.ldv > 1 << 24) return PRISM_ERR_SHAPE;              // a chunk's values within 32-bit offsets
     char* wv = ws + nc * a.HK * rec_k(DK);
     hipLaunchKernelGGL(delta_prep_kernel<DK>, dim3((unsigned)nc, (unsigned)a.HV), dim3(64), 0, st, a, ws, wv);
     PRISM_LAUNCH_CHECK();
-    hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)wgs), dim3(256), 0, st, a, ws, wv, (int)keys);
+    hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)wgs), dim3(512), 0, st, a, ws, wv, (int)keys);
     PRISM_LAUNCH_CHECK();
     return PRISM_OK;
 }
