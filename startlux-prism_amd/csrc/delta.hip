@@ -437,243 +437,259 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
 // of U's tokens, and the halves' sums (fp32, always the same two added) meet in LDS.  Two barriers per chunk:
 //   state waves   K S, halves out | halves in, R, X R out | U in, S <- ..., S out, next K S
 //   output waves  (rest of the last chunk's output) S in, Q S | U in, P U, halves out
-// Fragments come straight into registers, each group for the next chunk right after its last use, so that a load has
-// about a whole chunk's time.
+// Fragments come straight into registers, each group for the next chunk right after its last use and in the order of
+// their uses (loads complete in order: waiting for one waits for all before it), so that a load has a whole chunk's time.
+template <int DK>
+struct ScanShared {
+    v4f sx[2][DK / 16][64], kx[2][4][64], ux[2][6][64], ox[2][4][64];
+};
+
+// What a wave of delta_scan walks along: its fragments, factors and first token's row.
+struct ScanAt {
+    const char *rk, *rv;
+    const float* vec;
+    int64_t rks, rvs;                                         // bytes from a chunk's records to the next one's
+    int first, count, nc, head, c0, w;                        // c0: the lane's column; w: which 16 of the workgroup's 32
+};
+
+// K or Q: 4 token tiles, the half's k
+template <int DK, int HALF>
+__device__ __forceinline__ void load_rows(v4u (&f)[4][DK / 64], const char* r) {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int k = 0; k < DK / 64; k++)
+            f[i][k] = *reinterpret_cast<const v4u*>(r + (i * (DK / 32) + HALF * (DK / 64) + k) * kFrag);
+}
+// X diag(beta) or P: the columns of the half's tokens, token tiles from 2 HALF
+template <int HALF>
+__device__ __forceinline__ void load_tri(v4u (&f)[4][3], const char* r) {
+#pragma unroll
+    for (int i = 2 * HALF; i < 4; i++)
+#pragma unroll
+        for (int x = 0; x < 3; x++) f[i][x] = *reinterpret_cast<const v4u*>(r + (3 * tri(i, HALF) + x) * kFrag);
+}
+template <int HALF, int KH>
+__device__ __forceinline__ void mul_rows(v4f (&acc)[4], const v4u (&f)[4][KH], int k, const Split& s) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(f[i][k], s.l, acc[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(f[i][k], s.m, acc[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(f[i][k], s.h, acc[i]);
+}
+// acc += (three-part fragments)(three-part s), the small products first
+template <int HALF>
+__device__ __forceinline__ void mul_tri(v4f (&acc)[4], const v4u (&f)[4][3], const Split& s) {
+#pragma unroll
+    for (int p = 0; p < 6; p++) {
+        const int x = p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
+        const v4u& y = p == 2 ? s.l : p == 1 || p == 4 ? s.m : s.h;
+#pragma unroll
+        for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_bf16(f[i][x], y, acc[i]);
+    }
+}
+
+template <int DK, int DV, int HALF>
+__device__ __forceinline__ void scan_state(const DeltaArgs& a, ScanAt at, int slot, ScanShared<DK>& x) {
+    constexpr int KS = DK / 32, KH = KS / 2, DH = DK / 32;
+    const int lane = threadIdx.x & 63, g = lane >> 4, w = at.w;
+    float* st = a.state + slot * a.lds_ + (int64_t)at.head * DK * DV + at.c0;
+    v4u fk[4][KH], ft[4][3], kt[DH][2];
+    v4f s[DH], ek[2], ew[4];
+    uint32_t off[2][4];                                       // this half's tokens' values (bytes from the chunk's)
+    uint16_t v[2][4];
+    float ec;
+    const char* vp = reinterpret_cast<const char*>(a.v + (int64_t)at.first * a.ldv + at.head * a.hv_s + at.c0);
+    // rows past the chunk's end read its last row: their columns of X diag(beta) are zeros
+    auto offsets = [&](int left) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                off[i][r] = 2u * (uint32_t)a.ldv * (uint32_t)min(32 * HALF + 16 * i + 4 * g + r, left - 1);
+    };
+    auto load_v = [&] {                                       // with the factors of K S
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[i][r] = *reinterpret_cast<const uint16_t*>(vp + off[i][r]);
+#pragma unroll
+        for (int i = 0; i < 2; i++) ek[i] = *reinterpret_cast<const v4f*>(at.vec + 32 * HALF + 16 * i + 4 * g);
+    };
+    auto load_kt = [&] {                                      // with the factors of U and S
+#pragma unroll
+        for (int i = 0; i < 4; i++) ew[i] = *reinterpret_cast<const v4f*>(at.vec + 2 * kC + 16 * i + 4 * g);
+        ec = at.vec[3 * kC + lane];                           // (a copy per lane)
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int d = 0; d < DH; d++)
+                kt[d][e] = *reinterpret_cast<const v4u*>(at.rk + (8 * KS + 2 * (HALF * DH + d) + e) * kFrag);
+    };
+    offsets(at.count);
+    load_rows<DK, HALF>(fk, at.rk);
+    load_v();
+    load_tri<HALF>(ft, at.rv);
+    load_kt();
+#pragma unroll
+    for (int d = 0; d < DH; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[d][r] = st[(16 * (HALF * DH + d) + 4 * g + r) * DV];
+#pragma unroll
+    for (int d = 0; d < DH; d++) x.sx[w][HALF * DH + d][lane] = s[d];
+    for (int c = 0; c < at.nc; c++) {
+        const int left = at.count - (c + 1) * kC;             // rows after this chunk
+        if (left > 0) {                                       // (past the last chunk it is read again)
+            at.rk += at.rks, at.rv += at.rvs, at.vec += at.rvs / 4;
+            vp += 2 * kC * a.ldv;
+            if (left < kC) offsets(left);
+        }
+        v4f ks[4], u[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) ks[i] = u[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KH; k++) mul_rows<HALF, KH>(ks, fk, k, split8(s[2 * k], s[2 * k + 1]));
+        load_rows<DK, HALF>(fk, at.rk);
+        // the other half's tokens' sums out, this half's in
+        x.kx[w][2 - 2 * HALF][lane] = ks[2 - 2 * HALF];
+        x.kx[w][3 - 2 * HALF][lane] = ks[3 - 2 * HALF];
+        lds_barrier();
+        v4f rr[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            rr[i] = ks[2 * HALF + i] + x.kx[w][2 * HALF + i][lane];
+#pragma unroll
+            for (int r = 0; r < 4; r++) rr[i][r] = fmaf(-ek[i][r], rr[i][r], bf16_to_f32(v[i][r]));
+        }
+        load_v();
+        mul_tri<HALF>(u, ft, split8(rr[0], rr[1]));
+        load_tri<HALF>(ft, at.rv);
+#pragma unroll
+        for (int i = 2 * HALF; i < 4; i++) x.ux[w][i + 2 * HALF][lane] = u[i];
+        lds_barrier();
+        if (HALF == 0) {
+            u[2] += x.ux[w][4][lane];
+            u[3] += x.ux[w][5][lane];
+        } else {
+            u[0] = x.ux[w][0][lane];
+            u[1] = x.ux[w][1][lane];
+            u[2] += x.ux[w][2][lane];
+            u[3] += x.ux[w][3][lane];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) u[i] *= ew[i];
+#pragma unroll
+        for (int d = 0; d < DH; d++) s[d] *= ec;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const Split us = split8(u[2 * e], u[2 * e + 1]);
+#pragma unroll
+            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d][e], us.l, s[d]);
+#pragma unroll
+            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d][e], us.m, s[d]);
+#pragma unroll
+            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d][e], us.h, s[d]);
+        }
+        load_kt();
+#pragma unroll
+        for (int d = 0; d < DH; d++) x.sx[w][HALF * DH + d][lane] = s[d];
+    }
+#pragma unroll
+    for (int d = 0; d < DH; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) st[(16 * (HALF * DH + d) + 4 * g + r) * DV] = s[d][r];
+    lds_barrier();
+}
+
+template <int DK, int HALF>
+__device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShared<DK>& x) {
+    constexpr int KS = DK / 32, KH = KS / 2, DH = DK / 32;
+    const int lane = threadIdx.x & 63, g = lane >> 4, w = at.w;
+    v4u fk[4][KH], ft[4][3];
+    v4f eq[4], mine[2];
+    at.rk += 4 * KS * kFrag;
+    at.rv += 3 * kTri * kFrag;
+    at.vec += kC;
+    auto load_q = [&] {
+        load_rows<DK, HALF>(fk, at.rk);
+#pragma unroll
+        for (int i = 0; i < 4; i++) eq[i] = *reinterpret_cast<const v4f*>(at.vec + 16 * i + 4 * g);
+    };
+    load_q();
+    load_tri<HALF>(ft, at.rv);
+    float* out = a.out + (int64_t)at.first * a.ldo + at.head * a.ho_s + at.c0;
+    // the last chunk's sums of this half's tokens, joined and stored; `left` rows of it are there
+    auto finish = [&](int left) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const v4f y = mine[i] + x.ox[w][2 * HALF + i][lane];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int t = 32 * HALF + 16 * i + 4 * g + r;
+                if (left >= kC || t < left) out[(int64_t)t * a.ldo] = y[r];
+            }
+        }
+        out += kC * a.ldo;
+    };
+    for (int c = 0; c < at.nc; c++) {
+        if (at.count - (c + 1) * kC > 0) at.rk += at.rks, at.rv += at.rvs, at.vec += at.rvs / 4;
+        lds_barrier();
+        if (c) finish(kC);
+        v4f o[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KH; k++)
+            mul_rows<HALF, KH>(o, fk, k, split8(x.sx[w][HALF * DH + 2 * k][lane], x.sx[w][HALF * DH + 2 * k + 1][lane]));
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] *= eq[i];
+        load_q();
+        lds_barrier();
+        v4f u0 = x.ux[w][2 * HALF][lane], u1 = x.ux[w][2 * HALF + 1][lane];
+        if (HALF) {
+            u0 += x.ux[w][4][lane];
+            u1 += x.ux[w][5][lane];
+        }
+        mul_tri<HALF>(o, ft, split8(u0, u1));
+        load_tri<HALF>(ft, at.rv);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            x.ox[w][2 - 2 * HALF + i][lane] = o[2 - 2 * HALF + i];
+            mine[i] = o[2 * HALF + i];
+        }
+    }
+    lds_barrier();
+    finish(at.count - (at.nc - 1) * kC);
+}
+
 template <int DK, int DV>
 __global__ __launch_bounds__(512, 1) void delta_scan_kernel(DeltaArgs a, const char* wk, const char* wv, int keys) {
-    constexpr int KS = DK / 32, DT = DK / 16, CT = DV / 32, KH = KS / 2, DH = DT / 2;
-    __shared__ v4f sx[2][DT][64], kx[2][4][64], ux[2][6][64], ox[2][4][64];
+    constexpr int CT = DV / 32;
+    __shared__ ScanShared<DK> x;
     // the workgroups of one key head, which read the same K and Q, on one XCD (workgroup i runs on XCD i % 8)
     const int share = a.HV / a.HK, per = share * CT;
     const int grp = blockIdx.x / (8 * per), key = 8 * grp + blockIdx.x % 8, m = blockIdx.x / 8 % per;
     if (key >= keys) return;
-    const int b = key / a.HK, hk = key % a.HK, head = hk * share + m / CT;
-    int first, count, slot;
-    if (!delta_seq(a, b, first, count, slot)) return;
+    const int b = key / a.HK, hk = key % a.HK;
+    ScanAt at;
+    int slot;
+    if (!delta_seq(a, b, at.first, at.count, slot)) return;
+    at.head = hk * share + m / CT;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4, w = wave & 1, half = wave >> 1 & 1;
-    const int c0 = 32 * (m % CT) + 16 * w + col;              // this lane's column
-    const int nc = (count + kC - 1) / kC, base = first / kC + b;
-    const char* rk = wk + ((int64_t)base * a.HK + hk) * rec_k(DK) + lane * 16;
-    const char* rv = wv + ((int64_t)base * a.HV + head) * kRecV + lane * 16;
-    const float* vec = reinterpret_cast<const float*>(wv + ((int64_t)base * a.HV + head) * kRecV + 6 * kTri * kFrag);
-    const int64_t rks = (int64_t)a.HK * rec_k(DK), rvs = (int64_t)a.HV * kRecV;
-    // K or Q (4 token tiles, this half's k), X diag(beta) or P (token tiles from 2 half, columns half)
-    v4u fk[4][KH], ft[4][3];
-    auto load_rows = [&](const char* r) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int k = 0; k < KH; k++)
-                fk[i][k] = *reinterpret_cast<const v4u*>(r + (i * KS + half * KH + k) * kFrag);
-    };
-    auto load_tri = [&](const char* r) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (half && i < 2) continue;                      // (wave-uniform)
-#pragma unroll
-            for (int x = 0; x < 3; x++)
-                ft[i][x] = *reinterpret_cast<const v4u*>(r + (3 * (i < 2 ? i : 2 * i - 2 + half) + x) * kFrag);
-        }
-    };
-    if (wave < 4) {
-        float* st = a.state + slot * a.lds_ + (int64_t)head * DK * DV + c0;
-        v4f s[DH];
-#pragma unroll
-        for (int d = 0; d < DH; d++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) s[d][r] = st[(16 * (half * DH + d) + 4 * g + r) * DV];
-        v4u kt[DH][2];
-        v4f ek[2], ew[4];
-        uint32_t off[2][4];                                   // this half's tokens' values (bytes from the chunk's)
-        uint16_t v[2][4];
-        float ec;
-        const char* vp = reinterpret_cast<const char*>(a.v + (int64_t)first * a.ldv + head * a.hv_s + c0);
-        auto load_kt = [&](const char* r) {
-#pragma unroll
-            for (int d = 0; d < DH; d++)
-#pragma unroll
-                for (int x = 0; x < 2; x++)
-                    kt[d][x] = *reinterpret_cast<const v4u*>(r + (8 * KS + 2 * (half * DH + d) + x) * kFrag);
-        };
-        // rows past the chunk's end read its last row: their columns of X diag(beta) are zeros
-        auto offsets = [&](int left) {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    off[i][r] = 2u * (uint32_t)a.ldv * (uint32_t)min(32 * half + 16 * i + 4 * g + r, left - 1);
-        };
-        auto load_v = [&] {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) v[i][r] = *reinterpret_cast<const uint16_t*>(vp + off[i][r]);
-        };
-        auto load_vec = [&] {
-#pragma unroll
-            for (int i = 0; i < 2; i++) ek[i] = *reinterpret_cast<const v4f*>(vec + 32 * half + 16 * i + 4 * g);
-#pragma unroll
-            for (int i = 0; i < 4; i++) ew[i] = *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
-            ec = vec[3 * kC];
-        };
-        load_rows(rk);
-        load_tri(rv);
-        load_kt(rk);
-        offsets(count);
-        load_v();
-        load_vec();
-#pragma unroll
-        for (int d = 0; d < DH; d++) sx[w][half * DH + d][lane] = s[d];
-        for (int c = 0; c < nc; c++) {
-            const bool more = c + 1 < nc;                     // (past the last chunk it is read again)
-            rk += more ? rks : 0;
-            rv += more ? rvs : 0;
-            vec += more ? rvs / 4 : 0;
-            v4f ks[4], u[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) ks[i] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < KH; k++) {
-                const Split sp = split8(s[2 * k], s[2 * k + 1]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) ks[i] = mfma_bf16(fk[i][k], sp.l, ks[i]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) ks[i] = mfma_bf16(fk[i][k], sp.m, ks[i]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) ks[i] = mfma_bf16(fk[i][k], sp.h, ks[i]);
-            }
-            load_rows(rk);
-            // the other half's tokens' sums out, this half's in
-            v4f mine[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                kx[w][2 - 2 * half + i][lane] = half ? ks[i] : ks[2 + i];
-                mine[i] = half ? ks[2 + i] : ks[i];
-            }
-            lds_barrier();
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                mine[i] += kx[w][2 * half + i][lane];
-#pragma unroll
-                for (int r = 0; r < 4; r++) mine[i][r] = fmaf(-ek[i][r], mine[i][r], bf16_to_f32(v[i][r]));
-            }
-            if (more) {
-                vp += 2 * kC * a.ldv;
-                if (count - (c + 1) * kC < kC) offsets(count - (c + 1) * kC);
-            }
-            load_v();
-            const Split rs = split8(mine[0], mine[1]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) u[i] = v4f{0.f, 0.f, 0.f, 0.f};
-#define TRI(X, Y)                                                            \
-    if (!half) {                                                             \
-        u[0] = mfma_bf16(ft[0][X], rs.Y, u[0]);                              \
-        u[1] = mfma_bf16(ft[1][X], rs.Y, u[1]);                              \
-    }                                                                        \
-    u[2] = mfma_bf16(ft[2][X], rs.Y, u[2]);                                  \
-    u[3] = mfma_bf16(ft[3][X], rs.Y, u[3]);
-            TRI(2, h) TRI(1, m) TRI(0, l) TRI(1, h) TRI(0, m) TRI(0, h)
-            load_tri(rv);
-            if (!half) {
-                ux[w][0][lane] = u[0];
-                ux[w][1][lane] = u[1];
-            }
-            ux[w][2 + 2 * half][lane] = u[2];
-            ux[w][3 + 2 * half][lane] = u[3];
-            lds_barrier();
-            u[0] = ux[w][0][lane];
-            u[1] = ux[w][1][lane];
-            u[2] = ux[w][2][lane] + ux[w][4][lane];
-            u[3] = ux[w][3][lane] + ux[w][5][lane];
-#pragma unroll
-            for (int i = 0; i < 4; i++) u[i] *= ew[i];
-            const Split u0 = split8(u[0], u[1]), u1 = split8(u[2], u[3]);
-#pragma unroll
-            for (int d = 0; d < DH; d++) s[d] *= ec;
-#define COL(X, U)                                                            \
-    _Pragma("unroll") for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d][X], U, s[d]);
-            COL(0, u0.l) COL(0, u0.m) COL(0, u0.h) COL(1, u1.l) COL(1, u1.m) COL(1, u1.h)
-#undef COL
-            load_kt(rk);
-            load_vec();
-#pragma unroll
-            for (int d = 0; d < DH; d++) sx[w][half * DH + d][lane] = s[d];
-        }
-#pragma unroll
-        for (int d = 0; d < DH; d++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) st[(16 * (half * DH + d) + 4 * g + r) * DV] = s[d][r];
-        lds_barrier();
-    } else {
-        v4f eq[4], o[4];
-        rk += 4 * KS * kFrag;
-        rv += 3 * kTri * kFrag;
-        vec += kC;
-        auto load_vec = [&] {
-#pragma unroll
-            for (int i = 0; i < 4; i++) eq[i] = *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
-        };
-        load_rows(rk);
-        load_tri(rv);
-        load_vec();
-        float* out = a.out + (int64_t)first * a.ldo + head * a.ho_s + c0;
-        v4f mine[2];
-        // the last chunk's sums of this half's tokens, joined and stored; `left` rows of it are there
-        auto finish = [&](int left) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const v4f x = mine[i] + ox[w][2 * half + i][lane];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int t = 32 * half + 16 * i + 4 * g + r;
-                    if (left >= kC || t < left) out[(int64_t)t * a.ldo] = x[r];
-                }
-            }
-            out += kC * a.ldo;
-        };
-        for (int c = 0; c < nc; c++) {
-            const bool more = c + 1 < nc;
-            rk += more ? rks : 0;
-            rv += more ? rvs : 0;
-            vec += more ? rvs / 4 : 0;
-            lds_barrier();
-            if (c) finish(kC);
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < KH; k++) {
-                const Split sp = split8(sx[w][half * DH + 2 * k][lane], sx[w][half * DH + 2 * k + 1][lane]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = mfma_bf16(fk[i][k], sp.l, o[i]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = mfma_bf16(fk[i][k], sp.m, o[i]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[i] = mfma_bf16(fk[i][k], sp.h, o[i]);
-            }
-            load_rows(rk);
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[i] *= eq[i];
-            load_vec();
-            lds_barrier();
-            v4f x = ux[w][2 * half][lane], y = ux[w][2 * half + 1][lane];
-            if (half) {
-                x += ux[w][4][lane];
-                y += ux[w][5][lane];
-            }
-            const Split rs = split8(x, y);
-            v4f(&u)[4] = o;
-            TRI(2, h) TRI(1, m) TRI(0, l) TRI(1, h) TRI(0, m) TRI(0, h)
-#undef TRI
-            load_tri(rv);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                ox[w][2 - 2 * half + i][lane] = half ? o[i] : o[2 + i];
-                mine[i] = half ? o[2 + i] : o[i];
-            }
-        }
-        lds_barrier();
-        finish(count - (nc - 1) * kC);
+    at.w = wave & 1;
+    at.c0 = 32 * (m % CT) + 16 * at.w + (lane & 15);
+    at.nc = (at.count + kC - 1) / kC;
+    const int64_t id = at.first / kC + b;
+    at.rk = wk + (id * a.HK + hk) * rec_k(DK) + lane * 16;
+    at.rv = wv + (id * a.HV + at.head) * kRecV + lane * 16;
+    at.vec = reinterpret_cast<const float*>(wv + (id * a.HV + at.head) * kRecV + 6 * kTri * kFrag);
+    at.rks = (int64_t)a.HK * rec_k(DK), at.rvs = (int64_t)a.HV * kRecV;
+    switch (wave >> 1) {
+        case 0: return scan_state<DK, DV, 0>(a, at, slot, x);
+        case 1: return scan_state<DK, DV, 1>(a, at, slot, x);
+        case 2: return scan_out<DK, 0>(a, at, x);
+        default: return scan_out<DK, 1>(a, at, x);
     }
 }
 
