@@ -619,23 +619,25 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShar
     load_q();
     load_tri<HALF>(ft, at.rv);
     float* out = a.out + (int64_t)at.first * a.ldo + at.head * a.ho_s + at.c0;
-    // the last chunk's sums of this half's tokens, joined and stored; `left` rows of it are there
-    auto finish = [&](int left) {
+    // the last chunk's sums of this half's tokens, joined, then stored (`left` rows of it are there)
+    auto join = [&] {
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const v4f y = mine[i] + x.ox[w][2 * HALF + i][lane];
+        for (int i = 0; i < 2; i++) mine[i] += x.ox[w][2 * HALF + i][lane];
+    };
+    auto store = [&](int left) {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int t = 32 * HALF + 16 * i + 4 * g + r;
-                if (left >= kC || t < left) out[(int64_t)t * a.ldo] = y[r];
+                if (left >= kC || t < left) out[(int64_t)t * a.ldo] = mine[i][r];
             }
-        }
         out += kC * a.ldo;
     };
     for (int c = 0; c < at.nc; c++) {
         if (at.count - (c + 1) * kC > 0) at.rk += at.rks, at.rv += at.rvs, at.vec += at.rvs / 4;
         lds_barrier();
-        if (c) finish(kC);
+        if (c) join();
         v4f o[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
@@ -646,6 +648,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShar
         for (int i = 0; i < 4; i++) o[i] *= eq[i];
         load_q();
         lds_barrier();
+        if (c) store(kC);                                     // (here the state waves have more to do than these)
         v4f u0 = x.ux[w][2 * HALF][lane], u1 = x.ux[w][2 * HALF + 1][lane];
         if (HALF) {
             u0 += x.ux[w][4][lane];
@@ -660,7 +663,8 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShar
         }
     }
     lds_barrier();
-    finish(at.count - (at.nc - 1) * kC);
+    join();
+    store(at.count - (at.nc - 1) * kC);
 }
 
 template <int DK, int DV>
