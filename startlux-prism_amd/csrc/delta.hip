@@ -431,75 +431,67 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
         }
 }
 
-// A workgroup walks the chunks of one sequence and value head for 32 columns of the state: four waves to 16 columns, on
-// a SIMD each, two holding the halves of S's rows and taking what the next chunk waits for (K S, U, K^T U), two the
-// chunk's output (Q S, P U).  Products split over the summed index: a wave multiplies its half of S's rows, or its half
-// of U's tokens, and the halves' sums (fp32, always the same two added) meet in LDS.  Two barriers per chunk:
-//   state waves   K S, halves out | halves in, R, X R out | U in, S <- ..., S out, next K S
-//   output waves  (rest of the last chunk's output) S in, Q S | U in, P U, halves out
-// Fragments come straight into registers, each group for the next chunk right after its last use and in the order of
-// their uses (loads complete in order: waiting for one waits for all before it), so that a load has a whole chunk's time.
+// A workgroup walks the chunks of one sequence and value head for 32 columns of the state, twelve waves, three to a SIMD.
+// Four waves to 16 columns: two hold the halves of S's rows and take what the next chunk waits for (K S, U, K^T U), two
+// the chunk's output (Q S, P U); products split over the summed index: a wave multiplies its half of S's rows, or its half
+// of U's tokens, and the halves' sums (fp32, always the same two added) meet in LDS.  The other four waves bring the
+// fragments into LDS, each group while nobody reads it, and touch the lines of the chunk after the next, so that those
+// come from L2.  Two barriers per chunk:
+//   state waves   K S, halves out        | halves in, R, X R out  | U in, S <- ..., S out
+//   output waves  (P U of the last one)  | S in, Q S              | P U, halves out
+//   loading waves (Q, X, factors in)     | next K, P, K^T in      | next Q, X, factors in
 template <int DK>
 struct ScanShared {
+    v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], kt[DK / 16 * 2][64], x[3 * kTri][64], p[3 * kTri][64];
+    float vec[2][4 * kC];                                     // a chunk's factors, the next one's beside them
     v4f sx[2][DK / 16][64], kx[2][4][64], ux[2][6][64], ox[2][4][64];
+    uint32_t touched[64];
 };
 
-// What a wave of delta_scan walks along: its fragments, factors and first token's row.
+// What a wave of delta_scan walks along.
 struct ScanAt {
-    const char *rk, *rv;
-    const float* vec;
-    int64_t rks, rvs;                                         // bytes from a chunk's records to the next one's
     int first, count, nc, head, c0, w;                        // c0: the lane's column; w: which 16 of the workgroup's 32
 };
 
-// K or Q: 4 token tiles, the half's k
+// acc += (rows of K or Q, the half's k)(the half's rows of S)
 template <int DK, int HALF>
-__device__ __forceinline__ void load_rows(v4u (&f)[4][DK / 64], const char* r) {
+__device__ __forceinline__ void mul_rows(v4f (&acc)[4], const v4u (*f)[64], int k, const Split& s) {
+    const int lane = threadIdx.x & 63;
+    v4u r[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+    for (int i = 0; i < 4; i++) r[i] = f[i * (DK / 32) + HALF * (DK / 64) + k][lane];
 #pragma unroll
-        for (int k = 0; k < DK / 64; k++)
-            f[i][k] = *reinterpret_cast<const v4u*>(r + (i * (DK / 32) + HALF * (DK / 64) + k) * kFrag);
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.l, acc[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.m, acc[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.h, acc[i]);
 }
-// X diag(beta) or P: the columns of the half's tokens, token tiles from 2 HALF
+// acc += (X diag(beta) or P, the columns of the half's tokens)(three-part s), the small products first
 template <int HALF>
-__device__ __forceinline__ void load_tri(v4u (&f)[4][3], const char* r) {
-#pragma unroll
-    for (int i = 2 * HALF; i < 4; i++)
-#pragma unroll
-        for (int x = 0; x < 3; x++) f[i][x] = *reinterpret_cast<const v4u*>(r + (3 * tri(i, HALF) + x) * kFrag);
-}
-template <int HALF, int KH>
-__device__ __forceinline__ void mul_rows(v4f (&acc)[4], const v4u (&f)[4][KH], int k, const Split& s) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(f[i][k], s.l, acc[i]);
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(f[i][k], s.m, acc[i]);
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(f[i][k], s.h, acc[i]);
-}
-// acc += (three-part fragments)(three-part s), the small products first
-template <int HALF>
-__device__ __forceinline__ void mul_tri(v4f (&acc)[4], const v4u (&f)[4][3], const Split& s) {
+__device__ __forceinline__ void mul_tri(v4f (&acc)[4], const v4u (*f)[64], const Split& s) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int p = 0; p < 6; p++) {
         const int x = p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
         const v4u& y = p == 2 ? s.l : p == 1 || p == 4 ? s.m : s.h;
 #pragma unroll
-        for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_bf16(f[i][x], y, acc[i]);
+        for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_bf16(f[3 * tri(i, HALF) + x][lane], y, acc[i]);
     }
 }
 
 template <int DK, int DV, int HALF>
-__device__ __forceinline__ void scan_state(const DeltaArgs& a, ScanAt at, int slot, ScanShared<DK>& x) {
-    constexpr int KS = DK / 32, KH = KS / 2, DH = DK / 32;
+__device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at, int slot, ScanShared<DK>& x) {
+    constexpr int KH = DK / 64, DH = DK / 32;
     const int lane = threadIdx.x & 63, g = lane >> 4, w = at.w;
     float* st = a.state + slot * a.lds_ + (int64_t)at.head * DK * DV + at.c0;
-    v4u fk[4][KH], ft[4][3], kt[DH][2];
-    v4f s[DH], ek[2], ew[4];
+    v4f s[DH];
+#pragma unroll
+    for (int d = 0; d < DH; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) s[d][r] = st[(16 * (HALF * DH + d) + 4 * g + r) * DV];
     uint32_t off[2][4];                                       // this half's tokens' values (bytes from the chunk's)
     uint16_t v[2][4];
-    float ec;
     const char* vp = reinterpret_cast<const char*>(a.v + (int64_t)at.first * a.ldv + at.head * a.hv_s + at.c0);
     // rows past the chunk's end read its last row: their columns of X diag(beta) are zeros
     auto offsets = [&](int left) {
@@ -509,48 +501,25 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, ScanAt at, int sl
             for (int r = 0; r < 4; r++)
                 off[i][r] = 2u * (uint32_t)a.ldv * (uint32_t)min(32 * HALF + 16 * i + 4 * g + r, left - 1);
     };
-    auto load_v = [&] {                                       // with the factors of K S
+    auto load_v = [&] {
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
             for (int r = 0; r < 4; r++) v[i][r] = *reinterpret_cast<const uint16_t*>(vp + off[i][r]);
-#pragma unroll
-        for (int i = 0; i < 2; i++) ek[i] = *reinterpret_cast<const v4f*>(at.vec + 32 * HALF + 16 * i + 4 * g);
-    };
-    auto load_kt = [&] {                                      // with the factors of U and S
-#pragma unroll
-        for (int i = 0; i < 4; i++) ew[i] = *reinterpret_cast<const v4f*>(at.vec + 2 * kC + 16 * i + 4 * g);
-        ec = at.vec[3 * kC + lane];                           // (a copy per lane)
-#pragma unroll
-        for (int e = 0; e < 2; e++)
-#pragma unroll
-            for (int d = 0; d < DH; d++)
-                kt[d][e] = *reinterpret_cast<const v4u*>(at.rk + (8 * KS + 2 * (HALF * DH + d) + e) * kFrag);
     };
     offsets(at.count);
-    load_rows<DK, HALF>(fk, at.rk);
     load_v();
-    load_tri<HALF>(ft, at.rv);
-    load_kt();
-#pragma unroll
-    for (int d = 0; d < DH; d++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) s[d][r] = st[(16 * (HALF * DH + d) + 4 * g + r) * DV];
 #pragma unroll
     for (int d = 0; d < DH; d++) x.sx[w][HALF * DH + d][lane] = s[d];
+    lds_barrier();
     for (int c = 0; c < at.nc; c++) {
+        const float* vec = x.vec[c & 1];
         const int left = at.count - (c + 1) * kC;             // rows after this chunk
-        if (left > 0) {                                       // (past the last chunk it is read again)
-            at.rk += at.rks, at.rv += at.rvs, at.vec += at.rvs / 4;
-            vp += 2 * kC * a.ldv;
-            if (left < kC) offsets(left);
-        }
         v4f ks[4], u[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) ks[i] = u[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < KH; k++) mul_rows<HALF, KH>(ks, fk, k, split8(s[2 * k], s[2 * k + 1]));
-        load_rows<DK, HALF>(fk, at.rk);
+        for (int k = 0; k < KH; k++) mul_rows<DK, HALF>(ks, x.k, k, split8(s[2 * k], s[2 * k + 1]));
         // the other half's tokens' sums out, this half's in
         x.kx[w][2 - 2 * HALF][lane] = ks[2 - 2 * HALF];
         x.kx[w][3 - 2 * HALF][lane] = ks[3 - 2 * HALF];
@@ -558,13 +527,17 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, ScanAt at, int sl
         v4f rr[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
+            const v4f ek = *reinterpret_cast<const v4f*>(vec + 32 * HALF + 16 * i + 4 * g);
             rr[i] = ks[2 * HALF + i] + x.kx[w][2 * HALF + i][lane];
 #pragma unroll
-            for (int r = 0; r < 4; r++) rr[i][r] = fmaf(-ek[i][r], rr[i][r], bf16_to_f32(v[i][r]));
+            for (int r = 0; r < 4; r++) rr[i][r] = fmaf(-ek[r], rr[i][r], bf16_to_f32(v[i][r]));
         }
-        load_v();
-        mul_tri<HALF>(u, ft, split8(rr[0], rr[1]));
-        load_tri<HALF>(ft, at.rv);
+        if (left > 0) {
+            vp += 2 * kC * a.ldv;
+            if (left < kC) offsets(left);
+            load_v();
+        }
+        mul_tri<HALF>(u, x.x, split8(rr[0], rr[1]));
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++) x.ux[w][i + 2 * HALF][lane] = u[i];
         lds_barrier();
@@ -578,20 +551,23 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, ScanAt at, int sl
             u[3] += x.ux[w][3][lane];
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] *= ew[i];
+        for (int i = 0; i < 4; i++) u[i] *= *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
+        const float ec = vec[3 * kC];
 #pragma unroll
         for (int d = 0; d < DH; d++) s[d] *= ec;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const Split us = split8(u[2 * e], u[2 * e + 1]);
+            v4u kt[DH];
 #pragma unroll
-            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d][e], us.l, s[d]);
+            for (int d = 0; d < DH; d++) kt[d] = x.kt[2 * (HALF * DH + d) + e][lane];
 #pragma unroll
-            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d][e], us.m, s[d]);
+            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d], us.l, s[d]);
 #pragma unroll
-            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d][e], us.h, s[d]);
+            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d], us.m, s[d]);
+#pragma unroll
+            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d], us.h, s[d]);
         }
-        load_kt();
 #pragma unroll
         for (int d = 0; d < DH; d++) x.sx[w][HALF * DH + d][lane] = s[d];
     }
@@ -603,21 +579,10 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, ScanAt at, int sl
 }
 
 template <int DK, int HALF>
-__device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShared<DK>& x) {
-    constexpr int KS = DK / 32, KH = KS / 2, DH = DK / 32;
+__device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, ScanShared<DK>& x) {
+    constexpr int KH = DK / 64, DH = DK / 32;
     const int lane = threadIdx.x & 63, g = lane >> 4, w = at.w;
-    v4u fk[4][KH], ft[4][3];
-    v4f eq[4], mine[2];
-    at.rk += 4 * KS * kFrag;
-    at.rv += 3 * kTri * kFrag;
-    at.vec += kC;
-    auto load_q = [&] {
-        load_rows<DK, HALF>(fk, at.rk);
-#pragma unroll
-        for (int i = 0; i < 4; i++) eq[i] = *reinterpret_cast<const v4f*>(at.vec + 16 * i + 4 * g);
-    };
-    load_q();
-    load_tri<HALF>(ft, at.rv);
+    v4f mine[2];
     float* out = a.out + (int64_t)at.first * a.ldo + at.head * a.ho_s + at.c0;
     // the last chunk's sums of this half's tokens, joined, then stored (`left` rows of it are there)
     auto join = [&] {
@@ -634,8 +599,9 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShar
             }
         out += kC * a.ldo;
     };
+    lds_barrier();
     for (int c = 0; c < at.nc; c++) {
-        if (at.count - (c + 1) * kC > 0) at.rk += at.rks, at.rv += at.rvs, at.vec += at.rvs / 4;
+        const float* vec = x.vec[c & 1] + kC;
         lds_barrier();
         if (c) join();
         v4f o[4];
@@ -643,10 +609,9 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShar
         for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KH; k++)
-            mul_rows<HALF, KH>(o, fk, k, split8(x.sx[w][HALF * DH + 2 * k][lane], x.sx[w][HALF * DH + 2 * k + 1][lane]));
+            mul_rows<DK, HALF>(o, x.q, k, split8(x.sx[w][HALF * DH + 2 * k][lane], x.sx[w][HALF * DH + 2 * k + 1][lane]));
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] *= eq[i];
-        load_q();
+        for (int i = 0; i < 4; i++) o[i] *= *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
         lds_barrier();
         if (c) store(kC);                                     // (here the state waves have more to do than these)
         v4f u0 = x.ux[w][2 * HALF][lane], u1 = x.ux[w][2 * HALF + 1][lane];
@@ -654,8 +619,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShar
             u0 += x.ux[w][4][lane];
             u1 += x.ux[w][5][lane];
         }
-        mul_tri<HALF>(o, ft, split8(u0, u1));
-        load_tri<HALF>(ft, at.rv);
+        mul_tri<HALF>(o, x.p, split8(u0, u1));
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             x.ox[w][2 - 2 * HALF + i][lane] = o[2 - 2 * HALF + i];
@@ -667,10 +631,58 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, ScanAt at, ScanShar
     store(at.count - (at.nc - 1) * kC);
 }
 
+// Wave `q` of the four: every fourth fragment.  m of `per`, n of `heads`: this workgroup among those that read the same K
+// and Q, the same X and P; each touches its share of the lines two chunks on.
+template <int DK>
+__device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, const char* rv, int64_t rks, int64_t rvs, int q,
+                                          int m, int per, int n, int heads, ScanShared<DK>& x) {
+    constexpr int NK = 4 * (DK / 32), NT = DK / 16 * 2, NX = 3 * kTri;
+    const int lane = threadIdx.x & 63;
+    auto bring = [&](v4u (*to)[64], const char* from, int count) {
+        for (int i = q; i < count; i += 4) dma16(from + i * kFrag + lane * 16, to[i]);
+    };
+    auto factors = [&](int c, const char* r) {
+        if (q == 0) dma16(r + 2 * NX * kFrag + lane * 16, x.vec[c & 1]);
+    };
+    auto touch = [&](const char* k, const char* v) {
+        if (q == 1)
+            for (int i = m * 64 + lane; i < (int)(rec_k(DK) / 128); i += per * 64)
+                __builtin_amdgcn_global_load_lds(k + i * 128, (__attribute__((address_space(3))) void*)x.touched, 4, 0, 0);
+        if (q == 2)
+            for (int i = n * 64 + lane; i < (int)(kRecV / 128); i += heads * 64)
+                __builtin_amdgcn_global_load_lds(v + i * 128, (__attribute__((address_space(3))) void*)x.touched, 4, 0, 0);
+    };
+    bring(x.k, rk, NK);
+    bring(x.q, rk + NK * kFrag, NK);
+    bring(x.x, rv, NX);
+    factors(0, rv);
+    vm_wait<0>();
+    lds_barrier();
+    for (int c = 0; c < at.nc; c++) {
+        const bool more = c + 1 < at.nc;
+        lds_barrier();
+        if (more) bring(x.k, rk + rks, NK);
+        bring(x.p, rv + NX * kFrag, NX);
+        bring(x.kt, rk + 2 * NK * kFrag, NT);
+        vm_wait<0>();
+        lds_barrier();
+        if (more) {
+            bring(x.q, rk + rks + NK * kFrag, NK);
+            bring(x.x, rv + rvs, NX);
+            factors(c + 1, rv + rvs);
+            if (c + 2 < at.nc) touch(rk + 2 * rks, rv + 2 * rvs);
+        }
+        vm_wait<0>();
+        rk += rks, rv += rvs;
+    }
+    lds_barrier();
+}
+
 template <int DK, int DV>
-__global__ __launch_bounds__(512, 1) void delta_scan_kernel(DeltaArgs a, const char* wk, const char* wv, int keys) {
+__global__ __launch_bounds__(768, 3) void delta_scan_kernel(DeltaArgs a, const char* wk, const char* wv, int keys) {
     constexpr int CT = DV / 32;
-    __shared__ ScanShared<DK> x;
+    extern __shared__ __align__(16) char shared[];
+    ScanShared<DK>& x = *reinterpret_cast<ScanShared<DK>*>(shared);
     // the workgroups of one key head, which read the same K and Q, on one XCD (workgroup i runs on XCD i % 8)
     const int share = a.HV / a.HK, per = share * CT;
     const int grp = blockIdx.x / (8 * per), key = 8 * grp + blockIdx.x % 8, m = blockIdx.x / 8 % per;
@@ -684,17 +696,16 @@ __global__ __launch_bounds__(512, 1) void delta_scan_kernel(DeltaArgs a, const c
     at.w = wave & 1;
     at.c0 = 32 * (m % CT) + 16 * at.w + (lane & 15);
     at.nc = (at.count + kC - 1) / kC;
-    const int64_t id = at.first / kC + b;
-    at.rk = wk + (id * a.HK + hk) * rec_k(DK) + lane * 16;
-    at.rv = wv + (id * a.HV + at.head) * kRecV + lane * 16;
-    at.vec = reinterpret_cast<const float*>(wv + (id * a.HV + at.head) * kRecV + 6 * kTri * kFrag);
-    at.rks = (int64_t)a.HK * rec_k(DK), at.rvs = (int64_t)a.HV * kRecV;
     switch (wave >> 1) {
         case 0: return scan_state<DK, DV, 0>(a, at, slot, x);
         case 1: return scan_state<DK, DV, 1>(a, at, slot, x);
         case 2: return scan_out<DK, 0>(a, at, x);
-        default: return scan_out<DK, 1>(a, at, x);
+        case 3: return scan_out<DK, 1>(a, at, x);
+        default: break;
     }
+    const int64_t id = at.first / kC + b;
+    scan_load<DK>(at, wk + (id * a.HK + hk) * rec_k(DK), wv + (id * a.HV + at.head) * kRecV, (int64_t)a.HK * rec_k(DK),
+                  (int64_t)a.HV * kRecV, wave - 8, m, per, m % CT, CT, x);
 }
 
 static int64_t chunks(int64_t T, int64_t seqs) { return T / kC + seqs; }
@@ -708,7 +719,9 @@ static int launch_chunks(const DeltaArgs& a, char* ws, hipStream_t st) {
     char* wv = ws + nc * a.HK * rec_k(DK);
     hipLaunchKernelGGL(delta_prep_kernel<DK>, dim3((unsigned)nc, (unsigned)a.HV), dim3(64), 0, st, a, ws, wv);
     PRISM_LAUNCH_CHECK();
-    hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)wgs), dim3(512), 0, st, a, ws, wv, (int)keys);
+    allow_lds(delta_scan_kernel<DK, DV>, sizeof(ScanShared<DK>));
+    hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)wgs), dim3(768), sizeof(ScanShared<DK>), st, a, ws, wv,
+                       (int)keys);
     PRISM_LAUNCH_CHECK();
     return PRISM_OK;
 }
