@@ -451,6 +451,7 @@ struct ScanShared {
 // What a wave of delta_scan walks along.
 struct ScanAt {
     int first, count, nc, head, c0, w;                        // c0: the lane's column; w: which 16 of the workgroup's 32
+    int64_t rks, rvs;                                         // bytes from a chunk's records to the next one's
 };
 
 // acc += (rows of K or Q, the half's k)(the half's rows of S)
@@ -578,10 +579,19 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
     lds_barrier();
 }
 
+// rec: the key head's (HALF 0) or the head's (1) records, whose lines these waves touch two chunks ahead; m of `per`: this
+// workgroup among those that read them.
 template <int DK, int HALF>
-__device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, ScanShared<DK>& x) {
-    constexpr int KH = DK / 64, DH = DK / 32;
+__device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, const char* rec, int m, int per,
+                                         ScanShared<DK>& x) {
+    constexpr int KH = DK / 64, DH = DK / 32, LINES = (int)((HALF ? kRecV : rec_k(DK)) / 128);
     const int lane = threadIdx.x & 63, g = lane >> 4, w = at.w;
+    const int64_t step = HALF ? at.rvs : at.rks;
+    // (never waited for: these waves load nothing else)
+    auto touch = [&](const char* r) {
+        for (int i = (2 * m + w) * 64 + lane; i < LINES; i += per * 128)
+            __builtin_amdgcn_global_load_lds(r + i * 128, (__attribute__((address_space(3))) void*)x.touched, 4, 0, 0);
+    };
     v4f mine[2];
     float* out = a.out + (int64_t)at.first * a.ldo + at.head * a.ho_s + at.c0;
     // the last chunk's sums of this half's tokens, joined, then stored (`left` rows of it are there)
@@ -614,6 +624,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, S
         for (int i = 0; i < 4; i++) o[i] *= *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
         lds_barrier();
         if (c) store(kC);                                     // (here the state waves have more to do than these)
+        if (c + 2 < at.nc) touch(rec + (c + 2) * step);
         v4f u0 = x.ux[w][2 * HALF][lane], u1 = x.ux[w][2 * HALF + 1][lane];
         if (HALF) {
             u0 += x.ux[w][4][lane];
@@ -631,11 +642,10 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, S
     store(at.count - (at.nc - 1) * kC);
 }
 
-// Wave `q` of the four: every fourth fragment.  m of `per`, n of `heads`: this workgroup among those that read the same K
-// and Q, the same X and P; each touches its share of the lines two chunks on.
+// Wave `q` of the four: every fourth fragment.
 template <int DK>
-__device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, const char* rv, int64_t rks, int64_t rvs, int q,
-                                          int m, int per, int n, int heads, ScanShared<DK>& x) {
+__device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, const char* rv, int q, ScanShared<DK>& x) {
+    const int64_t rks = at.rks, rvs = at.rvs;
     constexpr int NK = 4 * (DK / 32), NT = DK / 16 * 2, NX = 3 * kTri;
     const int lane = threadIdx.x & 63;
     auto bring = [&](v4u (*to)[64], const char* from, int count) {
@@ -643,14 +653,6 @@ __device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, cons
     };
     auto factors = [&](int c, const char* r) {
         if (q == 0) dma16(r + 2 * NX * kFrag + lane * 16, x.vec[c & 1]);
-    };
-    auto touch = [&](const char* k, const char* v) {
-        if (q == 1)
-            for (int i = m * 64 + lane; i < (int)(rec_k(DK) / 128); i += per * 64)
-                __builtin_amdgcn_global_load_lds(k + i * 128, (__attribute__((address_space(3))) void*)x.touched, 4, 0, 0);
-        if (q == 2)
-            for (int i = n * 64 + lane; i < (int)(kRecV / 128); i += heads * 64)
-                __builtin_amdgcn_global_load_lds(v + i * 128, (__attribute__((address_space(3))) void*)x.touched, 4, 0, 0);
     };
     bring(x.k, rk, NK);
     bring(x.q, rk + NK * kFrag, NK);
@@ -670,7 +672,6 @@ __device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, cons
             bring(x.q, rk + rks + NK * kFrag, NK);
             bring(x.x, rv + rvs, NX);
             factors(c + 1, rv + rvs);
-            if (c + 2 < at.nc) touch(rk + 2 * rks, rv + 2 * rvs);
         }
         vm_wait<0>();
         rk += rks, rv += rvs;
@@ -696,16 +697,18 @@ __global__ __launch_bounds__(768, 3) void delta_scan_kernel(DeltaArgs a, const c
     at.w = wave & 1;
     at.c0 = 32 * (m % CT) + 16 * at.w + (lane & 15);
     at.nc = (at.count + kC - 1) / kC;
+    const int64_t id = at.first / kC + b;
+    const char* rk = wk + (id * a.HK + hk) * rec_k(DK);
+    const char* rv = wv + (id * a.HV + at.head) * kRecV;
+    at.rks = (int64_t)a.HK * rec_k(DK), at.rvs = (int64_t)a.HV * kRecV;
     switch (wave >> 1) {
         case 0: return scan_state<DK, DV, 0>(a, at, slot, x);
         case 1: return scan_state<DK, DV, 1>(a, at, slot, x);
-        case 2: return scan_out<DK, 0>(a, at, x);
-        case 3: return scan_out<DK, 1>(a, at, x);
+        case 2: return scan_out<DK, 0>(a, at, rk, m, per, x);
+        case 3: return scan_out<DK, 1>(a, at, rv, m % CT, CT, x);
         default: break;
     }
-    const int64_t id = at.first / kC + b;
-    scan_load<DK>(at, wk + (id * a.HK + hk) * rec_k(DK), wv + (id * a.HV + at.head) * kRecV, (int64_t)a.HK * rec_k(DK),
-                  (int64_t)a.HV * kRecV, wave - 8, m, per, m % CT, CT, x);
+    scan_load<DK>(at, rk, rv, wave - 8, x);
 }
 
 static int64_t chunks(int64_t T, int64_t seqs) { return T / kC + seqs; }
