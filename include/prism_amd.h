@@ -384,81 +384,123 @@ PRISM_API int64_t prism_mxfp4_split_workspace_bytes(int64_t N, int64_t K);
 
 /* ------------------------------------------------------------------------------------- token mixers (serving) */
 /*
- * The paged key-value cache of a full-attention layer: k_cache and v_cache [pages, page, HKV, D] (strides k_page, k_tok,
- * k_head and v_page, v_tok, v_head in elements, unit stride in D) of bf16 or (e4m3 = 1) OCP e4m3; an e4m3 cache may have
- * a scale per head (k_scale, v_scale fp32 [HKV], or null for 1): it holds x / scale clamped to +-448, nearest even, and
- * stands for value * scale.  table int32 [sequences, cols] (row stride table_ld): token t of sequence s lies in row
- * t % page of page table[s][t / page].  D 64, 128 or 256; page a power of two in 16 .. 65536; both caches 16-byte aligned
- * with strides of whole 16-byte units, a token stride of at most 2^26 elements.
+ * These entry points take their many arguments as one struct (host memory, read before the call returns) of 8-byte fields;
+ * strides are in elements.  They have no counterpart among the reference's quantized linear ops.
  *
- * prism_kv_append: token i < *n_rows, at position p = pos[i] of sequence s = seq[i] (seq null: i).  The first rot dims of
- * q and k turn by rope [rope_rows, rot] (fp32, row stride ldr: row p holds rot / 2 cosines, then the sines), pairs
- * (j, j + rot / 2), or (2 j, 2 j + 1) when adjacent = 1:
- *   a' = RN(RN(a cos) - RN(b sin)), b' = RN(RN(b cos) + RN(a sin)), rounded to the stored type.
- * q bf16 [T, HQ, D] -> q_out (which may be q; HQ = 0: no queries), k, v bf16 [T, HKV, D] -> the cache; row and head
- * strides in elements.  A token with no place (a position negative, past the table or the rotations; a sequence or page
- * out of range) is skipped.  rot = 0: no rotation.  Needs rot % 16 == 0, rot <= D, 16-byte aligned q, k, v, q_out and rope,
- * strides % 8 == 0 (ldr % 4).  No counterpart among the reference's quantized linear ops; nor have the entries below.
+ * The paged key-value cache of a full-attention layer: k and v [pages, page, heads, dim] (with unit stride in dim) of bf16
+ * or (e4m3 = 1) OCP e4m3; an e4m3 cache may have a scale per head (k_scale, v_scale fp32 [heads], or null for 1): it holds
+ * x / scale clamped to +-448, nearest even, and stands for value * scale.  table int32 [seqs, cols] (row stride
+ * table_ld): token t of sequence s lies in row t % page of page table[s][t / page].  dim 64, 128 or 256; page a power
+ * of two in 16 .. 65536; both caches 16-byte aligned with strides of whole 16-byte units, token strides of at most 2^26.
  */
-PRISM_API int prism_kv_append(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
-                              int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, uint16_t* q_out, int64_t ldo,
-                              int64_t ho_s, const float* rope, int64_t ldr, int64_t rope_rows, int64_t rot,
-                              int adjacent, const int32_t* pos, const int32_t* seq, void* k_cache, int64_t k_page,
-                              int64_t k_tok, int64_t k_head, void* v_cache, int64_t v_page, int64_t v_tok,
-                              int64_t v_head, int e4m3, const float* k_scale, const float* v_scale,
-                              const int32_t* table, int64_t table_ld, int64_t seqs, int64_t cols, int64_t pages,
-                              int64_t page, const int32_t* n_rows, int64_t T, int64_t HQ, int64_t HKV, int64_t D,
-                              void* stream);
+typedef struct {
+    void* k;
+    int64_t k_page, k_tok, k_head;
+    void* v;
+    int64_t v_page, v_tok, v_head;
+    int64_t e4m3;
+    const float* k_scale;
+    const float* v_scale;
+    const int32_t* table;
+    int64_t table_ld, seqs, cols, pages, page, heads, dim;
+} prism_kv_cache;
 
 /*
- * Attention of one new token per sequence over the cache: for i < *n_rows, out[i][h] = sum_t softmax_t(scale q[i][h] .
- * k_t) v_t over tokens t of max(0, lens[i] - window) .. lens[i] - 1 (window 0: all), head h on cache head h / (HQ / HKV);
- * no tokens: zeros.  lens counts past the table's capacity, cols page, are taken as that.  fp32 sums and softmax, the
- * weights in two bf16 parts; parts of a sequence (the split depends on all lengths) are joined in a fixed order through
- * `ws` (prism_kv_attend_workspace_bytes, no initial contents; 16-byte aligned; calls that overlap must not share it).
- * Rows >= *n_rows are untouched.  Needs HQ % HKV == 0, T <= 65535, 16-byte aligned q with strides % 8, 8-byte aligned out
- * with strides % 4, cols page < 2^31 - 65536.
+ * prism_kv_append: token i < *n_rows (of T), at position p = pos[i] of sequence s = seq[i] (seq null: i).  The first rot
+ * dims of q and k turn by rope [rope_rows, rot] (fp32, row stride ldr: row p holds rot / 2 cosines, then the sines), pairs
+ * (j, j + rot / 2), or (2 j, 2 j + 1) when adjacent = 1:
+ *   a' = RN(RN(a cos) - RN(b sin)), b' = RN(RN(b cos) + RN(a sin)), rounded to the stored type.
+ * q bf16 [T, hq, dim] -> q_out (which may be q; hq = 0: no queries), k, v bf16 [T, heads, dim] -> the cache; ld: row
+ * strides, hs: head strides.  A token with no place (a position negative, past the table or the rotations; a sequence or
+ * page out of range) is skipped.  rot = 0: no rotation.  Needs rot % 16 == 0, rot <= dim, 16-byte aligned q, k, v, q_out and
+ * rope, strides % 8 == 0 (ldr % 4).
  */
-PRISM_API int prism_kv_attend(const uint16_t* q, int64_t ldq, int64_t hq_s, const void* k_cache, int64_t k_page,
-                              int64_t k_tok, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_tok,
-                              int64_t v_head, int e4m3, const float* k_scale, const float* v_scale,
-                              const int32_t* table, int64_t table_ld, int64_t cols, int64_t pages, int64_t page,
-                              const int32_t* lens, uint16_t* out, int64_t ldo, int64_t ho_s, const int32_t* n_rows,
-                              int64_t T, int64_t HQ, int64_t HKV, int64_t D, float scale, int64_t window, void* ws,
-                              int64_t ws_bytes, void* stream);
+typedef struct {
+    prism_kv_cache cache;
+    const uint16_t* q;
+    int64_t q_ld, q_hs;
+    const uint16_t* k;
+    int64_t k_ld, k_hs;
+    const uint16_t* v;
+    int64_t v_ld, v_hs;
+    uint16_t* q_out;
+    int64_t o_ld, o_hs;
+    const float* rope;
+    int64_t ldr, rope_rows, rot, adjacent;
+    const int32_t* pos;
+    const int32_t* seq;
+    const int32_t* n_rows;
+    int64_t T, hq;
+} prism_kv_append_args;
+PRISM_API int prism_kv_append(const prism_kv_append_args* args, void* stream);
+
+/*
+ * prism_kv_attend: attention of one new token per sequence over the cache (T = cache.seqs sequences): for i < *n_rows,
+ * out[i][h] = sum_t softmax_t(scale q[i][h] . k_t) v_t over tokens t of max(0, lens[i] - window) .. lens[i] - 1 (window 0:
+ * all), head h of hq on cache head h / (hq / heads); no tokens: zeros.  lens past the table's capacity, cols page, count as
+ * that.  fp32 sums and softmax, the weights in two bf16 parts; parts of a sequence (the split depends on all lengths) are
+ * joined in a fixed order through ws (prism_kv_attend_workspace_bytes, no initial contents; 16-byte aligned; calls that
+ * overlap must not share it).  Rows >= *n_rows are untouched.  Needs hq % heads == 0, T <= 65535, 16-byte aligned q with
+ * strides % 8, 8-byte aligned out with strides % 4, cols page < 2^31 - 65536.
+ */
+typedef struct {
+    prism_kv_cache cache;
+    const uint16_t* q;
+    int64_t q_ld, q_hs;
+    uint16_t* out;
+    int64_t o_ld, o_hs;
+    const int32_t* lens;
+    const int32_t* n_rows;
+    int64_t hq, window;
+    double scale;
+    void* ws;
+    int64_t ws_bytes;
+} prism_kv_attend_args;
+PRISM_API int prism_kv_attend(const prism_kv_attend_args* args, void* stream);
 /* Bytes of ws for T sequences; 0 where nothing is split (ws may be null). */
-PRISM_API int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t cols,
+PRISM_API int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t hq, int64_t heads, int64_t dim, int64_t cols,
                                                   int64_t page);
 
 /*
- * The gated delta rule, per value head h with key head h / (HV / HK) and state S fp32 [DK, DV]:
+ * The gated delta rule, per value head h with key head h / (hv / hk) and state S fp32 [dk, dv]:
  *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q,
  * k and q first divided by sqrt(|.|^2 + eps) when norm = 1, q times scale either way; fp32 sums throughout.
- * q, k bf16 [T, HK, DK], v bf16 [T, HV, DV] (row and head strides in elements), g, beta fp32 [T, HV], out fp32
- * [T, HV, DV]; state [nslots, HV, DK, DV] contiguous per slot, slot_stride elements apart, updated in place; slots int32:
- * the state of each sequence (null: its number).  A sequence whose slot is out of range is skipped; two sequences must
- * not share one.  Needs DK, DV in {64, 128}, HV % HK == 0, 16-byte aligned tensors, strides % 8 (out and state % 4).
+ * q, k bf16 [T, hk, dk], v bf16 [T, hv, dv], g, beta fp32 [T, hv], out fp32 [T, hv, dv] (ld: row strides, hs: head
+ * strides); state [nslots, hv, dk, dv] contiguous per slot, slot_ld apart, updated in place; slots int32: the state of
+ * each sequence (null: its number).  A sequence whose slot is out of range is skipped; two sequences must not share one.
+ * Needs dk, dv in {64, 128}, hv % hk == 0, 16-byte aligned tensors, strides % 8 (out and state % 4), v_ld <= 2^24.
  *
- * prism_delta_step: row i < *n_rows is one token of sequence i.
- * prism_delta_prefill: sequence s is rows cu[s] .. cu[s + 1] - 1 (cu int32 [seqs + 1], non-decreasing within 0 .. T), in
+ * prism_delta_step: rows int32 [1]: row i < *rows (of T) is one token of sequence i; seqs, ws and ws_bytes are not read.
+ * prism_delta_prefill: rows int32 [seqs + 1], non-decreasing within 0 .. T: sequence s is rows[s] .. rows[s + 1] - 1, in
  * order.  ws: prism_delta_prefill_workspace_bytes (no initial contents, 16-byte aligned; calls that overlap must not
  * share it), null where that is 0.
  */
-PRISM_API int prism_delta_step(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
-                               int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, const float* g, int64_t ldg,
-                               const float* beta, int64_t ldb, float* state, int64_t slot_stride, int64_t nslots,
-                               const int32_t* slots, float* out, int64_t ldo, int64_t ho_s, const int32_t* n_rows,
-                               int64_t T, int64_t HK, int64_t HV, int64_t DK, int64_t DV, int norm, float scale,
-                               float eps, void* stream);
-PRISM_API int prism_delta_prefill(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
-                                  int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, const float* g,
-                                  int64_t ldg, const float* beta, int64_t ldb, float* state, int64_t slot_stride,
-                                  int64_t nslots, const int32_t* slots, float* out, int64_t ldo, int64_t ho_s,
-                                  const int32_t* cu, int64_t seqs, int64_t T, int64_t HK, int64_t HV, int64_t DK,
-                                  int64_t DV, int norm, float scale, float eps, void* ws, int64_t ws_bytes,
-                                  void* stream);
-PRISM_API int64_t prism_delta_prefill_workspace_bytes(int64_t T, int64_t seqs, int64_t HK, int64_t HV, int64_t DK,
-                                                      int64_t DV);
+typedef struct {
+    const uint16_t* q;
+    int64_t q_ld, q_hs;
+    const uint16_t* k;
+    int64_t k_ld, k_hs;
+    const uint16_t* v;
+    int64_t v_ld, v_hs;
+    const float* g;
+    int64_t g_ld;
+    const float* beta;
+    int64_t b_ld;
+    float* state;
+    int64_t slot_ld, nslots;
+    const int32_t* slots;
+    float* out;
+    int64_t o_ld, o_hs;
+    const int32_t* rows;
+    int64_t seqs, T, hk, hv, dk, dv, norm;
+    double scale, eps;
+    void* ws;
+    int64_t ws_bytes;
+} prism_delta_args;
+PRISM_API int prism_delta_step(const prism_delta_args* args, void* stream);
+PRISM_API int prism_delta_prefill(const prism_delta_args* args, void* stream);
+PRISM_API int64_t prism_delta_prefill_workspace_bytes(int64_t T, int64_t seqs, int64_t hk, int64_t hv, int64_t dk,
+                                                      int64_t dv);
 
 /*
  * Peak probes (measurement tooling: the reference's bench/csrc/mma_peak.cu:14-70 and bench/csrc/l2_bw.cu:8 for

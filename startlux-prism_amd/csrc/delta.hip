@@ -717,8 +717,7 @@ template <int DK, int DV>
 static int launch_chunks(const DeltaArgs& a, char* ws, hipStream_t st) {
     const int64_t nc = chunks(a.rows, a.seqs), keys = (int64_t)a.seqs * a.HK;
     const int64_t wgs = (keys + 7) / 8 * 8 * (a.HV / a.HK) * (DV / 32);
-    if (nc > INT32_MAX || a.HV > 65535 || wgs > INT32_MAX) return PRISM_ERR_SHAPE;
-    if (a.ldv > 1 << 24) return PRISM_ERR_SHAPE;              // a chunk's values within 32-bit offsets
+    if (nc > INT32_MAX || wgs > INT32_MAX) return PRISM_ERR_SHAPE;
     char* wv = ws + nc * a.HK * rec_k(DK);
     hipLaunchKernelGGL(delta_prep_kernel<DK>, dim3((unsigned)nc, (unsigned)a.HV), dim3(64), 0, st, a, ws, wv);
     PRISM_LAUNCH_CHECK();
@@ -726,20 +725,6 @@ static int launch_chunks(const DeltaArgs& a, char* ws, hipStream_t st) {
     hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)wgs), dim3(768), sizeof(ScanShared<DK>), st, a, ws, wv,
                        (int)keys);
     PRISM_LAUNCH_CHECK();
-    return PRISM_OK;
-}
-
-static int check(const DeltaArgs& a, int64_t rows, int64_t seqs, int64_t nslots, int64_t HK, int64_t HV, int64_t DK,
-                 int64_t DV) {
-    if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.state || !a.out || (a.norm != 0 && a.norm != 1)) return PRISM_ERR_ARG;
-    if ((DK != 64 && DK != 128) || (DV != 64 && DV != 128)) return PRISM_ERR_SHAPE;
-    if (HK < 1 || HV < HK || HV % HK || HV > 65536 || rows < 0 || rows > INT32_MAX || seqs < 0 || seqs > INT32_MAX)
-        return PRISM_ERR_SHAPE;
-    if (nslots < 0 || nslots > INT32_MAX || a.lds_ < HV * DK * DV) return PRISM_ERR_SHAPE;
-    if (!PRISM_ALIGNED(a.q, 16) || !PRISM_ALIGNED(a.k, 16) || !PRISM_ALIGNED(a.v, 16) || !PRISM_ALIGNED(a.out, 16) ||
-        !PRISM_ALIGNED(a.state, 16) || a.ldq % 8 || a.hq_s % 8 || a.ldk % 8 || a.hk_s % 8 || a.ldv % 8 || a.hv_s % 8 ||
-        a.ldo % 4 || a.ho_s % 4 || a.lds_ % 4)
-        return PRISM_ERR_ALIGN;
     return PRISM_OK;
 }
 
@@ -756,47 +741,51 @@ static int dispatch_chunks(const DeltaArgs& a, int64_t DK, int64_t DV, char* ws,
 // A handful of rows go token by token.
 static bool by_token(int64_t T) { return T <= 16; }
 
+static int64_t workspace_bytes(int64_t T, int64_t seqs, int64_t hk, int64_t hv, int64_t dk) {
+    if (T < 1 || seqs < 1 || hk < 1 || hv < 1 || (dk != 64 && dk != 128) || by_token(T)) return 0;
+    return chunks(T, seqs) * (hk * rec_k((int)dk) + hv * kRecV);
+}
+
+static_assert(sizeof(prism_delta_args) == 32 * 8, "8-byte fields throughout");
+
+// A call's arguments, checked and launched; seqs sequences, in chunks where a prompt's rows are given and many enough.
+static int run(const prism_delta_args& h, bool prompts, hipStream_t st) {
+    const int64_t seqs = prompts ? h.seqs : h.T;
+    if (!h.q || !h.k || !h.v || !h.g || !h.beta || !h.state || !h.out || !h.rows || (h.norm != 0 && h.norm != 1))
+        return PRISM_ERR_ARG;
+    if ((h.dk != 64 && h.dk != 128) || (h.dv != 64 && h.dv != 128)) return PRISM_ERR_SHAPE;
+    if (h.hk < 1 || h.hv < h.hk || h.hv % h.hk || h.hv > 65535 || h.T < 0 || h.T > INT32_MAX || seqs < 0 ||
+        seqs > INT32_MAX)
+        return PRISM_ERR_SHAPE;
+    if (h.nslots < 0 || h.nslots > INT32_MAX || h.slot_ld < h.hv * h.dk * h.dv) return PRISM_ERR_SHAPE;
+    if (h.v_ld > 1 << 24) return PRISM_ERR_SHAPE;             // a chunk's values within 32-bit offsets
+    if (!PRISM_ALIGNED(h.q, 16) || !PRISM_ALIGNED(h.k, 16) || !PRISM_ALIGNED(h.v, 16) || !PRISM_ALIGNED(h.out, 16) ||
+        !PRISM_ALIGNED(h.state, 16) || h.q_ld % 8 || h.q_hs % 8 || h.k_ld % 8 || h.k_hs % 8 || h.v_ld % 8 || h.v_hs % 8 ||
+        h.o_ld % 4 || h.o_hs % 4 || h.slot_ld % 4)
+        return PRISM_ERR_ALIGN;
+    const int64_t need = prompts ? workspace_bytes(h.T, seqs, h.hk, h.hv, h.dk) : 0;
+    if (need > 0 && (!h.ws || h.ws_bytes < need)) return PRISM_ERR_ARG;
+    if (need > 0 && !PRISM_ALIGNED(h.ws, 16)) return PRISM_ERR_ALIGN;
+    if (h.T == 0 || seqs == 0 || h.nslots == 0) return PRISM_OK;
+    const DeltaArgs a{h.q, h.k, h.v, h.q_ld, h.q_hs, h.k_ld, h.k_hs, h.v_ld, h.v_hs, h.g, h.beta, h.g_ld, h.b_ld, h.state,
+                      h.slot_ld, h.out, h.o_ld, h.o_hs, prompts ? h.rows : nullptr, h.slots, prompts ? nullptr : h.rows,
+                      (int)h.T, (int)seqs, (int)h.nslots, (int)h.hk, (int)h.hv, (int)h.norm, (float)h.scale, (float)h.eps};
+    return need > 0 ? dispatch_chunks(a, h.dk, h.dv, (char*)h.ws, st) : dispatch_rec(a, h.dk, h.dv, st);
+}
+
 }  // namespace prism
 
 using namespace prism;
 
-extern "C" int prism_delta_step(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
-                                int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, const float* g, int64_t ldg,
-                                const float* beta, int64_t ldb, float* state, int64_t slot_stride, int64_t nslots,
-                                const int32_t* slots, float* out, int64_t ldo, int64_t ho_s, const int32_t* n_rows,
-                                int64_t T, int64_t HK, int64_t HV, int64_t DK, int64_t DV, int norm, float scale,
-                                float eps, void* stream) {
-    const DeltaArgs a{q, k, v, ldq, hq_s, ldk, hk_s, ldv, hv_s, g, beta, ldg, ldb, state, slot_stride, out, ldo, ho_s,
-                      nullptr, slots, n_rows, (int)T, (int)T, (int)nslots, (int)HK, (int)HV, norm, scale, eps};
-    const int rc = check(a, T, T, nslots, HK, HV, DK, DV);
-    if (rc != PRISM_OK) return rc;
-    if (!n_rows) return PRISM_ERR_ARG;
-    if (T == 0 || nslots == 0) return PRISM_OK;
-    return dispatch_rec(a, DK, DV, (hipStream_t)stream);
+extern "C" int prism_delta_step(const prism_delta_args* args, void* stream) {
+    return args ? run(*args, false, (hipStream_t)stream) : (int)PRISM_ERR_ARG;
 }
 
-extern "C" int prism_delta_prefill(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
-                                   int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, const float* g,
-                                   int64_t ldg, const float* beta, int64_t ldb, float* state, int64_t slot_stride,
-                                   int64_t nslots, const int32_t* slots, float* out, int64_t ldo, int64_t ho_s,
-                                   const int32_t* cu, int64_t seqs, int64_t T, int64_t HK, int64_t HV, int64_t DK,
-                                   int64_t DV, int norm, float scale, float eps, void* ws, int64_t ws_bytes,
-                                   void* stream) {
-    const DeltaArgs a{q, k, v, ldq, hq_s, ldk, hk_s, ldv, hv_s, g, beta, ldg, ldb, state, slot_stride, out, ldo, ho_s,
-                      cu, slots, nullptr, (int)T, (int)seqs, (int)nslots, (int)HK, (int)HV, norm, scale, eps};
-    const int rc = check(a, T, seqs, nslots, HK, HV, DK, DV);
-    if (rc != PRISM_OK) return rc;
-    if (!cu) return PRISM_ERR_ARG;
-    const int64_t need = prism_delta_prefill_workspace_bytes(T, seqs, HK, HV, DK, DV);
-    if (need > 0 && (!ws || ws_bytes < need)) return PRISM_ERR_ARG;
-    if (need > 0 && !PRISM_ALIGNED(ws, 16)) return PRISM_ERR_ALIGN;
-    if (T == 0 || seqs == 0 || nslots == 0) return PRISM_OK;
-    if (by_token(T)) return dispatch_rec(a, DK, DV, (hipStream_t)stream);
-    return dispatch_chunks(a, DK, DV, (char*)ws, (hipStream_t)stream);
+extern "C" int prism_delta_prefill(const prism_delta_args* args, void* stream) {
+    return args ? run(*args, true, (hipStream_t)stream) : (int)PRISM_ERR_ARG;
 }
 
-extern "C" int64_t prism_delta_prefill_workspace_bytes(int64_t T, int64_t seqs, int64_t HK, int64_t HV, int64_t DK,
-                                                       int64_t DV) {
-    if (T < 1 || seqs < 1 || HK < 1 || HV < 1 || (DK != 64 && DK != 128) || by_token(T)) return 0;
-    return chunks(T, seqs) * (HK * rec_k((int)DK) + HV * kRecV);
+extern "C" int64_t prism_delta_prefill_workspace_bytes(int64_t T, int64_t seqs, int64_t hk, int64_t hv, int64_t dk,
+                                                       int64_t dv) {
+    return dv == 64 || dv == 128 ? workspace_bytes(T, seqs, hk, hv, dk) : 0;
 }

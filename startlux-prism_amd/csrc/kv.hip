@@ -4,6 +4,8 @@
 // The cache is [pages, page, heads, dim] of bf16 or e4m3 with any strides of its first three dims, so both memory
 // orders in use (token rows of all heads, or a page's rows of one head together) are the same code.  A page table
 // int32 [sequences, columns] names the pages of a sequence: token t lies in row t % page of page table[s][t / page].
+#include <type_traits>
+
 #include "common.h"
 
 namespace prism {
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // o[h] = sum_t softmax_t(scale q_h . k_t) v_t over a sequence's visible tokens, all query heads of one key head
 // together (they read the same keys and values), in one pass with a running maximum and sum per query head.
 //
-// A wave takes blocks of 32 tokens with no LDS: scores transposed, S^T = K Q^T (the keys as the MFMA's first operand,
+// A wave takes blocks of 32 tokens: scores transposed, S^T = K Q^T (the keys as the MFMA's first operand,
 // query heads its 16 columns), leave each lane the scores of ITS head (lane % 16) for tokens 4 g + r and 16 + 4 g + r
 // (g = lane / 16, r < 4).  O^T = V^T P^T wants in each lane 8 tokens of its head as second operand, and the order of
 // the 32 tokens along the product is free as long as both operands agree: taking them as the scores lie, P never
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // rounding is the only one that shows; the second MFMA is free beside the cache's bytes.
 //
 // Work is split on the device, from the lengths (a captured launch serves every batch): a unit is what the four waves
-// take in one round; `per` units to a workgroup bring the batch to about kTarget workgroups; a sequence gets
+// take in one round; `per` units to a workgroup bring the batch to about `target` workgroups; a sequence gets
 // max(1, ceil(units / per)) of them, shared evenly.  Sequences with one workgroup write their output; the others'
 // parts are joined by a second kernel in a fixed order, so results do not depend on timing.
 struct AttendArgs {
@@ -157,6 +159,7 @@ struct AttendArgs {
     const int32_t *lens, *n;
     float* part_o;                                            // [P, HQ, D]
     float* part_ml;                                           // [P, HQ, 2]
+    int2* plan;                                               // [T]: a sequence's first part and how many it has
     float scale;                                              // times log2 e
     int T, HQ, G, tiles, HT, window, target;
     Cache c;
@@ -186,9 +189,9 @@ __device__ __forceinline__ long long wave_sum(long long v) {
     return v;
 }
 
-// Work of part p (b < 0: none), or with p < 0 sequence `want`'s parts; the same in every lane.
+// Work of part p (b < 0: none); the same in every lane.
 template <int UNIT>
-__device__ __forceinline__ Plan make_plan(const AttendArgs& a, int p, int want) {
+__device__ __forceinline__ Plan make_plan(const AttendArgs& a, int p) {
     const int lane = threadIdx.x & 63;
     const int n = min(__ldg(a.n), a.T);
     int lo, len;
@@ -215,7 +218,7 @@ __device__ __forceinline__ Plan make_plan(const AttendArgs& a, int p, int want) 
         }
         const int tot = __shfl(incl, 63, kWave);
         const int mine = base + incl - nb;                    // first part of this lane's sequence
-        const bool hit = p < 0 ? b == want : nb > 0 && p >= mine && p < mine + nb;
+        const bool hit = nb > 0 && p >= mine && p < mine + nb;
         const uint64_t m = __ballot(hit);
         if (m) {
             const int src = __builtin_ctzll(m);
@@ -237,11 +240,6 @@ __device__ __forceinline__ Plan make_plan(const AttendArgs& a, int p, int want) 
     return r;
 }
 
-template <typename V>
-__device__ __forceinline__ V ld(const char* base, uint32_t off) {
-    return *reinterpret_cast<const V*>(base + off);
-}
-
 __device__ __forceinline__ v8bf as_bf(v4u x) { return __builtin_bit_cast(v8bf, x); }
 __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(a), as_bf(b), c, 0, 0, 0);
@@ -252,41 +250,40 @@ __device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, SEL));
 }
 
-// Registers of one 32-token block's keys and values, and the loads that fill them.
+// One 32-token block: its loads' sizes, and its values' registers.
 template <int D, bool F8>
 struct Block {
-    static constexpr int KL = F8 ? D / 64 : D / 32;           // 16-byte key loads per 16 tokens and lane
-    static constexpr int VB = (F8 ? 1 : 2) * D / 16;          // value bytes per token and lane
-    static constexpr int VW = VB / 4;                         // 4, 8 or 16 bytes a load (two of 16 for 32)
-    v4u k[2][KL];
+    static constexpr int RB = (F8 ? 1 : 2) * D;               // bytes of a token's row
+    static constexpr int L = RB / 64;                         // loads of 1 KB for 16 tokens
+    static constexpr int VB = RB / 16, VW = VB / 4;           // value bytes and words per token and lane
+    // LDS bytes of a wave: the keys and values, at the end 16 columns of O
+    static constexpr int STAGE = 4 * L * 1024 > 16 * (D + 4) * 4 ? 4 * L * 1024 : 16 * (D + 4) * 4;
     uint32_t v[2][4][VW];
 };
 
+// The lane's piece of its 8 tokens' values (4 g + r of each 16).
 template <int D, bool F8>
-__device__ __forceinline__ void load_k(Block<D, F8>& s, int a, const char* base, uint32_t off) {
+__device__ __forceinline__ void read_v(Block<D, F8>& s, const char* vl) {
+    using B = Block<D, F8>;
 #pragma unroll
-    for (int i = 0; i < Block<D, F8>::KL; i++) s.k[a][i] = ld<v4u>(base, off + 64 * i);
-}
-
-template <int D, bool F8>
-__device__ __forceinline__ void load_v(Block<D, F8>& s, int a, const char* base, uint32_t off, uint32_t step) {
-    constexpr int VW = Block<D, F8>::VW;
+    for (int a = 0; a < 2; a++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        if constexpr (VW == 1) {
-            s.v[a][r][0] = ld<uint32_t>(base, off + r * step);
-        } else if constexpr (VW == 2) {
-            const v2u x = ld<v2u>(base, off + r * step);
-            s.v[a][r][0] = x[0], s.v[a][r][1] = x[1];
-        } else {
+        for (int r = 0; r < 4; r++) {
+            const char* p = vl + (16 * a + r) * B::RB;
+            if constexpr (B::VW == 1) {
+                s.v[a][r][0] = *reinterpret_cast<const uint32_t*>(p);
+            } else if constexpr (B::VW == 2) {
+                const v2u x = *reinterpret_cast<const v2u*>(p);
+                s.v[a][r][0] = x[0], s.v[a][r][1] = x[1];
+            } else {
 #pragma unroll
-            for (int i = 0; i < VW / 4; i++) {                // dims 8 c .. and 128 + 8 c .. of 256 bf16
-                const v4u x = ld<v4u>(base, off + r * step + 256 * i);
+                for (int i = 0; i < B::VW / 4; i++) {         // dims 8 c .. and 128 + 8 c .. of 256 bf16
+                    const v4u x = *reinterpret_cast<const v4u*>(p + 256 * i);
 #pragma unroll
-                for (int w = 0; w < 4; w++) s.v[a][r][4 * i + w] = x[w];
+                    for (int w = 0; w < 4; w++) s.v[a][r][4 * i + w] = x[w];
+                }
             }
         }
-    }
 }
 
 // The dim that fragment f of O^T holds in row m (piece m).
@@ -327,11 +324,14 @@ __device__ __forceinline__ void turn_v(const Block<D, F8>& s, int q, v4u (&out)[
 
 template <int D, bool F8>
 __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
-    constexpr int UNIT = 32 * kWaves, F = D / 16, QF = D / 32;
-    extern __shared__ float lds[];                            // [4][16][D + 4] O, then [4][16] m, [4][16] l
-    const int ht = blockIdx.x % a.HT, part = blockIdx.x / a.HT;
-    const Plan pl = make_plan<UNIT>(a, part, 0);
+    using B = Block<D, F8>;
+    constexpr int UNIT = 32 * kWaves, F = D / 16, QF = D / 32, L = B::L;
+    extern __shared__ __align__(16) char lds[];               // per wave: keys, at the end 16 columns of O; then m and l
+    // a part's heads, whose rows lie side by side in a cache of token rows, on one XCD (workgroup i runs on XCD i % 8)
+    const int ht = blockIdx.x / 8 % a.HT, part = blockIdx.x / (8 * a.HT) * 8 + blockIdx.x % 8;
+    const Plan pl = make_plan<UNIT>(a, part);
     if (pl.b < 0) return;
+    if (a.plan && ht == 0 && pl.split == 0 && threadIdx.x == 0) a.plan[pl.b] = int2{pl.first, pl.splits};
     const int hk = ht / a.tiles, tile = ht % a.tiles;
     const int h0 = hk * a.G + 16 * tile, nh = min(16, a.G - 16 * tile);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -353,22 +353,53 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
     for (int f = 0; f < F; f++) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 
-    const int32_t* row = a.c.table + b * a.c.table_ld;
+    // the table through the scalar cache: a vector load would be waited for together with the values in flight before it
+    const auto* row = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
+        reinterpret_cast<uintptr_t>(a.c.table + b * a.c.table_ld));
     const int last = len > 0 ? (len - 1) & ~15 : 0;           // the last 16 tokens that are there
-    const uint32_t koff = (uint32_t)(col * a.c.k_tok) + 16 * g;
-    const uint32_t voff = (uint32_t)(4 * g * a.c.v_tok) + (D == 256 && !F8 ? 16 : Block<D, F8>::VB) * col;
+    // Keys and values go to LDS by DMA, 1 KB a load.  Keys: 16 tokens x 64 bytes, four neighbouring lanes a token's (the
+    // memory pipeline merges neighbouring lanes only), placed so that operand order reads without bank conflicts; values:
+    // whole rows.  Every wait on them is written out: the compiler would wait for all of them at each use.
+    const uint32_t koff = (uint32_t)((lane >> 2) * a.c.k_tok) + 16 * ((lane & 3) ^ lds_turn(lane >> 4));
+    const uint32_t voff = (uint32_t)(16 * lane / B::RB * a.c.v_tok) + 16 * lane % B::RB;
     const char* kb = a.c.k + hk * a.c.k_head;
     const char* vb = a.c.v + hk * a.c.v_head;
+    char* stage = lds + wave * B::STAGE;
+    const v4u* kl = reinterpret_cast<const v4u*>(stage) + 4 * col + (g ^ lds_turn(col >> 2));
+    const char* vl = stage + 2 * L * 1024 + 4 * g * B::RB + (D == 256 && !F8 ? 16 : B::VB) * col;
 
-    for (int t0 = begin + 32 * wave; t0 < end; t0 += UNIT) {
-        Block<D, F8> s;
+    int64_t page[2];
+    auto locate = [&](int t0) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) page[x] = row[min(t0 + 16 * x, last) >> a.c.shift];   // 16 tokens never cross a page
+    };
+    auto clamp = [&] {
+#pragma unroll
+        for (int x = 0; x < 2; x++) page[x] = min(max((int)page[x], 0), a.c.pages - 1);
+    };
+    auto at = [&](int t0, int x) { return (int64_t)(min(t0 + 16 * x, last) & ((1 << a.c.shift) - 1)); };
+    auto load_k = [&](int t0) {
 #pragma unroll
         for (int x = 0; x < 2; x++) {
-            const int t = min(t0 + 16 * x, last);             // 16 tokens never cross a page
-            const int64_t page = min(max(row[t >> a.c.shift], 0), a.c.pages - 1), at = t & ((1 << a.c.shift) - 1);
-            load_k<D, F8>(s, x, kb + page * a.c.k_page + at * a.c.k_tok, koff);
-            load_v<D, F8>(s, x, vb + page * a.c.v_page + at * a.c.v_tok, voff, (uint32_t)a.c.v_tok);
+            const char* p = kb + page[x] * a.c.k_page + at(t0, x) * a.c.k_tok + koff;
+#pragma unroll
+            for (int i = 0; i < L; i++) dma16(p + 64 * i, stage + (x * L + i) * 1024);
         }
+    };
+    auto load_v = [&](int t0) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const char* p = vb + page[x] * a.c.v_page + at(t0, x) * a.c.v_tok + voff;
+#pragma unroll
+            for (int i = 0; i < L; i++) dma16(p + i * (1024 / B::RB) * a.c.v_tok, stage + (2 * L + x * L + i) * 1024);
+        }
+    };
+    B s;
+    // One block of 32 tokens; with `more`, the next one's loads go out as this one's places in LDS become free.
+    auto block = [&](int t0, auto more) {
+        constexpr bool MORE = decltype(more)::value;
+        vm_wait<2 * L>();                                     // the keys are there (the values' loads came after theirs)
+        if (MORE) locate(t0 + UNIT);
         v4f st[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int x = 0; x < 2; x++)
@@ -376,18 +407,30 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
             for (int i = 0; i < QF; i++) {
                 v4u kf;
                 if constexpr (F8) {
-                    const uint32_t w0 = s.k[x][i / 2][2 * (i % 2)], w1 = s.k[x][i / 2][2 * (i % 2) + 1];
+                    const v4u w = kl[(x * L + i / 2) * 64];
+                    const uint32_t w0 = w[2 * (i % 2)], w1 = w[2 * (i % 2) + 1];
                     kf = v4u{e4m3x2_bf16<false>(w0), e4m3x2_bf16<true>(w0), e4m3x2_bf16<false>(w1),
                              e4m3x2_bf16<true>(w1)};
                 } else {
-                    kf = s.k[x][i];
+                    kf = kl[(x * L + i) * 64];
                 }
                 st[x] = mfma_bf16(kf, qf[i], st[x]);
             }
+        if (MORE) {
+            clamp();
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this block's keys are read
+            load_k(t0 + UNIT);
+        }
+        vm_wait<MORE ? 2 * L : 0>();                          // the values are there
+        read_v<D, F8>(s, vl);
+        if (MORE) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // ... and read
+            load_v(t0 + UNIT);
+        }
         float p[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) p[j] = mul_rn(st[j / 4][j % 4], sc);
-        if (t0 < lo || t0 + 32 > len) {
+        if (t0 < lo || (!MORE && t0 + 32 > len)) {
             // tokens outside get no weight, and their values, which may be anything (a page's unwritten rows), are zeroed
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -395,7 +438,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
                 const bool in = t >= lo && t < len;
                 p[j] = in ? p[j] : -INFINITY;
 #pragma unroll
-                for (int w = 0; w < Block<D, F8>::VW; w++) s.v[j / 4][j % 4][w] = in ? s.v[j / 4][j % 4][w] : 0;
+                for (int w = 0; w < B::VW; w++) s.v[j / 4][j % 4][w] = in ? s.v[j / 4][j % 4][w] : 0;
             }
         }
         float bm = p[0];
@@ -434,11 +477,20 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
                 o[4 * q + f] = mfma_bf16(vf[f], plo, o[4 * q + f]);
             }
         }
+    };
+    int t0 = begin + 32 * wave;
+    if (t0 < end) {
+        locate(t0);
+        clamp();
+        load_k(t0);
+        load_v(t0);
+        for (; t0 + UNIT < end; t0 += UNIT) block(t0, std::true_type{});
+        block(t0, std::false_type{});
     }
 
     // the four waves' columns, joined: each to the common maximum
     constexpr int LD = D + 4;
-    float* lm = lds + kWaves * 16 * LD;
+    float* lm = reinterpret_cast<float*>(lds + kWaves * B::STAGE);
     float* ll = lm + kWaves * 16;
     l += __shfl_xor(l, 16, kWave);
     l += __shfl_xor(l, 32, kWave);
@@ -446,7 +498,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
         lm[wave * 16 + lane] = m;
         ll[wave * 16 + lane] = l;
     }
-    float* mine = lds + (wave * 16 + col) * LD;
+    float* mine = reinterpret_cast<float*>(stage) + col * LD;
 #pragma unroll
     for (int f = 0; f < F; f++)
 #pragma unroll
@@ -465,7 +517,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
         for (int w = 0; w < kWaves; w++) {
             const float e = __builtin_amdgcn_exp2f(lm[16 * w + h] - ref);
             sum += e * ll[16 * w + h];
-            acc += e * *reinterpret_cast<const v4f*>(lds + (w * 16 + h) * LD + d);
+            acc += e * *reinterpret_cast<const v4f*>(lds + w * B::STAGE + (h * LD + d) * 4);
         }
         if (pl.splits == 1) {
             uint32_t u[4];
@@ -483,76 +535,101 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
     }
 }
 
-// Joins the parts of sequence blockIdx.y, query head blockIdx.x: 256 threads as 1024 / D groups of D / 4, each group
-// every 1024 / D-th part, then the groups in order.
+// Joins the parts of sequence blockIdx.y's query heads hb blockIdx.x ..: groups of D / 4 threads, `share` of them (a power
+// of two, as many as the parts need) to a head, each every share-th part in order, then the groups in order.
 template <int D>
-__global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a) {
-    constexpr int UNIT = 32 * kWaves, TC = D / 4, NG = 256 / TC;
+__global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int hb) {
+    constexpr int TC = D / 4, NG = 256 / TC;
     __shared__ float lds[NG][D + 4];
     __shared__ float red[NG];
-    const int h = blockIdx.x, b = blockIdx.y;
-    const Plan pl = make_plan<UNIT>(a, -1, b);
-    if (pl.b < 0 || pl.splits < 2) return;
-    const int64_t first = (int64_t)pl.first * a.HQ + h;
-    float mm = -INFINITY;
-    for (int i = threadIdx.x & 63; i < pl.splits; i += 64) mm = fmaxf(mm, a.part_ml[2 * (first + (int64_t)i * a.HQ)]);
-    mm = wave_max(mm);
-    const float ref = mm == -INFINITY ? 0.f : mm;
+    const int b = blockIdx.y, n = __ldg(a.n);
+    const int2 pl = a.plan[b];                                // (a row past n has none: not used)
+    if (b >= n || pl.y < 2) return;
     const int c = threadIdx.x % TC, grp = threadIdx.x / TC;
-    v4f acc = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-    for (int i = grp; i < pl.splits; i += NG) {
-        const int64_t at = first + (int64_t)i * a.HQ;
-        const float e = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
-        sum += e * a.part_ml[2 * at + 1];
-        acc += e * *reinterpret_cast<const v4f*>(a.part_o + at * D + 4 * c);
-    }
-    *reinterpret_cast<v4f*>(&lds[grp][4 * c]) = acc;
-    if (c == 0) red[grp] = sum;
-    __syncthreads();
-    if (grp) return;
-    for (int i = 1; i < NG; i++) {
-        acc += *reinterpret_cast<const v4f*>(&lds[i][4 * c]);
-        sum += red[i];
-    }
-    const int hk = h / a.G;
-    const float vs = a.c.v_scale ? __ldg(a.c.v_scale + hk) : 1.f;
-    uint32_t u[4];
+    int share = 2;
+    while (share < NG && share < pl.y) share *= 2;
+    share = min(share, NG);
+    const int heads = NG / share, sub = grp % share;
+    const int hend = min(a.HQ, (int)(blockIdx.x + 1) * hb);
+    for (int h0 = blockIdx.x * hb; h0 < hend; h0 += heads) {
+        const int h = h0 + grp / share;
+        v4f acc = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+        if (h < hend) {
+            const int64_t first = (int64_t)pl.x * a.HQ + h;
+            float mm = -INFINITY;
+            for (int i = c; i < pl.y; i += TC) mm = fmaxf(mm, a.part_ml[2 * (first + (int64_t)i * a.HQ)]);
 #pragma unroll
-    for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(sum == 0.f ? 0.f : div_rn(acc[j], sum) * vs);
-    *reinterpret_cast<v2u*>(a.out + b * a.ldo + h * a.ho_s + 4 * c) = v2u{u[0] | (u[1] << 16), u[2] | (u[3] << 16)};
+            for (int o = TC / 2; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, kWave));
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            for (int i = sub; i < pl.y; i += share) {
+                const int64_t at = first + (int64_t)i * a.HQ;
+                const float e = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
+                sum += e * a.part_ml[2 * at + 1];
+                acc += e * *reinterpret_cast<const v4f*>(a.part_o + at * D + 4 * c);
+            }
+        }
+        *reinterpret_cast<v4f*>(&lds[grp][4 * c]) = acc;
+        if (c == 0) red[grp] = sum;
+        __syncthreads();
+        if (h < hend && sub == 0) {
+            for (int i = 1; i < share; i++) {
+                acc += *reinterpret_cast<const v4f*>(&lds[grp + i][4 * c]);
+                sum += red[grp + i];
+            }
+            const float vs = a.c.v_scale ? __ldg(a.c.v_scale + h / a.G) : 1.f;
+            uint32_t u[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(sum == 0.f ? 0.f : div_rn(acc[j], sum) * vs);
+            *reinterpret_cast<v2u*>(a.out + b * a.ldo + h * a.ho_s + 4 * c) =
+                v2u{u[0] | (u[1] << 16), u[2] | (u[3] << 16)};
+        }
+        __syncthreads();
+    }
 }
 
-// Workgroups that a launch's work is split into, at most (beside one for each further sequence and head).
-constexpr int kTarget = 512;
+// LDS of a workgroup, and the workgroups that a launch's work is split into, at most (beside one for each further sequence
+// and head): as many as the CUs' LDS holds at a time, up to four a CU.  More parts balance ragged batches better and cost
+// the join more: 128 sequences of 100 - 4096 visible tokens, 8 heads of 64, 192 us with two a CU, 172 with four; one
+// sequence of 131071 tokens, 8 heads of 128 bf16 (LDS for two), 100 us with two, 106 with four.
+static int attend_lds(int64_t D, bool f8) {
+    const int64_t stage = 4 * (f8 ? D : 2 * D) / 64 * 1024, o = 16 * (D + 4) * 4;
+    return (int)(kWaves * (stage > o ? stage : o) + 2 * kWaves * 16 * 4);
+}
+static int attend_target(int64_t D, bool f8) {
+    const int fit = 160 * 1024 / attend_lds(D, f8);
+    return 256 * (fit < 4 ? fit : 4);
+}
 
-static int64_t attend_parts(int64_t T, int64_t HT, int64_t cap) {
-    const int64_t unit = 32 * kWaves, most = T * ((cap + unit - 1) / unit);
-    const int64_t split = kTarget / HT + 1 + T;
+// Parts that the grid holds: every sequence at most a part per unit, all together at most the target's share of a head and
+// one more each.
+static int64_t attend_parts(int64_t T, int64_t HT, int64_t cap, int target) {
+    const int64_t unit = 32 * kWaves, most = T * ((cap + unit - 1) / unit), split = target / HT + 1 + T;
     return most < split ? most : split;
 }
 
-// The cache's arguments, checked; strides in elements.
-static int make_cache(Cache& c, void* k, int64_t k_page, int64_t k_tok, int64_t k_head, void* v, int64_t v_page,
-                      int64_t v_tok, int64_t v_head, int e4m3, const float* k_scale, const float* v_scale,
-                      const int32_t* table, int64_t table_ld, int64_t seqs, int64_t cols, int64_t pages, int64_t page,
-                      int64_t HKV, int64_t D) {
-    if (!k || !v || !table || (e4m3 != 0 && e4m3 != 1)) return PRISM_ERR_ARG;
-    if (!e4m3 && (k_scale || v_scale)) return PRISM_ERR_ARG;
-    if (HKV < 1 || HKV > 65536 || (D != 64 && D != 128 && D != 256)) return PRISM_ERR_SHAPE;
-    if (page < 16 || page > 65536 || (page & (page - 1)) || pages < 1 || pages > INT32_MAX) return PRISM_ERR_SHAPE;
-    if (seqs < 1 || seqs > INT32_MAX || cols < 1 || cols > (1 << 27) || table_ld < cols) return PRISM_ERR_SHAPE;
-    const int64_t size = e4m3 ? 1 : 2, unit = 16 / size;
-    if (k_page < 0 || k_tok < 0 || k_head < 0 || v_page < 0 || v_tok < 0 || v_head < 0) return PRISM_ERR_SHAPE;
+// The cache's arguments, checked; strides from elements to bytes.
+static_assert(sizeof(prism_kv_cache) == 19 * 8 && sizeof(prism_kv_append_args) == 41 * 8 &&
+              sizeof(prism_kv_attend_args) == 32 * 8, "8-byte fields throughout");
+
+static int make_cache(Cache& c, const prism_kv_cache& h) {
+    if (!h.k || !h.v || !h.table || (h.e4m3 != 0 && h.e4m3 != 1)) return PRISM_ERR_ARG;
+    if (!h.e4m3 && (h.k_scale || h.v_scale)) return PRISM_ERR_ARG;
+    if (h.heads < 1 || h.heads > 65536 || (h.dim != 64 && h.dim != 128 && h.dim != 256)) return PRISM_ERR_SHAPE;
+    if (h.page < 16 || h.page > 65536 || (h.page & (h.page - 1)) || h.pages < 1 || h.pages > INT32_MAX)
+        return PRISM_ERR_SHAPE;
+    if (h.seqs < 1 || h.seqs > INT32_MAX || h.cols < 1 || h.cols > (1 << 27) || h.table_ld < h.cols) return PRISM_ERR_SHAPE;
+    const int64_t size = h.e4m3 ? 1 : 2, unit = 16 / size;
+    if (h.k_page < 0 || h.k_tok < 0 || h.k_head < 0 || h.v_page < 0 || h.v_tok < 0 || h.v_head < 0) return PRISM_ERR_SHAPE;
     // a token's offset within 16 of them is a 32-bit number of bytes
-    if (k_tok > (1 << 26) || v_tok > (1 << 26)) return PRISM_ERR_SHAPE;
-    if (!PRISM_ALIGNED(k, 16) || !PRISM_ALIGNED(v, 16) || k_page % unit || k_tok % unit || k_head % unit ||
-        v_page % unit || v_tok % unit || v_head % unit)
+    if (h.k_tok > (1 << 26) || h.v_tok > (1 << 26)) return PRISM_ERR_SHAPE;
+    if (!PRISM_ALIGNED(h.k, 16) || !PRISM_ALIGNED(h.v, 16) || h.k_page % unit || h.k_tok % unit || h.k_head % unit ||
+        h.v_page % unit || h.v_tok % unit || h.v_head % unit)
         return PRISM_ERR_ALIGN;
     int shift = 0;
-    while ((1 << shift) < page) shift++;
-    c = Cache{(char*)k, (char*)v, k_page * size, k_tok * size, k_head * size, v_page * size, v_tok * size,
-              v_head * size, k_scale, v_scale, table, table_ld, (int)seqs, (int)cols, (int)pages, shift};
+    while ((1 << shift) < h.page) shift++;
+    c = Cache{(char*)h.k, (char*)h.v, h.k_page * size, h.k_tok * size, h.k_head * size, h.v_page * size, h.v_tok * size,
+              h.v_head * size, h.k_scale, h.v_scale, h.table, h.table_ld, (int)h.seqs, (int)h.cols, (int)h.pages, shift};
     return PRISM_OK;
 }
 
@@ -560,42 +637,40 @@ static int make_cache(Cache& c, void* k, int64_t k_page, int64_t k_tok, int64_t 
 
 using namespace prism;
 
-extern "C" int prism_kv_append(const uint16_t* q, int64_t ldq, int64_t hq_s, const uint16_t* k, int64_t ldk,
-                               int64_t hk_s, const uint16_t* v, int64_t ldv, int64_t hv_s, uint16_t* q_out, int64_t ldo,
-                               int64_t ho_s, const float* rope, int64_t ldr, int64_t rope_rows, int64_t rot,
-                               int adjacent, const int32_t* pos, const int32_t* seq, void* k_cache, int64_t k_page,
-                               int64_t k_tok, int64_t k_head, void* v_cache, int64_t v_page, int64_t v_tok,
-                               int64_t v_head, int e4m3, const float* k_scale, const float* v_scale,
-                               const int32_t* table, int64_t table_ld, int64_t seqs, int64_t cols, int64_t pages,
-                               int64_t page, const int32_t* n_rows, int64_t T, int64_t HQ, int64_t HKV, int64_t D,
-                               void* stream) {
+extern "C" int prism_kv_append(const prism_kv_append_args* args, void* stream) {
+    if (!args) return PRISM_ERR_ARG;
+    const prism_kv_append_args& h = *args;
     AppendArgs a{};
-    const int rc = make_cache(a.c, k_cache, k_page, k_tok, k_head, v_cache, v_page, v_tok, v_head, e4m3, k_scale,
-                              v_scale, table, table_ld, seqs, cols, pages, page, HKV, D);
+    const int rc = make_cache(a.c, h.cache);
     if (rc != PRISM_OK) return rc;
-    if (!k || !v || !pos || !n_rows || (HQ > 0 && (!q || !q_out)) || (rot > 0 && !rope)) return PRISM_ERR_ARG;
-    if (adjacent != 0 && adjacent != 1) return PRISM_ERR_ARG;
-    if (T < 0 || T > INT32_MAX || HQ < 0 || HQ > 65536 || rot < 0 || rot > D || rot % 16) return PRISM_ERR_SHAPE;
-    if (rot > 0 && (ldr < rot || rope_rows < 1)) return PRISM_ERR_SHAPE;
-    if (!PRISM_ALIGNED(k, 16) || !PRISM_ALIGNED(v, 16) || ldk % 8 || hk_s % 8 || ldv % 8 || hv_s % 8)
+    const int64_t D = h.cache.dim, HKV = h.cache.heads;
+    if (!h.k || !h.v || !h.pos || !h.n_rows || (h.hq > 0 && (!h.q || !h.q_out)) || (h.rot > 0 && !h.rope))
+        return PRISM_ERR_ARG;
+    if (h.adjacent != 0 && h.adjacent != 1) return PRISM_ERR_ARG;
+    if (h.T < 0 || h.T > INT32_MAX || h.hq < 0 || h.hq > 65536 || h.rot < 0 || h.rot > D || h.rot % 16)
+        return PRISM_ERR_SHAPE;
+    if (h.rot > 0 && (h.ldr < h.rot || h.rope_rows < 1)) return PRISM_ERR_SHAPE;
+    if (!PRISM_ALIGNED(h.k, 16) || !PRISM_ALIGNED(h.v, 16) || h.k_ld % 8 || h.k_hs % 8 || h.v_ld % 8 || h.v_hs % 8)
         return PRISM_ERR_ALIGN;
-    if (HQ > 0 && (!PRISM_ALIGNED(q, 16) || !PRISM_ALIGNED(q_out, 16) || ldq % 8 || hq_s % 8 || ldo % 8 || ho_s % 8))
+    if (h.hq > 0 && (!PRISM_ALIGNED(h.q, 16) || !PRISM_ALIGNED(h.q_out, 16) || h.q_ld % 8 || h.q_hs % 8 || h.o_ld % 8 ||
+                     h.o_hs % 8))
         return PRISM_ERR_ALIGN;
-    if (rot > 0 && (!PRISM_ALIGNED(rope, 16) || ldr % 4)) return PRISM_ERR_ALIGN;
-    if (T == 0) return PRISM_OK;
-    a.q = q, a.k = k, a.v = v, a.qo = q_out;
-    a.ldq = ldq, a.hq_s = hq_s, a.ldk = ldk, a.hk_s = hk_s, a.ldv = ldv, a.hv_s = hv_s, a.ldo = ldo, a.ho_s = ho_s;
-    a.rope = rope, a.ldr = ldr, a.pos = pos, a.seq = seq, a.n = n_rows;
-    a.rope_rows = (int)(rope_rows < INT32_MAX ? rope_rows : INT32_MAX);
-    a.R = (int)rot, a.adjacent = adjacent, a.HQ = (int)HQ, a.HKV = (int)HKV;
+    if (h.rot > 0 && (!PRISM_ALIGNED(h.rope, 16) || h.ldr % 4)) return PRISM_ERR_ALIGN;
+    if (h.T == 0) return PRISM_OK;
+    a.q = h.q, a.k = h.k, a.v = h.v, a.qo = h.q_out;
+    a.ldq = h.q_ld, a.hq_s = h.q_hs, a.ldk = h.k_ld, a.hk_s = h.k_hs, a.ldv = h.v_ld, a.hv_s = h.v_hs;
+    a.ldo = h.o_ld, a.ho_s = h.o_hs;
+    a.rope = h.rope, a.ldr = h.ldr, a.pos = h.pos, a.seq = h.seq, a.n = h.n_rows;
+    a.rope_rows = (int)(h.rope_rows < INT32_MAX ? h.rope_rows : INT32_MAX);
+    a.R = (int)h.rot, a.adjacent = (int)h.adjacent, a.HQ = (int)h.hq, a.HKV = (int)HKV;
     // whole waves, as few idle lanes as the rows' pieces allow
-    const int64_t items = (HQ + 2 * HKV) * (D / 16), rows = (items + 255) / 256;
+    const int64_t items = (h.hq + 2 * HKV) * (D / 16), rows = (items + 255) / 256;
     const int tpb = (int)(((items + rows - 1) / rows + 63) / 64 * 64);
-    const dim3 grid((unsigned)T, (unsigned)((items + tpb - 1) / tpb));
+    const dim3 grid((unsigned)h.T, (unsigned)((items + tpb - 1) / tpb));
     const hipStream_t st = (hipStream_t)stream;
 #define AP(DD) \
     do { \
-        if (e4m3) hipLaunchKernelGGL((kv_append_kernel<DD, true>), grid, dim3(tpb), 0, st, a); \
+        if (h.cache.e4m3) hipLaunchKernelGGL((kv_append_kernel<DD, true>), grid, dim3(tpb), 0, st, a); \
         else hipLaunchKernelGGL((kv_append_kernel<DD, false>), grid, dim3(tpb), 0, st, a); \
     } while (0)
     if (D == 64) AP(64); else if (D == 128) AP(128); else AP(256);
@@ -604,65 +679,67 @@ extern "C" int prism_kv_append(const uint16_t* q, int64_t ldq, int64_t hq_s, con
     return PRISM_OK;
 }
 
-static int64_t attend_bytes(int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t cap) {
-    const int64_t G = HQ / HKV, HT = HKV * ((G + 15) / 16);
-    return attend_parts(T, HT, cap) * HQ * (D + 2) * 4;
-}
-
-extern "C" int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t HQ, int64_t HKV, int64_t D, int64_t cols,
+extern "C" int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t hq, int64_t heads, int64_t dim, int64_t cols,
                                                    int64_t page) {
-    if (T < 1 || HKV < 1 || HQ < HKV || HQ % HKV || D < 1 || cols < 1 || page < 1) return 0;
+    if (T < 1 || heads < 1 || hq < heads || hq % heads || dim < 1 || cols < 1 || page < 1) return 0;
     if (cols * page <= 32 * kWaves) return 0;                // one unit: nothing to join
-    return attend_bytes(T, HQ, HKV, D, cols * page);
+    // (the most parts that either cache type takes)
+    return attend_parts(T, heads * ((hq / heads + 15) / 16), cols * page, 4 * 256) * hq * (dim + 2) * 4 + T * 8;
 }
 
-extern "C" int prism_kv_attend(const uint16_t* q, int64_t ldq, int64_t hq_s, const void* k_cache, int64_t k_page,
-                               int64_t k_tok, int64_t k_head, const void* v_cache, int64_t v_page, int64_t v_tok,
-                               int64_t v_head, int e4m3, const float* k_scale, const float* v_scale,
-                               const int32_t* table, int64_t table_ld, int64_t cols, int64_t pages, int64_t page,
-                               const int32_t* lens, uint16_t* out, int64_t ldo, int64_t ho_s, const int32_t* n_rows,
-                               int64_t T, int64_t HQ, int64_t HKV, int64_t D, float scale, int64_t window, void* ws,
-                               int64_t ws_bytes, void* stream) {
-    AttendArgs a{};
+extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
+    if (!args) return PRISM_ERR_ARG;
+    const prism_kv_attend_args& h = *args;
+    const int64_t T = h.cache.seqs, HQ = h.hq, HKV = h.cache.heads, D = h.cache.dim, cols = h.cache.cols;
     if (T < 0 || T > 65535) return PRISM_ERR_SHAPE;
-    const int rc = make_cache(a.c, const_cast<void*>(k_cache), k_page, k_tok, k_head, const_cast<void*>(v_cache), v_page,
-                              v_tok, v_head, e4m3, k_scale, v_scale, table, table_ld, T > 0 ? T : 1, cols, pages, page,
-                              HKV, D);
+    AttendArgs a{};
+    prism_kv_cache hc = h.cache;
+    hc.seqs = T > 0 ? T : 1;
+    const int rc = make_cache(a.c, hc);
     if (rc != PRISM_OK) return rc;
-    if (!q || !lens || !out || !n_rows) return PRISM_ERR_ARG;
-    if (HQ < HKV || HQ % HKV || HQ > 65535 || window < 0 || cols * page > INT32_MAX - 65536) return PRISM_ERR_SHAPE;
-    if (!PRISM_ALIGNED(q, 16) || !PRISM_ALIGNED(out, 8) || ldq % 8 || hq_s % 8 || ldo % 4 || ho_s % 4)
+    if (!h.q || !h.lens || !h.out || !h.n_rows) return PRISM_ERR_ARG;
+    if (HQ < HKV || HQ % HKV || HQ > 65535 || h.window < 0 || cols * hc.page > INT32_MAX - 65536) return PRISM_ERR_SHAPE;
+    if (!PRISM_ALIGNED(h.q, 16) || !PRISM_ALIGNED(h.out, 8) || h.q_ld % 8 || h.q_hs % 8 || h.o_ld % 4 || h.o_hs % 4)
         return PRISM_ERR_ALIGN;
-    const int64_t need = prism_kv_attend_workspace_bytes(T, HQ, HKV, D, cols, page);
-    if (T > 0 && need > 0 && (!ws || ws_bytes < need)) return PRISM_ERR_ARG;
-    if (need > 0 && !PRISM_ALIGNED(ws, 16)) return PRISM_ERR_ALIGN;
+    const int64_t need = prism_kv_attend_workspace_bytes(T, HQ, HKV, D, cols, hc.page);
+    if (need > 0 && (!h.ws || h.ws_bytes < need)) return PRISM_ERR_ARG;
+    if (need > 0 && !PRISM_ALIGNED(h.ws, 16)) return PRISM_ERR_ALIGN;
     if (T == 0) return PRISM_OK;
     const int64_t G = HQ / HKV, tiles = (G + 15) / 16, HT = HKV * tiles;
-    const int64_t parts = attend_parts(T, HT, cols * page);
-    if (parts * HT > INT32_MAX) return PRISM_ERR_SHAPE;
-    a.q = q, a.out = out, a.ldq = ldq, a.hq_s = hq_s, a.ldo = ldo, a.ho_s = ho_s, a.lens = lens, a.n = n_rows;
-    a.part_o = (float*)ws;
-    a.part_ml = (float*)ws + parts * HQ * D;
-    a.scale = scale * 1.44269504088896340736f;
-    a.T = (int)T, a.HQ = (int)HQ, a.G = (int)G, a.tiles = (int)tiles, a.HT = (int)HT, a.target = kTarget;
-    a.window = (int)(window < INT32_MAX ? window : 0);
+    const bool f8 = hc.e4m3 != 0;
+    a.target = attend_target(D, f8);
+    const int64_t parts = attend_parts(T, HT, cols * hc.page, a.target), grid = (parts + 7) / 8 * 8 * HT;
+    if (grid > INT32_MAX) return PRISM_ERR_SHAPE;
+    a.q = h.q, a.out = h.out, a.ldq = h.q_ld, a.hq_s = h.q_hs, a.ldo = h.o_ld, a.ho_s = h.o_hs;
+    a.lens = h.lens, a.n = h.n_rows;
+    if (need > 0) {
+        a.part_o = (float*)h.ws;
+        a.part_ml = (float*)h.ws + parts * HQ * D;
+        a.plan = (int2*)((float*)h.ws + parts * HQ * (D + 2));
+    }
+    a.scale = (float)h.scale * 1.44269504088896340736f;
+    a.T = (int)T, a.HQ = (int)HQ, a.G = (int)G, a.tiles = (int)tiles, a.HT = (int)HT;
+    a.window = (int)(h.window < INT32_MAX ? h.window : 0);
     const hipStream_t st = (hipStream_t)stream;
-    const size_t lds = (size_t)(kWaves * 16 * (D + 4) + 2 * kWaves * 16) * 4;
 #define AT(DD, F8) \
     do { \
+        static_assert(Block<DD, F8>::STAGE % 16 == 0, "LDS alignment"); \
+        const int lds = attend_lds(DD, F8); \
         allow_lds(kv_attend_kernel<DD, F8>, lds); \
-        hipLaunchKernelGGL((kv_attend_kernel<DD, F8>), dim3((unsigned)(parts * HT)), dim3(256), lds, st, a); \
+        hipLaunchKernelGGL((kv_attend_kernel<DD, F8>), dim3((unsigned)grid), dim3(256), lds, st, a); \
     } while (0)
-    if (D == 64) { if (e4m3) AT(64, true); else AT(64, false); }
-    else if (D == 128) { if (e4m3) AT(128, true); else AT(128, false); }
-    else { if (e4m3) AT(256, true); else AT(256, false); }
+    if (D == 64) { if (f8) AT(64, true); else AT(64, false); }
+    else if (D == 128) { if (f8) AT(128, true); else AT(128, false); }
+    else { if (f8) AT(256, true); else AT(256, false); }
 #undef AT
     PRISM_LAUNCH_CHECK();
     if (need > 0) {
-        const dim3 grid((unsigned)HQ, (unsigned)T);
-        if (D == 64) hipLaunchKernelGGL(kv_join_kernel<64>, grid, dim3(256), 0, st, a);
-        else if (D == 128) hipLaunchKernelGGL(kv_join_kernel<128>, grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL(kv_join_kernel<256>, grid, dim3(256), 0, st, a);
+        // a workgroup per head while there are few (long sequences have many parts), else one for as many as it has groups
+        const int hb = T * HQ <= 1024 ? 1 : (int)(1024 / D);
+        const dim3 jg((unsigned)((HQ + hb - 1) / hb), (unsigned)T);
+        if (D == 64) hipLaunchKernelGGL(kv_join_kernel<64>, jg, dim3(256), 0, st, a, hb);
+        else if (D == 128) hipLaunchKernelGGL(kv_join_kernel<128>, jg, dim3(256), 0, st, a, hb);
+        else hipLaunchKernelGGL(kv_join_kernel<256>, jg, dim3(256), 0, st, a, hb);
         PRISM_LAUNCH_CHECK();
     }
     return PRISM_OK;

@@ -13,10 +13,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libprism_am
 
 _i64, _p, _int = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
 
-# the paged cache's arguments (both tensors with their page, token and head strides, e4m3, the scales) and the delta
-# rule's (q, k, v, g, beta, state, out with their strides)
-_CACHE = [_p, _i64, _i64, _i64] * 2 + [_int, _p, _p]
-_DELTA = [_p, _i64, _i64] * 3 + [_p, _i64] * 2 + [_p, _i64, _i64, _p] + [_p, _i64, _i64]
+_args = ctypes.c_char_p                     # a struct of 8-byte fields, packed by struct.Struct into bytes
 
 _SIGS = {
     "prism_version": (_int, []),
@@ -59,13 +56,11 @@ _SIGS = {
     "prism_mxfp4_gemm": (_int, [_p, _p, _int, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _int, _int, _p]),
     "prism_mxfp4_gemm_ws": (_int, [_p, _p, _int, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _int, _int, _p, _i64, _p]),
     "prism_mxfp4_split_workspace_bytes": (_i64, [_i64, _i64]),
-    "prism_kv_append": (_int, [_p, _i64, _i64] * 4 + [_p, _i64, _i64, _i64, _int, _p, _p] + _CACHE
-                        + [_p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p]),
-    "prism_kv_attend": (_int, [_p, _i64, _i64] + _CACHE + [_p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64,
-                                                           _i64, _i64, ctypes.c_float, _i64, _p, _i64, _p]),
+    "prism_kv_append": (_int, [_args, _p]),
+    "prism_kv_attend": (_int, [_args, _p]),
     "prism_kv_attend_workspace_bytes": (_i64, [_i64] * 6),
-    "prism_delta_step": (_int, _DELTA + [_p] + [_i64] * 5 + [_int, ctypes.c_float, ctypes.c_float, _p]),
-    "prism_delta_prefill": (_int, _DELTA + [_p] + [_i64] * 6 + [_int, ctypes.c_float, ctypes.c_float, _p, _i64, _p]),
+    "prism_delta_step": (_int, [_args, _p]),
+    "prism_delta_prefill": (_int, [_args, _p]),
     "prism_delta_prefill_workspace_bytes": (_i64, [_i64] * 6),
 }
 

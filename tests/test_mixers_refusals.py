@@ -17,12 +17,33 @@ def lib():
     return L.lib()
 
 
+def packed(layout, *fields):
+    return layout.pack(*(0 if f is None else f for f in fields))
+
+
+def test_packed_layouts_match_the_header():
+    """The Python layer packs as many 8-byte fields as the header's structs declare."""
+    import re
+    from prism_amd import delta, kv
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "prism_amd.h")).read()
+    count = {}
+    for body, name in re.findall(r"typedef struct \{(.*?)\} (prism_\w+);", src, re.S):
+        count[name] = sum(count["prism_kv_cache"] if f.split()[0] == "prism_kv_cache" else len(f.split(","))
+                          for f in body.split(";") if f.strip())
+    for layout, name in ((kv._APPEND, "prism_kv_append_args"), (kv._ATTEND, "prism_kv_attend_args"),
+                         (delta._ARGS, "prism_delta_args")):
+        assert layout.size == 8 * count[name], name
+
+
 def test_append_codes(lib):
+    from prism_amd import kv
+
     def call(q=P, k=P, rope=P, rot=64, ldr=64, adjacent=0, pos=P, kc=P, tok=128, e4m3=0, ks=None, cols=4, pages=8,
              page=16, T=1, HQ=2, D=64, ldk=128, qo=P):
-        return lib.prism_kv_append(q, 256, 64, k, ldk, 64, P, 128, 64, qo, 128, 64, rope, ldr, 100, rot, adjacent, pos,
-                                   None, kc, 4096, tok, 64, P, 4096, tok, 64, e4m3, ks, None, P, 4, 2, cols, pages, page,
-                                   P, T, HQ, 2, D, None)
+        return lib.prism_kv_append(packed(
+            kv._APPEND, kc, 4096, tok, 64, P, 4096, tok, 64, e4m3, ks, None, P, 4, 2, cols, pages, page, 2, D,
+            q, 256, 64, k, ldk, 64, P, 128, 64, qo, 128, 64, rope, ldr, 100, rot, adjacent, pos, None, P, T, HQ), None)
+    assert lib.prism_kv_append(None, None) == ARG
     assert call(T=0) == OK and call(T=0, HQ=0, q=None, qo=None) == OK and call(T=0, rot=0, rope=None, ldr=0) == OK
     assert call(k=None) == ARG and call(q=None) == ARG and call(rope=None) == ARG and call(pos=None) == ARG
     assert call(adjacent=2) == ARG and call(e4m3=2) == ARG and call(ks=P) == ARG      # a bf16 cache has no scales
@@ -34,9 +55,13 @@ def test_append_codes(lib):
 
 
 def test_attend_codes(lib):
+    from prism_amd import kv
+
     def call(q=P, lens=P, out=P, T=1, HQ=4, D=64, window=0, ws=P, ws_bytes=1 << 20, cols=16, page=16, ldq=256, ldo=256):
-        return lib.prism_kv_attend(q, ldq, 64, P, 4096, 128, 64, P, 4096, 128, 64, 0, None, None, P, cols, cols, 8, page,
-                                   lens, out, ldo, 64, P, T, HQ, 2, D, 0.125, window, ws, ws_bytes, None)
+        return lib.prism_kv_attend(packed(
+            kv._ATTEND, P, 4096, 128, 64, P, 4096, 128, 64, 0, None, None, P, cols, T, cols, 8, page, 2, D,
+            q, ldq, 64, out, ldo, 64, lens, P, HQ, window, 0.125, ws, ws_bytes), None)
+    assert lib.prism_kv_attend(None, None) == ARG
     assert call(T=0) == OK
     assert call(q=None) == ARG and call(lens=None) == ARG and call(ws=None) == ARG and call(ws_bytes=64) == ARG
     assert call(HQ=3) == SHAPE and call(HQ=0) == SHAPE and call(D=32) == SHAPE and call(window=-1) == SHAPE
@@ -49,18 +74,27 @@ def test_attend_codes(lib):
 
 
 def test_delta_codes(lib):
-    def call(q=P, state=P, n=P, T=1, HK=2, HV=4, DK=128, DV=128, norm=1, nslots=2, stride=None, ldv=512, fn="step"):
-        a = (q, 256, 128, P, 256, 128, P, ldv, 128, P, 4, P, 4, state, HV * DK * DV if stride is None else stride, nslots,
-             None, P, 512, 128, n)
-        if fn == "step":
-            return lib.prism_delta_step(*a, T, HK, HV, DK, DV, norm, 1.0, 1e-6, None)
-        return lib.prism_delta_prefill(*a, 1, T, HK, HV, DK, DV, norm, 1.0, 1e-6, None, 0, None)
+    from prism_amd import delta
+
+    def call(q=P, state=P, n=P, T=1, HK=2, HV=4, DK=128, DV=128, norm=1, nslots=2, stride=None, ldv=512, fn="step", seqs=1,
+             ws=None, ws_bytes=0):
+        return getattr(lib, "prism_delta_" + fn)(packed(
+            delta._ARGS, q, 256, 128, P, 256, 128, P, ldv, 128, P, 4, P, 4, state, HV * DK * DV if stride is None else stride,
+            nslots, None, P, 512, 128, n, seqs, T, HK, HV, DK, DV, norm, 1.0, 1e-6, ws, ws_bytes), None)
     for fn in ("step", "prefill"):
+        assert getattr(lib, "prism_delta_" + fn)(None, None) == ARG
         assert call(T=0, fn=fn) == OK
         assert call(q=None, fn=fn) == ARG and call(n=None, fn=fn) == ARG and call(norm=2, fn=fn) == ARG
         assert call(DK=96, fn=fn) == SHAPE and call(DV=256, fn=fn) == SHAPE and call(HV=5, fn=fn) == SHAPE
         assert call(HK=0, fn=fn) == SHAPE and call(T=-1, fn=fn) == SHAPE and call(stride=100, fn=fn) == SHAPE
+        assert call(ldv=(1 << 24) + 8, fn=fn) == SHAPE
         assert call(q=U, fn=fn) == ALIGN and call(state=U, fn=fn) == ALIGN and call(ldv=516, fn=fn) == ALIGN
+    b = lib.prism_delta_prefill_workspace_bytes
+    need = b(1000, 1, 2, 4, 128, 128)
+    assert need > 0 and b(1, 1, 2, 4, 128, 128) == 0 and b(1000, 1, 2, 4, 96, 128) == 0 and b(0, 1, 2, 4, 128, 128) == 0
+    assert call(fn="prefill", T=1000) == ARG and call(fn="prefill", T=1000, ws=P, ws_bytes=need - 1) == ARG
+    assert call(fn="prefill", T=1000, ws=U, ws_bytes=need) == ALIGN
+    assert call(fn="prefill", T=1000, seqs=-1) == SHAPE and call(fn="prefill", T=1000, seqs=0) == OK
 
 
 def _i32(*shape):
