@@ -149,16 +149,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // rounding is the only one that shows; the second MFMA is free beside the cache's bytes.
 //
 // Work is split on the device, from the lengths (a captured launch serves every batch): a unit is what the four waves
-// take in one round; `per` units to a workgroup bring the batch to about `target` workgroups; a sequence gets
-// max(1, ceil(units / per)) of them, shared evenly.  Sequences with one workgroup write their output; the others'
-// parts are joined by a second kernel in a fixed order, so results do not depend on timing.
+// take in one round (128 tokens); laid one after the other, the sequences' units are dealt out `per` to a workgroup, so
+// that `target` of them share all the work evenly, whatever the lengths.  A sequence within one workgroup gets its output
+// at once; the others' parts are joined by a second kernel in a fixed order, so results do not depend on timing.
 struct AttendArgs {
     const uint16_t* q;
     uint16_t* out;
     int64_t ldq, hq_s, ldo, ho_s;
     const int32_t *lens, *n;
-    float* part_o;                                            // [P, HQ, D]
-    float* part_ml;                                           // [P, HQ, 2]
+    float* part_o;                                            // [2 P, HQ, D]: two parts a workgroup
+    float* part_ml;                                           // [2 P, HQ, 2]
     int2* plan;                                               // [T]: a sequence's first part and how many it has
     float scale;                                              // times log2 e
     int T, HQ, G, tiles, HT, window, target;
@@ -166,10 +166,6 @@ struct AttendArgs {
 };
 
 constexpr int kWaves = 4;
-
-struct Plan {
-    int b, lo, len, begin, end, split, splits, first;         // first: index of the sequence's first part
-};
 
 template <int UNIT>
 __device__ __forceinline__ int vis_units(const AttendArgs& a, int len, int* lo_out, int* len_out) {
@@ -189,53 +185,44 @@ __device__ __forceinline__ long long wave_sum(long long v) {
     return v;
 }
 
-// Work of part p (b < 0: none); the same in every lane.
+// Where workgroup p's units begin: unit u = p per of all sequences' one after the other (a sequence without tokens has one,
+// for its zeros) lies in sequence b, `off` units from its start; `left` units to do.  The same in every lane; b < 0: none.
+struct Plan {
+    int b, off, left, per;
+};
 template <int UNIT>
 __device__ __forceinline__ Plan make_plan(const AttendArgs& a, int p) {
     const int lane = threadIdx.x & 63;
     const int n = min(__ldg(a.n), a.T);
     int lo, len;
     long long sum = 0;
-    for (int b = lane; b < n; b += 64) sum += vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len);
+    for (int b = lane; b < n; b += 64) sum += max(1, vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len));
     const long long total = wave_sum(sum);
-    const int per = max((int)((total * a.HT + a.target - 1) / a.target), 1);
-    int base = 0;
     Plan r;
     r.b = -1;
+    r.per = max((int)((total * a.HT + a.target - 1) / a.target), 1);
+    const long long u = (long long)p * r.per;
+    if (u >= total) return r;
+    r.left = (int)min((long long)r.per, total - u);
+    long long base = 0;
     for (int b0 = 0; b0 < n; b0 += 64) {
         const int b = b0 + lane;
-        int units = 0, nb = 0;
-        lo = len = 0;
-        if (b < n) {
-            units = vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len);
-            nb = max(1, (units + per - 1) / per);
-        }
-        int incl = nb;
+        const int units = b < n ? max(1, vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len)) : 0;
+        long long incl = units;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(incl, o, kWave);
+            const long long up = __shfl_up(incl, o, kWave);
             if (lane >= o) incl += up;
         }
-        const int tot = __shfl(incl, 63, kWave);
-        const int mine = base + incl - nb;                    // first part of this lane's sequence
-        const bool hit = nb > 0 && p >= mine && p < mine + nb;
-        const uint64_t m = __ballot(hit);
+        const long long at = u - (base + incl - units);       // from the start of this lane's sequence
+        const uint64_t m = __ballot(at >= 0 && at < units);
         if (m) {
             const int src = __builtin_ctzll(m);
-            const int u = __shfl(units, src, kWave), k = __shfl(nb, src, kWave);
             r.b = b0 + src;
-            r.lo = __shfl(lo, src, kWave);
-            r.len = __shfl(len, src, kWave);
-            r.first = __shfl(mine, src, kWave);
-            r.splits = k;
-            r.split = p - r.first;
-            const int each = u / k, more = u % k;             // the first `more` parts take one unit more
-            const int ub = r.split * each + min(r.split, more);
-            r.begin = (r.lo & ~15) + ub * UNIT;
-            r.end = min(r.len, (int)min((int64_t)r.begin + (int64_t)(each + (r.split < more)) * UNIT, (int64_t)INT32_MAX));
+            r.off = __shfl((int)at, src, kWave);
             break;
         }
-        base += tot;
+        base += __shfl(incl, 63, kWave);
     }
     return r;
 }
@@ -331,207 +318,220 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
     const int ht = blockIdx.x / 8 % a.HT, part = blockIdx.x / (8 * a.HT) * 8 + blockIdx.x % 8;
     const Plan pl = make_plan<UNIT>(a, part);
     if (pl.b < 0) return;
-    if (a.plan && ht == 0 && pl.split == 0 && threadIdx.x == 0) a.plan[pl.b] = int2{pl.first, pl.splits};
     const int hk = ht / a.tiles, tile = ht % a.tiles;
     const int h0 = hk * a.G + 16 * tile, nh = min(16, a.G - 16 * tile);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int b = __builtin_amdgcn_readfirstlane(pl.b), len = __builtin_amdgcn_readfirstlane(pl.len);
-    const int lo = __builtin_amdgcn_readfirstlane(pl.lo), end = __builtin_amdgcn_readfirstlane(pl.end);
-    const int begin = __builtin_amdgcn_readfirstlane(pl.begin);
+    int b = __builtin_amdgcn_readfirstlane(pl.b), off = __builtin_amdgcn_readfirstlane(pl.off);
+    int left = __builtin_amdgcn_readfirstlane(pl.left);
+    for (;;) {                                                // a sequence, or as much of it as is this workgroup's
+        int lo, len;
+        const int units = max(1, vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len)), seg = min(left, units - off);
+        const int begin = (lo & ~15) + off * UNIT;
+        const int end = seg == units - off ? len : begin + seg * UNIT;
+        const bool whole = seg == units;
 
-    v4u qf[QF];                                               // heads past the tile: zeros
+        v4u qf[QF];                                               // heads past the tile: zeros
 #pragma unroll
-    for (int i = 0; i < QF; i++) {
-        const int d = F8 ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
-        qf[i] = col < nh ? *reinterpret_cast<const v4u*>(a.q + b * a.ldq + (h0 + col) * a.hq_s + d) : v4u{0, 0, 0, 0};
-    }
-    const float sc = a.scale * (F8 && a.c.k_scale ? __ldg(a.c.k_scale + hk) : 1.f);
-
-    v4f o[F];
-#pragma unroll
-    for (int f = 0; f < F; f++) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-
-    // the table through the scalar cache: a vector load would be waited for together with the values in flight before it
-    const auto* row = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
-        reinterpret_cast<uintptr_t>(a.c.table + b * a.c.table_ld));
-    const int last = len > 0 ? (len - 1) & ~15 : 0;           // the last 16 tokens that are there
-    // Keys and values go to LDS by DMA, 1 KB a load.  Keys: 16 tokens x 64 bytes, four neighbouring lanes a token's (the
-    // memory pipeline merges neighbouring lanes only), placed so that operand order reads without bank conflicts; values:
-    // whole rows.  Every wait on them is written out: the compiler would wait for all of them at each use.
-    const uint32_t koff = (uint32_t)((lane >> 2) * a.c.k_tok) + 16 * ((lane & 3) ^ lds_turn(lane >> 4));
-    const uint32_t voff = (uint32_t)(16 * lane / B::RB * a.c.v_tok) + 16 * lane % B::RB;
-    const char* kb = a.c.k + hk * a.c.k_head;
-    const char* vb = a.c.v + hk * a.c.v_head;
-    char* stage = lds + wave * B::STAGE;
-    const v4u* kl = reinterpret_cast<const v4u*>(stage) + 4 * col + (g ^ lds_turn(col >> 2));
-    const char* vl = stage + 2 * L * 1024 + 4 * g * B::RB + (D == 256 && !F8 ? 16 : B::VB) * col;
-
-    int64_t page[2];
-    auto locate = [&](int t0) {
-#pragma unroll
-        for (int x = 0; x < 2; x++) page[x] = row[min(t0 + 16 * x, last) >> a.c.shift];   // 16 tokens never cross a page
-    };
-    auto clamp = [&] {
-#pragma unroll
-        for (int x = 0; x < 2; x++) page[x] = min(max((int)page[x], 0), a.c.pages - 1);
-    };
-    auto at = [&](int t0, int x) { return (int64_t)(min(t0 + 16 * x, last) & ((1 << a.c.shift) - 1)); };
-    auto load_k = [&](int t0) {
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const char* p = kb + page[x] * a.c.k_page + at(t0, x) * a.c.k_tok + koff;
-#pragma unroll
-            for (int i = 0; i < L; i++) dma16(p + 64 * i, stage + (x * L + i) * 1024);
+        for (int i = 0; i < QF; i++) {
+            const int d = F8 ? 64 * (i / 2) + 16 * g + 8 * (i % 2) : 32 * i + 8 * g;
+            qf[i] = col < nh ? *reinterpret_cast<const v4u*>(a.q + b * a.ldq + (h0 + col) * a.hq_s + d) : v4u{0, 0, 0, 0};
         }
-    };
-    auto load_v = [&](int t0) {
+        const float sc = a.scale * (F8 && a.c.k_scale ? __ldg(a.c.k_scale + hk) : 1.f);
+
+        v4f o[F];
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            const char* p = vb + page[x] * a.c.v_page + at(t0, x) * a.c.v_tok + voff;
+        for (int f = 0; f < F; f++) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+
+        // the table through the scalar cache: a vector load would be waited for together with the values in flight before it
+        const auto* row = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
+            reinterpret_cast<uintptr_t>(a.c.table + b * a.c.table_ld));
+        const int last = len > 0 ? (len - 1) & ~15 : 0;           // the last 16 tokens that are there
+        // Keys and values go to LDS by DMA, 1 KB a load.  Keys: 16 tokens x 64 bytes, four neighbouring lanes a token's (the
+        // memory pipeline merges neighbouring lanes only), placed so that operand order reads without bank conflicts; values:
+        // whole rows.  Every wait on them is written out: the compiler would wait for all of them at each use.
+        const uint32_t koff = (uint32_t)((lane >> 2) * a.c.k_tok) + 16 * ((lane & 3) ^ lds_turn(lane >> 4));
+        const uint32_t voff = (uint32_t)(16 * lane / B::RB * a.c.v_tok) + 16 * lane % B::RB;
+        const char* kb = a.c.k + hk * a.c.k_head;
+        const char* vb = a.c.v + hk * a.c.v_head;
+        char* stage = lds + wave * B::STAGE;
+        const v4u* kl = reinterpret_cast<const v4u*>(stage) + 4 * col + (g ^ lds_turn(col >> 2));
+        const char* vl = stage + 2 * L * 1024 + 4 * g * B::RB + (D == 256 && !F8 ? 16 : B::VB) * col;
+
+        int64_t page[2];
+        auto locate = [&](int t0) {
 #pragma unroll
-            for (int i = 0; i < L; i++) dma16(p + i * (1024 / B::RB) * a.c.v_tok, stage + (2 * L + x * L + i) * 1024);
-        }
-    };
-    B s;
-    // One block of 32 tokens; with `more`, the next one's loads go out as this one's places in LDS become free.
-    auto block = [&](int t0, auto more) {
-        constexpr bool MORE = decltype(more)::value;
-        vm_wait<2 * L>();                                     // the keys are there (the values' loads came after theirs)
-        if (MORE) locate(t0 + UNIT);
-        v4f st[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+            for (int x = 0; x < 2; x++) page[x] = row[min(t0 + 16 * x, last) >> a.c.shift];   // 16 tokens never cross a page
+        };
+        auto clamp = [&] {
 #pragma unroll
-        for (int x = 0; x < 2; x++)
+            for (int x = 0; x < 2; x++) page[x] = min(max((int)page[x], 0), a.c.pages - 1);
+        };
+        auto at = [&](int t0, int x) { return (int64_t)(min(t0 + 16 * x, last) & ((1 << a.c.shift) - 1)); };
+        auto load_k = [&](int t0) {
 #pragma unroll
-            for (int i = 0; i < QF; i++) {
-                v4u kf;
-                if constexpr (F8) {
-                    const v4u w = kl[(x * L + i / 2) * 64];
-                    const uint32_t w0 = w[2 * (i % 2)], w1 = w[2 * (i % 2) + 1];
-                    kf = v4u{e4m3x2_bf16<false>(w0), e4m3x2_bf16<true>(w0), e4m3x2_bf16<false>(w1),
-                             e4m3x2_bf16<true>(w1)};
-                } else {
-                    kf = kl[(x * L + i) * 64];
+            for (int x = 0; x < 2; x++) {
+                const char* p = kb + page[x] * a.c.k_page + at(t0, x) * a.c.k_tok + koff;
+#pragma unroll
+                for (int i = 0; i < L; i++) dma16(p + 64 * i, stage + (x * L + i) * 1024);
+            }
+        };
+        auto load_v = [&](int t0) {
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const char* p = vb + page[x] * a.c.v_page + at(t0, x) * a.c.v_tok + voff;
+#pragma unroll
+                for (int i = 0; i < L; i++) dma16(p + i * (1024 / B::RB) * a.c.v_tok, stage + (2 * L + x * L + i) * 1024);
+            }
+        };
+        B s;
+        // One block of 32 tokens; with `more`, the next one's loads go out as this one's places in LDS become free.
+        auto block = [&](int t0, auto more) {
+            constexpr bool MORE = decltype(more)::value;
+            vm_wait<2 * L>();                                     // the keys are there (the values' loads came after theirs)
+            if (MORE) locate(t0 + UNIT);
+            v4f st[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int i = 0; i < QF; i++) {
+                    v4u kf;
+                    if constexpr (F8) {
+                        const v4u w = kl[(x * L + i / 2) * 64];
+                        const uint32_t w0 = w[2 * (i % 2)], w1 = w[2 * (i % 2) + 1];
+                        kf = v4u{e4m3x2_bf16<false>(w0), e4m3x2_bf16<true>(w0), e4m3x2_bf16<false>(w1),
+                                 e4m3x2_bf16<true>(w1)};
+                    } else {
+                        kf = kl[(x * L + i) * 64];
+                    }
+                    st[x] = mfma_bf16(kf, qf[i], st[x]);
                 }
-                st[x] = mfma_bf16(kf, qf[i], st[x]);
+            if (MORE) {
+                clamp();
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this block's keys are read
+                load_k(t0 + UNIT);
             }
-        if (MORE) {
+            vm_wait<MORE ? 2 * L : 0>();                          // the values are there
+            read_v<D, F8>(s, vl);
+            if (MORE) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // ... and read
+                load_v(t0 + UNIT);
+            }
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) p[j] = mul_rn(st[j / 4][j % 4], sc);
+            if (t0 < lo || (!MORE && t0 + 32 > len)) {
+                // tokens outside get no weight, and their values, which may be anything (a page's unwritten rows), are zeroed
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int t = t0 + 16 * (j / 4) + 4 * g + j % 4;
+                    const bool in = t >= lo && t < len;
+                    p[j] = in ? p[j] : -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < B::VW; w++) s.v[j / 4][j % 4][w] = in ? s.v[j / 4][j % 4][w] : 0;
+                }
+            }
+            float bm = p[0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) bm = fmaxf(bm, p[j]);
+            bm = fmaxf(bm, __shfl_xor(bm, 16, kWave));
+            bm = fmaxf(bm, __shfl_xor(bm, 32, kWave));
+            const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.f : mn;
+            if (__any(mn > m)) {
+                const float al = __builtin_amdgcn_exp2f(m - ref);
+                l *= al;
+#pragma unroll
+                for (int f = 0; f < F; f++) o[f] *= al;
+            }
+            m = mn;
+            uint32_t hi[4], lw[4];
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float e0 = __builtin_amdgcn_exp2f(p[2 * w] - ref), e1 = __builtin_amdgcn_exp2f(p[2 * w + 1] - ref);
+                l += e0 + e1;
+                // the upper part strictly below the weight, so that the rest of a weight is never 0 (0 times an infinite
+                // value would be NaN, not infinite)
+                const uint32_t b0 = max(__float_as_uint(e0), 1u) - 1u, b1 = max(__float_as_uint(e1), 1u) - 1u;
+                hi[w] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+                const float r0 = e0 - __uint_as_float(b0 & 0xffff0000u), r1 = e1 - __uint_as_float(b1 & 0xffff0000u);
+                lw[w] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+            }
+            const v4u ph = {hi[0], hi[1], hi[2], hi[3]}, plo = {lw[0], lw[1], lw[2], lw[3]};
+#pragma unroll
+            for (int q = 0; q < F / 4; q++) {
+                v4u vf[4];
+                turn_v<D, F8>(s, q, vf);
+#pragma unroll
+                for (int f = 0; f < 4; f++) {
+                    o[4 * q + f] = mfma_bf16(vf[f], ph, o[4 * q + f]);
+                    o[4 * q + f] = mfma_bf16(vf[f], plo, o[4 * q + f]);
+                }
+            }
+        };
+        int t0 = begin + 32 * wave;
+        if (t0 < end) {
+            locate(t0);
             clamp();
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this block's keys are read
-            load_k(t0 + UNIT);
+            load_k(t0);
+            load_v(t0);
+            for (; t0 + UNIT < end; t0 += UNIT) block(t0, std::true_type{});
+            block(t0, std::false_type{});
         }
-        vm_wait<MORE ? 2 * L : 0>();                          // the values are there
-        read_v<D, F8>(s, vl);
-        if (MORE) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // ... and read
-            load_v(t0 + UNIT);
-        }
-        float p[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) p[j] = mul_rn(st[j / 4][j % 4], sc);
-        if (t0 < lo || (!MORE && t0 + 32 > len)) {
-            // tokens outside get no weight, and their values, which may be anything (a page's unwritten rows), are zeroed
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int t = t0 + 16 * (j / 4) + 4 * g + j % 4;
-                const bool in = t >= lo && t < len;
-                p[j] = in ? p[j] : -INFINITY;
-#pragma unroll
-                for (int w = 0; w < B::VW; w++) s.v[j / 4][j % 4][w] = in ? s.v[j / 4][j % 4][w] : 0;
-            }
-        }
-        float bm = p[0];
-#pragma unroll
-        for (int j = 1; j < 8; j++) bm = fmaxf(bm, p[j]);
-        bm = fmaxf(bm, __shfl_xor(bm, 16, kWave));
-        bm = fmaxf(bm, __shfl_xor(bm, 32, kWave));
-        const float mn = fmaxf(m, bm), ref = mn == -INFINITY ? 0.f : mn;
-        if (__any(mn > m)) {
-            const float al = __builtin_amdgcn_exp2f(m - ref);
-            l *= al;
-#pragma unroll
-            for (int f = 0; f < F; f++) o[f] *= al;
-        }
-        m = mn;
-        uint32_t hi[4], lw[4];
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float e0 = __builtin_amdgcn_exp2f(p[2 * w] - ref), e1 = __builtin_amdgcn_exp2f(p[2 * w + 1] - ref);
-            l += e0 + e1;
-            // the upper part strictly below the weight, so that the rest of a weight is never 0 (0 times an infinite
-            // value would be NaN, not infinite)
-            const uint32_t b0 = max(__float_as_uint(e0), 1u) - 1u, b1 = max(__float_as_uint(e1), 1u) - 1u;
-            hi[w] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-            const float r0 = e0 - __uint_as_float(b0 & 0xffff0000u), r1 = e1 - __uint_as_float(b1 & 0xffff0000u);
-            lw[w] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
-        }
-        const v4u ph = {hi[0], hi[1], hi[2], hi[3]}, plo = {lw[0], lw[1], lw[2], lw[3]};
-#pragma unroll
-        for (int q = 0; q < F / 4; q++) {
-            v4u vf[4];
-            turn_v<D, F8>(s, q, vf);
-#pragma unroll
-            for (int f = 0; f < 4; f++) {
-                o[4 * q + f] = mfma_bf16(vf[f], ph, o[4 * q + f]);
-                o[4 * q + f] = mfma_bf16(vf[f], plo, o[4 * q + f]);
-            }
-        }
-    };
-    int t0 = begin + 32 * wave;
-    if (t0 < end) {
-        locate(t0);
-        clamp();
-        load_k(t0);
-        load_v(t0);
-        for (; t0 + UNIT < end; t0 += UNIT) block(t0, std::true_type{});
-        block(t0, std::false_type{});
-    }
 
-    // the four waves' columns, joined: each to the common maximum
-    constexpr int LD = D + 4;
-    float* lm = reinterpret_cast<float*>(lds + kWaves * B::STAGE);
-    float* ll = lm + kWaves * 16;
-    l += __shfl_xor(l, 16, kWave);
-    l += __shfl_xor(l, 32, kWave);
-    if (lane < 16) {
-        lm[wave * 16 + lane] = m;
-        ll[wave * 16 + lane] = l;
-    }
-    float* mine = reinterpret_cast<float*>(stage) + col * LD;
-#pragma unroll
-    for (int f = 0; f < F; f++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) mine[dim_of<D, F8>(f, 4 * g + r)] = o[f][r];
-    __syncthreads();
-    const float vs = F8 && a.c.v_scale ? __ldg(a.c.v_scale + hk) : 1.f;
-    for (int i = threadIdx.x; i < nh * (D / 4); i += 256) {
-        const int h = i / (D / 4), d = 4 * (i % (D / 4));
-        float mm = lm[h];
-#pragma unroll
-        for (int w = 1; w < kWaves; w++) mm = fmaxf(mm, lm[16 * w + h]);
-        const float ref = mm == -INFINITY ? 0.f : mm;
-        float sum = 0.f;
-        v4f acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            const float e = __builtin_amdgcn_exp2f(lm[16 * w + h] - ref);
-            sum += e * ll[16 * w + h];
-            acc += e * *reinterpret_cast<const v4f*>(lds + w * B::STAGE + (h * LD + d) * 4);
+        // the four waves' columns, joined: each to the common maximum
+        constexpr int LD = D + 4;
+        float* lm = reinterpret_cast<float*>(lds + kWaves * B::STAGE);
+        float* ll = lm + kWaves * 16;
+        l += __shfl_xor(l, 16, kWave);
+        l += __shfl_xor(l, 32, kWave);
+        if (lane < 16) {
+            lm[wave * 16 + lane] = m;
+            ll[wave * 16 + lane] = l;
         }
-        if (pl.splits == 1) {
-            uint32_t u[4];
+        float* mine = reinterpret_cast<float*>(stage) + col * LD;
 #pragma unroll
-            for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(sum == 0.f ? 0.f : div_rn(acc[j], sum) * vs);
-            *reinterpret_cast<v2u*>(a.out + b * a.ldo + (h0 + h) * a.ho_s + d) = v2u{u[0] | (u[1] << 16), u[2] | (u[3] << 16)};
-        } else {
-            const int64_t at = (int64_t)part * a.HQ + h0 + h;
-            *reinterpret_cast<v4f*>(a.part_o + at * D + d) = acc;
-            if (d == 0) {
-                a.part_ml[2 * at] = mm;
-                a.part_ml[2 * at + 1] = sum;
+        for (int f = 0; f < F; f++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) mine[dim_of<D, F8>(f, 4 * g + r)] = o[f][r];
+        __syncthreads();
+        // its first part's number and how many it has: the rest's units by `per`
+        if (a.plan && off == 0 && ht == 0 && threadIdx.x == 0)
+            a.plan[b] = int2{part, 1 + (units - seg + pl.per - 1) / pl.per};
+        const float vs = F8 && a.c.v_scale ? __ldg(a.c.v_scale + hk) : 1.f;
+        const int64_t slot = 2 * (int64_t)part + (off == 0);      // of a workgroup's parts one ends a sequence, one begins one
+        for (int i = threadIdx.x; i < nh * (D / 4); i += 256) {
+            const int h = i / (D / 4), d = 4 * (i % (D / 4));
+            float mm = lm[h];
+#pragma unroll
+            for (int w = 1; w < kWaves; w++) mm = fmaxf(mm, lm[16 * w + h]);
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            float sum = 0.f;
+            v4f acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const float e = __builtin_amdgcn_exp2f(lm[16 * w + h] - ref);
+                sum += e * ll[16 * w + h];
+                acc += e * *reinterpret_cast<const v4f*>(lds + w * B::STAGE + (h * LD + d) * 4);
+            }
+            if (whole) {
+                uint32_t u[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(sum == 0.f ? 0.f : div_rn(acc[j], sum) * vs);
+                *reinterpret_cast<v2u*>(a.out + b * a.ldo + (h0 + h) * a.ho_s + d) = v2u{u[0] | (u[1] << 16), u[2] | (u[3] << 16)};
+            } else {
+                const int64_t to = slot * a.HQ + h0 + h;
+                *reinterpret_cast<v4f*>(a.part_o + to * D + d) = acc;
+                if (d == 0) {
+                    a.part_ml[2 * to] = mm;
+                    a.part_ml[2 * to + 1] = sum;
+                }
             }
         }
+        left -= seg;
+        if (left == 0) return;
+        b++, off = 0;
+        __syncthreads();                                          // the next sequence's loads overwrite what was joined
     }
 }
 
@@ -546,6 +546,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int hb) {
     const int2 pl = a.plan[b];                                // (a row past n has none: not used)
     if (b >= n || pl.y < 2) return;
     const int c = threadIdx.x % TC, grp = threadIdx.x / TC;
+    auto slot = [&](int i) { return 2 * (int64_t)(pl.x + i) + (i == 0); };
     int share = 2;
     while (share < NG && share < pl.y) share *= 2;
     share = min(share, NG);
@@ -556,14 +557,13 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int hb) {
         v4f acc = {0.f, 0.f, 0.f, 0.f};
         float sum = 0.f;
         if (h < hend) {
-            const int64_t first = (int64_t)pl.x * a.HQ + h;
             float mm = -INFINITY;
-            for (int i = c; i < pl.y; i += TC) mm = fmaxf(mm, a.part_ml[2 * (first + (int64_t)i * a.HQ)]);
+            for (int i = c; i < pl.y; i += TC) mm = fmaxf(mm, a.part_ml[2 * (slot(i) * a.HQ + h)]);
 #pragma unroll
             for (int o = TC / 2; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, kWave));
             const float ref = mm == -INFINITY ? 0.f : mm;
             for (int i = sub; i < pl.y; i += share) {
-                const int64_t at = first + (int64_t)i * a.HQ;
+                const int64_t at = slot(i) * a.HQ + h;
                 const float e = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
                 sum += e * a.part_ml[2 * at + 1];
                 acc += e * *reinterpret_cast<const v4f*>(a.part_o + at * D + 4 * c);
@@ -601,10 +601,9 @@ static int attend_target(int64_t D, bool f8) {
     return 256 * (fit < 4 ? fit : 4);
 }
 
-// Parts that the grid holds: every sequence at most a part per unit, all together at most the target's share of a head and
-// one more each.
+// Workgroups per head: all units at `per` each, no more than the target's share and no more than there are units.
 static int64_t attend_parts(int64_t T, int64_t HT, int64_t cap, int target) {
-    const int64_t unit = 32 * kWaves, most = T * ((cap + unit - 1) / unit), split = target / HT + 1 + T;
+    const int64_t unit = 32 * kWaves, most = T * ((cap + unit - 1) / unit), split = target / HT + 1;
     return most < split ? most : split;
 }
 
@@ -684,7 +683,7 @@ extern "C" int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t hq, int64_
     if (T < 1 || heads < 1 || hq < heads || hq % heads || dim < 1 || cols < 1 || page < 1) return 0;
     if (cols * page <= 32 * kWaves) return 0;                // one unit: nothing to join
     // (the most parts that either cache type takes)
-    return attend_parts(T, heads * ((hq / heads + 15) / 16), cols * page, 4 * 256) * hq * (dim + 2) * 4 + T * 8;
+    return 2 * attend_parts(T, heads * ((hq / heads + 15) / 16), cols * page, 4 * 256) * hq * (dim + 2) * 4 + T * 8;
 }
 
 extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
@@ -714,8 +713,8 @@ extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
     a.lens = h.lens, a.n = h.n_rows;
     if (need > 0) {
         a.part_o = (float*)h.ws;
-        a.part_ml = (float*)h.ws + parts * HQ * D;
-        a.plan = (int2*)((float*)h.ws + parts * HQ * (D + 2));
+        a.part_ml = (float*)h.ws + 2 * parts * HQ * D;
+        a.plan = (int2*)((float*)h.ws + 2 * parts * HQ * (D + 2));
     }
     a.scale = (float)h.scale * 1.44269504088896340736f;
     a.T = (int)T, a.HQ = (int)HQ, a.G = (int)G, a.tiles = (int)tiles, a.HT = (int)HT;
@@ -735,7 +734,7 @@ extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
     PRISM_LAUNCH_CHECK();
     if (need > 0) {
         // a workgroup per head while there are few (long sequences have many parts), else one for as many as it has groups
-        const int hb = T * HQ <= 1024 ? 1 : (int)(1024 / D);
+        const int hb = T * HQ <= 4096 ? 1 : (int)(1024 / D);
         const dim3 jg((unsigned)((HQ + hb - 1) / hb), (unsigned)T);
         if (D == 64) hipLaunchKernelGGL(kv_join_kernel<64>, jg, dim3(256), 0, st, a, hb);
         else if (D == 128) hipLaunchKernelGGL(kv_join_kernel<128>, jg, dim3(256), 0, st, a, hb);
