@@ -193,21 +193,30 @@ struct Plan {
 template <int UNIT>
 __device__ __forceinline__ Plan make_plan(const AttendArgs& a, int p) {
     const int lane = threadIdx.x & 63;
+    const int len0 = lane < a.T ? __ldg(a.lens + lane) : 0;   // (loads that need not wait for n)
     const int n = min(__ldg(a.n), a.T);
     int lo, len;
-    long long sum = 0;
-    for (int b = lane; b < n; b += 64) sum += max(1, vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len));
-    const long long total = wave_sum(sum);
+    const int units0 = lane < n ? max(1, vis_units<UNIT>(a, len0, &lo, &len)) : 0;
+    long long total = __builtin_amdgcn_readfirstlane(units0);
+    if (n > 1) {
+        long long sum = units0;
+        for (int b = lane + 64; b < n; b += 64) sum += max(1, vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len));
+        total = wave_sum(sum);
+    }
     Plan r;
     r.b = -1;
     r.per = max((int)((total * a.HT + a.target - 1) / a.target), 1);
     const long long u = (long long)p * r.per;
     if (u >= total) return r;
     r.left = (int)min((long long)r.per, total - u);
+    if (n == 1) {
+        r.b = 0, r.off = (int)u;
+        return r;
+    }
     long long base = 0;
     for (int b0 = 0; b0 < n; b0 += 64) {
         const int b = b0 + lane;
-        const int units = b < n ? max(1, vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len)) : 0;
+        const int units = b0 == 0 ? units0 : b < n ? max(1, vis_units<UNIT>(a, __ldg(a.lens + b), &lo, &len)) : 0;
         long long incl = units;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -344,12 +353,12 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
         for (int f = 0; f < F; f++) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
 
-        // the table through the scalar cache: a vector load would be waited for together with the values in flight before it
+  // the table through the scalar cache: a vector load would be waited for together with the values in flight before it
         const auto* row = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
             reinterpret_cast<uintptr_t>(a.c.table + b * a.c.table_ld));
         const int last = len > 0 ? (len - 1) & ~15 : 0;           // the last 16 tokens that are there
-        // Keys and values go to LDS by DMA, 1 KB a load.  Keys: 16 tokens x 64 bytes, four neighbouring lanes a token's (the
-        // memory pipeline merges neighbouring lanes only), placed so that operand order reads without bank conflicts; values:
+  // Keys and values go to LDS by DMA, 1 KB a load.  Keys: 16 tokens x 64 bytes, four neighbouring lanes a token's (the
+  // memory pipeline merges neighbouring lanes only), placed so that operand order reads without bank conflicts; values:
         // whole rows.  Every wait on them is written out: the compiler would wait for all of them at each use.
         const uint32_t koff = (uint32_t)((lane >> 2) * a.c.k_tok) + 16 * ((lane & 3) ^ lds_turn(lane >> 4));
         const uint32_t voff = (uint32_t)(16 * lane / B::RB * a.c.v_tok) + 16 * lane % B::RB;
@@ -362,7 +371,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
         int64_t page[2];
         auto locate = [&](int t0) {
 #pragma unroll
-            for (int x = 0; x < 2; x++) page[x] = row[min(t0 + 16 * x, last) >> a.c.shift];   // 16 tokens never cross a page
+            for (int x = 0; x < 2; x++) page[x] = row[min(t0 + 16 * x, last) >> a.c.shift];  // 16 tokens never cross a page
         };
         auto clamp = [&] {
 #pragma unroll
@@ -389,7 +398,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
         // One block of 32 tokens; with `more`, the next one's loads go out as this one's places in LDS become free.
         auto block = [&](int t0, auto more) {
             constexpr bool MORE = decltype(more)::value;
-            vm_wait<2 * L>();                                     // the keys are there (the values' loads came after theirs)
+            vm_wait<2 * L>();  // the keys are there (the values' loads came after theirs)
             if (MORE) locate(t0 + UNIT);
             v4f st[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -422,7 +431,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; j++) p[j] = mul_rn(st[j / 4][j % 4], sc);
             if (t0 < lo || (!MORE && t0 + 32 > len)) {
-                // tokens outside get no weight, and their values, which may be anything (a page's unwritten rows), are zeroed
+  // tokens outside get no weight, and their values, which may be anything (a page's unwritten rows), are zeroed
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int t = t0 + 16 * (j / 4) + 4 * g + j % 4;
@@ -499,7 +508,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
         if (a.plan && off == 0 && ht == 0 && threadIdx.x == 0)
             a.plan[b] = int2{part, 1 + (units - seg + pl.per - 1) / pl.per};
         const float vs = F8 && a.c.v_scale ? __ldg(a.c.v_scale + hk) : 1.f;
-        const int64_t slot = 2 * (int64_t)part + (off == 0);      // of a workgroup's parts one ends a sequence, one begins one
+        const int64_t slot = 2 * (int64_t)part + (off == 0);  // of a workgroup's parts one ends a sequence, one begins one
         for (int i = threadIdx.x; i < nh * (D / 4); i += 256) {
             const int h = i / (D / 4), d = 4 * (i % (D / 4));
             float mm = lm[h];
@@ -588,17 +597,17 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int hb) {
     }
 }
 
-// LDS of a workgroup, and the workgroups that a launch's work is split into, at most (beside one for each further sequence
-// and head): as many as the CUs' LDS holds at a time, up to four a CU.  More parts balance ragged batches better and cost
-// the join more: 128 sequences of 100 - 4096 visible tokens, 8 heads of 64, 192 us with two a CU, 172 with four; one
-// sequence of 131071 tokens, 8 heads of 128 bf16 (LDS for two), 100 us with two, 106 with four.
+// LDS of a workgroup, and how many workgroups a launch's work is dealt out to: as many as are there at a time, two a CU where
+// LDS holds them.  With 4 a CU (rows of 128 bytes leave LDS for them) 128 sequences of 100 - 4096 visible tokens, 8 heads of
+// 64, take 153 us instead of 148 and 64 of 8000 tokens, 8 heads of 128 e4m3, 189 instead of 180: every further part is more
+// to join.  One a CU: 131071 tokens, 8 heads of 128 bf16, 98 us instead of 100, but 256 sequences of 20 - 300 tokens 50
+// instead of 41.
 static int attend_lds(int64_t D, bool f8) {
     const int64_t stage = 4 * (f8 ? D : 2 * D) / 64 * 1024, o = 16 * (D + 4) * 4;
     return (int)(kWaves * (stage > o ? stage : o) + 2 * kWaves * 16 * 4);
 }
 static int attend_target(int64_t D, bool f8) {
-    const int fit = 160 * 1024 / attend_lds(D, f8);
-    return 256 * (fit < 4 ? fit : 4);
+    return 2 * attend_lds(D, f8) <= 160 * 1024 ? 512 : 256;
 }
 
 // Workgroups per head: all units at `per` each, no more than the target's share and no more than there are units.
@@ -682,8 +691,8 @@ extern "C" int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t hq, int64_
                                                    int64_t page) {
     if (T < 1 || heads < 1 || hq < heads || hq % heads || dim < 1 || cols < 1 || page < 1) return 0;
     if (cols * page <= 32 * kWaves) return 0;                // one unit: nothing to join
-    // (the most parts that either cache type takes)
-    return 2 * attend_parts(T, heads * ((hq / heads + 15) / 16), cols * page, 4 * 256) * hq * (dim + 2) * 4 + T * 8;
+    // (512: the most that either cache type is dealt out to)
+    return 2 * attend_parts(T, heads * ((hq / heads + 15) / 16), cols * page, 512) * hq * (dim + 2) * 4 + T * 8;
 }
 
 extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
@@ -733,7 +742,7 @@ extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
 #undef AT
     PRISM_LAUNCH_CHECK();
     if (need > 0) {
-        // a workgroup per head while there are few (long sequences have many parts), else one for as many as it has groups
+  // a workgroup per head while there are few (long sequences have many parts), else one for as many as it has groups
         const int hb = T * HQ <= 4096 ? 1 : (int)(1024 / D);
         const dim3 jg((unsigned)((HQ + hb - 1) / hb), (unsigned)T);
         if (D == 64) hipLaunchKernelGGL(kv_join_kernel<64>, jg, dim3(256), 0, st, a, hb);
