@@ -3,7 +3,8 @@
     python startlux-prism_amd/build.py [-j N]
 
 Each csrc/*.hip compiles to an object under csrc/_build/, then one shared library links next to the Python package
-(startlux-prism_amd/prism_amd/libprism_amd.so), which prism_amd._lib loads.  Flags:
+(startlux-prism_amd/prism_amd/libprism_amd.so), which prism_amd._lib loads.  csrc/host.cpp compiles with g++ to
+prism_amd/_host.so, the checked host path of prism_amd.kv and prism_amd.delta.  Flags of the HIP files:
   --offload-arch=gfx950                        MI355X / MI350X only; no other targets, no host fallback
   -fhip-fp32-correctly-rounded-divide-sqrt     '/' on fp32 is the IEEE division the quantizers are specified with
   -ffp-contract=off                            no implicit a*b+c contraction: roundings are the ones written
@@ -20,6 +21,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "_build")
 LIB = os.path.join(HERE, "prism_amd", "libprism_amd.so")
+HOST = os.path.join(HERE, "prism_amd", "_host.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-ffp-contract=off",
@@ -43,11 +45,28 @@ def _compile(src):
     return obj, err
 
 
+def _compile_host():
+    """csrc/host.cpp -> prism_amd/_host.so: the CPython extension that checks kv's and delta's tensors (host code only)."""
+    import sysconfig
+
+    from torch.utils import cpp_extension as C
+    tmp = HOST + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
+           *("-I" + p for p in (*C.include_paths(), sysconfig.get_paths()["include"])), os.path.join(CSRC, "host.cpp"),
+           "-o", tmp, *("-L" + p for p in C.library_paths()), "-lc10", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on csrc/host.cpp:\n{r.stderr}")
+    os.replace(tmp, HOST)
+
+
 def build(jobs=8, verbose=False):
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     with cf.ThreadPoolExecutor(max(1, jobs)) as ex:
+        host = ex.submit(_compile_host)
         res = list(ex.map(_compile, srcs))
+        host.result()
     for _, err in res:
         if err.strip() and verbose:
             print(err, file=sys.stderr)

@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libprism_am
 
 _i64, _p, _int = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int
 
-_args = ctypes.c_char_p                     # a struct of 8-byte fields, packed by struct.Struct into bytes
+_args = ctypes.c_char_p                     # a struct of 8-byte fields as packed bytes (the host extension passes its own)
 
 _SIGS = {
     "prism_version": (_int, []),
@@ -87,6 +87,38 @@ def lib():
 
 def exported_symbols():
     return list(_SIGS)
+
+
+_host = None
+
+
+def host():
+    """The host extension (csrc/host.cpp: the checked calls of kv and delta), bound to the loaded library's entries; raises
+    if it was not built."""
+    global _host
+    if _host is None:
+        try:
+            from . import _host as h
+        except ImportError as e:
+            raise PrismError(f"prism_amd/_host.so is missing or does not load ({e}): build it with python "
+                             "startlux-prism_amd/build.py") from e
+        from . import scratch
+        ws = scratch.Scratch(16 << 20)
+
+        def workspace(like, need, stream):
+            # the stream's own scratch, or (more than it holds; none under capture) the caching allocator's memory, which
+            # is the current stream's too
+            t = ws.get(like.device, False, need, stream) if need <= ws.nbytes else None
+            return torch.empty(need, dtype=torch.uint8, device=like.device) if t is None else t
+        h.bind(*(ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value for n in (
+            "prism_kv_append", "prism_kv_attend", "prism_kv_attend_workspace_bytes", "prism_delta_step",
+            "prism_delta_prefill", "prism_delta_prefill_workspace_bytes")), stream_of, workspace)
+        _host = h
+    return _host
+
+
+def fail(name, rc):
+    raise PrismError(f"{name}: {lib().prism_error_string(rc).decode()} (code {rc})")
 
 
 _checked = set()

@@ -1,20 +1,25 @@
 """What the token mixers refuse, on the CPU: the C entries' codes for bad pointers, sizes and alignment (placeholders that
 are never dereferenced), and the Python layer's TypeError / ValueError before any call."""
 import os
+import struct
+import types
 
 import pytest
 import torch
 
+# the C entries' structs: 8-byte fields, floating ones as doubles
+L = types.SimpleNamespace(_APPEND=struct.Struct("19q 12q 5q 5q"), _ATTEND=struct.Struct("19q 6q 4q d 2q"),
+                          _ARGS=struct.Struct("9q 4q 4q 3q q 7q 2d 2q"))
 OK, SHAPE, ALIGN, ARG = 0, 1, 2, 3
 P, U = 0x100000, 0x100001
 
 
 @pytest.fixture(scope="module")
 def lib():
-    from prism_amd import _lib as L
-    if not os.path.exists(L.LIB_PATH):
+    from prism_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
         pytest.skip("libprism_amd.so not built (run __graft_entry__.build())")
-    return L.lib()
+    return _lib.lib()
 
 
 def packed(layout, *fields):
@@ -22,26 +27,23 @@ def packed(layout, *fields):
 
 
 def test_packed_layouts_match_the_header():
-    """The Python layer packs as many 8-byte fields as the header's structs declare."""
+    """The layouts above have as many 8-byte fields as the header's structs declare."""
     import re
-    from prism_amd import delta, kv
     src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "prism_amd.h")).read()
     count = {}
     for body, name in re.findall(r"typedef struct \{(.*?)\} (prism_\w+);", src, re.S):
         count[name] = sum(count["prism_kv_cache"] if f.split()[0] == "prism_kv_cache" else len(f.split(","))
                           for f in body.split(";") if f.strip())
-    for layout, name in ((kv._APPEND, "prism_kv_append_args"), (kv._ATTEND, "prism_kv_attend_args"),
-                         (delta._ARGS, "prism_delta_args")):
+    for layout, name in ((L._APPEND, "prism_kv_append_args"), (L._ATTEND, "prism_kv_attend_args"),
+                         (L._ARGS, "prism_delta_args")):
         assert layout.size == 8 * count[name], name
 
 
 def test_append_codes(lib):
-    from prism_amd import kv
-
     def call(q=P, k=P, rope=P, rot=64, ldr=64, adjacent=0, pos=P, kc=P, tok=128, e4m3=0, ks=None, cols=4, pages=8,
              page=16, T=1, HQ=2, D=64, ldk=128, qo=P):
         return lib.prism_kv_append(packed(
-            kv._APPEND, kc, 4096, tok, 64, P, 4096, tok, 64, e4m3, ks, None, P, 4, 2, cols, pages, page, 2, D,
+            L._APPEND, kc, 4096, tok, 64, P, 4096, tok, 64, e4m3, ks, None, P, 4, 2, cols, pages, page, 2, D,
             q, 256, 64, k, ldk, 64, P, 128, 64, qo, 128, 64, rope, ldr, 100, rot, adjacent, pos, None, P, T, HQ), None)
     assert lib.prism_kv_append(None, None) == ARG
     assert call(T=0) == OK and call(T=0, HQ=0, q=None, qo=None) == OK and call(T=0, rot=0, rope=None, ldr=0) == OK
@@ -55,11 +57,9 @@ def test_append_codes(lib):
 
 
 def test_attend_codes(lib):
-    from prism_amd import kv
-
     def call(q=P, lens=P, out=P, T=1, HQ=4, D=64, window=0, ws=P, ws_bytes=1 << 20, cols=16, page=16, ldq=256, ldo=256):
         return lib.prism_kv_attend(packed(
-            kv._ATTEND, P, 4096, 128, 64, P, 4096, 128, 64, 0, None, None, P, cols, T, cols, 8, page, 2, D,
+            L._ATTEND, P, 4096, 128, 64, P, 4096, 128, 64, 0, None, None, P, cols, T, cols, 8, page, 2, D,
             q, ldq, 64, out, ldo, 64, lens, P, HQ, window, 0.125, ws, ws_bytes), None)
     assert lib.prism_kv_attend(None, None) == ARG
     assert call(T=0) == OK
@@ -74,12 +74,10 @@ def test_attend_codes(lib):
 
 
 def test_delta_codes(lib):
-    from prism_amd import delta
-
     def call(q=P, state=P, n=P, T=1, HK=2, HV=4, DK=128, DV=128, norm=1, nslots=2, stride=None, ldv=512, fn="step", seqs=1,
              ws=None, ws_bytes=0):
         return getattr(lib, "prism_delta_" + fn)(packed(
-            delta._ARGS, q, 256, 128, P, 256, 128, P, ldv, 128, P, 4, P, 4, state, HV * DK * DV if stride is None else stride,
+            L._ARGS, q, 256, 128, P, 256, 128, P, ldv, 128, P, 4, P, 4, state, HV * DK * DV if stride is None else stride,
             nslots, None, P, 512, 128, n, seqs, T, HK, HV, DK, DV, norm, 1.0, 1e-6, ws, ws_bytes), None)
     for fn in ("step", "prefill"):
         assert getattr(lib, "prism_delta_" + fn)(None, None) == ARG
@@ -105,7 +103,7 @@ def _bf(*shape):
     return torch.zeros(*shape, dtype=torch.bfloat16)
 
 
-def test_kv_python_checks():
+def test_kv_python_checks(lib):
     from prism_amd import kv
     kc, vc = kv.cache(4, 16, 2, 64, device="cpu")
     assert kc.shape == (4, 16, 2, 64) and kc.stride(2) == 16 * 64
@@ -150,7 +148,7 @@ def test_kv_python_checks():
     no(TypeError, lens=torch.zeros(3, dtype=torch.int64))
 
 
-def test_delta_python_checks():
+def test_delta_python_checks(lib):
     from prism_amd import delta
     f = torch.zeros
     good = dict(q=_bf(5, 2, 64), k=_bf(5, 2, 64), v=_bf(5, 4, 128), g=f(5, 4), beta=f(5, 4), state=f(6, 4, 64, 128),
