@@ -225,28 +225,40 @@ __device__ __forceinline__ bool find_chunk(const DeltaArgs& a, int id, int& firs
     return false;
 }
 
-// One wave per chunk (blockIdx.x) and value head (blockIdx.y).
+// One wave per chunk (blockIdx.x) and value head (blockIdx.y).  Rows are loaded in their own order (a row per lane would take
+// the memory pipeline four times as long) and become fragments through LDS.  The decays between tokens of different 16-row
+// tiles are products of three that are at most 1, so that 16 exponentials a lane (the diagonal tiles') and a few are enough
+// for 40.
 template <int DK>
 __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, char* wv) {
-    constexpr int KS = DK / 32, LD = kC + 4;
-    __shared__ __align__(16) float x[kC * LD];                // A, then X, in place; before that, K's rows (bf16)
+    constexpr int KS = DK / 32, LD = kC + 4, LK = DK + 8, PR = DK / 8;   // PR: 16-byte pieces of a row
+    __shared__ __align__(16) float x[kC * LD];                // K's, then Q's rows (bf16); A, then X, in place
     __shared__ double gsum[kC];
-    __shared__ float rkv[kC], rqv[kC], bev[kC];
-    static_assert(sizeof(x) >= kC * (DK + 2) * 2, "K's rows");
+    __shared__ float rkv[kC], rqv[kC], bev[kC], upv[kC], dnv[kC];
+    static_assert(sizeof(x) >= kC * LK * 2, "K's rows");
     int first, count;
     if (!find_chunk(a, blockIdx.x, first, count)) return;
     const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
-    const int head = blockIdx.y, share = a.HV / a.HK, hk = head / share;
-    const bool copies = head % share == 0;                    // this key head's K, Q and K^T fragments are this wave's to write
+    const int head = blockIdx.y, share = a.HV / a.HK, hk = head / share, part = head % share;
     char* rk = wk + ((int64_t)blockIdx.x * a.HK + hk) * rec_k(DK);
     char* rv = wv + ((int64_t)blockIdx.x * a.HV + head) * kRecV;
 
+    v4u kr[PR], qr[PR];                                       // rows past the chunk are zeros
+#pragma unroll
+    for (int i = 0; i < PR; i++) {
+        const int row = i * (64 / PR) + lane / PR;
+        const int64_t t = first + min(row, count - 1);
+        kr[i] = *reinterpret_cast<const v4u*>(a.k + t * a.ldk + hk * a.hk_s + 8 * (lane % PR));
+        qr[i] = *reinterpret_cast<const v4u*>(a.q + t * a.ldq + hk * a.hq_s + 8 * (lane % PR));
+    }
     // the chunk's gates, one token per lane, the sums in 64 bits: the differences G_i - G_j are then as exact as the g.
     // Below -1e4 a decay is 0 either way, and sums stay finite (-inf minus -inf would not be a number)
     {
         const bool in = lane < count;
-        float gv = in ? a.g[(int64_t)(first + lane) * a.ldg + head] : 0.f;
-        gv = gv < -1e4f ? -1e4f : gv;
+        const int64_t t = first + min(lane, count - 1);
+        const float be = a.beta[t * a.ldb + head];
+        float gv = a.g[t * a.ldg + head];
+        gv = !in ? 0.f : gv < -1e4f ? -1e4f : gv;
         double s = gv;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -254,60 +266,46 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
             if (lane >= o) s += up;
         }
         gsum[lane] = s;
-        bev[lane] = in ? a.beta[(int64_t)(first + lane) * a.ldb + head] : 0.f;
+        bev[lane] = in ? be : 0.f;
+        // from the last token before this one's tile, and to the last token of its tile
+        const double before = __shfl(s, (lane & 48) - 1, kWave), last = __shfl(s, lane | 15, kWave);
+        upv[lane] = expf((float)(s - (lane < 16 ? 0.0 : before)));
+        dnv[lane] = expf((float)(last - s));
     }
-    // K's and Q's rows as fragments: tile i's row col, dims 32 s + 8 g .. + 7; rows past the chunk are zeros
-    v4u kf[4][KS], qf[4][KS];
+    uint16_t* rows = reinterpret_cast<uint16_t*>(x);
+    auto put = [&](const v4u (&r)[PR]) {
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const bool in = 16 * i + col < count;
-        const int64_t t = first + (in ? 16 * i + col : 0);
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const v4u kk = *reinterpret_cast<const v4u*>(a.k + t * a.ldk + hk * a.hk_s + 32 * s + 8 * g);
-            const v4u qq = *reinterpret_cast<const v4u*>(a.q + t * a.ldq + hk * a.hq_s + 32 * s + 8 * g);
-            kf[i][s] = in ? kk : v4u{0, 0, 0, 0};
-            qf[i][s] = in ? qq : v4u{0, 0, 0, 0};
+        for (int i = 0; i < PR; i++) {
+            const int row = i * (64 / PR) + lane / PR;
+            *reinterpret_cast<v4u*>(rows + row * LK + 8 * (lane % PR)) = row < count ? r[i] : v4u{0, 0, 0, 0};
         }
-        float sk = 0.f, sq = 0.f;
+        __syncthreads();
+    };
+    // fragment (i, s): tile i's row col, dims 32 s + 8 g .. + 7
+    auto get = [&](v4u (&f)[4][KS]) {
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float k0 = __uint_as_float(kf[i][s][w] << 16), k1 = cut(__uint_as_float(kf[i][s][w]));
-                const float q0 = __uint_as_float(qf[i][s][w] << 16), q1 = cut(__uint_as_float(qf[i][s][w]));
-                sk = fmaf(k0, k0, fmaf(k1, k1, sk));
-                sq = fmaf(q0, q0, fmaf(q1, q1, sq));
-            }
-        sk += __shfl_xor(sk, 16, kWave);
-        sk += __shfl_xor(sk, 32, kWave);
-        sq += __shfl_xor(sq, 16, kWave);
-        sq += __shfl_xor(sq, 32, kWave);
-        if (g == 0) {
-            rkv[16 * i + col] = a.norm ? div_rn(1.f, sqrt_rn(sk + a.eps)) : 1.f;
-            rqv[16 * i + col] = (a.norm ? div_rn(1.f, sqrt_rn(sq + a.eps)) : 1.f) * a.scale;
-        }
-    }
-    if (copies) {
-        // K and Q: fragment (i, s), piece p (4 dims) of a row at lane 16 (p % 4) + row, half p / 4
-        uint16_t* rows = reinterpret_cast<uint16_t*>(x);
+            for (int s = 0; s < KS; s++) f[i][s] = *reinterpret_cast<const v4u*>(rows + (16 * i + col) * LK + 32 * s + 8 * g);
+    };
+    // as delta_scan's left operand, fragment (i, s): dims 32 s + 4 g + j, then 32 s + 16 + 4 g + j
+    auto copy = [&](char* to) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                char* fk = rk + (i * KS + s) * kFrag;
-                char* fq = fk + 4 * KS * kFrag;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int p = 2 * g + h, at = (16 * (p & 3) + col) * 16 + 8 * (p >> 2);
-                    *reinterpret_cast<v2u*>(fk + at) = v2u{kf[i][s][2 * h], kf[i][s][2 * h + 1]};
-                    *reinterpret_cast<v2u*>(fq + at) = v2u{qf[i][s][2 * h], qf[i][s][2 * h + 1]};
-                }
-#pragma unroll
-                for (int w = 0; w < 4; w++)
-                    *reinterpret_cast<uint32_t*>(rows + (16 * i + col) * (DK + 2) + 32 * s + 8 * g + 2 * w) = kf[i][s][w];
+                const uint16_t* r = rows + (16 * i + col) * LK + 32 * s + 4 * g;
+                const v2u lo = *reinterpret_cast<const v2u*>(r), hi = *reinterpret_cast<const v2u*>(r + 16);
+                *reinterpret_cast<v4u*>(to + (i * KS + s) * kFrag + lane * 16) = v4u{lo[0], lo[1], hi[0], hi[1]};
             }
-        __syncthreads();
+    };
+    v4u kf[4][KS], qf[4][KS];
+    put(kr);
+    get(kf);
+    // this key head's fragments of K, K^T and Q are written by its first, second and last value head's wave
+    if (part == 0) copy(rk);
+    if (part == (share > 1 ? 1 : 0)) {
         // K^T: fragment (d, s), row 16 d + col, tokens 32 s + 4 g + j and 32 s + 16 + 4 g + j
         char* ft = rk + 8 * KS * kFrag;
 #pragma unroll
@@ -316,60 +314,89 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
             for (int s = 0; s < 2; s++) {
                 uint32_t u[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) u[j] = rows[(32 * s + 16 * (j / 4) + 4 * g + j % 4) * (DK + 2) + 16 * d + col];
+                for (int j = 0; j < 8; j++) u[j] = rows[(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col];
                 *reinterpret_cast<v4u*>(ft + (2 * d + s) * kFrag + lane * 16) =
                     v4u{u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16)};
             }
+    }
+    put(qr);
+    get(qf);
+    if (part == share - 1) copy(rk + 4 * KS * kFrag);
+
+    // squares of the rows' lengths: the diagonals of K K^T and Q Q^T
+    if (a.norm) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v4f kk = {0.f, 0.f, 0.f, 0.f}, qq = kk;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                kk = mfma_bf16(kf[i][s], kf[i][s], kk);
+                qq = mfma_bf16(qf[i][s], qf[i][s], qq);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (4 * g + r == col) rkv[16 * i + col] = kk[r], rqv[16 * i + col] = qq[r];
+        }
+        __syncthreads();
+    }
+    {
+        const float sk = a.norm ? div_rn(1.f, sqrt_rn(rkv[lane] + a.eps)) : 1.f;
+        const float sq = (a.norm ? div_rn(1.f, sqrt_rn(rqv[lane] + a.eps)) : 1.f) * a.scale;
+        rkv[lane] = sk;
+        rqv[lane] = sq;
+        float* vec = reinterpret_cast<float*>(rv + 6 * kTri * kFrag);
+        const double gl = gsum[lane], gc = gsum[kC - 1];
+        const float e = expf((float)gl);
+        vec[lane] = e * sk;
+        vec[kC + lane] = e * sq;
+        vec[2 * kC + lane] = expf((float)(gc - gl)) * sk;
+        vec[3 * kC + lane] = expf((float)gc);
     }
     __syncthreads();
 
     // k_i . k_j and q_i . k_j, tiles j <= i, transposed: a lane holds row i = col for columns 4 g + r, which is a
     // fragment's order
-    v4f pt[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const double gi = gsum[16 * i + col];
-        const float ki = bev[16 * i + col] * rkv[16 * i + col], qi = rqv[16 * i + col];
+        const int row = 16 * i + col;
+        const double gi = gsum[row];
+        const float up = upv[row], ki = bev[row] * rkv[row], qi = rqv[row];
+        v4f pt[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            pt[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+            pt[j] = v4f{0.f, 0.f, 0.f, 0.f};
             if (j > i) continue;
-            v4f kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
+            v4f kk = {0.f, 0.f, 0.f, 0.f}, qk = kk, am, f;
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 kk = mfma_bf16(kf[j][s], kf[i][s], kk);
                 qk = mfma_bf16(kf[j][s], qf[i][s], qk);
             }
-            v4f am;
+            const int c0 = 16 * j + 4 * g;
+            if (i == j) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) f[r] = expf((float)(gi - gsum[c0 + r]));
+            } else {
+                const float mid = i == j + 1 ? up : up * expf((float)(gsum[16 * i - 1] - gsum[16 * j + 15]));
+#pragma unroll
+                for (int r = 0; r < 4; r++) f[r] = mid * dnv[c0 + r];
+            }
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int row = 16 * i + col, c = 16 * j + 4 * g + r;
-                const float f = expf((float)(gi - gsum[c])) * rkv[c];
-                am[r] = c < row ? f * ki * kk[r] : 0.f;
-                pt[i][j][r] = c <= row ? f * qi * qk[r] : 0.f;
+                f[r] *= rkv[c0 + r];
+                am[r] = c0 + r < row ? f[r] * ki * kk[r] : 0.f;
+                pt[j][r] = c0 + r <= row ? f[r] * qi * qk[r] : 0.f;
             }
-            *reinterpret_cast<v4f*>(x + (16 * i + col) * LD + 16 * j + 4 * g) = am;
+            *reinterpret_cast<v4f*>(x + row * LD + c0) = am;
         }
-    }
-    char* pa = rv + 3 * kTri * kFrag;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int s = 0; s <= i / 2; s++) {
-            const Split p = split8(pt[i][2 * s], pt[i][2 * s + 1]);
-            char* f = pa + 3 * tri(i, s) * kFrag + lane * 16;
-            *reinterpret_cast<v4u*>(f) = p.h;
-            *reinterpret_cast<v4u*>(f + kFrag) = p.m;
-            *reinterpret_cast<v4u*>(f + 2 * kFrag) = p.l;
+            const Split p = split8(pt[2 * s], pt[2 * s + 1]);
+            char* to = rv + 3 * (kTri + tri(i, s)) * kFrag + lane * 16;
+            *reinterpret_cast<v4u*>(to) = p.h;
+            *reinterpret_cast<v4u*>(to + kFrag) = p.m;
+            *reinterpret_cast<v4u*>(to + 2 * kFrag) = p.l;
         }
-    {
-        float* vec = reinterpret_cast<float*>(rv + 6 * kTri * kFrag);
-        const double gl = gsum[lane], gc = gsum[kC - 1];
-        const float e = expf((float)gl);
-        vec[lane] = e * rkv[lane];
-        vec[kC + lane] = e * rqv[lane];
-        vec[2 * kC + lane] = expf((float)(gc - gl)) * rkv[lane];
-        vec[3 * kC + lane] = expf((float)gc);
     }
     __syncthreads();
 
@@ -394,26 +421,45 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
         for (int i = 0; i < 16; i++) x[(16 * g + i) * LD + 16 * g + col] = v[i];
     }
     __syncthreads();
-    // the blocks below: X_ij = -X_ii sum_k A_ik X_kj, columns from the left, so that A_ij's place is free for X_ij
+    // the blocks below, X_ij = -X_ii sum_k A_ik X_kj, diagonal by diagonal: the X_kj are right operands as the accumulators
+    // they come in, so nothing is stored before all are there
+    {
+        v4f y[4][4];                                          // [i][j]; [i][i]: the diagonal blocks in the same form
 #pragma unroll
-    for (int j = 0; j < 3; j++)
+        for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int i = j + 1; i < 4; i++) {
-            v4f s = {0.f, 0.f, 0.f, 0.f}, y = s;
+            for (int r = 0; r < 4; r++) y[i][i][r] = x[(16 * i + 4 * g + r) * LD + 16 * i + col];
 #pragma unroll
-            for (int k = j; k < i; k++) {
-                const v4f am = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * k + 4 * g);
+        for (int d = 1; d < 4; d++) {
+            v4f s[4];
 #pragma unroll
-                for (int r = 0; r < 4; r++) s = mfma_f32(am[r], x[(16 * k + 4 * g + r) * LD + 16 * j + col], s);
+            for (int i = d; i < 4; i++) {
+                s[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = i - d; k < i; k++) {
+                    const v4f am = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * k + 4 * g);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[i] = mfma_f32(am[r], y[k][i - d][r], s[i]);
+                }
             }
-            const v4f xi = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * i + 4 * g);
 #pragma unroll
-            for (int r = 0; r < 4; r++) y = mfma_f32(xi[r], s[r], y);
-            __syncthreads();
+            for (int i = d; i < 4; i++) {
+                const v4f xi = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * i + 4 * g);
+                v4f z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; r++) x[(16 * i + 4 * g + r) * LD + 16 * j + col] = -y[r];
-            __syncthreads();
+                for (int r = 0; r < 4; r++) z = mfma_f32(xi[r], s[i][r], z);
+                y[i][i - d] = -z;
+            }
         }
+        __syncthreads();
+#pragma unroll
+        for (int i = 1; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < i; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[(16 * i + 4 * g + r) * LD + 16 * j + col] = y[i][j][r];
+    }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
