@@ -158,9 +158,14 @@ static int launch_rec(const DeltaArgs& a, hipStream_t st) {
 // Only S runs from chunk to chunk, so two kernels: delta_prep computes X diag(beta) and P of all chunks at once,
 // delta_scan walks each sequence's chunks.  The normalisation is row scales (rk, rq), so K and Q stay the bf16 they are.
 //
-// The products run on the bf16 MFMA at fp32's precision: an fp32 operand is three bf16 (x = hi + mid + lo, 8 bits each,
-// by truncation, exact), three products against K or Q, six against another such triple (what is dropped is below
-// 2^-24 of the terms).  That is 5 and 2.7 times the fp32 MFMA's rate.
+// The products run on the fp16 MFMA at nearly fp32's precision: an fp32 operand is two fp16, the value rounded to 11 bits and
+// what is left rounded to 11 more (to nearest: the error is below 2^-23 of the value), two products against K or Q, three
+// against another such pair (the fourth is below 2^-22 of the terms).  fp16's range is made to do by powers of two: every row
+// of K, Q, X and P and every column (lane) of S, R and U is scaled so that its largest value is about 2^14, which leaves the
+// lower halves normal down to 2^-28 of it; the powers are taken off with factors that are there anyway, or exactly after the
+// product.  bf16 operands (K and Q, 8 bits) fit one fp16.  Against three bf16 parts, which need no scales but three and six
+// products: the same error (1.6e-7 of the outputs), 16 of 24 and 9 of 18 MFMAs, two instructions a value for the parts
+// instead of 5.5, a third less of X and P to write and read.
 //
 // Everything that delta_scan multiplies from the left (K, Q, K^T, X diag(beta), P) lies in the workspace as MFMA
 // fragments, 1 KB each in lane order.  Inside a product the order of the summed index is free: taking it as an
@@ -172,7 +177,7 @@ constexpr int kFrag = 1024;                                   // bytes of a frag
 constexpr int kTri = 6;                                       // fragments (i, s) of a lower triangle: 16-row tile i, 32 columns s <= i / 2
 __host__ __device__ constexpr int tri(int i, int s) { return i < 2 ? i : 2 * i - 2 + s; }
 __host__ __device__ constexpr int64_t rec_k(int DK) { return (int64_t)(4 * (DK / 32) * 2 + DK / 16 * 2) * kFrag; }   // K, Q, K^T
-constexpr int64_t kRecV = 2 * 3 * kTri * kFrag + 4 * kC * 4;  // X diag(beta), P; row factors of K S and Q S, of U; e^(G_63)
+constexpr int64_t kRecV = 2 * 2 * kTri * kFrag + 5 * kC * 4;  // X diag(beta), P; factors: of K S, Q S, U, the output's; e^(G_63)
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
@@ -180,25 +185,67 @@ __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
 }
 __device__ __forceinline__ v4f mfma_f32(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// Eight fp32 (x then y) as three bf16 fragments.
-struct Split {
-    v4u h, m, l;
-};
-__device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-__device__ __forceinline__ uint32_t pack_hi(float a, float b) {
-    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+// LDS-DMA of 4 bytes a lane.
+__device__ __forceinline__ void dma4(const void* g, void* lds) {
+    __builtin_amdgcn_global_load_lds(g, (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
 }
-__device__ __forceinline__ Split split8(v4f x, v4f y) {
-    Split s;
+
+// fp16 operands
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ v4f mfma_f16(v4u a, v4u b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
+}
+
+// The power of two that brings values up to `most` to 2^14 .. 2^15, and its inverse.  Below 2^-60 it stays what it is there
+// (nothing overflows, and what such small values lose is far below the rest of their row or column); infinities and NaN
+// stay what they are.
+struct Pow2 {
+    float up, down;
+};
+__device__ __forceinline__ Pow2 pow2_of(float most) {
+    const uint32_t e = max(__float_as_uint(most) >> 23 & 0xff, 67u);
+    return Pow2{__uint_as_float((268 - e) << 23), __uint_as_float((e - 14) << 23)};
+}
+__device__ __forceinline__ float max_abs(float m, v4f x) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(x[r]));
+    return m;
+}
+// The largest of the four lanes of a column (lane % 16).
+__device__ __forceinline__ float column_max(float m) {
+    const uint32_t a = __float_as_uint(m);
+    const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    const uint32_t b = __float_as_uint(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+    const auto y = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+
+// Eight fp32 (x then y) times a power of two as two fp16 fragments: h = RN(x s), l = RN(x s - h), two values a pair of
+// instructions (the products are exact).
+struct Split {
+    v4u h, l;
+};
+__device__ __forceinline__ Split split8(v4f x, v4f y, float s) {
+    Split r;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         const float a = w < 2 ? x[2 * w] : y[2 * w - 4], b = w < 2 ? x[2 * w + 1] : y[2 * w - 3];
-        const float a1 = a - cut(a), b1 = b - cut(b);
-        s.h[w] = pack_hi(a, b);
-        s.m[w] = pack_hi(a1, b1);
-        s.l[w] = pack_hi(a1 - cut(a1), b1 - cut(b1));
+        uint32_t h, l;
+        asm("v_fma_mixlo_f16 %0, %1, %3, 0 op_sel_hi:[0,0,0]\n\t"
+            "v_fma_mixhi_f16 %0, %2, %3, 0 op_sel_hi:[0,0,0]" : "=&v"(h) : "v"(a), "v"(b), "v"(s));
+        asm("v_fma_mixlo_f16 %0, %1, %3, -%4 op_sel_hi:[0,0,1]\n\t"
+            "v_fma_mixhi_f16 %0, %2, %3, -%4 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
+            : "=&v"(l) : "v"(a), "v"(b), "v"(s), "v"(h));
+        r.h[w] = h;
+        r.l[w] = l;
     }
-    return s;
+    return r;
+}
+__device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+// Two bf16 times a power of two as two fp16 (exact within the range that the scale leaves).
+__device__ __forceinline__ uint32_t bf16x2_f16(uint32_t w, float s) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w << 16) * s,
+                                                                   cut(__uint_as_float(w)) * s));
 }
 
 // Chunk `id` of the workspace: sequence b's chunks start at id cu[b] / 64 + b, which leaves each sequence room for its
@@ -234,7 +281,7 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
     constexpr int KS = DK / 32, LD = kC + 4, LK = DK + 8, PR = DK / 8;   // PR: 16-byte pieces of a row
     __shared__ __align__(16) float x[kC * LD];                // K's, then Q's rows (bf16); A, then X, in place
     __shared__ double gsum[kC];
-    __shared__ float rkv[kC], rqv[kC], bev[kC], upv[kC], dnv[kC];
+    __shared__ float rkv[kC], rqv[kC], kup[kC], kdn[kC], qup[kC], bev[kC], upv[kC], dnv[kC], xdn[kC], odn[kC];
     static_assert(sizeof(x) >= kC * LK * 2, "K's rows");
     int first, count;
     if (!find_chunk(a, blockIdx.x, first, count)) return;
@@ -289,82 +336,82 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
 #pragma unroll
             for (int s = 0; s < KS; s++) f[i][s] = *reinterpret_cast<const v4u*>(rows + (16 * i + col) * LK + 32 * s + 8 * g);
     };
-    // as delta_scan's left operand, fragment (i, s): dims 32 s + 4 g + j, then 32 s + 16 + 4 g + j
-    auto copy = [&](char* to) {
+    // as delta_scan's left operand, scaled rows: fragment (i, s), dims 32 s + 4 g + j, then 32 s + 16 + 4 g + j
+    auto copy = [&](char* to, const float* up) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int s = 0; s < KS; s++) {
                 const uint16_t* r = rows + (16 * i + col) * LK + 32 * s + 4 * g;
                 const v2u lo = *reinterpret_cast<const v2u*>(r), hi = *reinterpret_cast<const v2u*>(r + 16);
-                *reinterpret_cast<v4u*>(to + (i * KS + s) * kFrag + lane * 16) = v4u{lo[0], lo[1], hi[0], hi[1]};
+                const float u = up[16 * i + col];
+                *reinterpret_cast<v4u*>(to + (i * KS + s) * kFrag + lane * 16) =
+                    v4u{bf16x2_f16(lo[0], u), bf16x2_f16(lo[1], u), bf16x2_f16(hi[0], u), bf16x2_f16(hi[1], u)};
             }
+    };
+    // the rows' lengths, from the diagonal of K K^T or Q Q^T: their scales and, if asked, the normalising factors
+    auto lengths = [&](const v4u (&f)[4][KS], float* unit, float* up, float scale) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v4f d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; s++) d = mfma_bf16(f[i][s], f[i][s], d);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (4 * g + r == col) unit[16 * i + col] = d[r];
+        }
+        __syncthreads();
+        const float sq = unit[lane];
+        const Pow2 p = pow2_of(sqrt_rn(sq));                  // (no value of a row is above its length)
+        unit[lane] = (a.norm ? div_rn(1.f, sqrt_rn(sq + a.eps)) : 1.f) * scale;
+        up[lane] = p.up;
+        __syncthreads();
+        return p.down;
     };
     v4u kf[4][KS], qf[4][KS];
     put(kr);
     get(kf);
+    kdn[lane] = lengths(kf, rkv, kup, 1.f);
     // this key head's fragments of K, K^T and Q are written by its first, second and last value head's wave
-    if (part == 0) copy(rk);
+    if (part == 0) copy(rk, kup);
     if (part == (share > 1 ? 1 : 0)) {
         // K^T: fragment (d, s), row 16 d + col, tokens 32 s + 4 g + j and 32 s + 16 + 4 g + j
         char* ft = rk + 8 * KS * kFrag;
 #pragma unroll
-        for (int d = 0; d < DK / 16; d++)
+        for (int s = 0; s < 2; s++) {
+            v4f up[2];
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                uint32_t u[8];
+            for (int e = 0; e < 2; e++) up[e] = *reinterpret_cast<const v4f*>(kup + 32 * s + 16 * e + 4 * g);
 #pragma unroll
-                for (int j = 0; j < 8; j++) u[j] = rows[(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col];
-                *reinterpret_cast<v4u*>(ft + (2 * d + s) * kFrag + lane * 16) =
-                    v4u{u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16)};
+            for (int d = 0; d < DK / 16; d++) {
+                float u[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    u[j] = bf16_to_f32(rows[(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col]) * up[j / 4][j % 4];
+                v4u w;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    w[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(u[2 * j], u[2 * j + 1]));
+                *reinterpret_cast<v4u*>(ft + (2 * d + s) * kFrag + lane * 16) = w;
             }
+        }
     }
     put(qr);
     get(qf);
-    if (part == share - 1) copy(rk + 4 * KS * kFrag);
-
-    // squares of the rows' lengths: the diagonals of K K^T and Q Q^T
-    if (a.norm) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v4f kk = {0.f, 0.f, 0.f, 0.f}, qq = kk;
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                kk = mfma_bf16(kf[i][s], kf[i][s], kk);
-                qq = mfma_bf16(qf[i][s], qf[i][s], qq);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (4 * g + r == col) rkv[16 * i + col] = kk[r], rqv[16 * i + col] = qq[r];
-        }
-        __syncthreads();
-    }
-    {
-        const float sk = a.norm ? div_rn(1.f, sqrt_rn(rkv[lane] + a.eps)) : 1.f;
-        const float sq = (a.norm ? div_rn(1.f, sqrt_rn(rqv[lane] + a.eps)) : 1.f) * a.scale;
-        rkv[lane] = sk;
-        rqv[lane] = sq;
-        float* vec = reinterpret_cast<float*>(rv + 6 * kTri * kFrag);
-        const double gl = gsum[lane], gc = gsum[kC - 1];
-        const float e = expf((float)gl);
-        vec[lane] = e * sk;
-        vec[kC + lane] = e * sq;
-        vec[2 * kC + lane] = expf((float)(gc - gl)) * sk;
-        vec[3 * kC + lane] = expf((float)gc);
-    }
-    __syncthreads();
+    const float qdn = lengths(qf, rqv, qup, a.scale);
+    if (part == share - 1) copy(rk + 4 * KS * kFrag, qup);
 
     // k_i . k_j and q_i . k_j, tiles j <= i, transposed: a lane holds row i = col for columns 4 g + r, which is a
     // fragment's order
+    v4f pt[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int row = 16 * i + col;
         const double gi = gsum[row];
         const float up = upv[row], ki = bev[row] * rkv[row], qi = rqv[row];
-        v4f pt[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            pt[j] = v4f{0.f, 0.f, 0.f, 0.f};
+            pt[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
             if (j > i) continue;
             v4f kk = {0.f, 0.f, 0.f, 0.f}, qk = kk, am, f;
 #pragma unroll
@@ -385,17 +432,9 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
             for (int r = 0; r < 4; r++) {
                 f[r] *= rkv[c0 + r];
                 am[r] = c0 + r < row ? f[r] * ki * kk[r] : 0.f;
-                pt[j][r] = c0 + r <= row ? f[r] * qi * qk[r] : 0.f;
+                pt[i][j][r] = c0 + r <= row ? f[r] * qi * qk[r] : 0.f;
             }
             *reinterpret_cast<v4f*>(x + row * LD + c0) = am;
-        }
-#pragma unroll
-        for (int s = 0; s <= i / 2; s++) {
-            const Split p = split8(pt[2 * s], pt[2 * s + 1]);
-            char* to = rv + 3 * (kTri + tri(i, s)) * kFrag + lane * 16;
-            *reinterpret_cast<v4u*>(to) = p.h;
-            *reinterpret_cast<v4u*>(to + kFrag) = p.m;
-            *reinterpret_cast<v4u*>(to + 2 * kFrag) = p.l;
         }
     }
     __syncthreads();
@@ -460,27 +499,50 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
                 for (int r = 0; r < 4; r++) x[(16 * i + 4 * g + r) * LD + 16 * j + col] = y[i][j][r];
     }
     __syncthreads();
+    // X diag(beta), and then P, whose columns take X's rows' scales (U's rows come out in them)
+    auto put_tri = [&](int i, const v4f (&h)[4], float* down, char* to) {
+        float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
+        for (int j = 0; j <= i; j++) m = max_abs(m, h[j]);
+        const Pow2 p = pow2_of(column_max(m));
+        down[16 * i + col] = p.down;
 #pragma unroll
         for (int s = 0; s <= i / 2; s++) {
-            v4f h[2];
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const int c = 32 * s + 16 * e + 4 * g;
-                h[e] = v4f{0.f, 0.f, 0.f, 0.f};
-                if (2 * s + e <= i) {
-                    h[e] = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + c);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) h[e][r] *= bev[c + r];
-                }
-            }
-            const Split p = split8(h[0], h[1]);
-            char* f = rv + 3 * tri(i, s) * kFrag + lane * 16;
-            *reinterpret_cast<v4u*>(f) = p.h;
-            *reinterpret_cast<v4u*>(f + kFrag) = p.m;
-            *reinterpret_cast<v4u*>(f + 2 * kFrag) = p.l;
+            const Split sp = split8(h[2 * s], h[2 * s + 1], p.up);
+            *reinterpret_cast<v4u*>(to + 2 * tri(i, s) * kFrag + lane * 16) = sp.h;
+            *reinterpret_cast<v4u*>(to + (2 * tri(i, s) + 1) * kFrag + lane * 16) = sp.l;
         }
+    };
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        v4f h[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            h[j] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (j <= i)
+                h[j] = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * j + 4 * g) *
+                       *reinterpret_cast<const v4f*>(bev + 16 * j + 4 * g);
+        }
+        put_tri(i, h, xdn, rv);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int j = 0; j <= i; j++) pt[i][j] *= *reinterpret_cast<const v4f*>(xdn + 16 * j + 4 * g);
+        put_tri(i, pt[i], odn, rv + 2 * kTri * kFrag);
+    }
+    __syncthreads();
+    {
+        float* vec = reinterpret_cast<float*>(rv + 4 * kTri * kFrag);
+        const double gl = gsum[lane], gc = gsum[kC - 1];
+        const float e = expf((float)gl), kd = rkv[lane] * kdn[lane], od = odn[lane];
+        vec[lane] = e * kd;
+        vec[kC + lane] = e * rqv[lane] * qdn * (1.f / od);    // (a power of two)
+        vec[2 * kC + lane] = expf((float)(gc - gl)) * kd * xdn[lane];
+        vec[3 * kC + lane] = od;
+        vec[4 * kC + lane] = expf((float)gc);
+    }
 }
 
 // A workgroup walks the chunks of one sequence and value head for 32 columns of the state, twelve waves, three to a SIMD.
@@ -494,8 +556,8 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
 //   loading waves (Q, X, factors in)     | next K, P, K^T in      | next Q, X, factors in
 template <int DK>
 struct ScanShared {
-    v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], kt[DK / 16 * 2][64], x[3 * kTri][64], p[3 * kTri][64];
-    float vec[2][4 * kC];                                     // a chunk's factors, the next one's beside them
+    v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], kt[DK / 16 * 2][64], x[2 * kTri][64], p[2 * kTri][64];
+    float vec[2][5 * kC];                                     // a chunk's factors, the next one's beside them
     v4f sx[2][DK / 16][64], kx[2][4][64], ux[2][6][64], ox[2][4][64];
     uint32_t touched[64];
 };
@@ -514,23 +576,23 @@ __device__ __forceinline__ void mul_rows(v4f (&acc)[4], const v4u (*f)[64], int 
 #pragma unroll
     for (int i = 0; i < 4; i++) r[i] = f[i * (DK / 32) + HALF * (DK / 64) + k][lane];
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.l, acc[i]);
+    for (int i = 0; i < 4; i++) acc[i] = mfma_f16(r[i], s.l, acc[i]);
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.m, acc[i]);
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.h, acc[i]);
+    for (int i = 0; i < 4; i++) acc[i] = mfma_f16(r[i], s.h, acc[i]);
 }
-// acc += (X diag(beta) or P, the columns of the half's tokens)(three-part s), the small products first
+// acc += (X diag(beta) or P, the columns of the half's tokens) s, the small products first
 template <int HALF>
 __device__ __forceinline__ void mul_tri(v4f (&acc)[4], const v4u (*f)[64], const Split& s) {
     const int lane = threadIdx.x & 63;
+    v4u h[4];
 #pragma unroll
-    for (int p = 0; p < 6; p++) {
-        const int x = p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
-        const v4u& y = p == 2 ? s.l : p == 1 || p == 4 ? s.m : s.h;
+    for (int i = 2 * HALF; i < 4; i++) h[i] = f[2 * tri(i, HALF)][lane];
 #pragma unroll
-        for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_bf16(f[3 * tri(i, HALF) + x][lane], y, acc[i]);
-    }
+    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(f[2 * tri(i, HALF) + 1][lane], s.h, acc[i]);
+#pragma unroll
+    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(h[i], s.l, acc[i]);
+#pragma unroll
+    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(h[i], s.h, acc[i]);
 }
 
 template <int DK, int DV, int HALF>
@@ -571,8 +633,14 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
         v4f ks[4], u[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) ks[i] = u[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        float sm = 0.f;
 #pragma unroll
-        for (int k = 0; k < KH; k++) mul_rows<DK, HALF>(ks, x.k, k, split8(s[2 * k], s[2 * k + 1]));
+        for (int d = 0; d < DH; d++) sm = max_abs(sm, s[d]);
+        const Pow2 sp = pow2_of(column_max(sm));
+#pragma unroll
+        for (int k = 0; k < KH; k++) mul_rows<DK, HALF>(ks, x.k, k, split8(s[2 * k], s[2 * k + 1], sp.up));
+#pragma unroll
+        for (int i = 0; i < 4; i++) ks[i] *= sp.down;
         // the other half's tokens' sums out, this half's in
         x.kx[w][2 - 2 * HALF][lane] = ks[2 - 2 * HALF];
         x.kx[w][3 - 2 * HALF][lane] = ks[3 - 2 * HALF];
@@ -590,7 +658,10 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
             if (left < kC) offsets(left);
             load_v();
         }
-        mul_tri<HALF>(u, x.x, split8(rr[0], rr[1]));
+        const Pow2 rp = pow2_of(column_max(max_abs(max_abs(0.f, rr[0]), rr[1])));
+        mul_tri<HALF>(u, x.x, split8(rr[0], rr[1], rp.up));
+#pragma unroll
+        for (int i = 2 * HALF; i < 4; i++) u[i] *= rp.down;
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++) x.ux[w][i + 2 * HALF][lane] = u[i];
         lds_barrier();
@@ -605,22 +676,29 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) u[i] *= *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
-        const float ec = vec[3 * kC];
+        float um = 0.f;
 #pragma unroll
-        for (int d = 0; d < DH; d++) s[d] *= ec;
+        for (int i = 0; i < 4; i++) um = max_abs(um, u[i]);
+        const Pow2 up = pow2_of(column_max(um));
+        v4f add[DH];
+#pragma unroll
+        for (int d = 0; d < DH; d++) add[d] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const Split us = split8(u[2 * e], u[2 * e + 1]);
+            const Split us = split8(u[2 * e], u[2 * e + 1], up.up);
             v4u kt[DH];
 #pragma unroll
             for (int d = 0; d < DH; d++) kt[d] = x.kt[2 * (HALF * DH + d) + e][lane];
 #pragma unroll
-            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d], us.l, s[d]);
+            for (int d = 0; d < DH; d++) add[d] = mfma_f16(kt[d], us.l, add[d]);
 #pragma unroll
-            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d], us.m, s[d]);
-#pragma unroll
-            for (int d = 0; d < DH; d++) s[d] = mfma_bf16(kt[d], us.h, s[d]);
+            for (int d = 0; d < DH; d++) add[d] = mfma_f16(kt[d], us.h, add[d]);
         }
+        const float ec = vec[4 * kC];
+#pragma unroll
+        for (int d = 0; d < DH; d++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) s[d][r] = fmaf(add[d][r], up.down, ec * s[d][r]);
 #pragma unroll
         for (int d = 0; d < DH; d++) x.sx[w][HALF * DH + d][lane] = s[d];
     }
@@ -642,14 +720,16 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
     // (never waited for: these waves load nothing else)
     auto touch = [&](const char* r) {
         for (int i = (2 * m + w) * 64 + lane; i < LINES; i += per * 128)
-            __builtin_amdgcn_global_load_lds(r + i * 128, (__attribute__((address_space(3))) void*)x.touched, 4, 0, 0);
+            dma4(r + i * 128, x.touched);
     };
     v4f mine[2];
     float* out = a.out + (int64_t)at.first * a.ldo + at.head * a.ho_s + at.c0;
     // the last chunk's sums of this half's tokens, joined, then stored (`left` rows of it are there)
-    auto join = [&] {
+    auto join = [&](int c) {
 #pragma unroll
-        for (int i = 0; i < 2; i++) mine[i] += x.ox[w][2 * HALF + i][lane];
+        for (int i = 0; i < 2; i++)
+            mine[i] = (mine[i] + x.ox[w][2 * HALF + i][lane]) *
+                      *reinterpret_cast<const v4f*>(x.vec[c & 1] + 3 * kC + 32 * HALF + 16 * i + 4 * g);
     };
     auto store = [&](int left) {
 #pragma unroll
@@ -665,15 +745,22 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
     for (int c = 0; c < at.nc; c++) {
         const float* vec = x.vec[c & 1] + kC;
         lds_barrier();
-        if (c) join();
+        if (c) join(c - 1);
         v4f o[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        v4f s[DH];
+        float sm = 0.f;
 #pragma unroll
-        for (int k = 0; k < KH; k++)
-            mul_rows<DK, HALF>(o, x.q, k, split8(x.sx[w][HALF * DH + 2 * k][lane], x.sx[w][HALF * DH + 2 * k + 1][lane]));
+        for (int d = 0; d < DH; d++) {
+            s[d] = x.sx[w][HALF * DH + d][lane];
+            sm = max_abs(sm, s[d]);
+        }
+        const Pow2 sp = pow2_of(column_max(sm));
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] *= *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
+        for (int k = 0; k < KH; k++) mul_rows<DK, HALF>(o, x.q, k, split8(s[2 * k], s[2 * k + 1], sp.up));
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] *= sp.down * *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
         lds_barrier();
         if (c) store(kC);                                     // (here the state waves have more to do than these)
         if (c + 2 < at.nc) touch(rec + (c + 2) * step);
@@ -682,7 +769,15 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
             u0 += x.ux[w][4][lane];
             u1 += x.ux[w][5][lane];
         }
-        mul_tri<HALF>(o, x.p, split8(u0, u1));
+        const Pow2 up = pow2_of(column_max(max_abs(max_abs(0.f, u0), u1)));
+        v4f pu[4];
+#pragma unroll
+        for (int i = 2 * HALF; i < 4; i++) pu[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        mul_tri<HALF>(pu, x.p, split8(u0, u1, up.up));
+#pragma unroll
+        for (int i = 2 * HALF; i < 4; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) o[i][r] = fmaf(pu[i][r], up.down, o[i][r]);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             x.ox[w][2 - 2 * HALF + i][lane] = o[2 - 2 * HALF + i];
@@ -690,7 +785,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
         }
     }
     lds_barrier();
-    join();
+    join(at.nc - 1);
     store(at.count - (at.nc - 1) * kC);
 }
 
@@ -698,13 +793,14 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
 template <int DK>
 __device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, const char* rv, int q, ScanShared<DK>& x) {
     const int64_t rks = at.rks, rvs = at.rvs;
-    constexpr int NK = 4 * (DK / 32), NT = DK / 16 * 2, NX = 3 * kTri;
+    constexpr int NK = 4 * (DK / 32), NT = DK / 16 * 2, NX = 2 * kTri;
     const int lane = threadIdx.x & 63;
     auto bring = [&](v4u (*to)[64], const char* from, int count) {
         for (int i = q; i < count; i += 4) dma16(from + i * kFrag + lane * 16, to[i]);
     };
     auto factors = [&](int c, const char* r) {
         if (q == 0) dma16(r + 2 * NX * kFrag + lane * 16, x.vec[c & 1]);
+        if (q == 1) dma4(r + (2 * NX + 1) * kFrag + lane * 4, x.vec[c & 1] + 4 * kC);
     };
     bring(x.k, rk, NK);
     bring(x.q, rk + NK * kFrag, NK);
