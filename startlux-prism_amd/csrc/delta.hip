@@ -553,11 +553,12 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
 // come from L2.  Two barriers per chunk:
 //   state waves   K S, halves out        | halves in, R, X R out  | U in, S <- ..., S out
 //   output waves  (P U of the last one)  | S in, Q S              | P U, halves out
-//   loading waves (Q, X, factors in)     | next K, P, K^T in      | next Q, X, factors in
+//   loading waves                        | next K in              | all else of the next chunk in
 template <int DK>
 struct ScanShared {
-    v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], kt[DK / 16 * 2][64], x[2 * kTri][64], p[2 * kTri][64];
-    float vec[2][5 * kC];                                     // a chunk's factors, the next one's beside them
+    v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], x[2 * kTri][64];
+    v4u kt[2][DK / 16 * 2][64], p[2][2 * kTri][64];           // a chunk's, the next one's beside them
+    float vec[2][5 * kC];                                     // the factors likewise
     v4f sx[2][DK / 16][64], kx[2][4][64], ux[2][6][64], ox[2][4][64];
     uint32_t touched[64];
 };
@@ -688,7 +689,7 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
             const Split us = split8(u[2 * e], u[2 * e + 1], up.up);
             v4u kt[DH];
 #pragma unroll
-            for (int d = 0; d < DH; d++) kt[d] = x.kt[2 * (HALF * DH + d) + e][lane];
+            for (int d = 0; d < DH; d++) kt[d] = x.kt[c & 1][2 * (HALF * DH + d) + e][lane];
 #pragma unroll
             for (int d = 0; d < DH; d++) add[d] = mfma_f16(kt[d], us.l, add[d]);
 #pragma unroll
@@ -773,7 +774,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
         v4f pu[4];
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++) pu[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        mul_tri<HALF>(pu, x.p, split8(u0, u1, up.up));
+        mul_tri<HALF>(pu, x.p[c & 1], split8(u0, u1, up.up));
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++)
 #pragma unroll
@@ -802,25 +803,24 @@ __device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, cons
         if (q == 0) dma16(r + 2 * NX * kFrag + lane * 16, x.vec[c & 1]);
         if (q == 1) dma4(r + (2 * NX + 1) * kFrag + lane * 4, x.vec[c & 1] + 4 * kC);
     };
+    auto later = [&](int c, const char* k, const char* v) {   // what chunk c needs after its first barrier
+        bring(x.q, k + NK * kFrag, NK);
+        bring(x.x, v, NX);
+        factors(c, v);
+        bring(x.p[c & 1], v + NX * kFrag, NX);
+        bring(x.kt[c & 1], k + 2 * NK * kFrag, NT);
+    };
     bring(x.k, rk, NK);
-    bring(x.q, rk + NK * kFrag, NK);
-    bring(x.x, rv, NX);
-    factors(0, rv);
+    later(0, rk, rv);
     vm_wait<0>();
     lds_barrier();
     for (int c = 0; c < at.nc; c++) {
         const bool more = c + 1 < at.nc;
         lds_barrier();
         if (more) bring(x.k, rk + rks, NK);
-        bring(x.p, rv + NX * kFrag, NX);
-        bring(x.kt, rk + 2 * NK * kFrag, NT);
         vm_wait<0>();
         lds_barrier();
-        if (more) {
-            bring(x.q, rk + rks + NK * kFrag, NK);
-            bring(x.x, rv + rvs, NX);
-            factors(c + 1, rv + rvs);
-        }
+        if (more) later(c + 1, rk + rks, rv + rvs);
         vm_wait<0>();
         rk += rks, rv += rvs;
     }
