@@ -273,6 +273,11 @@ __device__ __forceinline__ bool find_chunk(const DeltaArgs& a, int id, int& firs
     return false;
 }
 
+// The records go past the caches (delta_scan reads them after all are written): 8191 tokens 396 -> 379 us in all.
+__device__ __forceinline__ void put_frag(char* base, v4u v) {
+    __builtin_nontemporal_store(v, reinterpret_cast<v4u*>(base + (threadIdx.x & 63) * 16));
+}
+
 // One wave per chunk (blockIdx.x) and value head (blockIdx.y).  Rows are loaded in their own order (a row per lane would take
 // the memory pipeline four times as long) and become fragments through LDS.  The decays between tokens of different 16-row
 // tiles are products of three that are at most 1, so that 16 exponentials a lane (the diagonal tiles') and a few are enough
@@ -346,8 +351,8 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
                 const uint16_t* r = rows + (16 * i + col) * LK + 32 * s + 4 * g;
                 const v2u lo = *reinterpret_cast<const v2u*>(r), hi = *reinterpret_cast<const v2u*>(r + 16);
                 const float u = up[16 * i + col];
-                *reinterpret_cast<v4u*>(to + (i * KS + s) * kFrag + lane * 16) =
-                    v4u{bf16x2_f16(lo[0], u), bf16x2_f16(lo[1], u), bf16x2_f16(hi[0], u), bf16x2_f16(hi[1], u)};
+                put_frag(to + (i * KS + s) * kFrag,
+                         v4u{bf16x2_f16(lo[0], u), bf16x2_f16(lo[1], u), bf16x2_f16(hi[0], u), bf16x2_f16(hi[1], u)});
             }
     };
     // the rows' lengths, from the diagonal of K K^T or Q Q^T: their scales and, if asked, the normalising factors
@@ -393,7 +398,7 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     w[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(u[2 * j], u[2 * j + 1]));
-                *reinterpret_cast<v4u*>(ft + (2 * d + s) * kFrag + lane * 16) = w;
+                put_frag(ft + (2 * d + s) * kFrag, w);
             }
         }
     }
@@ -510,8 +515,8 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
 #pragma unroll
         for (int s = 0; s <= i / 2; s++) {
             const Split sp = split8(h[2 * s], h[2 * s + 1], p.up);
-            *reinterpret_cast<v4u*>(to + 2 * tri(i, s) * kFrag + lane * 16) = sp.h;
-            *reinterpret_cast<v4u*>(to + (2 * tri(i, s) + 1) * kFrag + lane * 16) = sp.l;
+            put_frag(to + 2 * tri(i, s) * kFrag, sp.h);
+            put_frag(to + (2 * tri(i, s) + 1) * kFrag, sp.l);
         }
     };
 #pragma unroll
@@ -570,31 +575,41 @@ struct ScanAt {
     int64_t rks, rvs;                                         // bytes from a chunk's records to the next one's
 };
 
-// acc += (rows of K or Q, the half's k)(the half's rows of S)
+// A product's fragments are read from LDS into registers.  The compiler spreads the reads over the phase; forced to its
+// start, to have their latency behind what the right operand still takes, they come as bursts that hold the others up:
+// 392 us for 8191 tokens instead of 372 (LDS moves some 370 KB a chunk, over half of what it can).
+// K or Q: 4 token tiles, the half's k
 template <int DK, int HALF>
-__device__ __forceinline__ void mul_rows(v4f (&acc)[4], const v4u (*f)[64], int k, const Split& s) {
-    const int lane = threadIdx.x & 63;
-    v4u r[4];
+__device__ __forceinline__ void read_rows(v4u (&r)[DK / 64][4], const v4u (*f)[64]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = f[i * (DK / 32) + HALF * (DK / 64) + k][lane];
+    for (int k = 0; k < DK / 64; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[k][i] = f[i * (DK / 32) + HALF * (DK / 64) + k][threadIdx.x & 63];
+}
+// X diag(beta) or P: the columns of the half's tokens
+template <int HALF>
+__device__ __forceinline__ void read_tri(v4u (&r)[4][2], const v4u (*f)[64]) {
+#pragma unroll
+    for (int i = 2 * HALF; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) r[i][e] = f[2 * tri(i, HALF) + e][threadIdx.x & 63];
+}
+// acc += r s
+__device__ __forceinline__ void mul_rows(v4f (&acc)[4], const v4u (&r)[4], const Split& s) {
 #pragma unroll
     for (int i = 0; i < 4; i++) acc[i] = mfma_f16(r[i], s.l, acc[i]);
 #pragma unroll
     for (int i = 0; i < 4; i++) acc[i] = mfma_f16(r[i], s.h, acc[i]);
 }
-// acc += (X diag(beta) or P, the columns of the half's tokens) s, the small products first
+// acc += r s, the small products first
 template <int HALF>
-__device__ __forceinline__ void mul_tri(v4f (&acc)[4], const v4u (*f)[64], const Split& s) {
-    const int lane = threadIdx.x & 63;
-    v4u h[4];
+__device__ __forceinline__ void mul_tri(v4f (&acc)[4], const v4u (&r)[4][2], const Split& s) {
 #pragma unroll
-    for (int i = 2 * HALF; i < 4; i++) h[i] = f[2 * tri(i, HALF)][lane];
+    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(r[i][1], s.h, acc[i]);
 #pragma unroll
-    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(f[2 * tri(i, HALF) + 1][lane], s.h, acc[i]);
+    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(r[i][0], s.l, acc[i]);
 #pragma unroll
-    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(h[i], s.l, acc[i]);
-#pragma unroll
-    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(h[i], s.h, acc[i]);
+    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(r[i][0], s.h, acc[i]);
 }
 
 template <int DK, int DV, int HALF>
@@ -633,6 +648,8 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
         const float* vec = x.vec[c & 1];
         const int left = at.count - (c + 1) * kC;             // rows after this chunk
         v4f ks[4], u[4];
+        v4u kr[KH][4], tr[4][2], tk[DH][2];
+        read_rows<DK, HALF>(kr, x.k);
 #pragma unroll
         for (int i = 0; i < 4; i++) ks[i] = u[i] = v4f{0.f, 0.f, 0.f, 0.f};
         float sm = 0.f;
@@ -640,20 +657,25 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
         for (int d = 0; d < DH; d++) sm = max_abs(sm, s[d]);
         const Pow2 sp = pow2_of(column_max(sm));
 #pragma unroll
-        for (int k = 0; k < KH; k++) mul_rows<DK, HALF>(ks, x.k, k, split8(s[2 * k], s[2 * k + 1], sp.up));
+        for (int k = 0; k < KH; k++) mul_rows(ks, kr[k], split8(s[2 * k], s[2 * k + 1], sp.up));
 #pragma unroll
         for (int i = 0; i < 4; i++) ks[i] *= sp.down;
         // the other half's tokens' sums out, this half's in
         x.kx[w][2 - 2 * HALF][lane] = ks[2 - 2 * HALF];
         x.kx[w][3 - 2 * HALF][lane] = ks[3 - 2 * HALF];
         lds_barrier();
-        v4f rr[2];
+        v4f rr[2], ek[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const v4f ek = *reinterpret_cast<const v4f*>(vec + 32 * HALF + 16 * i + 4 * g);
-            rr[i] = ks[2 * HALF + i] + x.kx[w][2 * HALF + i][lane];
+            rr[i] = x.kx[w][2 * HALF + i][lane];
+            ek[i] = *reinterpret_cast<const v4f*>(vec + 32 * HALF + 16 * i + 4 * g);
+        }
+        read_tri<HALF>(tr, x.x);
 #pragma unroll
-            for (int r = 0; r < 4; r++) rr[i][r] = fmaf(-ek[r], rr[i][r], bf16_to_f32(v[i][r]));
+        for (int i = 0; i < 2; i++) {
+            rr[i] += ks[2 * HALF + i];
+#pragma unroll
+            for (int r = 0; r < 4; r++) rr[i][r] = fmaf(-ek[i][r], rr[i][r], bf16_to_f32(v[i][r]));
         }
         if (left > 0) {
             vp += 2 * kC * a.ldv;
@@ -661,23 +683,28 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
             load_v();
         }
         const Pow2 rp = pow2_of(column_max(max_abs(max_abs(0.f, rr[0]), rr[1])));
-        mul_tri<HALF>(u, x.x, split8(rr[0], rr[1], rp.up));
+        mul_tri<HALF>(u, tr, split8(rr[0], rr[1], rp.up));
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++) u[i] *= rp.down;
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++) x.ux[w][i + 2 * HALF][lane] = u[i];
         lds_barrier();
-        if (HALF == 0) {
-            u[2] += x.ux[w][4][lane];
-            u[3] += x.ux[w][5][lane];
-        } else {
-            u[0] = x.ux[w][0][lane];
-            u[1] = x.ux[w][1][lane];
-            u[2] += x.ux[w][2][lane];
-            u[3] += x.ux[w][3][lane];
+        v4f ux[4], ew[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i >= 2 || HALF) ux[i] = x.ux[w][i < 2 || HALF ? i : i + 2][lane];
+            ew[i] = *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) u[i] *= *reinterpret_cast<const v4f*>(vec + 2 * kC + 16 * i + 4 * g);
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+            for (int d = 0; d < DH; d++) tk[d][e] = x.kt[c & 1][2 * (HALF * DH + d) + e][lane];
+        const float ec = vec[4 * kC];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (i >= 2 || HALF) u[i] += ux[i];                // (half 1 has no part of u[0], u[1]: zeros)
+            u[i] *= ew[i];
+        }
         float um = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; i++) um = max_abs(um, u[i]);
@@ -688,15 +715,11 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const Split us = split8(u[2 * e], u[2 * e + 1], up.up);
-            v4u kt[DH];
 #pragma unroll
-            for (int d = 0; d < DH; d++) kt[d] = x.kt[c & 1][2 * (HALF * DH + d) + e][lane];
+            for (int d = 0; d < DH; d++) add[d] = mfma_f16(tk[d][e], us.l, add[d]);
 #pragma unroll
-            for (int d = 0; d < DH; d++) add[d] = mfma_f16(kt[d], us.l, add[d]);
-#pragma unroll
-            for (int d = 0; d < DH; d++) add[d] = mfma_f16(kt[d], us.h, add[d]);
+            for (int d = 0; d < DH; d++) add[d] = mfma_f16(tk[d][e], us.h, add[d]);
         }
-        const float ec = vec[4 * kC];
 #pragma unroll
         for (int d = 0; d < DH; d++)
 #pragma unroll
@@ -739,7 +762,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int t = 32 * HALF + 16 * i + 4 * g + r;
-                if (left >= kC || t < left) out[(int64_t)t * a.ldo] = mine[i][r];
+                if (left >= kC || t < left) __builtin_nontemporal_store(mine[i][r], out + (int64_t)t * a.ldo);
             }
         out += kC * a.ldo;
     };
@@ -751,22 +774,26 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
         v4f o[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        v4f s[DH];
+        v4f s[DH], eq[4];
+        v4u qr[KH][4], tr[4][2];
+#pragma unroll
+        for (int d = 0; d < DH; d++) s[d] = x.sx[w][HALF * DH + d][lane];
+        read_rows<DK, HALF>(qr, x.q);
+#pragma unroll
+        for (int i = 0; i < 4; i++) eq[i] = *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
         float sm = 0.f;
 #pragma unroll
-        for (int d = 0; d < DH; d++) {
-            s[d] = x.sx[w][HALF * DH + d][lane];
-            sm = max_abs(sm, s[d]);
-        }
+        for (int d = 0; d < DH; d++) sm = max_abs(sm, s[d]);
         const Pow2 sp = pow2_of(column_max(sm));
 #pragma unroll
-        for (int k = 0; k < KH; k++) mul_rows<DK, HALF>(o, x.q, k, split8(s[2 * k], s[2 * k + 1], sp.up));
+        for (int k = 0; k < KH; k++) mul_rows(o, qr[k], split8(s[2 * k], s[2 * k + 1], sp.up));
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] *= sp.down * *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
+        for (int i = 0; i < 4; i++) o[i] *= sp.down * eq[i];
         lds_barrier();
         if (c) store(kC);                                     // (here the state waves have more to do than these)
         if (c + 2 < at.nc) touch(rec + (c + 2) * step);
         v4f u0 = x.ux[w][2 * HALF][lane], u1 = x.ux[w][2 * HALF + 1][lane];
+        read_tri<HALF>(tr, x.p[c & 1]);
         if (HALF) {
             u0 += x.ux[w][4][lane];
             u1 += x.ux[w][5][lane];
@@ -775,7 +802,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
         v4f pu[4];
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++) pu[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        mul_tri<HALF>(pu, x.p[c & 1], split8(u0, u1, up.up));
+        mul_tri<HALF>(pu, tr, split8(u0, u1, up.up));
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++)
 #pragma unroll
