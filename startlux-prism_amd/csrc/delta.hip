@@ -165,7 +165,7 @@ static int launch_rec(const DeltaArgs& a, hipStream_t st) {
 // of K, Q, X and P and every column (lane) of S, R and U is scaled so that its largest value is about 2^14, which leaves the
 // lower halves normal down to 2^-28 of it; the powers are taken off with factors that are there anyway, or exactly after the
 // product.  bf16 operands (K and Q, 8 bits) fit one fp16.  Against three bf16 parts, which need no scales but three and six
-// products: the same error (1.6e-7 of the outputs), 16 of 24 and 9 of 18 MFMAs, two instructions a value for the parts
+// products: the same error (1.6e-7 of the outputs), 16 of 24 and 9 of 18 MFMAs, three instructions a value for the parts
 // instead of 5.5, a third less of X and P to write and read.
 //
 // Everything that delta_scan multiplies from the left (K, Q, K^T, X diag(beta), P) lies in the workspace as MFMA
@@ -221,8 +221,11 @@ __device__ __forceinline__ float column_max(float m) {
     return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 
-// Eight fp32 (x then y) times a power of two as two fp16 fragments: h = RN(x s), l = RN(x s - h), two values a pair of
-// instructions (the products are exact).
+// Eight fp32 (x then y) times a power of two as two fp16 fragments: h = RN(x s), l = RN(x s - h), six instructions for two
+// values (products and differences are exact).  No inline assembly: the compiler does not put the wait states between it and
+// an MFMA that reads its result.
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 struct Split {
     v4u h, l;
 };
@@ -231,14 +234,10 @@ __device__ __forceinline__ Split split8(v4f x, v4f y, float s) {
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         const float a = w < 2 ? x[2 * w] : y[2 * w - 4], b = w < 2 ? x[2 * w + 1] : y[2 * w - 3];
-        uint32_t h, l;
-        asm("v_fma_mixlo_f16 %0, %1, %3, 0 op_sel_hi:[0,0,0]\n\t"
-            "v_fma_mixhi_f16 %0, %2, %3, 0 op_sel_hi:[0,0,0]" : "=&v"(h) : "v"(a), "v"(b), "v"(s));
-        asm("v_fma_mixlo_f16 %0, %1, %3, -%4 op_sel_hi:[0,0,1]\n\t"
-            "v_fma_mixhi_f16 %0, %2, %3, -%4 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
-            : "=&v"(l) : "v"(a), "v"(b), "v"(s), "v"(h));
-        r.h[w] = h;
-        r.l[w] = l;
+        const v2h h = __builtin_convertvector((v2f{a * s, b * s}), v2h);
+        const v2f d = {__builtin_fmaf(a, s, -(float)h[0]), __builtin_fmaf(b, s, -(float)h[1])};
+        r.h[w] = __builtin_bit_cast(uint32_t, h);
+        r.l[w] = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, v2h));
     }
     return r;
 }
