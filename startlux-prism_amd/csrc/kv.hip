@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // rounding is the only one that shows; the second MFMA is free beside the cache's bytes.
 //
 // Work is split on the device, from the lengths (a captured launch serves every batch): a unit is what the four waves
-// take in one round (128 tokens); laid one after the other, the sequences' units are dealt out `per` to a workgroup, so
+// take in one round (128 tokens of a head, or 32 of four); laid one after the other, the sequences' units are dealt out `per` to a workgroup, so
 // that `target` of them share all the work evenly, whatever the lengths.  A sequence within one workgroup gets its output
 // at once; the others' parts are joined by a second kernel in a fixed order, so results do not depend on timing.
 struct AttendArgs {
@@ -322,18 +322,20 @@ __device__ __forceinline__ void turn_v(const Block<D, F8>& s, int q, v4u (&out)[
     }
 }
 
-template <int D, bool F8>
+// SIDE: the four waves take four neighbouring heads of the same 32 tokens (unit: 32 tokens, no joining of waves) instead of
+// four blocks of one head's: where a token's heads lie side by side in memory, a workgroup then reads 4 of them in one run.
+template <int D, bool F8, bool SIDE>
 __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
     using B = Block<D, F8>;
-    constexpr int UNIT = 32 * kWaves, F = D / 16, QF = D / 32, L = B::L;
+    constexpr int WT = SIDE ? 1 : kWaves, UNIT = 32 * WT, F = D / 16, QF = D / 32, L = B::L;
     extern __shared__ __align__(16) char lds[];               // per wave: keys, at the end 16 columns of O; then m and l
     // a part's heads, whose rows lie side by side in a cache of token rows, on one XCD (workgroup i runs on XCD i % 8)
     const int ht = blockIdx.x / 8 % a.HT, part = blockIdx.x / (8 * a.HT) * 8 + blockIdx.x % 8;
     const Plan pl = make_plan<UNIT>(a, part);
     if (pl.b < 0) return;
-    const int hk = ht / a.tiles, tile = ht % a.tiles;
-    const int h0 = hk * a.G + 16 * tile, nh = min(16, a.G - 16 * tile);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hk = SIDE ? 4 * ht + wave : ht / a.tiles, tile = SIDE ? 0 : ht % a.tiles;
+    const int h0 = hk * a.G + 16 * tile, nh = min(16, a.G - 16 * tile);
     const int col = lane & 15, g = lane >> 4;
     int b = __builtin_amdgcn_readfirstlane(pl.b), off = __builtin_amdgcn_readfirstlane(pl.off);
     int left = __builtin_amdgcn_readfirstlane(pl.left);
@@ -482,7 +484,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
                 }
             }
         };
-        int t0 = begin + 32 * wave;
+        int t0 = begin + (SIDE ? 0 : 32 * wave);
         if (t0 < end) {
             locate(t0);
             clamp();
@@ -492,7 +494,7 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
             block(t0, std::false_type{});
         }
 
-        // the four waves' columns, joined: each to the common maximum
+        // the four waves' columns, joined: each to the common maximum (SIDE: a wave's own)
         constexpr int LD = D + 4;
         float* lm = reinterpret_cast<float*>(lds + kWaves * B::STAGE);
         float* ll = lm + kWaves * 16;
@@ -513,16 +515,17 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
             a.plan[b] = int2{part, 1 + (units - seg + pl.per - 1) / pl.per};
         const float vs = F8 && a.c.v_scale ? __ldg(a.c.v_scale + hk) : 1.f;
         const int64_t slot = 2 * (int64_t)part + (off == 0);  // of a workgroup's parts one ends a sequence, one begins one
-        for (int i = threadIdx.x; i < nh * (D / 4); i += 256) {
+        const int w0 = SIDE ? wave : 0;
+        for (int i = SIDE ? lane : threadIdx.x; i < nh * (D / 4); i += SIDE ? 64 : 256) {
             const int h = i / (D / 4), d = 4 * (i % (D / 4));
-            float mm = lm[h];
+            float mm = lm[16 * w0 + h];
 #pragma unroll
-            for (int w = 1; w < kWaves; w++) mm = fmaxf(mm, lm[16 * w + h]);
+            for (int w = 1; w < WT; w++) mm = fmaxf(mm, lm[16 * w + h]);
             const float ref = mm == -INFINITY ? 0.f : mm;
             float sum = 0.f;
             v4f acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < kWaves; w++) {
+            for (int w = w0; w < w0 + WT; w++) {
                 const float e = __builtin_amdgcn_exp2f(lm[16 * w + h] - ref);
                 sum += e * ll[16 * w + h];
                 acc += e * *reinterpret_cast<const v4f*>(lds + w * B::STAGE + (h * LD + d) * 4);
@@ -614,10 +617,19 @@ static int attend_target(int64_t D, bool f8) {
     return 2 * attend_lds(D, f8) <= 160 * 1024 ? 512 : 256;
 }
 
-// Workgroups per head: all units at `per` each, no more than the target's share and no more than there are units.
-static int64_t attend_parts(int64_t T, int64_t HT, int64_t cap, int target) {
-    const int64_t unit = 32 * kWaves, most = T * ((cap + unit - 1) / unit), split = target / HT + 1;
+// Workgroups per head (or four side by side): all units at `per` each, no more than the target's share and no more than
+// there are units.
+static int64_t attend_parts(int64_t T, int64_t HT, int64_t cap, int64_t unit, int target) {
+    const int64_t most = T * ((cap + unit - 1) / unit), split = target / HT + 1;
     return most < split ? most : split;
+}
+
+// Whether waves may take heads side by side: whole groups of four, a tile of query heads each, and enough sequences that the
+// parts, now of four heads each, are few.  With and without, rows of 8 heads: 128 sequences of 100 - 4096 visible tokens of 64
+// bf16 133.5 / 147.3 us, 64 of 8000 tokens of 128 365 / 390 (e4m3 199 / 234), 16 of 4000 of 64 34.7 / 37.6; but 8 of those
+// 20.6 / 19.6, one of 32768 28 / 21, and 16 of 300 - 500 tokens of 128 e4m3 13.7 / 12.6.
+static bool attend_side(int64_t T, int64_t hq, int64_t heads, int64_t cap) {
+    return heads % 4 == 0 && hq / heads <= 16 && T >= 16 && cap >= 1024;
 }
 
 // The cache's arguments, checked; strides from elements to bytes.
@@ -694,9 +706,14 @@ extern "C" int prism_kv_append(const prism_kv_append_args* args, void* stream) {
 extern "C" int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t hq, int64_t heads, int64_t dim, int64_t cols,
                                                    int64_t page) {
     if (T < 1 || heads < 1 || hq < heads || hq % heads || dim < 1 || cols < 1 || page < 1) return 0;
-    if (cols * page <= 32 * kWaves) return 0;                // one unit: nothing to join
-    // (512: the most that either cache type is dealt out to)
-    return 2 * attend_parts(T, heads * ((hq / heads + 15) / 16), cols * page, 512) * hq * (dim + 2) * 4 + T * 8;
+    // the most of both ways that the strides may choose, and of both cache types (512 workgroups)
+    const int64_t cap = cols * page, tiles = (hq / heads + 15) / 16;
+    int64_t parts = cap <= 32 * kWaves ? 0 : attend_parts(T, heads * tiles, cap, 32 * kWaves, 512);
+    if (attend_side(T, hq, heads, cap)) {
+        const int64_t side = attend_parts(T, heads / 4, cap, 32, 512);
+        if (side > parts) parts = side;
+    }
+    return parts ? 2 * parts * hq * (dim + 2) * 4 + T * 8 : 0;     // 0: one unit a sequence, nothing to join
 }
 
 extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
@@ -717,14 +734,17 @@ extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
     if (need > 0 && (!h.ws || h.ws_bytes < need)) return PRISM_ERR_ARG;
     if (need > 0 && !PRISM_ALIGNED(h.ws, 16)) return PRISM_ERR_ALIGN;
     if (T == 0) return PRISM_OK;
-    const int64_t G = HQ / HKV, tiles = (G + 15) / 16, HT = HKV * tiles;
+    const int64_t G = HQ / HKV, tiles = (G + 15) / 16, cap = cols * hc.page;
     const bool f8 = hc.e4m3 != 0;
+    const bool side = hc.k_head < hc.k_tok && hc.v_head < hc.v_tok && attend_side(T, HQ, HKV, cap);
+    const int64_t HT = side ? HKV / 4 : HKV * tiles, unit = side ? 32 : 32 * kWaves;
     a.target = attend_target(D, f8);
-    const int64_t parts = attend_parts(T, HT, cols * hc.page, a.target), grid = (parts + 7) / 8 * 8 * HT;
+    const int64_t parts = attend_parts(T, HT, cap, unit, a.target), grid = (parts + 7) / 8 * 8 * HT;
     if (grid > INT32_MAX) return PRISM_ERR_SHAPE;
     a.q = h.q, a.out = h.out, a.ldq = h.q_ld, a.hq_s = h.q_hs, a.ldo = h.o_ld, a.ho_s = h.o_hs;
     a.lens = h.lens, a.n = h.n_rows;
-    if (need > 0) {
+    const bool joins = cap > unit;
+    if (joins) {
         a.part_o = (float*)h.ws;
         a.part_ml = (float*)h.ws + 2 * parts * HQ * D;
         a.plan = (int2*)((float*)h.ws + 2 * parts * HQ * (D + 2));
@@ -737,15 +757,20 @@ extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
     do { \
         static_assert(Block<DD, F8>::STAGE % 16 == 0, "LDS alignment"); \
         const int lds = attend_lds(DD, F8); \
-        allow_lds(kv_attend_kernel<DD, F8>, lds); \
-        hipLaunchKernelGGL((kv_attend_kernel<DD, F8>), dim3((unsigned)grid), dim3(256), lds, st, a); \
+        if (side) { \
+            allow_lds(kv_attend_kernel<DD, F8, true>, lds); \
+            hipLaunchKernelGGL((kv_attend_kernel<DD, F8, true>), dim3((unsigned)grid), dim3(256), lds, st, a); \
+        } else { \
+            allow_lds(kv_attend_kernel<DD, F8, false>, lds); \
+            hipLaunchKernelGGL((kv_attend_kernel<DD, F8, false>), dim3((unsigned)grid), dim3(256), lds, st, a); \
+        } \
     } while (0)
     if (D == 64) { if (f8) AT(64, true); else AT(64, false); }
     else if (D == 128) { if (f8) AT(128, true); else AT(128, false); }
     else { if (f8) AT(256, true); else AT(256, false); }
 #undef AT
     PRISM_LAUNCH_CHECK();
-    if (need > 0) {
+    if (joins) {
   // a workgroup per head while there are few (long sequences have many parts), else one for as many as it has groups
         const int hb = T * HQ <= 4096 ? 1 : (int)(1024 / D);
         const dim3 jg((unsigned)((HQ + hb - 1) / hb), (unsigned)T);

@@ -243,6 +243,16 @@ def test_attend_live_rows_and_many_sequences(dev):
     check_attend(dev, lens, 4, 2, 64, 32, torch.bfloat16, "head", live=131)
 
 
+@pytest.mark.parametrize("hq,hkv,dim,window", [(8, 4, 64, 0), (4, 4, 128, 0), (64, 4, 64, 33), (28, 4, 128, 0), (24, 8, 256, 700),
+                                               (12, 12, 64, 1)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_attend_batches_over_token_rows(dev, hq, hkv, dim, window, dtype):
+    """Sixteen sequences and more over caches whose heads lie side by side, taken four at a time; some end a part, some
+    are empty, some are past the live rows."""
+    lens = [0, 1, 31, 32, 33, 2100, 64, 0, 0, 97, 1024, 15, 16, 17, 129, 1, 500, 0, 800]
+    check_attend(dev, lens, hq, hkv, dim, 16, dtype, "token", window=window, live=18, scaled=dtype == E4M3)
+
+
 def test_attend_peaked_scores(dev):
     """Scores of hundreds: one token takes nearly all of the weight, the running maximum moves often."""
     check_attend(dev, [900, 64], 4, 1, 128, 16, torch.bfloat16, "token", scale=1.0, q_std=4.0)
