@@ -1,6 +1,7 @@
-// The gated delta rule of a linear-attention layer in serving (gfx950).  Per value head, with the state S fp32 [DK, DV],
-// a = exp(g), key k and query q (normalised to length 1 in the kernel if asked, the query times a scale), all in fp32:
+// The gated delta rule of a linear-attention layer in serving (gfx950).  Per value head, with the state S fp32 [DK,
+// DV], a = exp(g), key k and query q (normalised to length 1 in the kernel if asked, the query times a scale):
 //   S <- a S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q.
+// States, sums and factors are fp32, a chunk's gate sums fp64.
 #include "common.h"
 
 namespace prism {
@@ -42,8 +43,10 @@ __device__ __forceinline__ float wave_addf(float v) {
 // A workgroup holds NC columns of one head's state in registers from its only read to its only write: thread t the
 // columns 4 (t % (NC / 4)) .. + 3 of the rows t / (NC / 4) + i RG.  Both sums over the rows, S^T k and S^T q, are taken
 // of the decayed state at once (o = S^T q + (q . k) u), so a token costs one exchange between the waves.  Each wave
-// holds its own copy of the token's key and query.  Bound by the state's bytes (loading a further token's inputs ahead did not
-// show: 1.5 us a token is the exchange's chain).
+// holds its own copy of the token's key and query.  A step of many rows is bound by the state's bytes: 256 rows of 32
+// heads of 128 x 128 (1.08 GB) 190 us, 5.7 TB/s; 40 rows of 48 heads (254 MB) 46 us, 5.5 TB/s (a copy in place of 1 GB:
+// 5.9).  Several tokens of a sequence are bound by the exchange's chain, 1.5 us a token; loading the next token's
+// inputs ahead did not show.
 template <int DK, int DV, int NC>
 __global__ __launch_bounds__(256) void delta_rec_kernel(DeltaArgs a) {
     constexpr int LC = NC / 4, RG = 256 / LC, RPT = DK / RG, E = DK / 64;
@@ -59,7 +62,8 @@ __global__ __launch_bounds__(256) void delta_rec_kernel(DeltaArgs a) {
     const int hk = head / (a.HV / a.HK);
     v4f s[RPT];
 #pragma unroll
-    for (int i = 0; i < RPT; i++) s[i] = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(st + (rg + i * RG) * DV));
+    for (int i = 0; i < RPT; i++)
+        s[i] = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(st + (rg + i * RG) * DV));
     for (int j = 0; j < count; j++) {
         const int64_t t = first + j;
         float kv[E], qv[E], kk = 0.f, qq = 0.f, qk = 0.f;
@@ -137,14 +141,15 @@ __global__ __launch_bounds__(256) void delta_rec_kernel(DeltaArgs a) {
     for (int i = 0; i < RPT; i++) __builtin_nontemporal_store(s[i], reinterpret_cast<v4f*>(st + (rg + i * RG) * DV));
 }
 
-// Columns per workgroup: 32 while that is what fills the card, the whole head (its 64 KB in one run) once there are heads
-// enough.  At 48 heads of 128 x 128: 1 row 4.5 us with 32, 4.8 with 64, 5.4 with 128 columns; 8 rows 10.5, 9.4, 10.1; 16 rows
-// 20.9, 20.7, 18.5; 256 rows of 32 heads 203, 203, 190 (5.7 TB/s; 214 without the non-temporal loads and stores).
+// Columns per workgroup: 32 while that is what fills the card, the whole head (its 64 KB in one run) once there are
+// heads enough.  At 48 heads of 128 x 128: 1 row 4.5 us with 32, 4.8 with 64, 5.4 with 128 columns; 8 rows 10.5, 9.4,
+// 10.1; 16 rows 20.9, 20.7, 18.5; 256 rows of 32 heads 203, 203, 190 (214 without the non-temporal loads and stores).
 template <int DK, int DV>
 static int launch_rec(const DeltaArgs& a, hipStream_t st) {
     const int64_t heads = (int64_t)a.seqs * a.HV;
     if (heads * (DV / 32) > INT32_MAX) return PRISM_ERR_SHAPE;
-#define RC(NC) hipLaunchKernelGGL((delta_rec_kernel<DK, DV, NC>), dim3((unsigned)(heads * (DV / (NC)))), dim3(256), 0, st, a)
+#define RC(NC) \
+    hipLaunchKernelGGL((delta_rec_kernel<DK, DV, NC>), dim3((unsigned)(heads * (DV / (NC)))), dim3(256), 0, st, a)
     if (heads >= 512) RC(DV);
     else if (heads >= 256) RC(64);
     else RC(32);
@@ -157,16 +162,21 @@ static int launch_rec(const DeltaArgs& a, hipStream_t st) {
 //   A_ij = beta_i e^(G_i - G_j) k_i . k_j (j < i),  X = (I + A)^-1,  U = X diag(beta) (V - diag(e^G) K S)
 //   O = diag(e^G) Q S + P U,  P_ij = e^(G_i - G_j) q_i . k_j (j <= i);  S <- e^(G_63) S + K^T diag(e^(G_63 - G)) U
 // Only S runs from chunk to chunk, so two kernels: delta_prep computes X diag(beta) and P of all chunks at once,
-// delta_scan walks each sequence's chunks.  The normalisation is row scales (rk, rq), so K and Q stay the bf16 they are.
+// delta_scan walks each sequence's chunks.  The normalisation is row scales (rk, rq), so K and Q stay the bf16 they
+// are.
 //
-// The products run on the fp16 MFMA at nearly fp32's precision: an fp32 operand is two fp16, the value rounded to 11 bits and
-// what is left rounded to 11 more (to nearest: the error is below 2^-23 of the value), two products against K or Q, three
-// against another such pair (the fourth is below 2^-22 of the terms).  fp16's range is made to do by powers of two: every row
-// of K, Q, X and P and every column (lane) of S, R and U is scaled so that its largest value is about 2^14, which leaves the
-// lower halves normal down to 2^-28 of it; the powers are taken off with factors that are there anyway, or exactly after the
-// product.  bf16 operands (K and Q, 8 bits) fit one fp16.  Against three bf16 parts, which need no scales but three and six
-// products: the same error (1.6e-7 of the outputs), 16 of 24 and 9 of 18 MFMAs, three instructions a value for the parts
-// instead of 5.5, a third less of X and P to write and read.
+// The products run on the fp16 MFMA at nearly fp32's precision: an fp32 operand is two fp16, the value rounded to 11
+// bits and what is left rounded to 11 more (to nearest: the error is below 2^-23 of the value), two products against K
+// or Q, three against another such pair (the fourth is below 2^-22 of the terms).  fp16's range is made to do by powers
+// of two: every row of K, Q, X and P and every column (lane) of S, R and U is scaled so that its largest value is about
+// 2^14, which leaves the lower halves normal down to 2^-28 of it; the powers are taken off with factors that are there
+// anyway, or exactly after the product.  bf16 operands (K and Q, 8 bits) fit one fp16.  Against three bf16 parts, which
+// need no scales but three and six products: the same error (1.7e-7 of the outputs), 16 of 24 and 9 of 18 MFMAs, a
+// third less of X and P to write and read; delta_scan 313 us instead of 326 (8191 tokens, 16 key and 48 value heads of
+// 128).
+//
+// A token's outputs depend on its own and earlier tokens only, but a value that is not finite reaches its whole chunk
+// (zeros of a triangle times infinity).
 //
 // Everything that delta_scan multiplies from the left (K, Q, K^T, X diag(beta), P) lies in the workspace as MFMA
 // fragments, 1 KB each in lane order.  Inside a product the order of the summed index is free: taking it as an
@@ -175,16 +185,20 @@ static int launch_rec(const DeltaArgs& a, hipStream_t st) {
 // without exchanging anything.
 constexpr int kC = 64;                                        // tokens per chunk
 constexpr int kFrag = 1024;                                   // bytes of a fragment: 64 lanes of 8 bf16
-constexpr int kTri = 6;                                       // fragments (i, s) of a lower triangle: 16-row tile i, 32 columns s <= i / 2
+constexpr int kTri = 6;       // fragments (i, s) of a lower triangle: 16-row tile i, 32 columns s <= i / 2
 __host__ __device__ constexpr int tri(int i, int s) { return i < 2 ? i : 2 * i - 2 + s; }
-__host__ __device__ constexpr int64_t rec_k(int DK) { return (int64_t)(4 * (DK / 32) * 2 + DK / 16 * 2) * kFrag; }   // K, Q, K^T
-constexpr int64_t kRecV = 2 * 2 * kTri * kFrag + 5 * kC * 4;  // X diag(beta), P; factors: of K S, Q S, U, the output's; e^(G_63)
+// K, Q, K^T
+__host__ __device__ constexpr int64_t rec_k(int DK) { return (int64_t)(4 * (DK / 32) * 2 + DK / 16 * 2) * kFrag; }
+// X diag(beta), P; factors: of K S, Q S, U, the output's; e^(G_63)
+constexpr int64_t kRecV = 2 * 2 * kTri * kFrag + 5 * kC * 4;
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ v4f mfma_f32(float a, float b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ v4f mfma_f32(float a, float b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
 
 // LDS-DMA of 4 bytes a lane.
 __device__ __forceinline__ void dma4(const void* g, void* lds) {
@@ -197,9 +211,9 @@ __device__ __forceinline__ v4f mfma_f16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// The power of two that brings values up to `most` to 2^14 .. 2^15, and its inverse.  Below 2^-60 it stays what it is there
-// (nothing overflows, and what such small values lose is far below the rest of their row or column); infinities and NaN
-// stay what they are.
+// The power of two that brings values up to `most` to 2^14 .. 2^15, and its inverse.  Below 2^-60 it stays what it is
+// there (nothing overflows, and what such small values lose is far below the rest of their row or column); infinities
+// and NaN stay what they are.
 struct Pow2 {
     float up, down;
 };
@@ -221,9 +235,9 @@ __device__ __forceinline__ float column_max(float m) {
     return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 
-// Eight fp32 (x then y) times a power of two as two fp16 fragments: h = RN(x s), l = RN(x s - h), six instructions for two
-// values (products and differences are exact).  No inline assembly: the compiler does not put the wait states between it and
-// an MFMA that reads its result.
+// Eight fp32 (x then y) times a power of two as two fp16 fragments: h = RN(x s), l = RN(x s - h); products and
+// differences are exact.  No inline assembly: the compiler does not put the wait states between it and an MFMA that
+// reads its result.
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 struct Split {
@@ -272,15 +286,17 @@ __device__ __forceinline__ bool find_chunk(const DeltaArgs& a, int id, int& firs
     return false;
 }
 
-// The records go past the caches (delta_scan reads them after all are written): 8191 tokens 396 -> 379 us in all.
+// The records go past the caches (delta_scan reads them after all are written): 8191 tokens 379 us in all instead of
+// 396.
 __device__ __forceinline__ void put_frag(char* base, v4u v) {
     __builtin_nontemporal_store(v, reinterpret_cast<v4u*>(base + (threadIdx.x & 63) * 16));
 }
 
-// One wave per chunk (blockIdx.x) and value head (blockIdx.y).  Rows are loaded in their own order (a row per lane would take
-// the memory pipeline four times as long) and become fragments through LDS.  The decays between tokens of different 16-row
-// tiles are products of three that are at most 1, so that 16 exponentials a lane (the diagonal tiles') and a few are enough
-// for 40.
+// One wave per chunk (blockIdx.x) and value head (blockIdx.y).  Rows are loaded in their own order (a row per lane
+// would take the memory pipeline four times as long) and become fragments through LDS.  The decays between tokens of
+// different 16-row tiles are products of three that are at most 1, so that 16 exponentials a lane (the diagonal tiles')
+// and a few are enough for 40.  One chunk takes 13 us, the chain of its steps; 8191 tokens of 16 key and 48 value heads
+// of 128 take 100 us, bound by the records' 255 MB (47 us without their stores).
 template <int DK>
 __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, char* wv) {
     constexpr int KS = DK / 32, LD = kC + 4, LK = DK + 8, PR = DK / 8;   // PR: 16-byte pieces of a row
@@ -339,7 +355,8 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int s = 0; s < KS; s++) f[i][s] = *reinterpret_cast<const v4u*>(rows + (16 * i + col) * LK + 32 * s + 8 * g);
+            for (int s = 0; s < KS; s++)
+                f[i][s] = *reinterpret_cast<const v4u*>(rows + (16 * i + col) * LK + 32 * s + 8 * g);
     };
     // as delta_scan's left operand, scaled rows: fragment (i, s), dims 32 s + 4 g + j, then 32 s + 16 + 4 g + j
     auto copy = [&](char* to, const float* up) {
@@ -392,7 +409,8 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
                 float u[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    u[j] = bf16_to_f32(rows[(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col]) * up[j / 4][j % 4];
+                    u[j] = bf16_to_f32(rows[(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col]) *
+                           up[j / 4][j % 4];
                 v4u w;
 #pragma unroll
                 for (int j = 0; j < 4; j++)
@@ -465,8 +483,8 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
         for (int i = 0; i < 16; i++) x[(16 * g + i) * LD + 16 * g + col] = v[i];
     }
     __syncthreads();
-    // the blocks below, X_ij = -X_ii sum_k A_ik X_kj, diagonal by diagonal: the X_kj are right operands as the accumulators
-    // they come in, so nothing is stored before all are there
+    // the blocks below, X_ij = -X_ii sum_k A_ik X_kj, diagonal by diagonal: the X_kj are right operands as the
+    // accumulators they come in, so nothing is stored before all are there
     {
         v4f y[4][4];                                          // [i][j]; [i][i]: the diagonal blocks in the same form
 #pragma unroll
@@ -550,15 +568,17 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
     }
 }
 
-// A workgroup walks the chunks of one sequence and value head for 32 columns of the state, twelve waves, three to a SIMD.
-// Four waves to 16 columns: two hold the halves of S's rows and take what the next chunk waits for (K S, U, K^T U), two
-// the chunk's output (Q S, P U); products split over the summed index: a wave multiplies its half of S's rows, or its half
-// of U's tokens, and the halves' sums (fp32, always the same two added) meet in LDS.  The other four waves bring the
-// fragments into LDS, each group while nobody reads it, and touch the lines of the chunk after the next, so that those
-// come from L2.  Two barriers per chunk:
+// A workgroup walks the chunks of one sequence and value head for 32 columns of the state, twelve waves, three to a
+// SIMD. Four waves to 16 columns: two hold the halves of S's rows and take what the next chunk waits for (K S, U, K^T
+// U), two the chunk's output (Q S, P U); products split over the summed index: a wave multiplies its half of S's rows,
+// or its half of U's tokens, and the halves' sums (fp32, always the same two added) meet in LDS.  The other four waves
+// bring the fragments into LDS, each group while nobody reads it, and touch the lines of the chunk after the next, so
+// that those come from L2.  Two barriers per chunk:
 //   state waves   K S, halves out        | halves in, R, X R out  | U in, S <- ..., S out
 //   output waves  (P U of the last one)  | S in, Q S              | P U, halves out
 //   loading waves                        | next K in              | all else of the next chunk in
+// Bound by that chain: a chunk takes some 5000 cycles, 3500 of them the state waves' alone, while LDS moves 370 KB
+// (2900 cycles).  8191 tokens of one sequence, 16 key and 48 value heads of 128 (192 workgroups): 280 us.
 template <int DK>
 struct ScanShared {
     v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], x[2 * kTri][64];
@@ -576,7 +596,7 @@ struct ScanAt {
 
 // A product's fragments are read from LDS into registers.  The compiler spreads the reads over the phase; forced to its
 // start, to have their latency behind what the right operand still takes, they come as bursts that hold the others up:
-// 392 us for 8191 tokens instead of 372 (LDS moves some 370 KB a chunk, over half of what it can).
+// 392 us for 8191 tokens instead of 372.
 // K or Q: 4 token tiles, the half's k
 template <int DK, int HALF>
 __device__ __forceinline__ void read_rows(v4u (&r)[DK / 64][4], const v4u (*f)[64]) {
@@ -733,8 +753,8 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
     lds_barrier();
 }
 
-// rec: the key head's (HALF 0) or the head's (1) records, whose lines these waves touch two chunks ahead; m of `per`: this
-// workgroup among those that read them.
+// rec: the key head's (HALF 0) or the head's (1) records, whose lines these waves touch two chunks ahead; m of `per`:
+// this workgroup among those that read them.
 template <int DK, int HALF>
 __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, const char* rec, int m, int per,
                                          ScanShared<DK>& x) {
@@ -913,8 +933,8 @@ static int dispatch_chunks(const DeltaArgs& a, int64_t DK, int64_t DV, char* ws,
     return DV == 64 ? launch_chunks<128, 64>(a, ws, st) : launch_chunks<128, 128>(a, ws, st);
 }
 
-// A few rows go token by token: 1.5 us each for a sequence's at 48 heads, against 19 us for its first chunk (12 rows 21 us,
-// 8 rows 15).
+// A few rows go token by token: 1.5 us each for a sequence's at 48 heads, against 19 us for its first chunk (12 rows 21
+// us, 8 rows 15).
 static bool by_token(int64_t T) { return T <= 12; }
 
 static int64_t workspace_bytes(int64_t T, int64_t seqs, int64_t hk, int64_t hv, int64_t dk) {

@@ -24,12 +24,12 @@ struct Cache {
 };
 
 // ------------------------------------------------------------------------------------------------------------ append
-// A thread takes 16 dims of one head as two pieces of 8 that a rotation in halves pairs: dims 8 j .. + 7 and
-// R / 2 + 8 j .. + 7 of the R rotated ones, the same split of the others.  Every piece is one 16-byte load, 16 bytes
-// (8 of e4m3) stored; neighbouring lanes hold neighbouring pieces.  One workgroup row per token (blockIdx.x), the
-// token's heads (queries, keys, values) over blockIdx.y.  Bound by memory: nothing is read or written twice; 8191 tokens of
-// 24 + 2 x 4 heads of 256 into an e4m3 cache (254 MB) 50 us, 5.1 TB/s, what a large copy reaches (53 us without the
-// non-temporal loads and cache stores; the queries are read again at once, so theirs are plain).
+// A thread takes 16 dims of one head as two pieces of 8 that a rotation in halves pairs: dims 8 j .. + 7 and R / 2 + 8
+// j .. + 7 of the R rotated ones, the same split of the others.  Every piece is one 16-byte load, 16 bytes (8 of e4m3)
+// stored; neighbouring lanes hold neighbouring pieces.  One workgroup row per token (blockIdx.x), the token's heads
+// (queries, keys, values) over blockIdx.y.  Bound by memory: nothing is read or written twice; 8191 tokens of 24 + 2 x
+// 4 heads of 256 into an e4m3 cache (254 MB) 50 us, 5.1 TB/s, what a large copy reaches (53 us without the non-temporal
+// loads and cache stores; the queries are read again at once, so theirs are plain).
 struct AppendArgs {
     const uint16_t *q, *k, *v;
     uint16_t* qo;
@@ -153,9 +153,16 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // rounding is the only one that shows; the second MFMA is free beside the cache's bytes.
 //
 // Work is split on the device, from the lengths (a captured launch serves every batch): a unit is what the four waves
-// take in one round (128 tokens of a head, or 32 of four); laid one after the other, the sequences' units are dealt out `per` to a workgroup, so
-// that `target` of them share all the work evenly, whatever the lengths.  A sequence within one workgroup gets its output
-// at once; the others' parts are joined by a second kernel in a fixed order, so results do not depend on timing.
+// take in one round (128 tokens of a head, or 32 of four); laid one after the other, the sequences' units are dealt out
+// `per` to a workgroup, so that `target` of them share all the work evenly, whatever the lengths.  A sequence within
+// one workgroup gets its output at once; the others' parts are joined by a second kernel in a fixed order, so results
+// do not depend on timing.
+//
+// Bound by the cache's bytes, read once: one sequence of 131071 tokens, 8 heads of 128 bf16 (537 MB), 98 us, 5.5 TB/s, 90
+// of them this kernel (6.0 TB/s, more than a copy moves) and 7 the joining one; 40 of up to 20000, 4 heads of 256 e4m3
+// (505 MB), 101 us, 5.0 TB/s; token rows of 8 heads of 64, 128 sequences of up to 4096 visible (613 MB), 134 us,
+// 4.6 TB/s (runs of 512 bytes a token; the same heads' rows by the page take 120).  A short call (613 tokens) is launches
+// and one chain of a unit's steps, 9 us.
 struct AttendArgs {
     const uint16_t* q;
     uint16_t* out;
@@ -189,8 +196,9 @@ __device__ __forceinline__ long long wave_sum(long long v) {
     return v;
 }
 
-// Where workgroup p's units begin: unit u = p per of all sequences' one after the other (a sequence without tokens has one,
-// for its zeros) lies in sequence b, `off` units from its start; `left` units to do.  The same in every lane; b < 0: none.
+// Where workgroup p's units begin: unit u = p per of all sequences' one after the other (a sequence without tokens has
+// one, for its zeros) lies in sequence b, `off` units from its start; `left` units to do.  The same in every lane; b <
+// 0: none.
 struct Plan {
     int b, off, left, per;
 };
@@ -322,8 +330,9 @@ __device__ __forceinline__ void turn_v(const Block<D, F8>& s, int q, v4u (&out)[
     }
 }
 
-// SIDE: the four waves take four neighbouring heads of the same 32 tokens (unit: 32 tokens, no joining of waves) instead of
-// four blocks of one head's: where a token's heads lie side by side in memory, a workgroup then reads 4 of them in one run.
+// SIDE: the four waves take four neighbouring heads of the same 32 tokens (unit: 32 tokens, no joining of waves)
+// instead of four blocks of one head's: where a token's heads lie side by side in memory, a workgroup then reads 4 of
+// them in one run.
 template <int D, bool F8, bool SIDE>
 __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
     using B = Block<D, F8>;
@@ -359,13 +368,15 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
         for (int f = 0; f < F; f++) o[f] = v4f{0.f, 0.f, 0.f, 0.f};
         float m = -INFINITY, l = 0.f;
 
-  // the table through the scalar cache: a vector load would be waited for together with the values in flight before it
+        // the table through the scalar cache: a vector load would be waited for together with the values in flight
+        // before it
         const auto* row = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
             reinterpret_cast<uintptr_t>(a.c.table + b * a.c.table_ld));
         const int last = len > 0 ? (len - 1) & ~15 : 0;           // the last 16 tokens that are there
-  // Keys and values go to LDS by DMA, 1 KB a load.  Keys: 16 tokens x 64 bytes, four neighbouring lanes a token's (the
-  // memory pipeline merges neighbouring lanes only), placed so that operand order reads without bank conflicts; values:
-        // whole rows.  Every wait on them is written out: the compiler would wait for all of them at each use.
+        // Keys and values go to LDS by DMA, 1 KB a load.  Keys: 16 tokens x 64 bytes, four neighbouring lanes a token's
+        // (the memory pipeline merges neighbouring lanes only), placed so that operand order reads without bank
+        // conflicts; values: whole rows.  Every wait on them is written out: the compiler would wait for all of them at
+        // each use.
         const uint32_t koff = (uint32_t)((lane >> 2) * a.c.k_tok) + 16 * ((lane & 3) ^ lds_turn(lane >> 4));
         const uint32_t voff = (uint32_t)(16 * lane / B::RB * a.c.v_tok) + 16 * lane % B::RB;
         const char* kb = a.c.k + hk * a.c.k_head;
@@ -437,7 +448,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; j++) p[j] = mul_rn(st[j / 4][j % 4], sc);
             if (t0 < lo || (!MORE && t0 + 32 > len)) {
-  // tokens outside get no weight, and their values, which may be anything (a page's unwritten rows), are zeroed
+                // tokens outside get no weight, and their values, which may be anything (a page's unwritten rows), are
+                // zeroed
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     const int t = t0 + 16 * (j / 4) + 4 * g + j % 4;
@@ -465,8 +477,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
             for (int w = 0; w < 4; w++) {
                 const float e0 = __builtin_amdgcn_exp2f(p[2 * w] - ref), e1 = __builtin_amdgcn_exp2f(p[2 * w + 1] - ref);
                 l += e0 + e1;
-                // the upper part strictly below the weight, so that the rest of a weight is never 0 (0 times an infinite
-                // value would be NaN, not infinite)
+                // the upper part strictly below the weight, so that the rest of a weight is never 0 (0 times an
+                // infinite value would be NaN, not infinite)
                 const uint32_t b0 = max(__float_as_uint(e0), 1u) - 1u, b1 = max(__float_as_uint(e1), 1u) - 1u;
                 hi[w] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
                 const float r0 = e0 - __uint_as_float(b0 & 0xffff0000u), r1 = e1 - __uint_as_float(b1 & 0xffff0000u);
@@ -534,7 +546,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
                 uint32_t u[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(sum == 0.f ? 0.f : div_rn(acc[j], sum) * vs);
-                *reinterpret_cast<v2u*>(a.out + b * a.ldo + (h0 + h) * a.ho_s + d) = v2u{u[0] | (u[1] << 16), u[2] | (u[3] << 16)};
+                *reinterpret_cast<v2u*>(a.out + b * a.ldo + (h0 + h) * a.ho_s + d) =
+                    v2u{u[0] | (u[1] << 16), u[2] | (u[3] << 16)};
             } else {
                 const int64_t to = slot * a.HQ + h0 + h;
                 *reinterpret_cast<v4f*>(a.part_o + to * D + d) = acc;
@@ -551,8 +564,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
     }
 }
 
-// Joins the parts of sequence blockIdx.y's query heads hb blockIdx.x ..: groups of D / 4 threads, `share` of them (a power
-// of two, as many as the parts need) to a head, each every share-th part in order, then the groups in order.
+// Joins the parts of sequence blockIdx.y's query heads hb blockIdx.x ..: groups of D / 4 threads, `share` of them (a
+// power of two, as many as the parts need) to a head, each every share-th part in order, then the groups in order.
 template <int D>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int hb) {
     constexpr int TC = D / 4, NG = 256 / TC;
@@ -604,11 +617,11 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int hb) {
     }
 }
 
-// LDS of a workgroup, and how many workgroups a launch's work is dealt out to: as many as are there at a time, two a CU where
-// LDS holds them.  With 4 a CU (rows of 128 bytes leave LDS for them) 128 sequences of 100 - 4096 visible tokens, 8 heads of
-// 64, take 153 us instead of 148 and 64 of 8000 tokens, 8 heads of 128 e4m3, 189 instead of 180: every further part is more
-// to join.  One a CU: 131071 tokens, 8 heads of 128 bf16, 98 us instead of 100, but 256 sequences of 20 - 300 tokens 50
-// instead of 41.
+// LDS of a workgroup, and how many workgroups a launch's work is dealt out to: as many as are there at a time, two a CU
+// where LDS holds them.  With 4 a CU (rows of 128 bytes leave LDS for them) 128 sequences of 100 - 4096 visible tokens,
+// 8 heads of 64, take 138 us instead of 133.5, 64 of 8000 tokens, 8 heads of 128 e4m3, 205 instead of 199: every further
+// part is more to join.  One a CU: 131071 tokens, 8 heads of 128 bf16, 98 us instead of 100, but 256 sequences of
+// 20 - 300 tokens 50 instead of 41.
 static int attend_lds(int64_t D, bool f8) {
     const int64_t stage = 4 * (f8 ? D : 2 * D) / 64 * 1024, o = 16 * (D + 4) * 4;
     return (int)(kWaves * (stage > o ? stage : o) + 2 * kWaves * 16 * 4);
@@ -624,10 +637,10 @@ static int64_t attend_parts(int64_t T, int64_t HT, int64_t cap, int64_t unit, in
     return most < split ? most : split;
 }
 
-// Whether waves may take heads side by side: whole groups of four, a tile of query heads each, and enough sequences that the
-// parts, now of four heads each, are few.  With and without, rows of 8 heads: 128 sequences of 100 - 4096 visible tokens of 64
-// bf16 133.5 / 147.3 us, 64 of 8000 tokens of 128 365 / 390 (e4m3 199 / 234), 16 of 4000 of 64 34.7 / 37.6; but 8 of those
-// 20.6 / 19.6, one of 32768 28 / 21, and 16 of 300 - 500 tokens of 128 e4m3 13.7 / 12.6.
+// Whether waves may take heads side by side: whole groups of four, a tile of query heads each, and enough sequences
+// that the parts, now of four heads each, are few.  With and without, rows of 8 heads: 128 sequences of 100 - 4096
+// visible tokens of 64 bf16 133.5 / 147.3 us, 64 of 8000 tokens of 128 365 / 390 (e4m3 199 / 234), 16 of 4000 of 64
+// 34.7 / 37.6; but 8 of those 20.6 / 19.6, one of 32768 28 / 21, and 16 of 300 - 500 tokens of 128 e4m3 13.7 / 12.6.
 static bool attend_side(int64_t T, int64_t hq, int64_t heads, int64_t cap) {
     return heads % 4 == 0 && hq / heads <= 16 && T >= 16 && cap >= 1024;
 }
@@ -771,7 +784,8 @@ extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
 #undef AT
     PRISM_LAUNCH_CHECK();
     if (joins) {
-  // a workgroup per head while there are few (long sequences have many parts), else one for as many as it has groups
+        // a workgroup per head while there are few (long sequences have many parts), else one for as many as it has
+        // groups
         const int hb = T * HQ <= 4096 ? 1 : (int)(1024 / D);
         const dim3 jg((unsigned)((HQ + hb - 1) / hb), (unsigned)T);
         if (D == 64) hipLaunchKernelGGL(kv_join_kernel<64>, jg, dim3(256), 0, st, a, hb);
