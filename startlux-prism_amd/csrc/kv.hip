@@ -160,8 +160,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 //
 // Bound by the cache's bytes, read once: one sequence of 131071 tokens, 8 heads of 128 bf16 (537 MB), 98 us, 5.5 TB/s, 90
 // of them this kernel (6.0 TB/s, more than a copy moves) and 7 the joining one; 40 of up to 20000, 4 heads of 256 e4m3
-// (505 MB), 101 us, 5.0 TB/s; token rows of 8 heads of 64, 128 sequences of up to 4096 visible (613 MB), 134 us,
-// 4.6 TB/s (runs of 512 bytes a token; the same heads' rows by the page take 120).  A short call (613 tokens) is launches
+// (505 MB), 101 us, 5.0 TB/s; token rows of 8 heads of 64, 128 sequences of up to 4096 visible (613 MB), 124 us,
+// 4.9 TB/s (runs of 512 bytes a token; the same heads' rows by the page take 120).  A short call (613 tokens) is launches
 // and one chain of a unit's steps, 9 us.
 struct AttendArgs {
     const uint16_t* q;
@@ -619,7 +619,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int hb) {
 
 // LDS of a workgroup, and how many workgroups a launch's work is dealt out to: as many as are there at a time, two a CU
 // where LDS holds them.  With 4 a CU (rows of 128 bytes leave LDS for them) 128 sequences of 100 - 4096 visible tokens,
-// 8 heads of 64, take 138 us instead of 133.5, 64 of 8000 tokens, 8 heads of 128 e4m3, 205 instead of 199: every further
+// 8 heads of 64, took 138 us instead of 133.5, 64 of 8000 tokens, 8 heads of 128 e4m3, 205 instead of 199: every further
 // part is more to join.  One a CU: 131071 tokens, 8 heads of 128 bf16, 98 us instead of 100, but 256 sequences of
 // 20 - 300 tokens 50 instead of 41.
 static int attend_lds(int64_t D, bool f8) {
@@ -639,8 +639,8 @@ static int64_t attend_parts(int64_t T, int64_t HT, int64_t cap, int64_t unit, in
 
 // Whether waves may take heads side by side: whole groups of four, a tile of query heads each, and enough sequences
 // that the parts, now of four heads each, are few.  With and without, rows of 8 heads: 128 sequences of 100 - 4096
-// visible tokens of 64 bf16 133.5 / 147.3 us, 64 of 8000 tokens of 128 365 / 390 (e4m3 199 / 234), 16 of 4000 of 64
-// 34.7 / 37.6; but 8 of those 20.6 / 19.6, one of 32768 28 / 21, and 16 of 300 - 500 tokens of 128 e4m3 13.7 / 12.6.
+// visible tokens of 64 bf16 124 / 146 us, 64 of 8000 tokens of 128 364 / 391 (e4m3 199 / 234), 16 of 4000 of 64
+// 34.7 / 37.6; but 8 of those 20.5 / 19.5, one of 32768 28 / 21, and 16 of 300 - 500 tokens of 128 e4m3 13.2 / 11.7.
 static bool attend_side(int64_t T, int64_t hq, int64_t heads, int64_t cap) {
     return heads % 4 == 0 && hq / heads <= 16 && T >= 16 && cap >= 1024;
 }
@@ -784,9 +784,10 @@ extern "C" int prism_kv_attend(const prism_kv_attend_args* args, void* stream) {
 #undef AT
     PRISM_LAUNCH_CHECK();
     if (joins) {
-        // a workgroup per head while there are few (long sequences have many parts), else one for as many as it has
-        // groups
-        const int hb = T * HQ <= 4096 ? 1 : (int)(1024 / D);
+        // a workgroup per head while there are few (long sequences have many parts), else one for a quarter as many as
+        // it has groups: 128 sequences of 64 heads of 64 take 124 - 127 us in all, 130 with half as many, 137 with as
+        // many (a chain of loads after the other), 131 with one
+        const int hb = T * HQ <= 4096 ? 1 : (int)(256 / D);
         const dim3 jg((unsigned)((HQ + hb - 1) / hb), (unsigned)T);
         if (D == 64) hipLaunchKernelGGL(kv_join_kernel<64>, jg, dim3(256), 0, st, a, hb);
         else if (D == 128) hipLaunchKernelGGL(kv_join_kernel<128>, jg, dim3(256), 0, st, a, hb);
