@@ -287,41 +287,43 @@ __device__ __forceinline__ bool find_chunk(const DeltaArgs& a, int id, int& firs
 }
 
 // The records go past the caches (delta_scan reads them after all are written): 8191 tokens 379 us in all instead of
-// 396.
+// 396 when that was measured.
 __device__ __forceinline__ void put_frag(char* base, v4u v) {
     __builtin_nontemporal_store(v, reinterpret_cast<v4u*>(base + (threadIdx.x & 63) * 16));
 }
 
-// One wave per chunk (blockIdx.x) and value head (blockIdx.y).  Rows are loaded in their own order (a row per lane
-// would take the memory pipeline four times as long) and become fragments through LDS.  The decays between tokens of
-// different 16-row tiles are products of three that are at most 1, so that 16 exponentials a lane (the diagonal tiles')
-// and a few are enough for 40.  One chunk takes 13 us, the chain of its steps; 8191 tokens of 16 key and 48 value heads
-// of 128 take 100 us, bound by the records' 255 MB (47 us without their stores).
+// A workgroup per chunk (blockIdx.x) and value head (blockIdx.y), a wave per 16 of the chunk's rows (of X's columns
+// where the system is solved).  Rows are loaded in their own order (a row per lane would take the memory pipeline four
+// times as long) and become fragments through LDS.  The decays between tokens of different 16-row tiles are products of
+// three that are at most 1, so that a diagonal tile's exponentials and a few are enough.  One chunk takes 9 us, the
+// chain of its steps, and 8191 tokens of 16 key and 48 value heads of 128 take 86 us, the records' 255 MB for the most
+// part; with one wave for all four tiles 13 and 100 us, with each wave inverting its own diagonal block 9.4 and 109.
 template <int DK>
-__global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, char* wv) {
-    constexpr int KS = DK / 32, LD = kC + 4, LK = DK + 8, PR = DK / 8;   // PR: 16-byte pieces of a row
-    __shared__ __align__(16) float x[kC * LD];                // K's, then Q's rows (bf16); A, then X, in place
+__global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* wk, char* wv) {
+    constexpr int KS = DK / 32, LD = kC + 4, LK = DK + 8, PR = DK / 8, NL = 16 * PR / 64;  // PR: 16-byte pieces of a row
+    __shared__ __align__(16) uint16_t rows[2][kC * LK];       // K's and Q's rows; then A, then X, in place
     __shared__ double gsum[kC];
-    __shared__ float rkv[kC], rqv[kC], kup[kC], kdn[kC], qup[kC], bev[kC], upv[kC], dnv[kC], xdn[kC], odn[kC];
-    static_assert(sizeof(x) >= kC * LK * 2, "K's rows");
+    __shared__ float rkv[kC], rqv[kC], kup[kC], kdn[kC], qup[kC], qdn[kC], bev[kC], upv[kC], dnv[kC], xdn[kC], odn[kC];
+    static_assert(sizeof(rows) >= kC * LD * 4, "A");
+    float* x = reinterpret_cast<float*>(rows);
     int first, count;
     if (!find_chunk(a, blockIdx.x, first, count)) return;
-    const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const int head = blockIdx.y, share = a.HV / a.HK, hk = head / share, part = head % share;
+    const int own = 16 * w + col;                             // this lane's row where a fragment's rows are lanes
     char* rk = wk + ((int64_t)blockIdx.x * a.HK + hk) * rec_k(DK);
     char* rv = wv + ((int64_t)blockIdx.x * a.HV + head) * kRecV;
 
-    v4u kr[PR], qr[PR];                                       // rows past the chunk are zeros
+    v4u kr[NL], qr[NL];                                       // rows past the chunk are zeros
 #pragma unroll
-    for (int i = 0; i < PR; i++) {
-        const int row = i * (64 / PR) + lane / PR;
-        const int64_t t = first + min(row, count - 1);
+    for (int i = 0; i < NL; i++) {
+        const int64_t t = first + min(16 * w + i * (64 / PR) + lane / PR, count - 1);
         kr[i] = *reinterpret_cast<const v4u*>(a.k + t * a.ldk + hk * a.hk_s + 8 * (lane % PR));
         qr[i] = *reinterpret_cast<const v4u*>(a.q + t * a.ldq + hk * a.hq_s + 8 * (lane % PR));
     }
     // the chunk's gates, one token per lane, the sums in 64 bits: the differences G_i - G_j are then as exact as the g.
     // Below -1e4 a decay is 0 either way, and sums stay finite (-inf minus -inf would not be a number)
-    {
+    if (w == 0) {
         const bool in = lane < count;
         const int64_t t = first + min(lane, count - 1);
         const float be = a.beta[t * a.ldb + head];
@@ -340,62 +342,51 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
         upv[lane] = expf((float)(s - (lane < 16 ? 0.0 : before)));
         dnv[lane] = expf((float)(last - s));
     }
-    uint16_t* rows = reinterpret_cast<uint16_t*>(x);
-    auto put = [&](const v4u (&r)[PR]) {
-        __syncthreads();
 #pragma unroll
-        for (int i = 0; i < PR; i++) {
-            const int row = i * (64 / PR) + lane / PR;
-            *reinterpret_cast<v4u*>(rows + row * LK + 8 * (lane % PR)) = row < count ? r[i] : v4u{0, 0, 0, 0};
+    for (int i = 0; i < NL; i++) {
+        const int row = 16 * w + i * (64 / PR) + lane / PR, at = row * LK + 8 * (lane % PR);
+        *reinterpret_cast<v4u*>(rows[0] + at) = row < count ? kr[i] : v4u{0, 0, 0, 0};
+        *reinterpret_cast<v4u*>(rows[1] + at) = row < count ? qr[i] : v4u{0, 0, 0, 0};
+    }
+    __syncthreads();
+    // fragment s of tile i: its row col, dims 32 s + 8 g .. + 7
+    auto get = [&](v4u (&f)[KS], const uint16_t* r, int i) {
+#pragma unroll
+        for (int s = 0; s < KS; s++) f[s] = *reinterpret_cast<const v4u*>(r + (16 * i + col) * LK + 32 * s + 8 * g);
+    };
+    // the tile's rows' lengths, from the diagonal of K K^T or Q Q^T: their scales and, if asked, the normalising
+    // factors
+    auto lengths = [&](const v4u (&f)[KS], float* unit, float* up, float* down, float scale) {
+        v4f d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KS; s++) d = mfma_bf16(f[s], f[s], d);
+        const float sq = col & 2 ? (col & 1 ? d[3] : d[2]) : (col & 1 ? d[1] : d[0]);
+        if (g == col >> 2) {
+            const Pow2 p = pow2_of(sqrt_rn(sq));              // (no value of a row is above its length)
+            unit[own] = (a.norm ? div_rn(1.f, sqrt_rn(sq + a.eps)) : 1.f) * scale;
+            up[own] = p.up;
+            down[own] = p.down;
         }
-        __syncthreads();
     };
-    // fragment (i, s): tile i's row col, dims 32 s + 8 g .. + 7
-    auto get = [&](v4u (&f)[4][KS]) {
+    v4u kf[KS], qf[KS];
+    get(kf, rows[0], w);
+    get(qf, rows[1], w);
+    lengths(kf, rkv, kup, kdn, 1.f);
+    lengths(qf, rqv, qup, qdn, a.scale);
+    __syncthreads();
+    // as delta_scan's left operand, scaled rows: fragment (w, s), dims 32 s + 4 g + j, then 32 s + 16 + 4 g + j
+    auto copy = [&](char* to, const uint16_t* from, const float* up) {
+        const float u = up[own];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-                f[i][s] = *reinterpret_cast<const v4u*>(rows + (16 * i + col) * LK + 32 * s + 8 * g);
-    };
-    // as delta_scan's left operand, scaled rows: fragment (i, s), dims 32 s + 4 g + j, then 32 s + 16 + 4 g + j
-    auto copy = [&](char* to, const float* up) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const uint16_t* r = rows + (16 * i + col) * LK + 32 * s + 4 * g;
-                const v2u lo = *reinterpret_cast<const v2u*>(r), hi = *reinterpret_cast<const v2u*>(r + 16);
-                const float u = up[16 * i + col];
-                put_frag(to + (i * KS + s) * kFrag,
-                         v4u{bf16x2_f16(lo[0], u), bf16x2_f16(lo[1], u), bf16x2_f16(hi[0], u), bf16x2_f16(hi[1], u)});
-            }
-    };
-    // the rows' lengths, from the diagonal of K K^T or Q Q^T: their scales and, if asked, the normalising factors
-    auto lengths = [&](const v4u (&f)[4][KS], float* unit, float* up, float scale) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v4f d = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KS; s++) d = mfma_bf16(f[i][s], f[i][s], d);
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (4 * g + r == col) unit[16 * i + col] = d[r];
+        for (int s = 0; s < KS; s++) {
+            const uint16_t* r = from + own * LK + 32 * s + 4 * g;
+            const v2u lo = *reinterpret_cast<const v2u*>(r), hi = *reinterpret_cast<const v2u*>(r + 16);
+            put_frag(to + (w * KS + s) * kFrag,
+                     v4u{bf16x2_f16(lo[0], u), bf16x2_f16(lo[1], u), bf16x2_f16(hi[0], u), bf16x2_f16(hi[1], u)});
         }
-        __syncthreads();
-        const float sq = unit[lane];
-        const Pow2 p = pow2_of(sqrt_rn(sq));                  // (no value of a row is above its length)
-        unit[lane] = (a.norm ? div_rn(1.f, sqrt_rn(sq + a.eps)) : 1.f) * scale;
-        up[lane] = p.up;
-        __syncthreads();
-        return p.down;
     };
-    v4u kf[4][KS], qf[4][KS];
-    put(kr);
-    get(kf);
-    kdn[lane] = lengths(kf, rkv, kup, 1.f);
-    // this key head's fragments of K, K^T and Q are written by its first, second and last value head's wave
-    if (part == 0) copy(rk, kup);
+    // this key head's fragments of K, K^T and Q are written by its first, second and last value head's workgroup
+    if (part == 0) copy(rk, rows[0], kup);
     if (part == (share > 1 ? 1 : 0)) {
         // K^T: fragment (d, s), row 16 d + col, tokens 32 s + 4 g + j and 32 s + 16 + 4 g + j
         char* ft = rk + 8 * KS * kFrag;
@@ -405,66 +396,67 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
 #pragma unroll
             for (int e = 0; e < 2; e++) up[e] = *reinterpret_cast<const v4f*>(kup + 32 * s + 16 * e + 4 * g);
 #pragma unroll
-            for (int d = 0; d < DK / 16; d++) {
+            for (int e = 0; e < DK / 64; e++) {
+                const int d = w * (DK / 64) + e;
                 float u[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    u[j] = bf16_to_f32(rows[(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col]) *
+                    u[j] = bf16_to_f32(rows[0][(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col]) *
                            up[j / 4][j % 4];
-                v4u w;
+                v4u o;
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    w[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(u[2 * j], u[2 * j + 1]));
-                put_frag(ft + (2 * d + s) * kFrag, w);
+                    o[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(u[2 * j], u[2 * j + 1]));
+                put_frag(ft + (2 * d + s) * kFrag, o);
             }
         }
     }
-    put(qr);
-    get(qf);
-    const float qdn = lengths(qf, rqv, qup, a.scale);
-    if (part == share - 1) copy(rk + 4 * KS * kFrag, qup);
+    if (part == share - 1) copy(rk + 4 * KS * kFrag, rows[1], qup);
 
-    // k_i . k_j and q_i . k_j, tiles j <= i, transposed: a lane holds row i = col for columns 4 g + r, which is a
+    // k_i . k_j and q_i . k_j, tiles j <= i = w, transposed: a lane holds row `own` for columns 4 g + r, which is a
     // fragment's order
-    v4f pt[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int row = 16 * i + col;
-        const double gi = gsum[row];
-        const float up = upv[row], ki = bev[row] * rkv[row], qi = rqv[row];
+    v4f pt[4], am[4];
+    {
+        const double gi = gsum[own];
+        const float up = upv[own], ki = bev[own] * rkv[own], qi = rqv[own];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            pt[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-            if (j > i) continue;
-            v4f kk = {0.f, 0.f, 0.f, 0.f}, qk = kk, am, f;
+            pt[j] = am[j] = v4f{0.f, 0.f, 0.f, 0.f};
+            if (j > w) continue;
+            v4f kk = {0.f, 0.f, 0.f, 0.f}, qk = kk, f;
+            v4u kj[KS];
+            get(kj, rows[0], j);
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                kk = mfma_bf16(kf[j][s], kf[i][s], kk);
-                qk = mfma_bf16(kf[j][s], qf[i][s], qk);
+                kk = mfma_bf16(kj[s], kf[s], kk);
+                qk = mfma_bf16(kj[s], qf[s], qk);
             }
             const int c0 = 16 * j + 4 * g;
-            if (i == j) {
+            if (w == j) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) f[r] = expf((float)(gi - gsum[c0 + r]));
             } else {
-                const float mid = i == j + 1 ? up : up * expf((float)(gsum[16 * i - 1] - gsum[16 * j + 15]));
+                const float mid = w == j + 1 ? up : up * expf((float)(gsum[16 * w - 1] - gsum[16 * j + 15]));
 #pragma unroll
                 for (int r = 0; r < 4; r++) f[r] = mid * dnv[c0 + r];
             }
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 f[r] *= rkv[c0 + r];
-                am[r] = c0 + r < row ? f[r] * ki * kk[r] : 0.f;
-                pt[i][j][r] = c0 + r <= row ? f[r] * qi * qk[r] : 0.f;
+                am[j][r] = c0 + r < own ? f[r] * ki * kk[r] : 0.f;
+                pt[j][r] = c0 + r <= own ? f[r] * qi * qk[r] : 0.f;
             }
-            *reinterpret_cast<v4f*>(x + row * LD + c0) = am;
         }
     }
+    __syncthreads();                                          // K's and Q's rows are read
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        if (j <= w) *reinterpret_cast<v4f*>(x + own * LD + 16 * j + 4 * g) = am[j];
     __syncthreads();
 
     // the four diagonal blocks of I + A inverted at once by forward substitution, a column per lane
-    {
-        const float* d = x + 16 * g * LD + 16 * g;
+    if (w == 0) {
+        float* d = x + 16 * g * LD + 16 * g;
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -478,90 +470,80 @@ __global__ __launch_bounds__(64) void delta_prep_kernel(DeltaArgs a, char* wk, c
             }
             v[i] = s;
         }
-        __syncthreads();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
+        __builtin_amdgcn_wave_barrier();                      // (the wave's reads come before its writes)
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[(16 * g + i) * LD + 16 * g + col] = v[i];
+        for (int i = 0; i < 16; i++) d[i * LD + col] = v[i];
     }
     __syncthreads();
-    // the blocks below, X_ij = -X_ii sum_k A_ik X_kj, diagonal by diagonal: the X_kj are right operands as the
-    // accumulators they come in, so nothing is stored before all are there
+    // the blocks below, X_ij = -X_ii sum_k A_ik X_kj, column j = w: the X_kj are right operands as the accumulators
+    // they come in, so nothing is stored before all are there
     {
-        v4f y[4][4];                                          // [i][j]; [i][i]: the diagonal blocks in the same form
+        v4f y[4];                                             // [i - w]
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) y[i][i][r] = x[(16 * i + 4 * g + r) * LD + 16 * i + col];
+        for (int r = 0; r < 4; r++) y[0][r] = x[(16 * w + 4 * g + r) * LD + own];
 #pragma unroll
         for (int d = 1; d < 4; d++) {
-            v4f s[4];
+            const int i = w + d;
+            if (i > 3) continue;
+            v4f s = {0.f, 0.f, 0.f, 0.f}, z = s;
 #pragma unroll
-            for (int i = d; i < 4; i++) {
-                s[i] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < d; k++) {
+                const v4f m = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * (w + k) + 4 * g);
 #pragma unroll
-                for (int k = i - d; k < i; k++) {
-                    const v4f am = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * k + 4 * g);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) s[i] = mfma_f32(am[r], y[k][i - d][r], s[i]);
-                }
+                for (int r = 0; r < 4; r++) s = mfma_f32(m[r], y[k][r], s);
             }
+            const v4f xi = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * i + 4 * g);
 #pragma unroll
-            for (int i = d; i < 4; i++) {
-                const v4f xi = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * i + 4 * g);
-                v4f z = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int r = 0; r < 4; r++) z = mfma_f32(xi[r], s[i][r], z);
-                y[i][i - d] = -z;
-            }
+            for (int r = 0; r < 4; r++) z = mfma_f32(xi[r], s[r], z);
+            y[d] = -z;
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 1; i < 4; i++)
+        for (int d = 1; d < 4; d++)
+            if (w + d < 4)
 #pragma unroll
-            for (int j = 0; j < i; j++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) x[(16 * i + 4 * g + r) * LD + 16 * j + col] = y[i][j][r];
+                for (int r = 0; r < 4; r++) x[(16 * (w + d) + 4 * g + r) * LD + own] = y[d][r];
     }
     __syncthreads();
     // X diag(beta), and then P, whose columns take X's rows' scales (U's rows come out in them)
-    auto put_tri = [&](int i, const v4f (&h)[4], float* down, char* to) {
+    auto put_tri = [&](const v4f (&h)[4], float* down, char* to) {
         float m = 0.f;
 #pragma unroll
-        for (int j = 0; j <= i; j++) m = max_abs(m, h[j]);
+        for (int j = 0; j < 4; j++) m = max_abs(m, h[j]);     // (zeros right of the diagonal)
         const Pow2 p = pow2_of(column_max(m));
-        down[16 * i + col] = p.down;
+        down[own] = p.down;
 #pragma unroll
-        for (int s = 0; s <= i / 2; s++) {
+        for (int s = 0; s < 2; s++) {
+            if (s > w / 2) continue;
             const Split sp = split8(h[2 * s], h[2 * s + 1], p.up);
-            put_frag(to + 2 * tri(i, s) * kFrag, sp.h);
-            put_frag(to + (2 * tri(i, s) + 1) * kFrag, sp.l);
+            put_frag(to + 2 * tri(w, s) * kFrag, sp.h);
+            put_frag(to + (2 * tri(w, s) + 1) * kFrag, sp.l);
         }
     };
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
+    {
         v4f h[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             h[j] = v4f{0.f, 0.f, 0.f, 0.f};
-            if (j <= i)
-                h[j] = *reinterpret_cast<const v4f*>(x + (16 * i + col) * LD + 16 * j + 4 * g) *
+            if (j <= w)
+                h[j] = *reinterpret_cast<const v4f*>(x + own * LD + 16 * j + 4 * g) *
                        *reinterpret_cast<const v4f*>(bev + 16 * j + 4 * g);
         }
-        put_tri(i, h, xdn, rv);
+        put_tri(h, xdn, rv);
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-#pragma unroll
-        for (int j = 0; j <= i; j++) pt[i][j] *= *reinterpret_cast<const v4f*>(xdn + 16 * j + 4 * g);
-        put_tri(i, pt[i], odn, rv + 2 * kTri * kFrag);
-    }
+    for (int j = 0; j < 4; j++)
+        if (j <= w) pt[j] *= *reinterpret_cast<const v4f*>(xdn + 16 * j + 4 * g);
+    put_tri(pt, odn, rv + 2 * kTri * kFrag);
     __syncthreads();
-    {
+    if (w == 0) {
         float* vec = reinterpret_cast<float*>(rv + 4 * kTri * kFrag);
         const double gl = gsum[lane], gc = gsum[kC - 1];
         const float e = expf((float)gl), kd = rkv[lane] * kdn[lane], od = odn[lane];
         vec[lane] = e * kd;
-        vec[kC + lane] = e * rqv[lane] * qdn * (1.f / od);    // (a power of two)
+        vec[kC + lane] = e * rqv[lane] * qdn[lane] * (1.f / od);  // (a power of two)
         vec[2 * kC + lane] = expf((float)(gc - gl)) * kd * xdn[lane];
         vec[3 * kC + lane] = od;
         vec[4 * kC + lane] = expf((float)gc);
@@ -914,7 +896,7 @@ static int launch_chunks(const DeltaArgs& a, char* ws, hipStream_t st) {
     const int64_t wgs = (keys + 7) / 8 * 8 * (a.HV / a.HK) * (DV / 32);
     if (nc > INT32_MAX || wgs > INT32_MAX) return PRISM_ERR_SHAPE;
     char* wv = ws + nc * a.HK * rec_k(DK);
-    hipLaunchKernelGGL(delta_prep_kernel<DK>, dim3((unsigned)nc, (unsigned)a.HV), dim3(64), 0, st, a, ws, wv);
+    hipLaunchKernelGGL(delta_prep_kernel<DK>, dim3((unsigned)nc, (unsigned)a.HV), dim3(256), 0, st, a, ws, wv);
     PRISM_LAUNCH_CHECK();
     allow_lds(delta_scan_kernel<DK, DV>, sizeof(ScanShared<DK>));
     hipLaunchKernelGGL((delta_scan_kernel<DK, DV>), dim3((unsigned)wgs), dim3(768), sizeof(ScanShared<DK>), st, a, ws, wv,
@@ -933,12 +915,13 @@ static int dispatch_chunks(const DeltaArgs& a, int64_t DK, int64_t DV, char* ws,
     return DV == 64 ? launch_chunks<128, 64>(a, ws, st) : launch_chunks<128, 128>(a, ws, st);
 }
 
-// A few rows go token by token: 1.5 us each for a sequence's at 48 heads, against 19 us for its first chunk (12 rows 21
-// us, 8 rows 15).
-static bool by_token(int64_t T) { return T <= 12; }
+// A few rows go token by token: 1.5 us each for a sequence's at 48 heads, against 15.5 us for its first chunk (one
+// sequence of 6 rows 12.3 us, 8 rows 15.8, 10 rows 18.6; 12 rows of 6 sequences 8.1 against 18.3, of one 21.8 against
+// 15.8).
+static bool by_token(int64_t T, int64_t seqs) { return T <= (seqs > 1 ? 12 : 8); }
 
 static int64_t workspace_bytes(int64_t T, int64_t seqs, int64_t hk, int64_t hv, int64_t dk) {
-    if (T < 1 || seqs < 1 || hk < 1 || hv < 1 || (dk != 64 && dk != 128) || by_token(T)) return 0;
+    if (T < 1 || seqs < 1 || hk < 1 || hv < 1 || (dk != 64 && dk != 128) || by_token(T, seqs)) return 0;
     return chunks(T, seqs) * (hk * rec_k((int)dk) + hv * kRecV);
 }
 
