@@ -149,8 +149,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 // leaves its lane, and neither do the maximum, the sum and the rescaling of O^T's columns (all of head lane % 16).
 // V's operand needs 8 tokens of one dim per lane: a lane loads its 8 tokens' rows in pieces of D / 16 dims (16 lanes
 // a whole row, contiguous) and turns the 8 x D/16 block with one v_perm per register.
-// P is split into two bf16 parts (truncated, then the rest), so the weights carry 16 bits and the output's one bf16
-// rounding is the only one that shows; the second MFMA is free beside the cache's bytes.
+// P is split into three bf16 parts, each what the last one left (the first two cut, the third rounded: within 2^-23 of the
+// weight), so the weights carry fp32's bits and the output's one bf16 rounding is the only one that shows.  The further
+// MFMAs are free beside the cache's bytes: with two parts, cut, the same times (98.7 and 98.7, 101.4 and 101.8, 126.8 and 126.7
+// us for the three sizes below), and outputs that lean toward zero by 1e-5, what the weights lose and their sum does not.
 //
 // Work is split on the device, from the lengths (a captured launch serves every batch): a unit is what the four waves
 // take in one round (128 tokens of a head, or 32 of four); laid one after the other, the sequences' units are dealt out
@@ -252,6 +254,16 @@ __device__ __forceinline__ v8bf as_bf(v4u x) { return __builtin_bit_cast(v8bf, x
 __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(a), as_bf(b), c, 0, 0, 0);
 }
+// Two weights' upper parts as bf16, each cut to 8 bits strictly below the weight, and what is left of them.  What is left
+// of a weight is then never 0: a part of 0 times an infinite value would be NaN, where the weight itself gives infinity.
+__device__ __forceinline__ uint32_t below(float e0, float e1, float& r0, float& r1) {
+    const uint32_t b0 = max(__float_as_uint(e0), 1u) - 1u, b1 = max(__float_as_uint(e1), 1u) - 1u;
+    r0 = e0 - __uint_as_float(b0 & 0xffff0000u), r1 = e1 - __uint_as_float(b1 & 0xffff0000u);
+    return __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+}
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+
 // Two e4m3 bytes (SEL: the upper two) as two bf16, exactly.
 template <bool SEL>
 __device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
@@ -472,19 +484,18 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
                 for (int f = 0; f < F; f++) o[f] *= al;
             }
             m = mn;
-            uint32_t hi[4], lw[4];
+            uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 const float e0 = __builtin_amdgcn_exp2f(p[2 * w] - ref), e1 = __builtin_amdgcn_exp2f(p[2 * w + 1] - ref);
                 l += e0 + e1;
-                // the upper part strictly below the weight, so that the rest of a weight is never 0 (0 times an
-                // infinite value would be NaN, not infinite)
-                const uint32_t b0 = max(__float_as_uint(e0), 1u) - 1u, b1 = max(__float_as_uint(e1), 1u) - 1u;
-                hi[w] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
-                const float r0 = e0 - __uint_as_float(b0 & 0xffff0000u), r1 = e1 - __uint_as_float(b1 & 0xffff0000u);
-                lw[w] = __builtin_amdgcn_perm(__float_as_uint(r1), __float_as_uint(r0), 0x07060302u);
+                float r0, r1, s0, s1;
+                hi[w] = below(e0, e1, r0, r1);
+                mid[w] = below(r0, r1, s0, s1);
+                lo[w] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{s0, s1}), v2bf));
             }
-            const v4u ph = {hi[0], hi[1], hi[2], hi[3]}, plo = {lw[0], lw[1], lw[2], lw[3]};
+            const v4u ph = {hi[0], hi[1], hi[2], hi[3]}, pm = {mid[0], mid[1], mid[2], mid[3]},
+                      pl = {lo[0], lo[1], lo[2], lo[3]};
 #pragma unroll
             for (int q = 0; q < F / 4; q++) {
                 v4u vf[4];
@@ -492,7 +503,8 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
 #pragma unroll
                 for (int f = 0; f < 4; f++) {
                     o[4 * q + f] = mfma_bf16(vf[f], ph, o[4 * q + f]);
-                    o[4 * q + f] = mfma_bf16(vf[f], plo, o[4 * q + f]);
+                    o[4 * q + f] = mfma_bf16(vf[f], pm, o[4 * q + f]);
+                    o[4 * q + f] = mfma_bf16(vf[f], pl, o[4 * q + f]);
                 }
             }
         };

@@ -55,8 +55,8 @@ def attend(q, k_cache, v_cache, table, lens, out, n, T, scale=None, window=0, k_
     holds counts as what it holds); window > 0: only the last `window` of them.  A sequence without tokens gets zeros.
     scale None: dim ** -0.5.
 
-    q, out bf16 [>= T, heads, dim], unit stride in dim.  Softmax and sums in fp32, the weights in two bf16 parts (16 bits),
-    the output rounded once.  Results do not depend on timing; how a sequence's length is split, and so the order of its
+    q, out bf16 [>= T, heads, dim], unit stride in dim.  Softmax, weights and sums in fp32 (the products take the weights as
+    three bf16 parts), the output rounded once.  Results do not depend on timing; how a sequence's length is split, and so the order of its
     sums, depends on the batch.  Table entries of visible tokens must name pages (others read some page, never memory
     outside the cache)."""
     if n is None:
