@@ -363,7 +363,8 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
         const float sq = col & 2 ? (col & 1 ? d[3] : d[2]) : (col & 1 ? d[1] : d[0]);
         if (g == col >> 2) {
             const Pow2 p = pow2_of(sqrt_rn(sq));              // (no value of a row is above its length)
-            unit[own] = (a.norm ? div_rn(1.f, sqrt_rn(sq + a.eps)) : 1.f) * scale;
+            // (rows past the chunk are zeros, whose length eps = 0 would divide by)
+            unit[own] = own < count ? (a.norm ? div_rn(1.f, sqrt_rn(sq + a.eps)) : 1.f) * scale : 0.f;
             up[own] = p.up;
             down[own] = p.down;
         }

@@ -1,0 +1,34 @@
+"""prism_amd.delta on the GPU where its forms can go wrong: normalising without an eps, with the checks and tolerances of
+test_delta_gpu."""
+import pytest
+import torch
+
+from test_delta_gpu import compare, inputs, recurrence, split
+
+pytestmark = pytest.mark.gpu
+
+
+def check_prefill(dev, lens, hk, hv, dk, dv, seed=0, eps=1e-6, lead=0, tail=0):
+    """Prompts of these lengths after `lead` rows of none, `tail` rows of none behind; every state and row of out checked."""
+    from prism_amd import delta
+    T, states = lead + sum(lens) + tail, len(lens) + 1
+    proj, g, beta, state = inputs(T, hk, hv, dk, dv, states, seed)
+    cu = [lead + sum(lens[:i]) for i in range(len(lens) + 1)]
+    spans = list(zip(cu, cu[1:]))
+    slots = torch.randperm(states, generator=torch.Generator().manual_seed(seed))[:len(lens)].int()
+    q, k, v = split(proj, hk, hv, dk, dv)
+    want = recurrence(q, k, v, g, beta, state, spans, slots.tolist(), True, dk ** -0.5, eps)
+    dq, dk_, dv_ = split(proj.to(dev), hk, hv, dk, dv)
+    ds, out = state.to(dev), torch.full((T, hv, dv), float("nan"), device=dev)
+    delta.prefill(dq, dk_, dv_, g.to(dev), beta.to(dev), ds, out, torch.tensor(cu, dtype=torch.int32, device=dev), T,
+                  slots=slots.to(dev), eps=eps)
+    assert torch.equal(torch.isnan(out.cpu()), torch.isnan(want[0]))
+    compare(out, ds, *want, spans, v, dk, state)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-60])                    # (the second is 0 in fp32)
+@pytest.mark.parametrize("lens", [[1], [5], [64], [65], [77], [130], [70, 0, 3, 129, 64, 31]])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 64)])
+def test_prefill_without_eps(dev, lens, eps, dk, dv):
+    """Lengths that leave a chunk unfilled: the rows past its end have no length to divide by."""
+    check_prefill(dev, lens, 2, 4, dk, dv, seed=sum(lens), eps=eps)
