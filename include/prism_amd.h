@@ -464,8 +464,8 @@ PRISM_API int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t hq, int64_t
 /*
  * The gated delta rule, per value head h with key head h / (hv / hk) and state S fp32 [dk, dv]:
  *   S <- exp(g) S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q,
- * k and q first divided by sqrt(|.|^2 + eps) when norm = 1, q times scale either way; fp32 sums and state
- * (prompts' products take fp32 operands as two fp16 parts, 22 bits).
+ * k and q first divided by sqrt(|.|^2 + eps) when norm = 1, q times scale either way; fp32 sums, state and operands (of
+ * prompts' products as three bf16 parts each).
  * q, k bf16 [T, hk, dk], v bf16 [T, hv, dv], g, beta fp32 [T, hv], out fp32 [T, hv, dv] (ld: row strides, hs: head
  * strides); state [nslots, hv, dk, dv] contiguous per slot, slot_ld apart, updated in place; slots int32: the state of
  * each sequence (null: its number).  A sequence whose slot is out of range is skipped; two sequences must not share one.

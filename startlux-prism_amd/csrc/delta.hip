@@ -165,18 +165,15 @@ static int launch_rec(const DeltaArgs& a, hipStream_t st) {
 // delta_scan walks each sequence's chunks.  The normalisation is row scales (rk, rq), so K and Q stay the bf16 they
 // are.
 //
-// The products run on the fp16 MFMA at nearly fp32's precision: an fp32 operand is two fp16, the value rounded to 11
-// bits and what is left rounded to 11 more (to nearest: the error is below 2^-23 of the value), two products against K
-// or Q, three against another such pair (the fourth is below 2^-22 of the terms).  fp16's range is made to do by powers
-// of two: every row of K, Q, X and P and every column (lane) of S, R and U is scaled so that its largest value is about
-// 2^14, which leaves the lower halves normal down to 2^-28 of it; the powers are taken off with factors that are there
-// anyway, or exactly after the product.  bf16 operands (K and Q, 8 bits) fit one fp16.  Against three bf16 parts, which
-// need no scales but three and six products: the same error (1.7e-7 of the outputs), 16 of 24 and 9 of 18 MFMAs, a
-// third less of X and P to write and read; delta_scan 313 us instead of 326 (8191 tokens, 16 key and 48 value heads of
-// 128).
+// The products run on the bf16 MFMA at fp32's precision and range: an fp32 operand is three bf16 that add up to it (S, R
+// and U cut, 8 bits after 8; X and P each the rounding of what the last part left), three products against K or Q, which
+// are bf16, six against another such triple (the three dropped ones are below 2^-23 of the terms).  Every value keeps its
+// own exponent, so no value's size touches another's bits.  Pairs of fp16 under powers of two shared by a column need two
+// and three products (8191 tokens, 16 key and 48 value heads of 128: 352 us instead of 381), but what a value keeps then
+// depends on the largest of its column: a token's update was rounded by, or lost to, a large value that came after it.
 //
-// A token's outputs depend on its own and earlier tokens only, but a value that is not finite reaches its whole chunk
-// (zeros of a triangle times infinity).
+// A token's outputs depend on its own and earlier tokens only, whatever finite values the later ones hold; a value that is
+// not finite reaches its whole chunk (zeros of a triangle times infinity).
 //
 // Everything that delta_scan multiplies from the left (K, Q, K^T, X diag(beta), P) lies in the workspace as MFMA
 // fragments, 1 KB each in lane order.  Inside a product the order of the summed index is free: taking it as an
@@ -189,8 +186,8 @@ constexpr int kTri = 6;       // fragments (i, s) of a lower triangle: 16-row ti
 __host__ __device__ constexpr int tri(int i, int s) { return i < 2 ? i : 2 * i - 2 + s; }
 // K, Q, K^T
 __host__ __device__ constexpr int64_t rec_k(int DK) { return (int64_t)(4 * (DK / 32) * 2 + DK / 16 * 2) * kFrag; }
-// X diag(beta), P; factors: of K S, Q S, U, the output's; e^(G_63)
-constexpr int64_t kRecV = 2 * 2 * kTri * kFrag + 5 * kC * 4;
+// X diag(beta), P, three parts each (two side by side, the third of all behind them); factors of K S, of Q S and of U; e^(G_63)
+constexpr int64_t kRecV = 2 * 3 * kTri * kFrag + 4 * kC * 4;
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
@@ -205,61 +202,47 @@ __device__ __forceinline__ void dma4(const void* g, void* lds) {
     __builtin_amdgcn_global_load_lds(g, (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
 }
 
-// fp16 operands
-typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ v4f mfma_f16(v4u a, v4u b, v4f c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-}
-
-// The power of two that brings values up to `most` to 2^14 .. 2^15, and its inverse.  Below 2^-60 it stays what it is
-// there (nothing overflows, and what such small values lose is far below the rest of their row or column); infinities
-// and NaN stay what they are.
-struct Pow2 {
-    float up, down;
-};
-__device__ __forceinline__ Pow2 pow2_of(float most) {
-    const uint32_t e = max(__float_as_uint(most) >> 23 & 0xff, 67u);
-    return Pow2{__uint_as_float((268 - e) << 23), __uint_as_float((e - 14) << 23)};
-}
-__device__ __forceinline__ float max_abs(float m, v4f x) {
-#pragma unroll
-    for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(x[r]));
-    return m;
-}
-// The largest of the four lanes of a column (lane % 16).
-__device__ __forceinline__ float column_max(float m) {
-    const uint32_t a = __float_as_uint(m);
-    const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
-    const uint32_t b = __float_as_uint(fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
-    const auto y = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-}
-
-// Eight fp32 (x then y) times a power of two as two fp16 fragments: h = RN(x s), l = RN(x s - h); products and
-// differences are exact.  No inline assembly: the compiler does not put the wait states between it and an MFMA that
+// Eight fp32 (x then y) as three bf16 fragments, of which the first two round: h = RN(x), m = RN(x - h), l = x - h - m.  All
+// differences are exact.  No inline assembly here: the compiler does not put the wait states between it and an MFMA that
 // reads its result.
 typedef float v2f __attribute__((ext_vector_type(2)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 struct Split {
-    v4u h, l;
+    v4u h, m, l;
 };
-__device__ __forceinline__ Split split8(v4f x, v4f y, float s) {
+__device__ __forceinline__ uint32_t bf16x2(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2bf));
+}
+__device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ Split split_rn(v4f x, v4f y) {
+    Split r;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        float a = w < 2 ? x[2 * w] : y[2 * w - 4], b = w < 2 ? x[2 * w + 1] : y[2 * w - 3];
+        r.h[w] = bf16x2(a, b);
+        a -= low_half(r.h[w]), b -= high_half(r.h[w]);
+        r.m[w] = bf16x2(a, b);
+        r.l[w] = bf16x2(a - low_half(r.m[w]), b - high_half(r.m[w]));
+    }
+    return r;
+}
+// The same with parts cut to 8 bits, which is faster (8191 tokens 381 us, with rounded ones in the scan 396).
+__device__ __forceinline__ uint32_t upper(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float rest(float x) { return x - high_half(__float_as_uint(x)); }
+__device__ __forceinline__ Split split_cut(v4f x, v4f y) {
     Split r;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         const float a = w < 2 ? x[2 * w] : y[2 * w - 4], b = w < 2 ? x[2 * w + 1] : y[2 * w - 3];
-        const v2h h = __builtin_convertvector((v2f{a * s, b * s}), v2h);
-        const v2f d = {__builtin_fmaf(a, s, -(float)h[0]), __builtin_fmaf(b, s, -(float)h[1])};
-        r.h[w] = __builtin_bit_cast(uint32_t, h);
-        r.l[w] = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, v2h));
+        const float a1 = rest(a), b1 = rest(b);
+        r.h[w] = upper(a, b);
+        r.m[w] = upper(a1, b1);
+        r.l[w] = upper(rest(a1), rest(b1));
     }
     return r;
-}
-__device__ __forceinline__ float cut(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-// Two bf16 times a power of two as two fp16 (exact within the range that the scale leaves).
-__device__ __forceinline__ uint32_t bf16x2_f16(uint32_t w, float s) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__uint_as_float(w << 16) * s,
-                                                                   cut(__uint_as_float(w)) * s));
 }
 
 // Chunk `id` of the workspace: sequence b's chunks start at id cu[b] / 64 + b, which leaves each sequence room for its
@@ -303,7 +286,7 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
     constexpr int KS = DK / 32, LD = kC + 4, LK = DK + 8, PR = DK / 8, NL = 16 * PR / 64;  // PR: 16-byte pieces of a row
     __shared__ __align__(16) uint16_t rows[2][kC * LK];       // K's and Q's rows; then A, then X, in place
     __shared__ double gsum[kC];
-    __shared__ float rkv[kC], rqv[kC], kup[kC], kdn[kC], qup[kC], qdn[kC], bev[kC], upv[kC], dnv[kC], xdn[kC], odn[kC];
+    __shared__ float rkv[kC], rqv[kC], bev[kC], upv[kC], dnv[kC];
     static_assert(sizeof(rows) >= kC * LD * 4, "A");
     float* x = reinterpret_cast<float*>(rows);
     int first, count;
@@ -354,65 +337,50 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
 #pragma unroll
         for (int s = 0; s < KS; s++) f[s] = *reinterpret_cast<const v4u*>(r + (16 * i + col) * LK + 32 * s + 8 * g);
     };
-    // the tile's rows' lengths, from the diagonal of K K^T or Q Q^T: their scales and, if asked, the normalising
-    // factors
-    auto lengths = [&](const v4u (&f)[KS], float* unit, float* up, float* down, float scale) {
+    // the tile's rows' normalising factors, if asked, from their lengths: the diagonal of K K^T or Q Q^T
+    auto lengths = [&](const v4u (&f)[KS], float* unit, float scale) {
         v4f d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < KS; s++) d = mfma_bf16(f[s], f[s], d);
         const float sq = col & 2 ? (col & 1 ? d[3] : d[2]) : (col & 1 ? d[1] : d[0]);
-        if (g == col >> 2) {
-            const Pow2 p = pow2_of(sqrt_rn(sq));              // (no value of a row is above its length)
-            // (rows past the chunk are zeros, whose length eps = 0 would divide by)
+        // (rows past the chunk are zeros, whose length eps = 0 would divide by)
+        if (g == col >> 2)
             unit[own] = own < count ? (a.norm ? div_rn(1.f, sqrt_rn(sq + a.eps)) : 1.f) * scale : 0.f;
-            up[own] = p.up;
-            down[own] = p.down;
-        }
     };
     v4u kf[KS], qf[KS];
     get(kf, rows[0], w);
     get(qf, rows[1], w);
-    lengths(kf, rkv, kup, kdn, 1.f);
-    lengths(qf, rqv, qup, qdn, a.scale);
+    lengths(kf, rkv, 1.f);
+    lengths(qf, rqv, a.scale);
     __syncthreads();
-    // as delta_scan's left operand, scaled rows: fragment (w, s), dims 32 s + 4 g + j, then 32 s + 16 + 4 g + j
-    auto copy = [&](char* to, const uint16_t* from, const float* up) {
-        const float u = up[own];
+    // as delta_scan's left operand: fragment (w, s), dims 32 s + 4 g + j, then 32 s + 16 + 4 g + j
+    auto copy = [&](char* to, const uint16_t* from) {
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const uint16_t* r = from + own * LK + 32 * s + 4 * g;
             const v2u lo = *reinterpret_cast<const v2u*>(r), hi = *reinterpret_cast<const v2u*>(r + 16);
-            put_frag(to + (w * KS + s) * kFrag,
-                     v4u{bf16x2_f16(lo[0], u), bf16x2_f16(lo[1], u), bf16x2_f16(hi[0], u), bf16x2_f16(hi[1], u)});
+            put_frag(to + (w * KS + s) * kFrag, v4u{lo[0], lo[1], hi[0], hi[1]});
         }
     };
     // this key head's fragments of K, K^T and Q are written by its first, second and last value head's workgroup
-    if (part == 0) copy(rk, rows[0], kup);
+    if (part == 0) copy(rk, rows[0]);
     if (part == (share > 1 ? 1 : 0)) {
         // K^T: fragment (d, s), row 16 d + col, tokens 32 s + 4 g + j and 32 s + 16 + 4 g + j
         char* ft = rk + 8 * KS * kFrag;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            v4f up[2];
-#pragma unroll
-            for (int e = 0; e < 2; e++) up[e] = *reinterpret_cast<const v4f*>(kup + 32 * s + 16 * e + 4 * g);
+        for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int e = 0; e < DK / 64; e++) {
                 const int d = w * (DK / 64) + e;
-                float u[8];
+                uint32_t u[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    u[j] = bf16_to_f32(rows[0][(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col]) *
-                           up[j / 4][j % 4];
-                v4u o;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    o[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(u[2 * j], u[2 * j + 1]));
-                put_frag(ft + (2 * d + s) * kFrag, o);
+                    u[j] = rows[0][(32 * s + 16 * (j / 4) + 4 * g + j % 4) * LK + 16 * d + col];
+                put_frag(ft + (2 * d + s) * kFrag,
+                         v4u{u[0] | (u[1] << 16), u[2] | (u[3] << 16), u[4] | (u[5] << 16), u[6] | (u[7] << 16)});
             }
-        }
     }
-    if (part == share - 1) copy(rk + 4 * KS * kFrag, rows[1], qup);
+    if (part == share - 1) copy(rk + 4 * KS * kFrag, rows[1]);
 
     // k_i . k_j and q_i . k_j, tiles j <= i = w, transposed: a lane holds row `own` for columns 4 g + r, which is a
     // fragment's order
@@ -507,21 +475,18 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
                 for (int r = 0; r < 4; r++) x[(16 * (w + d) + 4 * g + r) * LD + own] = y[d][r];
     }
     __syncthreads();
-    // X diag(beta), and then P, whose columns take X's rows' scales (U's rows come out in them)
-    auto put_tri = [&](const v4f (&h)[4], float* down, char* to) {
-        float m = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) m = max_abs(m, h[j]);     // (zeros right of the diagonal)
-        const Pow2 p = pow2_of(column_max(m));
-        down[own] = p.down;
+    // X diag(beta) and P
+    auto put_tri = [&](const v4f (&h)[4], char* to) {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             if (s > w / 2) continue;
-            const Split sp = split8(h[2 * s], h[2 * s + 1], p.up);
+            const Split sp = split_rn(h[2 * s], h[2 * s + 1]);  // (zeros right of the diagonal)
             put_frag(to + 2 * tri(w, s) * kFrag, sp.h);
-            put_frag(to + (2 * tri(w, s) + 1) * kFrag, sp.l);
+            put_frag(to + (2 * tri(w, s) + 1) * kFrag, sp.m);
+            put_frag(to + (2 * kTri + tri(w, s)) * kFrag, sp.l);
         }
     };
+    put_tri(pt, rv + 3 * kTri * kFrag);
     {
         v4f h[4];
 #pragma unroll
@@ -531,23 +496,16 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
                 h[j] = *reinterpret_cast<const v4f*>(x + own * LD + 16 * j + 4 * g) *
                        *reinterpret_cast<const v4f*>(bev + 16 * j + 4 * g);
         }
-        put_tri(h, xdn, rv);
+        put_tri(h, rv);
     }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (j <= w) pt[j] *= *reinterpret_cast<const v4f*>(xdn + 16 * j + 4 * g);
-    put_tri(pt, odn, rv + 2 * kTri * kFrag);
-    __syncthreads();
     if (w == 0) {
-        float* vec = reinterpret_cast<float*>(rv + 4 * kTri * kFrag);
+        float* vec = reinterpret_cast<float*>(rv + 6 * kTri * kFrag);
         const double gl = gsum[lane], gc = gsum[kC - 1];
-        const float e = expf((float)gl), kd = rkv[lane] * kdn[lane], od = odn[lane];
-        vec[lane] = e * kd;
-        vec[kC + lane] = e * rqv[lane] * qdn[lane] * (1.f / od);  // (a power of two)
-        vec[2 * kC + lane] = expf((float)(gc - gl)) * kd * xdn[lane];
-        vec[3 * kC + lane] = od;
-        vec[4 * kC + lane] = expf((float)gc);
+        const float e = expf((float)gl);
+        vec[lane] = e * rkv[lane];
+        vec[kC + lane] = e * rqv[lane];
+        vec[2 * kC + lane] = expf((float)(gc - gl)) * rkv[lane];
+        vec[3 * kC + lane] = expf((float)gc);
     }
 }
 
@@ -559,14 +517,15 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
 // that those come from L2.  Two barriers per chunk:
 //   state waves   K S, halves out        | halves in, R, X R out  | U in, S <- ..., S out
 //   output waves  (P U of the last one)  | S in, Q S              | P U, halves out
-//   loading waves                        | next K in              | all else of the next chunk in
+//   loading waves                        | next K in, P's last    | all else of the next chunk in
+//                                        | parts
 // Bound by that chain: a chunk takes some 5000 cycles, 3500 of them the state waves' alone, while LDS moves 370 KB
 // (2900 cycles).  8191 tokens of one sequence, 16 key and 48 value heads of 128 (192 workgroups): 280 us.
 template <int DK>
 struct ScanShared {
-    v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], x[2 * kTri][64];
+    v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], x[3 * kTri][64], pl[kTri][64];
     v4u kt[2][DK / 16 * 2][64], p[2][2 * kTri][64];           // a chunk's, the next one's beside them
-    float vec[2][5 * kC];                                     // the factors likewise
+    float vec[2][4 * kC];                                     // the factors likewise
     v4f sx[2][DK / 16][64], kx[2][4][64], ux[2][6][64], ox[2][4][64];
     uint32_t touched[64];
 };
@@ -588,30 +547,35 @@ __device__ __forceinline__ void read_rows(v4u (&r)[DK / 64][4], const v4u (*f)[6
 #pragma unroll
         for (int i = 0; i < 4; i++) r[k][i] = f[i * (DK / 32) + HALF * (DK / 64) + k][threadIdx.x & 63];
 }
-// X diag(beta) or P: the columns of the half's tokens
+// X diag(beta) or P, the parts that lie side by side and the third ones: the columns of the half's tokens
 template <int HALF>
-__device__ __forceinline__ void read_tri(v4u (&r)[4][2], const v4u (*f)[64]) {
+__device__ __forceinline__ void read_tri(v4u (&r)[4][3], const v4u (*hm)[64], const v4u (*l)[64]) {
 #pragma unroll
-    for (int i = 2 * HALF; i < 4; i++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) r[i][e] = f[2 * tri(i, HALF) + e][threadIdx.x & 63];
+    for (int i = 2 * HALF; i < 4; i++) {
+        r[i][0] = hm[2 * tri(i, HALF)][threadIdx.x & 63];
+        r[i][1] = hm[2 * tri(i, HALF) + 1][threadIdx.x & 63];
+        r[i][2] = l[tri(i, HALF)][threadIdx.x & 63];
+    }
 }
 // acc += r s
 __device__ __forceinline__ void mul_rows(v4f (&acc)[4], const v4u (&r)[4], const Split& s) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = mfma_f16(r[i], s.l, acc[i]);
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.l, acc[i]);
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[i] = mfma_f16(r[i], s.h, acc[i]);
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.m, acc[i]);
+#pragma unroll
+    for (int i = 0; i < 4; i++) acc[i] = mfma_bf16(r[i], s.h, acc[i]);
 }
 // acc += r s, the small products first
 template <int HALF>
-__device__ __forceinline__ void mul_tri(v4f (&acc)[4], const v4u (&r)[4][2], const Split& s) {
+__device__ __forceinline__ void mul_tri(v4f (&acc)[4], const v4u (&r)[4][3], const Split& s) {
 #pragma unroll
-    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(r[i][1], s.h, acc[i]);
+    for (int p = 0; p < 6; p++) {
+        const int e = p == 0 ? 2 : p == 1 || p == 3 ? 1 : 0;
+        const v4u& y = p == 2 ? s.l : p == 1 || p == 4 ? s.m : s.h;
 #pragma unroll
-    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(r[i][0], s.l, acc[i]);
-#pragma unroll
-    for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_f16(r[i][0], s.h, acc[i]);
+        for (int i = 2 * HALF; i < 4; i++) acc[i] = mfma_bf16(r[i][e], y, acc[i]);
+    }
 }
 
 template <int DK, int DV, int HALF>
@@ -650,18 +614,12 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
         const float* vec = x.vec[c & 1];
         const int left = at.count - (c + 1) * kC;             // rows after this chunk
         v4f ks[4], u[4];
-        v4u kr[KH][4], tr[4][2], tk[DH][2];
+        v4u kr[KH][4], tr[4][3], tk[DH][2];
         read_rows<DK, HALF>(kr, x.k);
 #pragma unroll
         for (int i = 0; i < 4; i++) ks[i] = u[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        float sm = 0.f;
 #pragma unroll
-        for (int d = 0; d < DH; d++) sm = max_abs(sm, s[d]);
-        const Pow2 sp = pow2_of(column_max(sm));
-#pragma unroll
-        for (int k = 0; k < KH; k++) mul_rows(ks, kr[k], split8(s[2 * k], s[2 * k + 1], sp.up));
-#pragma unroll
-        for (int i = 0; i < 4; i++) ks[i] *= sp.down;
+        for (int k = 0; k < KH; k++) mul_rows(ks, kr[k], split_cut(s[2 * k], s[2 * k + 1]));
         // the other half's tokens' sums out, this half's in
         x.kx[w][2 - 2 * HALF][lane] = ks[2 - 2 * HALF];
         x.kx[w][3 - 2 * HALF][lane] = ks[3 - 2 * HALF];
@@ -672,7 +630,7 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
             rr[i] = x.kx[w][2 * HALF + i][lane];
             ek[i] = *reinterpret_cast<const v4f*>(vec + 32 * HALF + 16 * i + 4 * g);
         }
-        read_tri<HALF>(tr, x.x);
+        read_tri<HALF>(tr, x.x, x.x + 2 * kTri);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             rr[i] += ks[2 * HALF + i];
@@ -684,10 +642,7 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
             if (left < kC) offsets(left);
             load_v();
         }
-        const Pow2 rp = pow2_of(column_max(max_abs(max_abs(0.f, rr[0]), rr[1])));
-        mul_tri<HALF>(u, tr, split8(rr[0], rr[1], rp.up));
-#pragma unroll
-        for (int i = 2 * HALF; i < 4; i++) u[i] *= rp.down;
+        mul_tri<HALF>(u, tr, split_cut(rr[0], rr[1]));
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++) x.ux[w][i + 2 * HALF][lane] = u[i];
         lds_barrier();
@@ -701,31 +656,29 @@ __device__ __forceinline__ void scan_state(const DeltaArgs& a, const ScanAt& at,
         for (int e = 0; e < 2; e++)
 #pragma unroll
             for (int d = 0; d < DH; d++) tk[d][e] = x.kt[c & 1][2 * (HALF * DH + d) + e][lane];
-        const float ec = vec[4 * kC];
+        const float ec = vec[3 * kC];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if (i >= 2 || HALF) u[i] += ux[i];                // (half 1 has no part of u[0], u[1]: zeros)
             u[i] *= ew[i];
         }
-        float um = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) um = max_abs(um, u[i]);
-        const Pow2 up = pow2_of(column_max(um));
         v4f add[DH];
 #pragma unroll
         for (int d = 0; d < DH; d++) add[d] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const Split us = split8(u[2 * e], u[2 * e + 1], up.up);
+            const Split us = split_cut(u[2 * e], u[2 * e + 1]);
 #pragma unroll
-            for (int d = 0; d < DH; d++) add[d] = mfma_f16(tk[d][e], us.l, add[d]);
+            for (int d = 0; d < DH; d++) add[d] = mfma_bf16(tk[d][e], us.l, add[d]);
 #pragma unroll
-            for (int d = 0; d < DH; d++) add[d] = mfma_f16(tk[d][e], us.h, add[d]);
+            for (int d = 0; d < DH; d++) add[d] = mfma_bf16(tk[d][e], us.m, add[d]);
+#pragma unroll
+            for (int d = 0; d < DH; d++) add[d] = mfma_bf16(tk[d][e], us.h, add[d]);
         }
 #pragma unroll
         for (int d = 0; d < DH; d++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) s[d][r] = fmaf(add[d][r], up.down, ec * s[d][r]);
+            for (int r = 0; r < 4; r++) s[d][r] = fmaf(ec, s[d][r], add[d][r]);
 #pragma unroll
         for (int d = 0; d < DH; d++) x.sx[w][HALF * DH + d][lane] = s[d];
     }
@@ -752,11 +705,9 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
     v4f mine[2];
     float* out = a.out + (int64_t)at.first * a.ldo + at.head * a.ho_s + at.c0;
     // the last chunk's sums of this half's tokens, joined, then stored (`left` rows of it are there)
-    auto join = [&](int c) {
+    auto join = [&] {
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            mine[i] = (mine[i] + x.ox[w][2 * HALF + i][lane]) *
-                      *reinterpret_cast<const v4f*>(x.vec[c & 1] + 3 * kC + 32 * HALF + 16 * i + 4 * g);
+        for (int i = 0; i < 2; i++) mine[i] += x.ox[w][2 * HALF + i][lane];
     };
     auto store = [&](int left) {
 #pragma unroll
@@ -772,43 +723,36 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
     for (int c = 0; c < at.nc; c++) {
         const float* vec = x.vec[c & 1] + kC;
         lds_barrier();
-        if (c) join(c - 1);
+        if (c) join();
         v4f o[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] = v4f{0.f, 0.f, 0.f, 0.f};
         v4f s[DH], eq[4];
-        v4u qr[KH][4], tr[4][2];
+        v4u qr[KH][4], tr[4][3];
 #pragma unroll
         for (int d = 0; d < DH; d++) s[d] = x.sx[w][HALF * DH + d][lane];
         read_rows<DK, HALF>(qr, x.q);
 #pragma unroll
         for (int i = 0; i < 4; i++) eq[i] = *reinterpret_cast<const v4f*>(vec + 16 * i + 4 * g);
-        float sm = 0.f;
 #pragma unroll
-        for (int d = 0; d < DH; d++) sm = max_abs(sm, s[d]);
-        const Pow2 sp = pow2_of(column_max(sm));
+        for (int k = 0; k < KH; k++) mul_rows(o, qr[k], split_cut(s[2 * k], s[2 * k + 1]));
 #pragma unroll
-        for (int k = 0; k < KH; k++) mul_rows(o, qr[k], split8(s[2 * k], s[2 * k + 1], sp.up));
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] *= sp.down * eq[i];
+        for (int i = 0; i < 4; i++) o[i] *= eq[i];
         lds_barrier();
         if (c) store(kC);                                     // (here the state waves have more to do than these)
         if (c + 2 < at.nc) touch(rec + (c + 2) * step);
         v4f u0 = x.ux[w][2 * HALF][lane], u1 = x.ux[w][2 * HALF + 1][lane];
-        read_tri<HALF>(tr, x.p[c & 1]);
+        read_tri<HALF>(tr, x.p[c & 1], x.pl);
         if (HALF) {
             u0 += x.ux[w][4][lane];
             u1 += x.ux[w][5][lane];
         }
-        const Pow2 up = pow2_of(column_max(max_abs(max_abs(0.f, u0), u1)));
         v4f pu[4];
 #pragma unroll
         for (int i = 2 * HALF; i < 4; i++) pu[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        mul_tri<HALF>(pu, tr, split8(u0, u1, up.up));
+        mul_tri<HALF>(pu, tr, split_cut(u0, u1));
 #pragma unroll
-        for (int i = 2 * HALF; i < 4; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) o[i][r] = fmaf(pu[i][r], up.down, o[i][r]);
+        for (int i = 2 * HALF; i < 4; i++) o[i] += pu[i];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             x.ox[w][2 - 2 * HALF + i][lane] = o[2 - 2 * HALF + i];
@@ -816,7 +760,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
         }
     }
     lds_barrier();
-    join(at.nc - 1);
+    join();
     store(at.count - (at.nc - 1) * kC);
 }
 
@@ -824,20 +768,19 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
 template <int DK>
 __device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, const char* rv, int q, ScanShared<DK>& x) {
     const int64_t rks = at.rks, rvs = at.rvs;
-    constexpr int NK = 4 * (DK / 32), NT = DK / 16 * 2, NX = 2 * kTri;
+    constexpr int NK = 4 * (DK / 32), NT = DK / 16 * 2, NX = 3 * kTri;
     const int lane = threadIdx.x & 63;
     auto bring = [&](v4u (*to)[64], const char* from, int count) {
         for (int i = q; i < count; i += 4) dma16(from + i * kFrag + lane * 16, to[i]);
     };
     auto factors = [&](int c, const char* r) {
         if (q == 0) dma16(r + 2 * NX * kFrag + lane * 16, x.vec[c & 1]);
-        if (q == 1) dma4(r + (2 * NX + 1) * kFrag + lane * 4, x.vec[c & 1] + 4 * kC);
     };
     auto later = [&](int c, const char* k, const char* v) {   // what chunk c needs after its first barrier
         bring(x.q, k + NK * kFrag, NK);
         bring(x.x, v, NX);
         factors(c, v);
-        bring(x.p[c & 1], v + NX * kFrag, NX);
+        bring(x.p[c & 1], v + NX * kFrag, 2 * kTri);
         bring(x.kt[c & 1], k + 2 * NK * kFrag, NT);
     };
     bring(x.k, rk, NK);
@@ -847,6 +790,7 @@ __device__ __forceinline__ void scan_load(const ScanAt& at, const char* rk, cons
     for (int c = 0; c < at.nc; c++) {
         const bool more = c + 1 < at.nc;
         lds_barrier();
+        bring(x.pl, rv + (NX + 2 * kTri) * kFrag, kTri);
         if (more) bring(x.k, rk + rks, NK);
         vm_wait<0>();
         lds_barrier();

@@ -15,7 +15,7 @@ Per value head, with its state S fp32 [dk, dv], a = exp(g), key k and query q of
               must not share a slot in one call.
   out         fp32 [>= T, value heads, dv], what quant.gated_norm_q8 / gated_norm_g read
 
-Sums, states and norms are fp32; `prefill`'s products take their fp32 operands as two fp16 parts (22 bits).  As the other
+Sums, states and norms are fp32, and so are the operands of `prefill`'s products (as three bf16 parts each).  As the other
 producers: outputs are the caller's buffers, calls go to torch's current stream and can be captured.
 """
 from . import _lib as L

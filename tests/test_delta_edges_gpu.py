@@ -32,3 +32,29 @@ def check_prefill(dev, lens, hk, hv, dk, dv, seed=0, eps=1e-6, lead=0, tail=0):
 def test_prefill_without_eps(dev, lens, eps, dk, dv):
     """Lengths that leave a chunk unfilled: the rows past its end have no length to divide by."""
     check_prefill(dev, lens, 2, 4, dk, dv, seed=sum(lens), eps=eps)
+
+
+@pytest.mark.parametrize("what,factor", [("value", 2.0 ** 20), ("value", 2.0 ** 40), ("value", 2.0 ** 70), ("key", 2.0 ** 20)])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 64)])
+def test_prefill_tokens_keep_their_own_size(dev, what, factor, dk, dv):
+    """One token far above the others, and the state cleared some tokens later: the tokens before the one and from the
+    clearing on are held to the bounds of their own sizes, as if the large one were not there.  (A large key makes the
+    update no contraction: its state is cleared at once, and its own token is not held to anything.)"""
+    from prism_amd import delta
+    T, hk, hv, big, clear = 190, 2, 4, 100, 140 if what == "value" else 101
+    norm = what == "value"
+    proj, g, beta, state = inputs(T, hk, hv, dk, dv, 1, 21)
+    if not norm:
+        proj *= dk ** -0.5
+    q, k, v = split(proj, hk, hv, dk, dv)
+    (v if what == "value" else k)[big] *= factor
+    g[clear] = float("-inf")
+    want_out, want_state = recurrence(q, k, v, g, beta, state, [(0, T)], [0], norm, dk ** -0.5)
+    dq, dk_, dv_ = split(proj.to(dev), hk, hv, dk, dv)
+    ds, out = state.to(dev), torch.empty(T, hv, dv, device=dev)
+    delta.prefill(dq, dk_, dv_, g.to(dev), beta.to(dev), ds, out, torch.tensor([0, T], dtype=torch.int32, device=dev), T,
+                  norm=norm)
+    for begin, end in ((0, big), (clear, T)) + (((big, clear),) if norm else ()):
+        part = torch.full_like(want_out, float("nan"))
+        part[begin:end] = want_out[begin:end]
+        compare(out, ds, part, want_state, [(begin, end)], v[begin:end], dk, state)
