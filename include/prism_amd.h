@@ -437,7 +437,7 @@ PRISM_API int prism_kv_append(const prism_kv_append_args* args, void* stream);
 /*
  * prism_kv_attend: attention of one new token per sequence over the cache (T = cache.seqs sequences): for i < *n_rows,
  * out[i][h] = sum_t softmax_t(scale q[i][h] . k_t) v_t over tokens t of max(0, lens[i] - window) .. lens[i] - 1 (window 0:
- * all), head h of hq on cache head h / (hq / heads); no tokens: zeros.  lens past the table's capacity, cols page, count as
+ * all), head h of hq on cache head h / (hq / heads); no tokens: zeros; scores all -inf (q . k is fp32): NaN.  lens past the table's capacity, cols page, count as
  * that.  fp32 sums, softmax and weights (in three bf16 parts); parts of a sequence (the split depends on all lengths) are
  * joined in a fixed order through ws (prism_kv_attend_workspace_bytes, no initial contents; 16-byte aligned; calls that
  * overlap must not share it).  Rows >= *n_rows are untouched.  Needs hq % heads == 0, T <= 65535, 16-byte aligned q with

@@ -555,9 +555,10 @@ __global__ __launch_bounds__(256, 2) void kv_attend_kernel(AttendArgs a) {
                 acc += e * *reinterpret_cast<const v4f*>(lds + w * B::STAGE + (h * LD + d) * 4);
             }
             if (whole) {
+                // zeros without tokens; with tokens whose scores are all -inf 0 / 0, as the softmax is
                 uint32_t u[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(sum == 0.f ? 0.f : div_rn(acc[j], sum) * vs);
+                for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(len == 0 ? 0.f : div_rn(acc[j], sum) * vs);
                 *reinterpret_cast<v2u*>(a.out + b * a.ldo + (h0 + h) * a.ho_s + d) =
                     v2u{u[0] | (u[1] << 16), u[2] | (u[3] << 16)};
             } else {
@@ -621,7 +622,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttendArgs a, int hb) {
             const float vs = a.c.v_scale ? __ldg(a.c.v_scale + h / a.G) : 1.f;
             uint32_t u[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(sum == 0.f ? 0.f : div_rn(acc[j], sum) * vs);
+            for (int j = 0; j < 4; j++) u[j] = f32_to_bf16(div_rn(acc[j], sum) * vs);     // (two parts: there are tokens)
             *reinterpret_cast<v2u*>(a.out + b * a.ldo + h * a.ho_s + 4 * c) =
                 v2u{u[0] | (u[1] << 16), u[2] | (u[3] << 16)};
         }

@@ -52,13 +52,13 @@ def append(q, k, v, rope, pos, table, k_cache, v_cache, q_out, n, T, seq=None, p
 def attend(q, k_cache, v_cache, table, lens, out, n, T, scale=None, window=0, k_scale=None, v_scale=None):
     """out[i] = softmax(scale q[i] K^T) V over the cached tokens of sequence i (i < n[0] <= T), query head h on the cache's
     head h // (heads / kv heads).  lens int32 [>= T]: tokens in the cache, the new one among them (more than the table
-    holds counts as what it holds); window > 0: only the last `window` of them.  A sequence without tokens gets zeros.
-    scale None: dim ** -0.5.
+    holds counts as what it holds); window > 0: only the last `window` of them.  A sequence without tokens gets zeros; one
+    whose scores are all -inf (q . k is fp32: it overflows) NaN, as softmax gives.  scale None: dim ** -0.5.
 
-    q, out bf16 [>= T, heads, dim], unit stride in dim.  Softmax, weights and sums in fp32 (the products take the weights as
-    three bf16 parts), the output rounded once.  Results do not depend on timing; how a sequence's length is split, and so the order of its
-    sums, depends on the batch.  Table entries of visible tokens must name pages (others read some page, never memory
-    outside the cache)."""
+    q, out bf16 [>= T, heads, dim], unit stride in dim.  Softmax, weights and sums in fp32 (the products take the weights
+    as three bf16 parts), the output rounded once.  Results do not depend on timing; how a sequence's length is split, and
+    so the order of its sums, depends on the batch.  Table entries of visible tokens must name pages (others read some
+    page, never memory outside the cache)."""
     if n is None:
         n = _live(n, T, q.device)
     rc = (L._host or L.host()).kv_attend(q, k_cache, v_cache, table, lens, out, n, T, scale, window, k_scale, v_scale)
