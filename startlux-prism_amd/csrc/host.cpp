@@ -77,15 +77,29 @@ const char* type_name(at::ScalarType t) {
 }
 
 // [>= T, heads, dim]; the strides of rows and heads (0 where there is one).
-const void* heads(PyObject* o, const char* name, int64_t T, int64_t n, int64_t dim, int dev, int64_t* ld, int64_t* hs,
-                  at::ScalarType type = at::kBFloat16) {
+const at::Tensor& rows_of(PyObject* o, const char* name, int64_t T, int64_t n, int64_t dim, int dev, int64_t* ld, int64_t* hs,
+                          at::ScalarType type) {
     const at::Tensor& t = tensor(o, name);
     if (t.scalar_type() != type || t.dim() != 3 || t.size(0) < T || t.size(1) != n || t.size(2) != dim ||
         t.stride(2) != 1 || device(t) != dev)
         refuse(name, t, type, "[>= " + std::to_string(T) + ", " + std::to_string(n) + ", " + std::to_string(dim) + "]", dev);
     *ld = t.size(0) > 1 ? t.stride(0) : 0;
     *hs = n > 1 ? t.stride(1) : 0;
-    return t.const_data_ptr();
+    return t;
+}
+
+const uint16_t* heads(PyObject* o, const char* name, int64_t T, int64_t n, int64_t dim, int dev, int64_t* ld, int64_t* hs) {
+    return static_cast<const uint16_t*>(rows_of(o, name, T, n, dim, dev, ld, hs, at::kBFloat16).const_data_ptr());
+}
+
+// An output's memory, its own: a copy-on-write clone gets it here.  Taken before the inputs' pointers, which may lie in the
+// same storage.
+void* written(const at::Tensor& t) { return t.mutable_data_ptr(); }
+
+template <typename E>
+E* out_heads(PyObject* o, const char* name, int64_t T, int64_t n, int64_t dim, int dev, int64_t* ld, int64_t* hs,
+             at::ScalarType type) {
+    return static_cast<E*>(written(rows_of(o, name, T, n, dim, dev, ld, hs, type)));
 }
 
 const int32_t* ints(PyObject* o, const char* name, int64_t least, int dev) {
@@ -122,7 +136,8 @@ const float* scales(PyObject* o, const char* name, int64_t n, bool e4m3, int dev
     return static_cast<const float*>(t.const_data_ptr());
 }
 
-// The caches, their scales and the page table of at least `rows` rows.
+// The caches (WRITE: outputs), their scales and the page table of at least `rows` rows.
+template <bool WRITE>
 void cache(prism_kv_cache& c, PyObject* ko, PyObject* vo, PyObject* kso, PyObject* vso, PyObject* to, int64_t rows, int dev) {
     const at::Tensor &k = tensor(ko, "k_cache"), &v = tensor(vo, "v_cache"), &t = tensor(to, "table");
     const at::ScalarType ty = k.scalar_type();
@@ -137,7 +152,8 @@ void cache(prism_kv_cache& c, PyObject* ko, PyObject* vo, PyObject* kso, PyObjec
         raise(PyExc_ValueError, "a page must hold a power of two of tokens, at least 16");
     if (c.pages < 1 || c.heads < 1) raise(PyExc_ValueError, "the caches must not be empty");
     const bool many = c.pages > 1, heads = c.heads > 1;       // (the stride of a single page or head is not used)
-    c.k = const_cast<void*>(k.const_data_ptr()), c.v = const_cast<void*>(v.const_data_ptr());
+    c.k = WRITE ? written(k) : const_cast<void*>(k.const_data_ptr());
+    c.v = WRITE ? written(v) : const_cast<void*>(v.const_data_ptr());
     c.k_page = many ? k.stride(0) : 0, c.k_tok = k.stride(1), c.k_head = heads ? k.stride(2) : 0;
     c.v_page = many ? v.stride(0) : 0, c.v_tok = v.stride(1), c.v_head = heads ? v.stride(2) : 0;
     c.e4m3 = ty == at::kFloat8_e4m3fn;
@@ -179,7 +195,10 @@ void need_args(Py_ssize_t got, Py_ssize_t want) {
     if (got != want) raise(PyExc_TypeError, std::to_string(want) + " arguments, got " + std::to_string(got));
 }
 
-int64_t heads_of(const at::Tensor& t) { return t.dim() == 3 ? t.size(1) : -1; }
+int64_t heads_of(const at::Tensor& t) {
+    if (t.dim() != 3) raise(PyExc_ValueError, "q must be [rows, heads, dim]; got " + list(t.sizes()));
+    return t.size(1);
+}
 
 int do_append(PyObject* const* a, Py_ssize_t n) {
     need_args(n, 15);
@@ -187,15 +206,15 @@ int do_append(PyObject* const* a, Py_ssize_t n) {
     prism_kv_append_args h{};
     const int dev = device(tensor(a[K], "k"));
     h.T = integer(a[T], "T");
-    cache(h.cache, a[KC], a[VC], a[KS], a[VS], a[TABLE], 1, dev);
-    h.k = static_cast<const uint16_t*>(heads(a[K], "k", h.T, h.cache.heads, h.cache.dim, dev, &h.k_ld, &h.k_hs));
-    h.v = static_cast<const uint16_t*>(heads(a[V], "v", h.T, h.cache.heads, h.cache.dim, dev, &h.v_ld, &h.v_hs));
+    cache<true>(h.cache, a[KC], a[VC], a[KS], a[VS], a[TABLE], 1, dev);
     if ((a[Q] == Py_None) != (a[QO] == Py_None)) raise(PyExc_ValueError, "append: q and q_out go together");
     if (a[Q] != Py_None) {
         h.hq = heads_of(tensor(a[Q], "q"));
-        h.q = static_cast<const uint16_t*>(heads(a[Q], "q", h.T, h.hq, h.cache.dim, dev, &h.q_ld, &h.q_hs));
-        h.q_out = static_cast<uint16_t*>(const_cast<void*>(heads(a[QO], "q_out", h.T, h.hq, h.cache.dim, dev, &h.o_ld, &h.o_hs)));
+        h.q_out = out_heads<uint16_t>(a[QO], "q_out", h.T, h.hq, h.cache.dim, dev, &h.o_ld, &h.o_hs, at::kBFloat16);
+        h.q = heads(a[Q], "q", h.T, h.hq, h.cache.dim, dev, &h.q_ld, &h.q_hs);
     }
+    h.k = heads(a[K], "k", h.T, h.cache.heads, h.cache.dim, dev, &h.k_ld, &h.k_hs);
+    h.v = heads(a[V], "v", h.T, h.cache.heads, h.cache.dim, dev, &h.v_ld, &h.v_hs);
     if (a[ROPE] != Py_None) {
         const at::Tensor& r = tensor(a[ROPE], "rope");
         if (r.scalar_type() != at::kFloat || r.dim() != 2 || r.size(1) % 16 || r.size(1) < 1 || r.size(1) > h.cache.dim ||
@@ -222,11 +241,12 @@ int do_attend(PyObject* const* a, Py_ssize_t n) {
     const at::Tensor& q = tensor(a[Q], "q");
     const int dev = device(q);
     const int64_t rows = integer(a[T], "T");
-    cache(h.cache, a[KC], a[VC], a[KS], a[VS], a[TABLE], rows, dev);
-    h.cache.seqs = rows;
     h.hq = heads_of(q);
-    h.q = static_cast<const uint16_t*>(heads(a[Q], "q", rows, h.hq, h.cache.dim, dev, &h.q_ld, &h.q_hs));
-    h.out = static_cast<uint16_t*>(const_cast<void*>(heads(a[OUT], "out", rows, h.hq, h.cache.dim, dev, &h.o_ld, &h.o_hs)));
+    const at::Tensor& k = tensor(a[KC], "k_cache");
+    h.out = out_heads<uint16_t>(a[OUT], "out", rows, h.hq, k.dim() == 4 ? k.size(3) : -1, dev, &h.o_ld, &h.o_hs, at::kBFloat16);
+    cache<false>(h.cache, a[KC], a[VC], a[KS], a[VS], a[TABLE], rows, dev);
+    h.cache.seqs = rows;
+    h.q = heads(a[Q], "q", rows, h.hq, h.cache.dim, dev, &h.q_ld, &h.q_hs);
     if (h.hq < h.cache.heads || h.hq % h.cache.heads)
         raise(PyExc_ValueError, "attend: the query heads must be a multiple of the cache's heads");
     h.window = integer(a[WINDOW], "window");
@@ -254,22 +274,22 @@ int do_delta(PyObject* const* a, Py_ssize_t n, bool prompts) {
     if (prompts && (r.dim() != 1 || r.size(0) < 1)) raise(PyExc_ValueError, "cu must be int32 [sequences + 1]");
     h.seqs = prompts ? r.size(0) - 1 : h.T;
     h.hk = q.size(1), h.dk = q.size(2), h.hv = v.size(1), h.dv = v.size(2);
-    h.q = static_cast<const uint16_t*>(heads(a[Q], "q", h.T, h.hk, h.dk, dev, &h.q_ld, &h.q_hs));
-    h.k = static_cast<const uint16_t*>(heads(a[K], "k", h.T, h.hk, h.dk, dev, &h.k_ld, &h.k_hs));
-    h.v = static_cast<const uint16_t*>(heads(a[V], "v", h.T, h.hv, h.dv, dev, &h.v_ld, &h.v_hs));
     if ((h.dk != 64 && h.dk != 128) || (h.dv != 64 && h.dv != 128)) raise(PyExc_ValueError, "the heads' dims must be 64 or 128");
     if (h.hk < 1 || h.hv < h.hk || h.hv % h.hk) raise(PyExc_ValueError, "the value heads must be a multiple of the key heads");
-    h.g = gates(a[G], "g", h.T, h.hv, dev, &h.g_ld);
-    h.beta = gates(a[BETA], "beta", h.T, h.hv, dev, &h.b_ld);
     const at::Tensor& s = tensor(a[STATE], "state");
     if (s.scalar_type() != at::kFloat || s.dim() != 4 || s.size(1) != h.hv || s.size(2) != h.dk || s.size(3) != h.dv ||
         s.stride(3) != 1 || s.stride(2) != h.dv || (h.hv > 1 && s.stride(1) != h.dk * h.dv) || device(s) != dev)
         refuse("state", s, at::kFloat,
                "[slots, " + std::to_string(h.hv) + ", " + std::to_string(h.dk) + ", " + std::to_string(h.dv) +
                    "], contiguous per slot", dev);
-    h.state = static_cast<float*>(const_cast<void*>(s.const_data_ptr()));
+    h.state = static_cast<float*>(written(s));
     h.nslots = s.size(0), h.slot_ld = s.size(0) > 1 ? s.stride(0) : h.hv * h.dk * h.dv;
-    h.out = static_cast<float*>(const_cast<void*>(heads(a[OUT], "out", h.T, h.hv, h.dv, dev, &h.o_ld, &h.o_hs, at::kFloat)));
+    h.out = out_heads<float>(a[OUT], "out", h.T, h.hv, h.dv, dev, &h.o_ld, &h.o_hs, at::kFloat);
+    h.q = heads(a[Q], "q", h.T, h.hk, h.dk, dev, &h.q_ld, &h.q_hs);
+    h.k = heads(a[K], "k", h.T, h.hk, h.dk, dev, &h.k_ld, &h.k_hs);
+    h.v = heads(a[V], "v", h.T, h.hv, h.dv, dev, &h.v_ld, &h.v_hs);
+    h.g = gates(a[G], "g", h.T, h.hv, dev, &h.g_ld);
+    h.beta = gates(a[BETA], "beta", h.T, h.hv, dev, &h.b_ld);
     h.slots = a[SLOTS] == Py_None ? nullptr : ints(a[SLOTS], "slots", h.seqs, dev);
     h.rows = prompts ? ints(a[ROWS], "cu", h.seqs + 1, dev) : live(a[ROWS], dev);
     h.norm = PyObject_IsTrue(a[NORM]);

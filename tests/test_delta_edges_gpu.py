@@ -58,3 +58,21 @@ def test_prefill_tokens_keep_their_own_size(dev, what, factor, dk, dv):
         part = torch.full_like(want_out, float("nan"))
         part[begin:end] = want_out[begin:end]
         compare(out, ds, part, want_state, [(begin, end)], v[begin:end], dk, state)
+
+
+@pytest.mark.parametrize("form", ["step", "prefill"])
+def test_clones_keep_what_they_were_made_of(dev, form):
+    """States and outputs that are copy-on-write clones: the tensors they were made of stay as they are."""
+    from prism_amd import delta
+    T, hk, hv, dk, dv = 20, 2, 4, 64, 64
+    proj, g, beta, state = (x.to(dev) for x in inputs(T, hk, hv, dk, dv, T, 31))
+    q, k, v = split(proj, hk, hv, dk, dv)
+    out = torch.zeros(T, hv, dv, device=dev)
+    s, o = torch._lazy_clone(state), torch._lazy_clone(out)
+    before = state.clone()
+    if form == "step":
+        delta.step(q, k, v, g, beta, s, o, None, T)
+    else:
+        delta.prefill(q, k, v, g, beta, s, o, torch.tensor([0, T], dtype=torch.int32, device=dev), T)
+    assert torch.equal(state, before) and (out == 0).all()
+    assert not torch.equal(s, state) and (o != 0).any()

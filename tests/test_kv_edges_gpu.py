@@ -35,3 +35,23 @@ def test_attend_scores_of_minus_infinity(dev, lens, dim):
         t = n // 3
         assert torch.isnan(out[i, :2]).all()
         assert torch.equal(out[i, 2:], vc[int(table[i, t // page]), t % page, 1].expand(2, dim))
+
+
+def test_clones_keep_what_they_were_made_of(dev):
+    """Caches and outputs that are copy-on-write clones: the tensors they were made of stay as they are, the caches that
+    attend reads stay shared."""
+    from prism_amd import kv
+    g = torch.Generator().manual_seed(5)
+    kc, vc = kv.cache(4, 16, 2, 64, device=dev)
+    q, k, v = (torch.randn(3, h, 64, generator=g).to(torch.bfloat16).to(dev) for h in (4, 2, 2))
+    turned, out = torch.zeros_like(q), torch.zeros_like(q)
+    table = torch.arange(3, dtype=torch.int32, device=dev).view(3, 1)
+    ones = torch.ones(3, dtype=torch.int32, device=dev)
+    lk, lv, lt, lo = (torch._lazy_clone(x) for x in (kc, vc, turned, out))
+    kv.append(q, k, v, None, ones - 1, table, lk, lv, lt, None, 3)
+    assert (kc == 0).all() and (vc == 0).all() and (turned == 0).all()
+    assert torch.equal(lk[:3, 0], k) and torch.equal(lv[:3, 0], v) and torch.equal(lt, q)
+    rk, rv = torch._lazy_clone(lk), torch._lazy_clone(lv)
+    kv.attend(q, rk, rv, table, ones, lo, None, 3)
+    assert (out == 0).all() and torch.equal(lo, v.repeat_interleave(2, 1))
+    assert torch._C._is_cow_tensor(rk) and torch._C._is_cow_tensor(rv)
