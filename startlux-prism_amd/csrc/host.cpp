@@ -8,6 +8,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -93,13 +94,19 @@ const uint16_t* heads(PyObject* o, const char* name, int64_t T, int64_t n, int64
 }
 
 // An output's memory, its own: a copy-on-write clone gets it here.  Taken before the inputs' pointers, which may lie in the
-// same storage.
-void* written(const at::Tensor& t) { return t.mutable_data_ptr(); }
+// same storage.  An output expanded over rows or heads is refused, as torch does where it writes in place: all of them
+// would be written to one place.
+void* written(const at::Tensor& t, const char* name) {
+    if (at::has_internal_overlap(t) == at::MemOverlap::Yes)
+        raise(PyExc_ValueError, std::string(name) + " is written and must not be expanded; got " + list(t.sizes()) +
+                                    ", strides " + list(t.strides()));
+    return t.mutable_data_ptr();
+}
 
 template <typename E>
 E* out_heads(PyObject* o, const char* name, int64_t T, int64_t n, int64_t dim, int dev, int64_t* ld, int64_t* hs,
              at::ScalarType type) {
-    return static_cast<E*>(written(rows_of(o, name, T, n, dim, dev, ld, hs, type)));
+    return static_cast<E*>(written(rows_of(o, name, T, n, dim, dev, ld, hs, type), name));
 }
 
 const int32_t* ints(PyObject* o, const char* name, int64_t least, int dev) {
@@ -152,8 +159,8 @@ void cache(prism_kv_cache& c, PyObject* ko, PyObject* vo, PyObject* kso, PyObjec
         raise(PyExc_ValueError, "a page must hold a power of two of tokens, at least 16");
     if (c.pages < 1 || c.heads < 1) raise(PyExc_ValueError, "the caches must not be empty");
     const bool many = c.pages > 1, heads = c.heads > 1;       // (the stride of a single page or head is not used)
-    c.k = WRITE ? written(k) : const_cast<void*>(k.const_data_ptr());
-    c.v = WRITE ? written(v) : const_cast<void*>(v.const_data_ptr());
+    c.k = WRITE ? written(k, "k_cache") : const_cast<void*>(k.const_data_ptr());
+    c.v = WRITE ? written(v, "v_cache") : const_cast<void*>(v.const_data_ptr());
     c.k_page = many ? k.stride(0) : 0, c.k_tok = k.stride(1), c.k_head = heads ? k.stride(2) : 0;
     c.v_page = many ? v.stride(0) : 0, c.v_tok = v.stride(1), c.v_head = heads ? v.stride(2) : 0;
     c.e4m3 = ty == at::kFloat8_e4m3fn;
@@ -282,7 +289,7 @@ int do_delta(PyObject* const* a, Py_ssize_t n, bool prompts) {
         refuse("state", s, at::kFloat,
                "[slots, " + std::to_string(h.hv) + ", " + std::to_string(h.dk) + ", " + std::to_string(h.dv) +
                    "], contiguous per slot", dev);
-    h.state = static_cast<float*>(written(s));
+    h.state = static_cast<float*>(written(s, "state"));
     h.nslots = s.size(0), h.slot_ld = s.size(0) > 1 ? s.stride(0) : h.hv * h.dk * h.dv;
     h.out = out_heads<float>(a[OUT], "out", h.T, h.hv, h.dv, dev, &h.o_ld, &h.o_hs, at::kFloat);
     h.q = heads(a[Q], "q", h.T, h.hk, h.dk, dev, &h.q_ld, &h.q_hs);

@@ -48,3 +48,17 @@ def test_outputs_that_are_copy_on_write_clones(name):
     for k, x in lazy.items():
         if torch.is_tensor(x):
             assert torch._C._is_cow_tensor(x) == (k not in outputs), k
+
+
+@pytest.mark.parametrize("name", ["append", "attend", "step", "prefill"])
+def test_expanded_outputs_are_refused(name):
+    """An output of which several rows, heads or pages are one place is refused; inputs may be expanded."""
+    fn, args, outputs = calls()[name]
+    for k, x in args.items():
+        if not torch.is_tensor(x):
+            continue
+        for d in range(x.dim() - 1):
+            if x.shape[d] > 1:
+                wide = {**args, k: x.narrow(d, 0, 1).expand(x.shape)}
+                with pytest.raises(ValueError if k in outputs else RuntimeError):
+                    fn(**wide)
