@@ -238,7 +238,8 @@ int do_append(PyObject* const* a, Py_ssize_t n) {
     h.pos = ints(a[POS], "pos", h.T, dev);
     h.seq = a[SEQ] == Py_None ? nullptr : ints(a[SEQ], "seq", h.T, dev);
     h.n_rows = live(a[N], dev);
-    return g_append(&h, stream_of(a[K]));
+    void* stream = stream_of(a[K]);
+    return h.T == 0 ? 0 : g_append(&h, stream);              // (no rows: their tensors may have no memory)
 }
 
 int do_attend(PyObject* const* a, Py_ssize_t n) {
@@ -262,6 +263,7 @@ int do_attend(PyObject* const* a, Py_ssize_t n) {
     h.n_rows = live(a[N], dev);
     h.scale = a[SCALE] == Py_None ? 1 / std::sqrt((double)h.cache.dim) : number(a[SCALE], "scale");
     void* stream = stream_of(a[Q]);
+    if (rows == 0) return 0;
     Workspace ws;
     h.ws_bytes = g_attend_ws(rows, h.hq, h.cache.heads, h.cache.dim, h.cache.cols, h.cache.page);
     if (h.ws_bytes) ws.get(a[Q], h.ws_bytes, stream);
@@ -304,6 +306,7 @@ int do_delta(PyObject* const* a, Py_ssize_t n, bool prompts) {
     h.scale = a[SCALE] == Py_None ? 1 / std::sqrt((double)h.dk) : number(a[SCALE], "scale");
     h.eps = number(a[EPS], "eps");
     void* stream = stream_of(a[Q]);
+    if (h.T == 0 || h.seqs == 0 || h.nslots == 0) return 0;
     if (!prompts) return g_step(&h, stream);
     Workspace ws;
     h.ws_bytes = g_prefill_ws(h.T, h.seqs, h.hk, h.hv, h.dk, h.dv);

@@ -76,3 +76,17 @@ def test_clones_keep_what_they_were_made_of(dev, form):
         delta.prefill(q, k, v, g, beta, s, o, torch.tensor([0, T], dtype=torch.int32, device=dev), T)
     assert torch.equal(state, before) and (out == 0).all()
     assert not torch.equal(s, state) and (o != 0).any()
+
+
+@pytest.mark.parametrize("T,slots", [(0, 3), (0, 0), (5, 0)])
+def test_calls_without_rows_or_states(dev, T, slots):
+    """No rows, no prompts, or no state that a sequence could have: nothing is done."""
+    from prism_amd import delta
+    bf = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=dev)             # noqa: E731
+    f = lambda *s: torch.zeros(*s, device=dev)                                    # noqa: E731
+    state, out = f(slots, 4, 64, 128) + 2, f(T, 4, 128) + 3
+    args = (bf(T, 2, 64), bf(T, 2, 64), bf(T, 4, 128), f(T, 4), f(T, 4), state, out)
+    delta.step(*args, torch.tensor([T], dtype=torch.int32, device=dev), T)
+    delta.prefill(*args, torch.tensor([0, T], dtype=torch.int32, device=dev), T)
+    delta.prefill(*args, torch.zeros(1, dtype=torch.int32, device=dev), T)
+    assert (state == 2).all() and (out == 3).all()

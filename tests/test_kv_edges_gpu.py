@@ -55,3 +55,16 @@ def test_clones_keep_what_they_were_made_of(dev):
     kv.attend(q, rk, rv, table, ones, lo, None, 3)
     assert (out == 0).all() and torch.equal(lo, v.repeat_interleave(2, 1))
     assert torch._C._is_cow_tensor(rk) and torch._C._is_cow_tensor(rv)
+
+
+def test_calls_without_rows(dev):
+    """T = 0 with tensors of no rows does nothing."""
+    from prism_amd import kv
+    kc, vc = kv.cache(4, 16, 2, 64, device=dev)
+    bf = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device=dev)             # noqa: E731
+    ints = lambda *s: torch.empty(*s, dtype=torch.int32, device=dev)              # noqa: E731
+    n = torch.zeros(1, dtype=torch.int32, device=dev)
+    kv.append(bf(0, 4, 64), bf(0, 2, 64), bf(0, 2, 64), torch.empty(9, 32, device=dev), ints(0), ints(1, 4), kc, vc,
+              bf(0, 4, 64), n, 0)
+    kv.attend(bf(0, 4, 64), kc, vc, ints(0, 4), ints(0), bf(0, 4, 64), n, 0)
+    assert (kc == 0).all() and (vc == 0).all()
