@@ -4,7 +4,8 @@
 
 Each csrc/*.hip compiles to an object under csrc/_build/, then one shared library links next to the Python package
 (startlux-prism_amd/prism_amd/libprism_amd.so), which prism_amd._lib loads.  csrc/host.cpp compiles with g++ to
-prism_amd/_host.so, the checked host path of prism_amd.kv and prism_amd.delta.  Flags of the HIP files:
+prism_amd/_host.so, the checked host path of prism_amd.kv and prism_amd.delta; without torch or g++ that one is left out
+and the library is complete for its C ABI.  Flags of the HIP files:
   --offload-arch=gfx950                        MI355X / MI350X only; no other targets, no host fallback
   -fhip-fp32-correctly-rounded-divide-sqrt     '/' on fp32 is the IEEE division the quantizers are specified with
   -ffp-contract=off                            no implicit a*b+c contraction: roundings are the ones written
@@ -46,27 +47,36 @@ def _compile(src):
 
 
 def _compile_host():
-    """csrc/host.cpp -> prism_amd/_host.so: the CPython extension that checks kv's and delta's tensors (host code only)."""
+    """csrc/host.cpp -> prism_amd/_host.so: the CPython extension that checks kv's and delta's tensors (host code only).
+    Returns why it cannot be built here (no torch, no C++ compiler), else None."""
     import sysconfig
 
-    from torch.utils import cpp_extension as C
+    try:
+        from torch.utils import cpp_extension as C
+    except ImportError as e:
+        return str(e)
     tmp = HOST + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
            *("-I" + p for p in (*C.include_paths(), sysconfig.get_paths()["include"])), os.path.join(CSRC, "host.cpp"),
            "-o", tmp, *("-L" + p for p in C.library_paths()), "-lc10", "-ltorch_cpu", "-ltorch_python"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+    except FileNotFoundError as e:
+        return str(e)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on csrc/host.cpp:\n{r.stderr}")
+        raise RuntimeError(f"{cmd[0]} failed on csrc/host.cpp:\n{r.stderr}")
     os.replace(tmp, HOST)
+    return None
 
 
 def build(jobs=8, verbose=False):
+    """The library, and where torch and a C++ compiler are there the Python package's host extension.  The library and its C
+    ABI need neither: without them the extension is left out (an older one too, whose structs may differ), and said so."""
     os.makedirs(OBJ, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     with cf.ThreadPoolExecutor(max(1, jobs)) as ex:
         host = ex.submit(_compile_host)
         res = list(ex.map(_compile, srcs))
-        host.result()
     for _, err in res:
         if err.strip() and verbose:
             print(err, file=sys.stderr)
@@ -77,6 +87,12 @@ def build(jobs=8, verbose=False):
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
+    missing = host.result()
+    if missing:
+        if os.path.exists(HOST):
+            os.remove(HOST)
+        print(f"{HOST} is not built ({missing}): prism_amd.kv and prism_amd.delta need it, the C ABI does not",
+              file=sys.stderr)
     return LIB
 
 
