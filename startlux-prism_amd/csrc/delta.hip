@@ -33,6 +33,13 @@ __device__ __forceinline__ bool delta_seq(const DeltaArgs& a, int b, int& first,
     return count > 0 && slot >= 0 && slot < a.nslots;
 }
 
+// What the lanes of a wave pass each other through LDS is in order at this point: the hardware keeps a wave's LDS operations
+// in theirs, the fence keeps the compiler from moving them.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ float wave_addf(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
@@ -88,6 +95,7 @@ __global__ __launch_bounds__(256) void delta_rec_kernel(DeltaArgs a) {
             kq[wave][0][e * 64 + lane] = kv[e] * rk;
             kq[wave][1][e * 64 + lane] = qv[e] * rq;
         }
+        wave_lds_order();                                     // (the last token's readers are past its barrier)
         v4f w1 = {0.f, 0.f, 0.f, 0.f}, w2 = w1;
         float kr[RPT];
 #pragma unroll
@@ -439,8 +447,7 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
             }
             v[i] = s;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
-        __builtin_amdgcn_wave_barrier();                      // (the wave's reads come before its writes)
+        wave_lds_order();                                     // (the wave's reads come before its writes)
 #pragma unroll
         for (int i = 0; i < 16; i++) d[i * LD + col] = v[i];
     }
