@@ -704,7 +704,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
     constexpr int KH = DK / 64, DH = DK / 32, LINES = (int)((HALF ? kRecV : rec_k(DK)) / 128);
     const int lane = threadIdx.x & 63, g = lane >> 4, w = at.w;
     const int64_t step = HALF ? at.rvs : at.rks;
-    // (never waited for: these waves load nothing else)
+    // (waited for once, at the end: nobody reads what they bring, but it has landed before the LDS is another workgroup's)
     auto touch = [&](const char* r) {
         for (int i = (2 * m + w) * 64 + lane; i < LINES; i += per * 128)
             dma4(r + i * 128, x.touched);
@@ -766,6 +766,7 @@ __device__ __forceinline__ void scan_out(const DeltaArgs& a, const ScanAt& at, c
             mine[i] = o[2 * HALF + i];
         }
     }
+    vm_wait<0>();
     lds_barrier();
     join();
     store(at.count - (at.nc - 1) * kC);

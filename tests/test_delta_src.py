@@ -30,3 +30,14 @@ def test_lanes_of_a_wave_exchange_in_order(name, write, read):
     assert "wave_lds_order();" in code[code.index(write):code.index(read)]
     order = body("wave_lds_order")
     assert "__builtin_amdgcn_fence(__ATOMIC_ACQ_REL" in order and "__builtin_amdgcn_wave_barrier()" in order
+
+
+def test_the_last_touches_have_landed_before_the_workgroup_ends():
+    """scan_out's touched lines come by DMA into LDS that nobody reads: they are waited for before its last barrier, outside
+    the loop over the chunks."""
+    code = body("scan_out")
+    loop = code.index("for (int c = 0; c < at.nc; c++) {")
+    end = code.rindex("lds_barrier();")
+    assert loop < code.index("touch(rec +") < code.rindex("vm_wait<0>();", 0, end) < end
+    between = code[code.rindex("}", 0, end):end]
+    assert "vm_wait<0>();" in between
