@@ -469,7 +469,7 @@ PRISM_API int64_t prism_kv_attend_workspace_bytes(int64_t T, int64_t hq, int64_t
  * q, k bf16 [T, hk, dk], v bf16 [T, hv, dv], g, beta fp32 [T, hv], out fp32 [T, hv, dv] (ld: row strides, hs: head
  * strides); state [nslots, hv, dk, dv] contiguous per slot, slot_ld apart, updated in place; slots int32: the state of
  * each sequence (null: its number).  A sequence whose slot is out of range is skipped; two sequences must not share one.
- * Needs dk, dv in {64, 128}, hv % hk == 0, 16-byte aligned tensors, strides % 8 (out and state % 4), v_ld <= 2^24.
+ * Needs dk, dv in {64, 128}, hv % hk == 0, 16-byte aligned tensors, strides % 8 (out and state % 4), v_ld in 0 .. 2^24.
  *
  * prism_delta_step: rows int32 [1]: row i < *rows (of T) is one token of sequence i; seqs, ws and ws_bytes are not read.
  * prism_delta_prefill: rows int32 [seqs + 1], non-decreasing within 0 .. T: sequence s is rows[s] .. rows[s + 1] - 1, in

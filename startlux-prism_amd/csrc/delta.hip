@@ -890,7 +890,7 @@ static int run(const prism_delta_args& h, bool prompts, hipStream_t st) {
         seqs > INT32_MAX)
         return PRISM_ERR_SHAPE;
     if (h.nslots < 0 || h.nslots > INT32_MAX || h.slot_ld < h.hv * h.dk * h.dv) return PRISM_ERR_SHAPE;
-    if (h.v_ld > 1 << 24) return PRISM_ERR_SHAPE;             // a chunk's values within 32-bit offsets
+    if (h.v_ld < 0 || h.v_ld > 1 << 24) return PRISM_ERR_SHAPE;   // a chunk's values within unsigned 32-bit offsets
     if (!PRISM_ALIGNED(h.q, 16) || !PRISM_ALIGNED(h.k, 16) || !PRISM_ALIGNED(h.v, 16) || !PRISM_ALIGNED(h.out, 16) ||
         !PRISM_ALIGNED(h.state, 16) || h.q_ld % 8 || h.q_hs % 8 || h.k_ld % 8 || h.k_hs % 8 || h.v_ld % 8 || h.v_hs % 8 ||
         h.o_ld % 4 || h.o_hs % 4 || h.slot_ld % 4)
