@@ -1,5 +1,5 @@
-"""prism_amd.delta on the GPU where its forms can go wrong: normalising without an eps, with the checks and tolerances of
-test_delta_gpu."""
+"""prism_amd.delta on the GPU where its forms can go wrong: normalising without an eps, values of very different sizes or
+not finite, clones, empty calls, many sequences, strides with gaps.  Checks and tolerances are test_delta_gpu's."""
 import pytest
 import torch
 
@@ -90,3 +90,81 @@ def test_calls_without_rows_or_states(dev, T, slots):
     delta.prefill(*args, torch.tensor([0, T], dtype=torch.int32, device=dev), T)
     delta.prefill(*args, torch.zeros(1, dtype=torch.int32, device=dev), T)
     assert (state == 2).all() and (out == 3).all()
+
+
+def test_prefill_more_sequences_than_a_wave_has_lanes(dev):
+    """130 short and empty prompts, some of more than a chunk and some past the 64th, rows of none on both sides."""
+    lens = [(7 * i * i + 3 * i) % 9 for i in range(130)]
+    lens[3], lens[63], lens[64], lens[90], lens[129] = 70, 129, 65, 64, 200
+    check_prefill(dev, lens, 1, 2, 64, 64, seed=41, lead=5, tail=3)
+
+
+@pytest.mark.parametrize("lead", [1, 5, 63, 64, 70])
+def test_prefill_rows_before_the_first_sequence(dev, lead):
+    check_prefill(dev, [130, 0, 7, 64], 1, 2, 64, 128, seed=lead, lead=lead, tail=2)
+
+
+@pytest.mark.parametrize("form", ["step", "prefill"])
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 128)])
+def test_rows_and_slots_with_gaps(dev, form, dk, dv):
+    """out between other columns, padded state slots, gates as column ranges of wider rows: the same bits as from whole
+    tensors, and nothing beside them written."""
+    from prism_amd import delta
+    hk, hv, T, seqs = 2, 4, 90, 3
+    proj, g, beta, state = (x.to(dev) for x in inputs(T, hk, hv, dk, dv, T, 51))
+    q, k, v = split(proj, hk, hv, dk, dv)
+    count = torch.tensor([T] if form == "step" else [0, 60, 61, T], dtype=torch.int32, device=dev)
+    call = delta.step if form == "step" else delta.prefill
+    states = T if form == "step" else seqs
+
+    want_s, want_o = state[:states].clone(), torch.zeros(T, hv, dv, device=dev)
+    call(q, k, v, g, beta, want_s, want_o, count, T)
+
+    wide_o = torch.full((T, hv + 2, dv + 8), 7.0, device=dev)
+    size = hv * dk * dv
+    wide_s = torch.full((states, size + 12), 7.0, device=dev)
+    s = wide_s.as_strided((states, hv, dk, dv), (size + 12, dk * dv, dv, 1))
+    s.copy_(state[:states])
+    gates = torch.cat([torch.full((T, 3), 9.0, device=dev), g, beta, torch.full((T, 2), 9.0, device=dev)], 1)
+    o = wide_o[:, 1:hv + 1, 4:dv + 4]
+    call(q, k, v, gates[:, 3:hv + 3], gates[:, hv + 3:2 * hv + 3], s, o, count, T)
+    assert torch.equal(o, want_o) and torch.equal(s, want_s)
+    o.fill_(7.0)
+    assert (wide_o == 7).all() and (wide_s[:, size:] == 7).all()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("where", ["v", "k", "state", "g"])
+def test_prefill_values_that_are_not_finite_stay_in_their_sequence_and_head(dev, bad, where):
+    """Other sequences, other heads and earlier chunks of the same sequence keep their bits; the sequence's later rows and
+    its state show it."""
+    from prism_amd import delta
+    hk, hv, dk, dv, T = 2, 4, 128, 64, 300
+    proj, g, beta, state = (x.to(dev) for x in inputs(T, hk, hv, dk, dv, 3, 61))
+    cu = torch.tensor([0, 90, 240, T], dtype=torch.int32, device=dev)
+
+    def run():
+        q, k, v = split(proj, hk, hv, dk, dv)
+        s, o = state.clone(), torch.zeros(T, hv, dv, device=dev)
+        delta.prefill(q, k, v, g, beta, s, o, cu, T)
+        return o, s
+    want_o, want_s = run()
+    _, k, v = split(proj, hk, hv, dk, dv)
+    t, first = 160, 154                                          # sequence 1, its second chunk (rows 154 .. 217)
+    if where == "v":
+        v[t, 2, 5] = bad
+    elif where == "k":
+        k[t, 1, 5] = bad
+    elif where == "g":
+        g[t, 2] = bad if bad != bad else float("nan")
+    else:
+        state[1, 2, 3, 4], first = bad, 90
+    heads = [2, 3] if where == "k" else [2]                      # (a key head's value heads)
+    o, s = run()
+    clean = torch.ones(T, hv, dtype=torch.bool, device=dev)
+    clean[first:240, heads] = False
+    assert torch.equal(o[clean], want_o[clean])
+    rest = torch.ones(3, hv, dtype=torch.bool, device=dev)
+    rest[1, heads] = False
+    assert torch.equal(s[rest], want_s[rest])
+    assert not torch.isfinite(o[t, 2]).all() and not torch.isfinite(s[1, 2]).all()

@@ -1,4 +1,5 @@
-"""prism_amd.kv on the GPU where its kernels can go wrong: scores past fp32's range."""
+"""prism_amd.kv on the GPU where its kernels can go wrong: scores past fp32's range, clones, empty calls, caches of two
+memory orders."""
 import pytest
 import torch
 
@@ -68,3 +69,34 @@ def test_calls_without_rows(dev):
               bf(0, 4, 64), n, 0)
     kv.attend(bf(0, 4, 64), kc, vc, ints(0, 4), ints(0), bf(0, 4, 64), n, 0)
     assert (kc == 0).all() and (vc == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_caches_of_different_orders(dev, dtype):
+    """Keys by the page's heads and values by token rows, and the other way round: append and attend give the bits of
+    caches of one order (fewer than 16 sequences: the order does not choose the form)."""
+    from prism_amd import kv
+    g = torch.Generator().manual_seed(7)
+    T, hq, hkv, dim, page, cols = 5, 8, 4, 128, 32, 9
+    lens = torch.tensor([1, 40, 288, 100, 64], dtype=torch.int32, device=dev)
+    table = torch.randperm(T * cols, generator=g).view(T, cols).int().to(dev)
+    shape = (T * cols, page, hkv, dim)
+    old = [torch.randn(shape, generator=g).to(dtype).to(dev) for _ in range(2)]
+    q, k, v = (torch.randn(T, h, dim, generator=g).to(torch.bfloat16).to(dev) for h in (hq, hkv, hkv))
+    rope = kv.rope_table(cols * page, 64, device=dev)
+
+    def order(x, by_head):
+        c = torch.empty(shape[0], hkv, page, dim, dtype=dtype, device=dev).transpose(1, 2) if by_head else \
+            torch.empty(shape, dtype=dtype, device=dev)
+        c.copy_(x)
+        return c
+
+    def run(k_by_head, v_by_head):
+        kc, vc = order(old[0], k_by_head), order(old[1], v_by_head)
+        turned, out = torch.empty_like(q), torch.empty_like(q)
+        kv.append(q, k, v, rope, lens - 1, table, kc, vc, turned, None, T)
+        kv.attend(turned, kc, vc, table, lens, out, None, T)
+        return [x.contiguous().view(torch.uint8) for x in (kc, vc, turned, out)]
+    want = run(True, True)
+    for ways in ((True, False), (False, True), (False, False)):
+        assert all(torch.equal(a, b) for a, b in zip(run(*ways), want))
