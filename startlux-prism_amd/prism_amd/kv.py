@@ -40,7 +40,8 @@ def append(q, k, v, rope, pos, table, k_cache, v_cache, q_out, n, T, seq=None, p
     multiple of 16 up to dim: the first R dims turn, in pairs (j, j + R / 2) with pairs="half" or (2 j, 2 j + 1) with
     pairs="adjacent": (a, b) -> (a cos - b sin, b cos + a sin) in fp32, rounded once to the type that is stored.  q_out may
     be q.  A token whose place is none is skipped, its q_out row untouched: a position that is negative or past the table
-    or the rotations, a sequence or a page out of range.  Two tokens with one place: either's value."""
+    or the rotations, a sequence or a page out of range.  Two tokens with one place leave a mixture of both there (each
+    piece of 8 dims is one's or the other's)."""
     if n is None:
         n = _live(n, T, k.device)
     rc = (L._host or L.host()).kv_append(q, k, v, rope, pos, table, k_cache, v_cache, q_out, n, T, seq, pairs, k_scale,
