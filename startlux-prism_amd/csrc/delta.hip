@@ -287,8 +287,9 @@ __device__ __forceinline__ void put_frag(char* base, v4u v) {
 // where the system is solved).  Rows are loaded in their own order (a row per lane would take the memory pipeline four
 // times as long) and become fragments through LDS.  The decays between tokens of different 16-row tiles are products of
 // three that are at most 1, so that a diagonal tile's exponentials and a few are enough.  One chunk takes 9 us, the
-// chain of its steps, and 8191 tokens of 16 key and 48 value heads of 128 take 86 us, the records' 255 MB for the most
-// part; with one wave for all four tiles 13 and 100 us, with each wave inverting its own diagonal block 9.4 and 109.
+// chain of its steps, and 8191 tokens of 16 key and 48 value heads of 128 take 92 us, the records' 333 MB for the most
+// part.  With a third less of X and P (255 MB, 86 us) one wave for all four tiles took 13 and 100 us, each wave inverting
+// its own diagonal block 9.4 and 109.
 template <int DK>
 __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* wk, char* wv) {
     constexpr int KS = DK / 32, LD = kC + 4, LK = DK + 8, PR = DK / 8, NL = 16 * PR / 64;  // PR: 16-byte pieces of a row
@@ -526,8 +527,10 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
 //   output waves  (P U of the last one)  | S in, Q S              | P U, halves out
 //   loading waves                        | next K in, P's last    | all else of the next chunk in
 //                                        | parts
-// Bound by that chain: a chunk takes some 5000 cycles, 3500 of them the state waves' alone, while LDS moves 370 KB
-// (2900 cycles).  8191 tokens of one sequence, 16 key and 48 value heads of 128 (192 workgroups): 280 us.
+// Bound by that chain where there are no more workgroups than CUs: 8191 tokens of one sequence, 16 key and 48 value heads of
+// 128 (192 workgroups) take 284 us, 2.2 a chunk, and 208 with the state waves' work alone; LDS moves 390 KB a chunk (some 3100
+// cycles).  158 KB of LDS leave one workgroup a CU: 1500 tokens in 5 prompts with 32 value heads are 640 workgroups, 40 us
+// for 13 chunks a CU.
 template <int DK>
 struct ScanShared {
     v4u k[4 * (DK / 32)][64], q[4 * (DK / 32)][64], x[3 * kTri][64], pl[kTri][64];
@@ -545,7 +548,7 @@ struct ScanAt {
 
 // A product's fragments are read from LDS into registers.  The compiler spreads the reads over the phase; forced to its
 // start, to have their latency behind what the right operand still takes, they come as bursts that hold the others up:
-// 392 us for 8191 tokens instead of 372.
+// 392 us for 8191 tokens instead of 372 (with operands of two parts).
 // K or Q: 4 token tiles, the half's k
 template <int DK, int HALF>
 __device__ __forceinline__ void read_rows(v4u (&r)[DK / 64][4], const v4u (*f)[64]) {
@@ -868,9 +871,10 @@ static int dispatch_chunks(const DeltaArgs& a, int64_t DK, int64_t DV, char* ws,
     return DV == 64 ? launch_chunks<128, 64>(a, ws, st) : launch_chunks<128, 128>(a, ws, st);
 }
 
-// A few rows go token by token: 1.5 us each for a sequence's at 48 heads, against 15.5 us for its first chunk (one
-// sequence of 6 rows 12.3 us, 8 rows 15.8, 10 rows 18.6; 12 rows of 6 sequences 8.1 against 18.3, of one 21.8 against
-// 15.8).
+// A few rows go token by token: 1.5 us each for a sequence's at 48 heads, against 15.3 us for its first chunk (one
+// sequence of 6 rows 12.3 us, 8 rows 15.4, 10 rows 18.5; 12 rows of 6 sequences 10.4 against 35).  The rule sees the rows
+// in all, not the prompts' lengths, which are on the device: many short prompts go in chunks and take a chunk's records
+// (2.6 MB at 16 and 48 heads of 128) and time each, 189 us for 40 prompts of 4 rows.
 static bool by_token(int64_t T, int64_t seqs) { return T <= (seqs > 1 ? 12 : 8); }
 
 static int64_t workspace_bytes(int64_t T, int64_t seqs, int64_t hk, int64_t hv, int64_t dk) {

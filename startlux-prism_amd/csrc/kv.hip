@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
 //
 // Bound by the cache's bytes, read once: one sequence of 131071 tokens, 8 heads of 128 bf16 (537 MB), 98 us, 5.5 TB/s, 90
 // of them this kernel (6.0 TB/s, more than a copy moves) and 7 the joining one; 40 of up to 20000, 4 heads of 256 e4m3
-// (505 MB), 101 us, 5.0 TB/s; token rows of 8 heads of 64, 128 sequences of up to 4096 visible (613 MB), 124 us,
+// (505 MB), 101 us, 5.0 TB/s; token rows of 8 heads of 64, 128 sequences of up to 4096 visible (613 MB), 125 us,
 // 4.9 TB/s (runs of 512 bytes a token; the same heads' rows by the page take 120).  A short call (613 tokens) is launches
 // and one chain of a unit's steps, 9 us.
 struct AttendArgs {
@@ -653,7 +653,9 @@ static int64_t attend_parts(int64_t T, int64_t HT, int64_t cap, int64_t unit, in
 // Whether waves may take heads side by side: whole groups of four, a tile of query heads each, and enough sequences
 // that the parts, now of four heads each, are few.  With and without, rows of 8 heads: 128 sequences of 100 - 4096
 // visible tokens of 64 bf16 124 / 146 us, 64 of 8000 tokens of 128 364 / 391 (e4m3 199 / 234), 16 of 4000 of 64
-// 34.7 / 37.6; but 8 of those 20.5 / 19.5, one of 32768 28 / 21, and 16 of 300 - 500 tokens of 128 e4m3 13.2 / 11.7.
+// 34.7 / 37.6; but 8 of those 20.5 / 19.5, one of 32768 28 / 21, and 16 of 300 - 500 tokens of 128 e4m3 13.2 / 11.7.  The
+// lengths are on the device, so the rule sees the rows of the batch and the room of the table: short sequences in a table
+// with room for long ones take this form as well.
 static bool attend_side(int64_t T, int64_t hq, int64_t heads, int64_t cap) {
     return heads % 4 == 0 && hq / heads <= 16 && T >= 16 && cap >= 1024;
 }
