@@ -180,8 +180,8 @@ static int launch_rec(const DeltaArgs& a, hipStream_t st) {
 // and three products (8191 tokens, 16 key and 48 value heads of 128: 352 us instead of 381), but what a value keeps then
 // depends on the largest of its column: a token's update was rounded by, or lost to, a large value that came after it.
 //
-// A token's outputs depend on its own and earlier tokens only, whatever finite values the later ones hold; a value that is
-// not finite reaches its whole chunk (zeros of a triangle times infinity).
+// A token's outputs depend on its own and earlier tokens only, whatever finite values the later ones hold; what is not finite,
+// an input or a product past fp32's range, reaches its whole chunk (zeros of a triangle times infinity).
 //
 // Everything that delta_scan multiplies from the left (K, Q, K^T, X diag(beta), P) lies in the workspace as MFMA
 // fragments, 1 KB each in lane order.  Inside a product the order of the summed index is free: taking it as an
@@ -521,12 +521,11 @@ __global__ __launch_bounds__(256, 4) void delta_prep_kernel(DeltaArgs a, char* w
 // SIMD. Four waves to 16 columns: two hold the halves of S's rows and take what the next chunk waits for (K S, U, K^T
 // U), two the chunk's output (Q S, P U); products split over the summed index: a wave multiplies its half of S's rows,
 // or its half of U's tokens, and the halves' sums (fp32, always the same two added) meet in LDS.  The other four waves
-// bring the fragments into LDS, each group while nobody reads it, and touch the lines of the chunk after the next, so
-// that those come from L2.  Two barriers per chunk:
+// bring the fragments into LDS, each group while nobody reads it; the output waves touch the lines of the chunk after the
+// next, so that those come from L2.  Two barriers per chunk:
 //   state waves   K S, halves out        | halves in, R, X R out  | U in, S <- ..., S out
 //   output waves  (P U of the last one)  | S in, Q S              | P U, halves out
-//   loading waves                        | next K in, P's last    | all else of the next chunk in
-//                                        | parts
+//   loading waves                        | next K, P's thirds in  | all else of the next chunk in
 // Bound by that chain where there are no more workgroups than CUs: 8191 tokens of one sequence, 16 key and 48 value heads of
 // 128 (192 workgroups) take 284 us, 2.2 a chunk, and 208 with the state waves' work alone; LDS moves 390 KB a chunk (some 3100
 // cycles).  158 KB of LDS leave one workgroup a CU: 1500 tokens in 5 prompts with 32 value heads are 640 workgroups, 40 us

@@ -34,8 +34,8 @@ def step(q, k, v, g, beta, state, out, n, T, slots=None, norm=True, scale=None, 
 def prefill(q, k, v, g, beta, state, out, cu, T, slots=None, norm=True, scale=None, eps=1e-6):
     """Sequence s is rows cu[s] .. cu[s + 1] - 1 (cu int32 [sequences + 1] on the device, non-decreasing, within 0 .. T),
     continued from its state, which is left as after its last row (module comment).  A sequence may be empty; rows outside
-    every sequence are untouched.  A value that is not finite may show in the outputs of up to 63 earlier tokens of its
-    sequence as well (they are computed together)."""
+    every sequence are untouched.  What is not finite (an input, or a product past fp32's range) may show in the outputs of
+    up to 63 earlier tokens of its sequence as well (they are computed together)."""
     rc = (L._host or L.host()).delta_prefill(q, k, v, g, beta, state, out, cu, T, slots, norm, scale, eps)
     if rc:
         L.fail("prism_delta_prefill", rc)
