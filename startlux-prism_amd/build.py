@@ -4,7 +4,7 @@
 
 Each csrc/*.hip compiles to an object under csrc/_build/, then one shared library links next to the Python package
 (startlux-prism_amd/prism_amd/libprism_amd.so), which prism_amd._lib loads.  csrc/host.cpp compiles with g++ to
-prism_amd/_host.so, the checked host path of prism_amd.kv and prism_amd.delta; without torch or g++ that one is left out
+prism_amd/_host.so, the checked host path of prism_amd.kv, delta, fp8 and moe; without torch or g++ that one is left out
 and the library is complete for its C ABI.  Flags of the HIP files:
   --offload-arch=gfx950                        MI355X / MI350X only; no other targets, no host fallback
   -fhip-fp32-correctly-rounded-divide-sqrt     '/' on fp32 is the IEEE division the quantizers are specified with
@@ -47,7 +47,7 @@ def _compile(src):
 
 
 def _compile_host():
-    """csrc/host.cpp -> prism_amd/_host.so: the CPython extension that checks kv's and delta's tensors (host code only).
+    """csrc/host.cpp -> prism_amd/_host.so: the CPython extension that checks the tensors of kv, delta, fp8 and moe (host code only).
     Returns why it cannot be built here (no torch, no C++ compiler), else None."""
     import sysconfig
 
@@ -91,7 +91,7 @@ def build(jobs=8, verbose=False):
     if missing:
         if os.path.exists(HOST):
             os.remove(HOST)
-        print(f"{HOST} is not built ({missing}): prism_amd.kv and prism_amd.delta need it, the C ABI does not",
+        print(f"{HOST} is not built ({missing}): prism_amd.kv, delta, fp8 and moe need it, the C ABI does not",
               file=sys.stderr)
     return LIB
 

@@ -1,0 +1,528 @@
+// 8-bit floating point projections with block scales for gfx950: the activation quantizer, the weight packer and the GEMM.
+//
+//   y[m][j] = sum_b as[m][b] ws[j / 128][b] (sum_i a[m][128 b + i] w[j][128 b + i])
+//
+// A block's inner sum is one v_mfma_scale_f32_16x16x128_f8f6f4 (unit scales) from a zero accumulator; its four values of a
+// lane are then folded into the fp32 sums by one fma each with as ws.  A operand: the weights, lane 16 g + r row r, bytes
+// 16 p .. of piece p = inputs 64 p + 16 g .. + 15; B operand: the activations likewise (any order of the inputs serves, so
+// long as both share it); D, lane 16 g + r: activation row r, weight rows 4 g .. + 3.  So as is one value of a lane per 16
+// rows, and ws one of the wave.
+//
+// Inside the MFMA the 8 products of a lane's 8 neighbouring bytes are aligned on the largest of them with 13 bits kept below
+// it (measured: beside a product of 2^16 one of 2^3 counts, one of 2^2 does not), the groups are added in fp32.  So a
+// product p is off by at most 2^-13 max of its group; on normal values with a shared scale the sum is 1.5e-5 off (2-norm),
+// against the 1.7e-3 of the bf16 output.  v_mfma_f32_16x16x32_fp8_fp8 gives the same bits at half the rate.
+#include "common.h"
+#include "fp8.h"
+
+namespace prism {
+
+// ---------------------------------------------------------------------------------------------------------- quantizers
+// e4m3 codes of two values already divided by their scale, nearest even; |v| <= 448 (1 + 2^-23) unless not finite.
+// v_cvt_pk_fp8_f32 saturates to NaN only past 464; NaN stays NaN, an infinity becomes NaN.
+__device__ __forceinline__ uint32_t e4m3_pk4(float a, float b, float c, float d) {
+    int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
+}
+
+__device__ __forceinline__ float block_scale(float amax) { return div_rn(fmaxf(amax, kAmaxMin), kE4m3Max); }
+
+// 16 neighbouring lanes per (row, 128 inputs), 8 inputs each, U such units per thread a grid apart (the loads of all go out
+// first).  VEC: 16-byte loads (aligned rows, k % 8 == 0).
+template <bool F32, bool VEC, int U>
+__global__ __launch_bounds__(256) void fp8_quant_kernel(const void* __restrict__ x, int64_t x_ld, uint8_t* __restrict__ q,
+                                                        int64_t q_ld, float* __restrict__ s, int64_t s_ld,
+                                                        const int32_t* __restrict__ n_rows, int T, int k, int KB) {
+    const int live = min(T, __ldg(n_rows));
+    const int64_t units = (int64_t)live * KB, step = (int64_t)gridDim.x * 16;
+    const int sub = threadIdx.x & 15;
+    int64_t u0 = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    for (; u0 < units; u0 += step * U) {
+        float v[U][8];
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int64_t u = u0 + j * step;
+            if (u >= units) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[j][i] = 0.f;
+                continue;
+            }
+            const int row = (int)(u / KB), c = (int)(u % KB) * 128 + sub * 8;
+            if (VEC) {
+                if (c < k) {
+                    if (F32) {
+                        const v4f* p = reinterpret_cast<const v4f*>(reinterpret_cast<const float*>(x) + row * x_ld + c);
+                        const v4f lo = __builtin_nontemporal_load(p), hi = __builtin_nontemporal_load(p + 1);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) v[j][i] = lo[i], v[j][4 + i] = hi[i];
+                    } else {
+                        const v4u p = __builtin_nontemporal_load(
+                            reinterpret_cast<const v4u*>(reinterpret_cast<const uint16_t*>(x) + row * x_ld + c));
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            v[j][2 * i] = bf16_to_f32(p[i] & 0xffff), v[j][2 * i + 1] = __uint_as_float(p[i] & 0xffff0000u);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[j][i] = 0.f;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    v[j][i] = 0.f;
+                    if (c + i < k)
+                        v[j][i] = F32 ? reinterpret_cast<const float*>(x)[row * x_ld + c + i]
+                                      : bf16_to_f32(reinterpret_cast<const uint16_t*>(x)[row * x_ld + c + i]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const int64_t u = u0 + j * step;
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(v[j][i]));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+            if (u >= units) continue;
+            const int row = (int)(u / KB), b = (int)(u % KB);
+            const float sc = block_scale(m);
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = div_rn(v[j][i], sc);
+            const v2u codes = {e4m3_pk4(y[0], y[1], y[2], y[3]), e4m3_pk4(y[4], y[5], y[6], y[7])};
+            *reinterpret_cast<v2u*>(q + row * q_ld + b * 128 + sub * 8) = codes;
+            if (sub == 0) s[row * s_ld + b] = sc;
+        }
+    }
+}
+
+// One workgroup per 128 x 128 block: thread t holds row t / 2's 64 inputs of half t % 2.
+__global__ __launch_bounds__(256) void fp8_pack_kernel(const void* __restrict__ w, int f32, int64_t ld,
+                                                       uint8_t* __restrict__ chunks, float* __restrict__ ws, int n, int k,
+                                                       int KB) {
+    __shared__ float red[4];
+    const int b = blockIdx.x, nb = blockIdx.y, t = threadIdx.x, row = nb * 128 + t / 2, half = t & 1;
+    float v[64], m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 64; i++) {
+        const int c = b * 128 + half * 64 + i;
+        v[i] = 0.f;
+        if (row < n && c < k)
+            v[i] = f32 ? reinterpret_cast<const float*>(w)[row * ld + c]
+                       : bf16_to_f32(reinterpret_cast<const uint16_t*>(w)[row * ld + c]);
+        m = fmaxf(m, fabsf(v[i]));
+    }
+    m = wave_max(m);
+    if ((t & 63) == 0) red[t >> 6] = m;
+    __syncthreads();
+    const float sc = block_scale(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    if (t == 0) ws[(int64_t)nb * KB + b] = sc;
+    if (row >= (n + 15) / 16 * 16) return;
+    uint8_t* c = chunks + ((int64_t)(row / 16) * KB + b) * 2048 + half * 1024 + (row & 15) * 16;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            o[i] = e4m3_pk4(div_rn(v[16 * g + 4 * i], sc), div_rn(v[16 * g + 4 * i + 1], sc),
+                            div_rn(v[16 * g + 4 * i + 2], sc), div_rn(v[16 * g + 4 * i + 3], sc));
+        *reinterpret_cast<v4u*>(c + 256 * g) = v4u{o[0], o[1], o[2], o[3]};
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- GEMM
+__device__ __forceinline__ v8i join8(v4i lo, v4i hi) { return v8i{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}; }
+
+__device__ __forceinline__ v4f fp8_mfma(v8i w, v8i a) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, a, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+}
+
+__device__ __forceinline__ v4f fold(v4f t, float s, v4f acc) {
+    return v4f{__builtin_fmaf(t.x, s, acc.x), __builtin_fmaf(t.y, s, acc.y), __builtin_fmaf(t.z, s, acc.z),
+               __builtin_fmaf(t.w, s, acc.w)};
+}
+
+struct Fp8Gemm {
+    const uint8_t* a;
+    int64_t a_ld;
+    const float* as;
+    int64_t as_ld;
+    const uint8_t* w;
+    const float* ws;
+    void* out;
+    int64_t o_ld;
+    const int32_t* n_rows;
+    float* part;             // split K: fp32 [splits][T][n rounded up to 4]
+    int T, n, k, KB, NT;     // NT: 16-row weight tiles
+    int vec;                 // the output's rows take whole stores of four
+};
+
+// Four outputs of row m, columns j .. j + 3 (those below n).
+template <int EPI>
+__device__ __forceinline__ void store4(const Fp8Gemm& g, int m, int j, v4f y) {
+    if (EPI == 0) {
+        uint16_t* o = reinterpret_cast<uint16_t*>(g.out) + m * g.o_ld + j;
+        if (g.vec && j + 3 < g.n) {
+            *reinterpret_cast<v2u*>(o) = v2u{f32_to_bf16(y.x) | f32_to_bf16(y.y) << 16, f32_to_bf16(y.z) | f32_to_bf16(y.w) << 16};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (j + i < g.n) o[i] = (uint16_t)f32_to_bf16(y[i]);
+        }
+    } else {
+        float* o = reinterpret_cast<float*>(g.out) + m * g.o_ld + j;
+        if (g.vec && j + 3 < g.n) {
+            v4f* p = reinterpret_cast<v4f*>(o);
+            const v4f h = *p;
+            *p = v4f{add_rn(h.x, y.x), add_rn(h.y, y.y), add_rn(h.z, y.z), add_rn(h.w, y.w)};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (j + i < g.n) o[i] = add_rn(o[i], y[i]);
+        }
+    }
+}
+
+// Few rows (up to 16 MT): a workgroup owns NW2 16-row weight tiles, its 8 waves take the blocks of 128 inputs in turn (wave w
+// block w, w + 8, ...) straight from memory into registers, D blocks ahead, and add their sums through LDS, wave after wave.
+// Blocks past the end and rows past the live ones read as zeros (the buffers' range), so the loop has no branches.
+constexpr int kStreamWaves = 8;
+template <int MT, int NW2, int D, int EPI>
+__global__ __launch_bounds__(64 * kStreamWaves) void fp8_stream_kernel(Fp8Gemm g) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, gr = lane >> 4;
+    const int t0 = blockIdx.x * NW2, m0 = blockIdx.y * 16 * MT;
+    const int live = min(g.T, __ldg(g.n_rows)) - m0;
+    if (live <= 0) return;
+    const int tiles = min(NW2, g.NT - t0), KB = g.KB;
+    const uint32_t tile = (uint32_t)KB * 2048;
+    const __amdgpu_buffer_rsrc_t wr = buf_rsrc_n(g.w + (int64_t)t0 * tile, tiles * tile);
+    const uint32_t rows = min(live, 16 * MT);
+    const __amdgpu_buffer_rsrc_t ar = buf_rsrc_n(g.a + m0 * g.a_ld, (uint32_t)((rows - 1) * g.a_ld + KB * 128));
+    const __amdgpu_buffer_rsrc_t sr = buf_rsrc_n(g.as + m0 * g.as_ld, (uint32_t)((rows - 1) * g.as_ld + KB) * 4);
+    const float* ws = g.ws + (int64_t)(t0 / 8) * KB;             // (NW2 tiles lie in one block of 128 rows)
+    constexpr uint32_t kOut = 0x80000000u;
+    uint32_t aoff[MT], soff[MT];
+#pragma unroll
+    for (int c = 0; c < MT; c++) {
+        const int m = 16 * c + r;
+        aoff[c] = m < live ? (uint32_t)(m * g.a_ld + 16 * gr) : kOut;
+        soff[c] = m < live ? (uint32_t)(m * g.as_ld) * 4 : kOut;
+    }
+    struct Stage {
+        v4i w[NW2][2], a[MT][2];
+        float s[MT];
+    } st[D];
+    auto issue = [&](Stage& x, int b) {
+        const uint32_t out = b < KB ? 0u : kOut;                  // (wave-uniform)
+#pragma unroll
+        for (int t = 0; t < NW2; t++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) x.w[t][p] = buf_load16<kBufNT>(wr, (lane * 16 + p * 1024 + t * tile + b * 2048u) | out, 0);
+#pragma unroll
+        for (int c = 0; c < MT; c++) {
+#pragma unroll
+            for (int p = 0; p < 2; p++) x.a[c][p] = buf_load16(ar, (aoff[c] + 64 * p + b * 128u) | out, 0);
+            x.s[c] = __uint_as_float(buf_load4(sr, (soff[c] + b * 4u) | out, 0));
+        }
+    };
+    v4f acc[NW2][MT];
+#pragma unroll
+    for (int t = 0; t < NW2; t++)
+#pragma unroll
+        for (int c = 0; c < MT; c++) acc[t][c] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < D; d++) issue(st[d], w + d * kStreamWaves);
+    for (int b = w; b < KB; b += D * kStreamWaves) {
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            const int at = b + d * kStreamWaves;
+            const float sw = ws[min(at, KB - 1)];
+#pragma unroll
+            for (int c = 0; c < MT; c++) {
+                const v8i a = join8(st[d].a[c][0], st[d].a[c][1]);
+                const float s = mul_rn(st[d].s[c], sw);
+#pragma unroll
+                for (int t = 0; t < NW2; t++)
+                    acc[t][c] = fold(fp8_mfma(join8(st[d].w[t][0], st[d].w[t][1]), a), s, acc[t][c]);
+            }
+            issue(st[d], at + D * kStreamWaves);
+        }
+    }
+    v4f* red = reinterpret_cast<v4f*>(lds);
+#pragma unroll
+    for (int t = 0; t < NW2; t++)
+#pragma unroll
+        for (int c = 0; c < MT; c++) red[((t * MT + c) * kStreamWaves + w) * 64 + lane] = acc[t][c];
+    __syncthreads();
+    for (int i = w; i < NW2 * MT; i += kStreamWaves) {
+        v4f y = red[i * kStreamWaves * 64 + lane];
+        for (int j = 1; j < kStreamWaves; j++) {
+            const v4f z = red[(i * kStreamWaves + j) * 64 + lane];
+            y = v4f{add_rn(y.x, z.x), add_rn(y.y, z.y), add_rn(y.z, z.z), add_rn(y.w, z.w)};
+        }
+        const int m = 16 * (i % MT) + r, j = (t0 + i / MT) * 16 + 4 * gr;
+        if (m < live) store4<EPI>(g, m0 + m, j, y);
+    }
+}
+
+// Many rows: WM x WN waves of 16 AR activation rows by 64 weight rows; both operands by LDS-DMA, NS stages of 128 inputs.
+// Weight chunks lie in LDS as in memory (a lane's fragments are contiguous); an activation row's 128 bytes lie as eight
+// 16-byte pieces, piece c of row r at slot c ^ (r % 8), so that eight neighbouring lanes copy one row and the 16 rows of a
+// fragment read lie on distinct banks.
+template <int WM, int WN, int AR>
+struct Fp8Tile {
+    static constexpr int W = WM * WN, TW = 4 * WN, TA = AR * WM;
+    static constexpr int AQ = TW * 2048, AS = AQ + TA * 2048, BYTES = AS + TA * 64;
+    static constexpr int WD = TW * 2 / W, AD = TA * 2 / W;            // 1 KB copies per wave and stage
+    static_assert(WD * W == TW * 2 && AD * W == TA * 2, "whole copies");
+};
+
+// EPI 2: fp32 partial sums of this part of K to g.part.
+template <int WM, int WN, int AR, int NS, int EPI, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n, int splits) {
+    using S = Fp8Tile<WM, WN, AR>;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, gr = lane >> 4;
+    const int tiles = tiles_m * tiles_n, part = blockIdx.x / tiles;       // (a part's tiles together, as their order wants)
+    int pm, pn;
+    xcd_tile_coords(blockIdx.x % tiles, tiles_m, tiles_n, pm, pn);
+    const int m0 = pm * 16 * S::TA, t0 = pn * S::TW, KB = g.KB;
+    const int live = min(g.T, __ldg(g.n_rows));
+    if (m0 >= live) return;
+    const int b0 = (int)((int64_t)KB * part / splits), b1 = (int)((int64_t)KB * (part + 1) / splits);
+
+    const uint8_t* wsrc[S::WD];
+    const uint8_t* asrc[S::AD];
+#pragma unroll
+    for (int i = 0; i < S::WD; i++) {
+        const int c = w * S::WD + i, t = min(t0 + c / 2, g.NT - 1);
+        wsrc[i] = g.w + ((int64_t)t * KB + b0) * 2048 + (c & 1) * 1024 + lane * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < S::AD; i++) {
+        const int row = (w * S::AD + i) * 8 + lane / 8, m = min(m0 + row, live - 1);
+        asrc[i] = g.a + m * g.a_ld + b0 * 128 + (((lane & 7) ^ (row & 7)) * 16);
+    }
+    // a wave's scales: 64 rows of the tile (waves past the tile's rows copy none)
+    const bool sc = w * 64 < 16 * S::TA;
+    const float* ssrc = g.as + min(m0 + w * 64 + lane, live - 1) * g.as_ld + b0;
+    auto issue = [&](int b, int buf) {
+        uint8_t* l = lds + buf * S::BYTES;
+#pragma unroll
+        for (int i = 0; i < S::WD; i++) dma16(wsrc[i] + b * 2048, l + (w * S::WD + i) * 1024);
+#pragma unroll
+        for (int i = 0; i < S::AD; i++) dma16(asrc[i] + b * 128, l + S::AQ + (w * S::AD + i) * 1024);
+        if (sc) __builtin_amdgcn_global_load_lds(ssrc + b, (__attribute__((address_space(3))) void*)(l + S::AS + w * 256), 4, 0, 0);
+    };
+    static_assert(S::TA % 4 == 0, "scales are copied 64 rows at a time");
+
+    const int wn = w % WN, wm = w / WN;
+    const float* ws = g.ws + (int64_t)min((t0 + 4 * wn) / 8, (g.NT - 1) / 8) * KB + b0;
+    v4f acc[4][AR];
+#pragma unroll
+    for (int a = 0; a < 4; a++)
+#pragma unroll
+        for (int c = 0; c < AR; c++) acc[a][c] = v4f{0.f, 0.f, 0.f, 0.f};
+    const int nb = b1 - b0;
+#pragma unroll
+    for (int i = 0; i < NS - 1; i++)
+        if (i < nb) issue(i, i);
+    for (int b = 0; b < nb; b++) {
+        // the copies of stage b are there: at most those of the NS - 2 later stages are in flight
+        constexpr int kCopies = S::WD + S::AD + 1;
+        const int pend = min(nb - 1, b + NS - 2) - b;
+        if (NS >= 3 && pend >= 1 && sc) vm_wait<kCopies*(NS - 2)>();
+        else if (NS >= 3 && pend >= 1) vm_wait<(kCopies - 1) * (NS - 2)>();
+        else vm_wait<0>();
+        lds_barrier();
+        if (b + NS - 1 < nb) issue(b + NS - 1, (b + NS - 1) % NS);
+        const uint8_t* l = lds + (b % NS) * S::BYTES;
+        const float sw = ws[b];
+        v8i wf[4];
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            const uint8_t* p = l + (4 * wn + a) * 2048 + lane * 16;
+            wf[a] = join8(*reinterpret_cast<const v4i*>(p), *reinterpret_cast<const v4i*>(p + 1024));
+        }
+#pragma unroll
+        for (int c = 0; c < AR; c++) {
+            const int row = 16 * (AR * wm + c) + r;
+            const uint8_t* p = l + S::AQ + row * 128;
+            const v8i af = join8(*reinterpret_cast<const v4i*>(p + ((gr ^ (r & 7)) * 16)),
+                                 *reinterpret_cast<const v4i*>(p + (((4 + gr) ^ (r & 7)) * 16)));
+            const float s = mul_rn(*reinterpret_cast<const float*>(l + S::AS + row * 4), sw);
+#pragma unroll
+            for (int a = 0; a < 4; a++) acc[a][c] = fold(fp8_mfma(wf[a], af), s, acc[a][c]);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < AR; c++) {
+        const int m = m0 + 16 * (AR * wm + c) + r;
+        if (m >= live) continue;
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            const int j = 16 * (t0 + 4 * wn + a) + 4 * gr;
+            if (EPI == 2) {
+                const int64_t n4 = (g.n + 3) & ~3;
+                if (j < n4) *reinterpret_cast<v4f*>(g.part + ((int64_t)part * g.T + m) * n4 + j) = acc[a][c];
+            } else if (j < g.n) {
+                store4<EPI>(g, m, j, acc[a][c]);
+            }
+        }
+    }
+}
+
+// The parts of a split K added in their order: a thread per four outputs.
+template <int EPI>
+__global__ __launch_bounds__(256) void fp8_join_kernel(Fp8Gemm g, int splits) {
+    const int live = min(g.T, __ldg(g.n_rows)), n4 = (g.n + 3) & ~3;
+    const int m = blockIdx.y, j = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (m >= live || j >= n4) return;
+    const float* p = g.part + (int64_t)m * n4 + j;
+    v4f y = *reinterpret_cast<const v4f*>(p);
+    for (int i = 1; i < splits; i++) {
+        const v4f z = *reinterpret_cast<const v4f*>(p + (int64_t)i * g.T * n4);
+        y = v4f{add_rn(y.x, z.x), add_rn(y.y, z.y), add_rn(y.z, z.z), add_rn(y.w, z.w)};
+    }
+    store4<EPI>(g, m, j, y);
+}
+
+// ------------------------------------------------------------------------------------------------------------- choice
+struct Fp8Plan {
+    int kind;            // 0 stream, 1 tile 64 x 128 (two waves of 64 x 64), 2 tile 256 x 256
+    int mt, splits;
+};
+
+inline Fp8Plan fp8_plan(int64_t T, int64_t n, int64_t k) {
+    const int64_t NT = (n + 15) / 16, KB = (k + 127) / 128;
+    if (T <= 64) return {0, (int)((T + 15) / 16), 1};
+    const int64_t big = ((T + 255) / 256) * ((NT + 15) / 16);
+    if (big >= 200) return {2, 8, 1};
+    const int64_t tiles = ((T + 127) / 128) * ((NT + 7) / 8);
+    int64_t s = 512 / (tiles > 512 ? 512 : tiles);
+    if (s > KB / 8) s = KB / 8;
+    if (s < 1) s = 1;
+    if (s > 8) s = 8;
+    return {1, 4, (int)s};
+}
+
+}  // namespace prism
+
+using namespace prism;
+
+extern "C" int prism_fp8_pack(const void* w, int f32, int64_t ld, uint8_t* chunks, float* ws, int64_t n, int64_t k,
+                              void* stream) {
+    if (!w || !chunks || !ws || (f32 != 0 && f32 != 1)) return PRISM_ERR_ARG;
+    if (n < 1 || k < 1 || n > kFp8MaxDim || k > kFp8MaxDim || ld < k) return PRISM_ERR_SHAPE;
+    if (!PRISM_ALIGNED(chunks, 16)) return PRISM_ERR_ALIGN;
+    const int KB = (int)((k + 127) / 128);
+    hipLaunchKernelGGL(fp8_pack_kernel, dim3(KB, (unsigned)((n + 127) / 128)), dim3(256), 0, (hipStream_t)stream, w, f32, ld,
+                       chunks, ws, (int)n, (int)k, KB);
+    PRISM_LAUNCH_CHECK();
+    return PRISM_OK;
+}
+
+extern "C" int prism_fp8_quant(const prism_fp8_quant_args* args, void* stream) {
+    if (!args) return PRISM_ERR_ARG;
+    const prism_fp8_quant_args& h = *args;
+    if (!h.x || !h.q || !h.s || !h.n_rows || (h.f32 != 0 && h.f32 != 1)) return PRISM_ERR_ARG;
+    const int64_t KB = (h.k + 127) / 128;
+    if (h.T < 0 || h.T > INT32_MAX || h.k < 1 || h.k > kFp8MaxDim || h.x_ld < 0 || h.q_ld < 0 || h.s_ld < 0)
+        return PRISM_ERR_SHAPE;
+    if (h.T > 1 && (h.q_ld < 128 * KB || h.s_ld < KB)) return PRISM_ERR_SHAPE;
+    if (!PRISM_ALIGNED(h.q, 8) || h.q_ld % 8) return PRISM_ERR_ALIGN;
+    if (h.T == 0) return PRISM_OK;
+    const bool vec = h.k % 8 == 0 && PRISM_ALIGNED(h.x, 16) && h.x_ld % (h.f32 ? 4 : 8) == 0;
+    const int64_t groups = (h.T * KB + 15) / 16;
+    const hipStream_t st = (hipStream_t)stream;
+#define FQ(F, V, U) \
+    hipLaunchKernelGGL((fp8_quant_kernel<F, V, U>), dim3((unsigned)((groups + U - 1) / U < 4096 ? (groups + U - 1) / U : 4096)), \
+                       dim3(256), 0, st, h.x, h.x_ld, h.q, h.q_ld, h.s, h.s_ld, h.n_rows, (int)h.T, (int)h.k, (int)KB)
+    const bool many = groups >= 2048;
+    if (h.f32) {
+        if (!vec) FQ(true, false, 1); else if (many) FQ(true, true, 2); else FQ(true, true, 1);
+    } else {
+        if (!vec) FQ(false, false, 1); else if (many) FQ(false, true, 4); else FQ(false, true, 1);
+    }
+#undef FQ
+    PRISM_LAUNCH_CHECK();
+    return PRISM_OK;
+}
+
+extern "C" int64_t prism_fp8_gemm_workspace_bytes(int64_t T, int64_t n, int64_t k) {
+    if (T < 1 || n < 1 || k < 1) return 0;
+    const Fp8Plan p = fp8_plan(T, n, k);
+    return p.splits > 1 ? (int64_t)p.splits * T * ((n + 3) & ~3) * 4 : 0;
+}
+
+extern "C" int prism_fp8_gemm(const prism_fp8_gemm_args* args, void* stream) {
+    if (!args) return PRISM_ERR_ARG;
+    const prism_fp8_gemm_args& h = *args;
+    if (!h.a || !h.as || !h.w || !h.ws || !h.out || !h.n_rows || (h.epi != 0 && h.epi != 1)) return PRISM_ERR_ARG;
+    if (h.T < 0 || h.T > INT32_MAX / 512 || h.n < 1 || h.k < 1 || h.n > kFp8MaxDim || h.k > kFp8MaxDim) return PRISM_ERR_SHAPE;
+    const int64_t KB = (h.k + 127) / 128;
+    // (the few rows' operands are reached by 31-bit offsets)
+    if (h.a_ld < 0 || h.as_ld < 0 || h.o_ld < 0 || h.a_ld > kFp8MaxLd || h.as_ld > kFp8MaxLd) return PRISM_ERR_SHAPE;
+    if (h.T > 1 && h.o_ld < h.n) return PRISM_ERR_SHAPE;
+    if (!PRISM_ALIGNED(h.a, 16) || !PRISM_ALIGNED(h.w, 16) || h.a_ld % 16 || !PRISM_ALIGNED(h.as, 4)) return PRISM_ERR_ALIGN;
+    if (!PRISM_ALIGNED(h.out, h.epi ? 4 : 2)) return PRISM_ERR_ALIGN;
+    if (h.T == 0) return PRISM_OK;
+    const int64_t need = prism_fp8_gemm_workspace_bytes(h.T, h.n, h.k);
+    if (need > 0 && (!h.wsp || h.wsp_bytes < need)) return PRISM_ERR_ARG;
+    if (need > 0 && !PRISM_ALIGNED(h.wsp, 16)) return PRISM_ERR_ALIGN;
+    Fp8Gemm g{h.a, h.a_ld, h.as, h.as_ld, h.w, h.ws, h.out, h.o_ld, h.n_rows, (float*)h.wsp, (int)h.T, (int)h.n, (int)h.k,
+              (int)KB, (int)((h.n + 15) / 16), 0};
+    g.vec = h.o_ld % 4 == 0 && PRISM_ALIGNED(h.out, h.epi ? 16 : 8);
+    const Fp8Plan p = fp8_plan(h.T, h.n, h.k);
+    const hipStream_t st = (hipStream_t)stream;
+#define EP(f) do { if (h.epi) f(1); else f(0); } while (0)
+    if (p.kind == 0) {
+#define ST(MT, NW, D, E) do { \
+        const size_t bytes = (size_t)MT * NW * kStreamWaves * 1024; \
+        allow_lds(fp8_stream_kernel<MT, NW, D, E>, bytes); \
+        hipLaunchKernelGGL((fp8_stream_kernel<MT, NW, D, E>), dim3((g.NT + NW - 1) / NW, (unsigned)((h.T + 16 * MT - 1) / (16 * MT))), \
+                           dim3(64 * kStreamWaves), bytes, st, g); \
+    } while (0)
+#define S1(E) ST(1, 1, 3, E)
+#define S2(E) ST(2, 2, 2, E)
+#define S3(E) ST(3, 2, 2, E)
+#define S4(E) ST(4, 2, 2, E)
+        if (p.mt == 1) EP(S1); else if (p.mt == 2) EP(S2); else if (p.mt == 3) EP(S3); else EP(S4);
+#undef S1
+#undef S2
+#undef S3
+#undef S4
+#undef ST
+    } else {
+#define TL(WM, WN, AR, NS, E, OCC) do { \
+        using S = Fp8Tile<WM, WN, AR>; \
+        const int tm = (int)((h.T + 16 * S::TA - 1) / (16 * S::TA)), tn = (g.NT + S::TW - 1) / S::TW; \
+        allow_lds(fp8_tile_kernel<WM, WN, AR, NS, E, OCC>, (size_t)S::BYTES * NS); \
+        hipLaunchKernelGGL((fp8_tile_kernel<WM, WN, AR, NS, E, OCC>), dim3((unsigned)(tm * tn * p.splits)), dim3(64 * WM * WN), \
+                           (size_t)S::BYTES * NS, st, g, tm, tn, p.splits); \
+    } while (0)
+#define T2(E) TL(2, 4, 8, 2, E, 2)
+#define T1(E) TL(2, 2, 4, 2, E, 2)
+        if (p.kind == 2) {
+            EP(T2);
+        } else if (p.splits == 1) {
+            EP(T1);
+        } else {
+            T1(2);
+            PRISM_LAUNCH_CHECK();
+            const dim3 grid((unsigned)((((g.n + 3) / 4) + 255) / 256), (unsigned)h.T);
+            if (h.epi) hipLaunchKernelGGL((fp8_join_kernel<1>), grid, dim3(256), 0, st, g, p.splits);
+            else hipLaunchKernelGGL((fp8_join_kernel<0>), grid, dim3(256), 0, st, g, p.splits);
+        }
+#undef T1
+#undef T2
+#undef TL
+    }
+#undef EP
+    PRISM_LAUNCH_CHECK();
+    return PRISM_OK;
+}

@@ -1,4 +1,4 @@
-// The host path of prism_amd.kv and prism_amd.delta: checks a call's tensors, fills the C entry's struct and calls it.  A
+// The host path of prism_amd.kv, delta, fp8 and moe: checks a call's tensors, fills the C entry's struct and calls it.  A
 // decode-size call is bound by the host, and a dozen tensors' shapes, strides, types and pointers cost Python some 10 us;
 // here they cost a few hundred ns.  A CPython extension over torch's tensors (prism_amd/_host.so); the C entries' addresses
 // come from the loaded library (bind), so nothing is linked to it.
@@ -27,7 +27,14 @@ int64_t (*g_attend_ws)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
 int (*g_step)(const prism_delta_args*, void*);
 int (*g_prefill)(const prism_delta_args*, void*);
 int64_t (*g_prefill_ws)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
+int (*g_fp8_quant)(const prism_fp8_quant_args*, void*);
+int (*g_fp8_gemm)(const prism_fp8_gemm_args*, void*);
+int64_t (*g_fp8_gemm_ws)(int64_t, int64_t, int64_t);
+int (*g_route)(const prism_moe_route_args*, void*);
+int (*g_experts)(const prism_moe_experts_args*, void*);
+int64_t (*g_experts_ws)(int64_t, int64_t, int64_t);
 PyObject* g_stream_of;                                        // tensor -> stream handle (raises off the GPU)
+PyObject* g_stream_here;                                      // the same, refusing a device that is not the current one
 PyObject* g_workspace;                                        // (tensor, bytes, stream handle) -> tensor
 
 [[noreturn]] void raise(PyObject* kind, const std::string& what) {
@@ -67,7 +74,8 @@ const at::Tensor& tensor(PyObject* o, const char* name) {
 int device(const at::Tensor& t) { return t.is_cuda() ? (int)t.get_device() : -1; }
 
 const char* type_name(at::ScalarType t) {
-    return t == at::kBFloat16 ? "bf16" : t == at::kFloat ? "fp32" : t == at::kInt ? "int32" : "of another type";
+    return t == at::kBFloat16 ? "bf16" : t == at::kFloat ? "fp32" : t == at::kInt ? "int32" :
+           t == at::kFloat8_e4m3fn ? "float8_e4m3fn" : t == at::kByte ? "uint8" : "of another type";
 }
 
 [[noreturn]] void refuse(const char* name, const at::Tensor& t, at::ScalarType type, const std::string& want, int dev) {
@@ -173,8 +181,8 @@ void cache(prism_kv_cache& c, PyObject* ko, PyObject* vo, PyObject* kso, PyObjec
 }
 
 // torch's current stream on the tensors' device; raises if that is no GPU of this library.
-void* stream_of(PyObject* like) {
-    PyObject* s = PyObject_CallFunctionObjArgs(g_stream_of, like, nullptr);
+void* stream_of(PyObject* like, bool here = false) {
+    PyObject* s = PyObject_CallFunctionObjArgs(here ? g_stream_here : g_stream_of, like, nullptr);
     if (!s) throw Raised{};
     void* p = PyLong_AsVoidPtr(s);
     Py_DECREF(s);
@@ -315,6 +323,177 @@ int do_delta(PyObject* const* a, Py_ssize_t n, bool prompts) {
     return g_prefill(&h, stream);
 }
 
+// [>= T, cols], any stride of rows.
+const at::Tensor& matrix(PyObject* o, const char* name, at::ScalarType type, int64_t T, int64_t cols, int dev, int64_t* ld) {
+    const at::Tensor& t = tensor(o, name);
+    if (t.scalar_type() != type || t.dim() != 2 || t.size(0) < T || t.size(1) != cols || (cols > 1 && t.stride(1) != 1) ||
+        device(t) != dev)
+        refuse(name, t, type, "[>= " + std::to_string(T) + ", " + std::to_string(cols) + "]", dev);
+    *ld = t.size(0) > 1 ? t.stride(0) : cols;
+    return t;
+}
+
+template <typename E>
+const E* in_matrix(PyObject* o, const char* name, at::ScalarType type, int64_t T, int64_t cols, int dev, int64_t* ld) {
+    return static_cast<const E*>(matrix(o, name, type, T, cols, dev, ld).const_data_ptr());
+}
+template <typename E>
+E* out_matrix(PyObject* o, const char* name, at::ScalarType type, int64_t T, int64_t cols, int dev, int64_t* ld) {
+    return static_cast<E*>(written(matrix(o, name, type, T, cols, dev, ld), name));
+}
+
+// [>= T, cols or (0) any number], fp32 or bf16; whether fp32.
+const void* wide_or_bf16(PyObject* o, const char* name, int64_t T, int64_t* cols, int64_t* ld, int64_t* f32) {
+    const at::Tensor& t = tensor(o, name);
+    if (t.dim() != 2) raise(PyExc_ValueError, std::string(name) + " must be [rows, columns]; got " + list(t.sizes()));
+    *f32 = t.scalar_type() == at::kFloat;
+    *cols = t.size(1);
+    return matrix(o, name, *f32 ? at::kFloat : at::kBFloat16, T, *cols, device(t), ld).const_data_ptr();
+}
+
+// An fp8.F8 (chunks, scales, n, k) of one weight (experts 0) or of so many.
+struct Weight {
+    const uint8_t* q;
+    const float* s;
+    int64_t n, k;
+};
+Weight weight(PyObject* o, const char* name, int64_t experts, int dev) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) raise(PyExc_TypeError, std::string(name) + " must be an fp8.F8");
+    const at::Tensor &q = tensor(PyTuple_GET_ITEM(o, 0), name), &s = tensor(PyTuple_GET_ITEM(o, 1), name);
+    const int64_t n = integer(PyTuple_GET_ITEM(o, 2), name), k = integer(PyTuple_GET_ITEM(o, 3), name);
+    if (q.scalar_type() != at::kByte || s.scalar_type() != at::kFloat)
+        raise(PyExc_TypeError, std::string(name) + " must hold uint8 chunks and fp32 scales (fp8.pack, fp8.from_rows)");
+    const int64_t KB = (k + 127) / 128, d = experts ? 1 : 0;
+    const bool ok = n > 0 && k > 0 && q.dim() == 3 + d && s.dim() == 2 + d && q.size(d) == (n + 15) / 16 && q.size(d + 1) == KB &&
+                    q.size(d + 2) == 2048 && s.size(d) == (n + 127) / 128 && s.size(d + 1) == KB &&
+                    (!experts || (q.size(0) == experts && s.size(0) == experts)) && q.is_contiguous() && s.is_contiguous() &&
+                    device(q) == dev && device(s) == dev;
+    if (!ok)
+        raise(PyExc_ValueError, std::string(name) + " must be " + (experts ? std::to_string(experts) + " weights" : "one weight") +
+                                    " as fp8.pack or fp8.from_rows leaves it, on the other tensors' device; got chunks " +
+                                    list(q.sizes()) + ", scales " + list(s.sizes()) + " for n " + std::to_string(n) + ", k " +
+                                    std::to_string(k));
+    return {static_cast<const uint8_t*>(q.const_data_ptr()), static_cast<const float*>(s.const_data_ptr()), n, k};
+}
+
+int64_t epilogue(PyObject* o) {
+    const int64_t e = integer(o, "epi");
+    if (e != 0 && e != 1) raise(PyExc_ValueError, "epi must be 0 (bf16) or 1 (added into fp32)");
+    return e;
+}
+
+int do_fp8_quant(PyObject* const* a, Py_ssize_t n) {
+    need_args(n, 5);
+    enum { X, Q, S, N, T };
+    prism_fp8_quant_args h{};
+    const int dev = device(tensor(a[X], "x"));
+    h.T = integer(a[T], "T");
+    wide_or_bf16(a[X], "x", h.T, &h.k, &h.x_ld, &h.f32);
+    const int64_t KB = (h.k + 127) / 128;
+    h.q = out_matrix<uint8_t>(a[Q], "q", at::kFloat8_e4m3fn, h.T, 128 * KB, dev, &h.q_ld);
+    h.s = out_matrix<float>(a[S], "s", at::kFloat, h.T, KB, dev, &h.s_ld);
+    h.x = tensor(a[X], "x").const_data_ptr();
+    h.n_rows = live(a[N], dev);
+    void* stream = stream_of(a[X], true);
+    return h.T == 0 || h.k == 0 ? 0 : g_fp8_quant(&h, stream);
+}
+
+int do_fp8_gemm(PyObject* const* a, Py_ssize_t n) {
+    need_args(n, 7);
+    enum { A, AS, W, OUT, N, T, EPI };
+    prism_fp8_gemm_args h{};
+    const int dev = device(tensor(a[A], "a_q"));
+    h.T = integer(a[T], "T");
+    h.epi = epilogue(a[EPI]);
+    const Weight w = weight(a[W], "w", 0, dev);
+    h.w = w.q, h.ws = w.s, h.n = w.n, h.k = w.k;
+    const int64_t KB = (h.k + 127) / 128;
+    h.out = out_matrix<void>(a[OUT], "out", h.epi ? at::kFloat : at::kBFloat16, h.T, h.n, dev, &h.o_ld);
+    h.a = in_matrix<uint8_t>(a[A], "a_q", at::kFloat8_e4m3fn, h.T, 128 * KB, dev, &h.a_ld);
+    h.as = in_matrix<float>(a[AS], "a_s", at::kFloat, h.T, KB, dev, &h.as_ld);
+    h.n_rows = live(a[N], dev);
+    void* stream = stream_of(a[A], true);
+    if (h.T == 0) return 0;
+    Workspace ws;
+    h.wsp_bytes = g_fp8_gemm_ws(h.T, h.n, h.k);
+    if (h.wsp_bytes) ws.get(a[A], h.wsp_bytes, stream);
+    h.wsp = ws.ptr;
+    return g_fp8_gemm(&h, stream);
+}
+
+int do_route(PyObject* const* a, Py_ssize_t n) {
+    need_args(n, 9);
+    enum { X, IDS, W, N, T, SCORE, BIAS, RENORM, SCALE };
+    prism_moe_route_args h{};
+    const int dev = device(tensor(a[X], "logits"));
+    h.T = integer(a[T], "T");
+    wide_or_bf16(a[X], "logits", h.T, &h.E, &h.x_ld, &h.f32);
+    const at::Tensor& ids = tensor(a[IDS], "ids");
+    if (ids.dim() != 2) raise(PyExc_ValueError, "ids must be [rows, experts per token]; got " + list(ids.sizes()));
+    h.top = ids.size(1);
+    h.ids = out_matrix<int32_t>(a[IDS], "ids", at::kInt, h.T, h.top, dev, &h.ids_ld);
+    h.w = out_matrix<float>(a[W], "weights", at::kFloat, h.T, h.top, dev, &h.w_ld);
+    h.x = tensor(a[X], "logits").const_data_ptr();
+    if (h.E < 1 || h.E > 1024) raise(PyExc_ValueError, "route: 1 to 1024 experts");
+    if (h.top < 1 || h.top > 16 || h.top > h.E) raise(PyExc_ValueError, "route: 1 to 16 experts per token, no more than there are");
+    const char* score = PyUnicode_Check(a[SCORE]) ? PyUnicode_AsUTF8(a[SCORE]) : nullptr;
+    if (!score) PyErr_Clear();
+    h.sigmoid = score && std::string(score) == "sigmoid";
+    if (!h.sigmoid && !(score && std::string(score) == "softmax"))
+        raise(PyExc_ValueError, "route: score must be \"softmax\" or \"sigmoid\"");
+    if (a[BIAS] != Py_None) {
+        const at::Tensor& b = tensor(a[BIAS], "bias");
+        if (!h.sigmoid) raise(PyExc_ValueError, "route: a bias goes with score=\"sigmoid\"");
+        if (b.scalar_type() != at::kFloat || b.dim() != 1 || b.size(0) != h.E || (h.E > 1 && b.stride(0) != 1) || device(b) != dev)
+            refuse("bias", b, at::kFloat, "[" + std::to_string(h.E) + "]", dev);
+        h.bias = static_cast<const float*>(b.const_data_ptr());
+    }
+    const int renorm = PyObject_IsTrue(a[RENORM]);
+    if (renorm < 0) throw Raised{};
+    h.renorm = renorm;
+    h.scale = number(a[SCALE], "scale");
+    h.n_rows = live(a[N], dev);
+    void* stream = stream_of(a[X], true);
+    return h.T == 0 ? 0 : g_route(&h, stream);
+}
+
+int do_experts(PyObject* const* a, Py_ssize_t n) {
+    need_args(n, 10);
+    enum { X, IDS, WT, GATE, UP, DOWN, OUT, N, T, EPI };
+    prism_moe_experts_args h{};
+    const int dev = device(tensor(a[X], "x"));
+    h.T = integer(a[T], "T");
+    h.epi = epilogue(a[EPI]);
+    const at::Tensor& ids = tensor(a[IDS], "ids");
+    if (ids.dim() != 2) raise(PyExc_ValueError, "ids must be [rows, experts per token]; got " + list(ids.sizes()));
+    h.top = ids.size(1);
+    if (h.top < 1 || h.top > 16) raise(PyExc_ValueError, "experts: 1 to 16 experts per token");
+    if (!PyTuple_Check(a[GATE]) || PyTuple_GET_SIZE(a[GATE]) != 4) raise(PyExc_TypeError, "gate must be an fp8.F8");
+    const at::Tensor& gq = tensor(PyTuple_GET_ITEM(a[GATE], 0), "gate");
+    h.E = gq.dim() == 4 ? gq.size(0) : 0;
+    if (h.E < 1) raise(PyExc_ValueError, "gate must hold the weights of every expert: chunks [experts, ...]");
+    const Weight g = weight(a[GATE], "gate", h.E, dev), u = weight(a[UP], "up", h.E, dev), d = weight(a[DOWN], "down", h.E, dev);
+    h.I = g.n, h.H = g.k;
+    if (u.n != h.I || u.k != h.H || d.n != h.H || d.k != h.I)
+        raise(PyExc_ValueError, "experts: gate and up must be [I, H] weights, down [H, I]; got gate [" + std::to_string(g.n) + ", " +
+                                    std::to_string(g.k) + "], up [" + std::to_string(u.n) + ", " + std::to_string(u.k) +
+                                    "], down [" + std::to_string(d.n) + ", " + std::to_string(d.k) + "]");
+    if (h.H % 16 || h.I % 16) raise(PyExc_ValueError, "experts: H and I must be multiples of 16");
+    h.gate = g.q, h.gate_s = g.s, h.up = u.q, h.up_s = u.s, h.down = d.q, h.down_s = d.s;
+    h.out = out_matrix<void>(a[OUT], "out", h.epi ? at::kFloat : at::kBFloat16, h.T, h.H, dev, &h.o_ld);
+    h.x = in_matrix<uint16_t>(a[X], "x", at::kBFloat16, h.T, h.H, dev, &h.x_ld);
+    h.ids = in_matrix<int32_t>(a[IDS], "ids", at::kInt, h.T, h.top, dev, &h.ids_ld);
+    h.w = in_matrix<float>(a[WT], "weights", at::kFloat, h.T, h.top, dev, &h.w_ld);
+    h.n_rows = live(a[N], dev);
+    void* stream = stream_of(a[X], true);
+    if (h.T == 0) return 0;
+    Workspace ws;
+    h.wsp_bytes = g_experts_ws(h.T, h.top, h.I);
+    ws.get(a[X], h.wsp_bytes, stream);
+    h.wsp = ws.ptr;
+    return g_experts(&h, stream);
+}
+
 template <typename F>
 PyObject* guarded(F&& f) {
     try {
@@ -333,12 +512,17 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarde
 PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return do_delta(a, n, false); }); }
 PyObject* py_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return do_delta(a, n, true); }); }
 
-// bind(addresses of the six C entries, stream_of, workspace)
+PyObject* py_fp8_quant(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return do_fp8_quant(a, n); }); }
+PyObject* py_fp8_gemm(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return do_fp8_gemm(a, n); }); }
+PyObject* py_route(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return do_route(a, n); }); }
+PyObject* py_experts(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded([&] { return do_experts(a, n); }); }
+
+// bind(addresses of the twelve C entries, stream_of, stream_here, workspace)
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&] {
-        need_args(n, 8);
-        void* p[6];
-        for (int i = 0; i < 6; i++) {
+        need_args(n, 15);
+        void* p[12];
+        for (int i = 0; i < 12; i++) {
             p[i] = PyLong_AsVoidPtr(a[i]);
             if (!p[i]) raise(PyExc_ValueError, "bind: an address is missing");
         }
@@ -348,11 +532,17 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
         g_step = reinterpret_cast<decltype(g_step)>(p[3]);
         g_prefill = reinterpret_cast<decltype(g_prefill)>(p[4]);
         g_prefill_ws = reinterpret_cast<decltype(g_prefill_ws)>(p[5]);
-        Py_INCREF(a[6]);
-        Py_INCREF(a[7]);
+        g_fp8_quant = reinterpret_cast<decltype(g_fp8_quant)>(p[6]);
+        g_fp8_gemm = reinterpret_cast<decltype(g_fp8_gemm)>(p[7]);
+        g_fp8_gemm_ws = reinterpret_cast<decltype(g_fp8_gemm_ws)>(p[8]);
+        g_route = reinterpret_cast<decltype(g_route)>(p[9]);
+        g_experts = reinterpret_cast<decltype(g_experts)>(p[10]);
+        g_experts_ws = reinterpret_cast<decltype(g_experts_ws)>(p[11]);
+        for (int i = 12; i < 15; i++) Py_INCREF(a[i]);
         Py_XDECREF(g_stream_of);
+        Py_XDECREF(g_stream_here);
         Py_XDECREF(g_workspace);
-        g_stream_of = a[6], g_workspace = a[7];
+        g_stream_of = a[12], g_stream_here = a[13], g_workspace = a[14];
         return 0;
     });
 }
@@ -363,10 +553,14 @@ PyMethodDef methods[] = {
     FAST("kv_attend", py_attend, "prism_kv_attend after checks; see prism_amd.kv.attend"),
     FAST("delta_step", py_step, "prism_delta_step after checks; see prism_amd.delta.step"),
     FAST("delta_prefill", py_prefill, "prism_delta_prefill after checks; see prism_amd.delta.prefill"),
-    FAST("bind", py_bind, "addresses of the C entries, then stream_of and workspace"),
+    FAST("fp8_quant", py_fp8_quant, "prism_fp8_quant after checks; see prism_amd.fp8.quantize_act"),
+    FAST("fp8_gemm", py_fp8_gemm, "prism_fp8_gemm after checks; see prism_amd.fp8.gemm"),
+    FAST("moe_route", py_route, "prism_moe_route after checks; see prism_amd.moe.route"),
+    FAST("moe_experts", py_experts, "prism_moe_experts after checks; see prism_amd.moe.experts"),
+    FAST("bind", py_bind, "addresses of the C entries, then stream_of, stream_here and workspace"),
     {nullptr, nullptr, 0, nullptr},
 };
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of prism_amd.kv and prism_amd.delta.", -1, methods,
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of prism_amd.kv, delta, fp8 and moe.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -62,6 +62,13 @@ _SIGS = {
     "prism_delta_step": (_int, [_args, _p]),
     "prism_delta_prefill": (_int, [_args, _p]),
     "prism_delta_prefill_workspace_bytes": (_i64, [_i64] * 6),
+    "prism_fp8_pack": (_int, [_p, _int, _i64, _p, _p, _i64, _i64, _p]),
+    "prism_fp8_quant": (_int, [_args, _p]),
+    "prism_fp8_gemm": (_int, [_args, _p]),
+    "prism_fp8_gemm_workspace_bytes": (_i64, [_i64] * 3),
+    "prism_moe_route": (_int, [_args, _p]),
+    "prism_moe_experts": (_int, [_args, _p]),
+    "prism_moe_experts_workspace_bytes": (_i64, [_i64] * 3),
 }
 
 _lib = None
@@ -93,7 +100,7 @@ _host = None
 
 
 def host():
-    """The host extension (csrc/host.cpp: the checked calls of kv and delta), bound to the loaded library's entries; raises
+    """The host extension (csrc/host.cpp: the checked calls of kv, delta, fp8 and moe), bound to the loaded library's entries; raises
     if it was not built."""
     global _host
     if _host is None:
@@ -112,7 +119,9 @@ def host():
             return torch.empty(need, dtype=torch.uint8, device=like.device) if t is None else t
         h.bind(*(ctypes.cast(getattr(lib(), n), ctypes.c_void_p).value for n in (
             "prism_kv_append", "prism_kv_attend", "prism_kv_attend_workspace_bytes", "prism_delta_step",
-            "prism_delta_prefill", "prism_delta_prefill_workspace_bytes")), stream_of, workspace)
+            "prism_delta_prefill", "prism_delta_prefill_workspace_bytes", "prism_fp8_quant", "prism_fp8_gemm",
+            "prism_fp8_gemm_workspace_bytes", "prism_moe_route", "prism_moe_experts", "prism_moe_experts_workspace_bytes")),
+            stream_of, stream_here, workspace)
         _host = h
     return _host
 
@@ -145,6 +154,15 @@ def stream_of(t):
     if t.is_cuda and dev.index in _checked:
         return raw_stream(dev.index)
     return raw_stream(_check_device(dev))
+
+
+def stream_here(t):
+    """The same, for a tensor of the current device only: a launch goes to the current device's queues."""
+    s = stream_of(t)
+    if t.device.index != torch.cuda.current_device():
+        raise PrismError(f"the tensors are on device {t.device.index}, the current device is {torch.cuda.current_device()}: "
+                         "call under torch.cuda.device(...)")
+    return s
 
 
 def ptr(t):
