@@ -604,7 +604,7 @@ typedef struct {
     int64_t wsp_bytes;
 } prism_moe_experts_args;
 PRISM_API int prism_moe_experts(const prism_moe_experts_args* args, void* stream);
-PRISM_API int64_t prism_moe_experts_workspace_bytes(int64_t T, int64_t top, int64_t I);
+PRISM_API int64_t prism_moe_experts_workspace_bytes(int64_t T, int64_t top, int64_t H, int64_t I);
 
 /*
  * Peak probes (measurement tooling: the reference's bench/csrc/mma_peak.cu:14-70 and bench/csrc/l2_bw.cu:8 for

@@ -186,7 +186,8 @@ __device__ __forceinline__ void store4(const Fp8Gemm& g, int m, int j, v4f y) {
 
 // Few rows (up to 16 MT): a workgroup owns NW2 16-row weight tiles, its 8 waves take the blocks of 128 inputs in turn (wave w
 // block w, w + 8, ...) straight from memory into registers, D blocks ahead, and add their sums through LDS, wave after wave.
-// Blocks past the end and rows past the live ones read as zeros (the buffers' range), so the loop has no branches.
+// Rows past the live ones read as zeros (the buffer's range), blocks past the last as the last against zeros, so the loop has
+// no branches.
 constexpr int kStreamWaves = 8;
 template <int MT, int NW2, int D, int EPI>
 __global__ __launch_bounds__(64 * kStreamWaves) void fp8_stream_kernel(Fp8Gemm g) {
@@ -196,13 +197,13 @@ __global__ __launch_bounds__(64 * kStreamWaves) void fp8_stream_kernel(Fp8Gemm g
     const int t0 = blockIdx.x * NW2, m0 = blockIdx.y * 16 * MT;
     const int live = min(g.T, __ldg(g.n_rows)) - m0;
     if (live <= 0) return;
-    const int tiles = min(NW2, g.NT - t0), KB = g.KB;
+    const int tiles = g.NT - t0, KB = g.KB;
     const uint32_t tile = (uint32_t)KB * 2048;
-    const __amdgpu_buffer_rsrc_t wr = buf_rsrc_n(g.w + (int64_t)t0 * tile, tiles * tile);
+    const __amdgpu_buffer_rsrc_t wr = buf_rsrc(g.w + (int64_t)t0 * tile);
     const uint32_t rows = min(live, 16 * MT);
     const __amdgpu_buffer_rsrc_t ar = buf_rsrc_n(g.a + m0 * g.a_ld, (uint32_t)((rows - 1) * g.a_ld + KB * 128));
     const __amdgpu_buffer_rsrc_t sr = buf_rsrc_n(g.as + m0 * g.as_ld, (uint32_t)((rows - 1) * g.as_ld + KB) * 4);
-    const float* ws = g.ws + (int64_t)(t0 / 8) * KB;             // (NW2 tiles lie in one block of 128 rows)
+    const __amdgpu_buffer_rsrc_t br = buf_rsrc(g.ws + (int64_t)(t0 / 8) * KB);   // (NW2 tiles lie in one block of 128 rows)
     constexpr uint32_t kOut = 0x80000000u;
     uint32_t aoff[MT], soff[MT];
 #pragma unroll
@@ -213,19 +214,20 @@ __global__ __launch_bounds__(64 * kStreamWaves) void fp8_stream_kernel(Fp8Gemm g
     }
     struct Stage {
         v4i w[NW2][2], a[MT][2];
-        float s[MT];
+        float s[MT], sw;
     } st[D];
     auto issue = [&](Stage& x, int b) {
-        const uint32_t out = b < KB ? 0u : kOut;                  // (wave-uniform)
+        const uint32_t bc = min(b, KB - 1), out = b < KB ? 0u : kOut;                  // (wave-uniform)
+        x.sw = __uint_as_float(buf_load4(br, 0, bc * 4));
 #pragma unroll
         for (int t = 0; t < NW2; t++)
 #pragma unroll
-            for (int p = 0; p < 2; p++) x.w[t][p] = buf_load16<kBufNT>(wr, (lane * 16 + p * 1024 + t * tile + b * 2048u) | out, 0);
+            for (int p = 0; p < 2; p++) x.w[t][p] = buf_load16<kBufNT>(wr, lane * 16 + p * 1024, min(t, tiles - 1) * tile + bc * 2048);
 #pragma unroll
         for (int c = 0; c < MT; c++) {
 #pragma unroll
-            for (int p = 0; p < 2; p++) x.a[c][p] = buf_load16(ar, (aoff[c] + 64 * p + b * 128u) | out, 0);
-            x.s[c] = __uint_as_float(buf_load4(sr, (soff[c] + b * 4u) | out, 0));
+            for (int p = 0; p < 2; p++) x.a[c][p] = buf_load16(ar, (aoff[c] | out) + 64 * p, bc * 128);
+            x.s[c] = __uint_as_float(buf_load4(sr, soff[c], bc * 4));
         }
     };
     v4f acc[NW2][MT];
@@ -239,11 +241,10 @@ __global__ __launch_bounds__(64 * kStreamWaves) void fp8_stream_kernel(Fp8Gemm g
 #pragma unroll
         for (int d = 0; d < D; d++) {
             const int at = b + d * kStreamWaves;
-            const float sw = ws[min(at, KB - 1)];
 #pragma unroll
             for (int c = 0; c < MT; c++) {
                 const v8i a = join8(st[d].a[c][0], st[d].a[c][1]);
-                const float s = mul_rn(st[d].s[c], sw);
+                const float s = mul_rn(st[d].s[c], st[d].sw);
 #pragma unroll
                 for (int t = 0; t < NW2; t++)
                     acc[t][c] = fold(fp8_mfma(join8(st[d].w[t][0], st[d].w[t][1]), a), s, acc[t][c]);
@@ -328,6 +329,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8Gemm g, 
 #pragma unroll
         for (int c = 0; c < AR; c++) acc[a][c] = v4f{0.f, 0.f, 0.f, 0.f};
     const int nb = b1 - b0;
+    float sw_next = ws[0];
 #pragma unroll
     for (int i = 0; i < NS - 1; i++)
         if (i < nb) issue(i, i);
@@ -341,7 +343,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void fp8_tile_kernel(Fp8Gemm g, 
         lds_barrier();
         if (b + NS - 1 < nb) issue(b + NS - 1, (b + NS - 1) % NS);
         const uint8_t* l = lds + (b % NS) * S::BYTES;
-        const float sw = ws[b];
+        const float sw = sw_next;
+        sw_next = ws[min(b + 1, nb - 1)];
         v8i wf[4];
 #pragma unroll
         for (int a = 0; a < 4; a++) {

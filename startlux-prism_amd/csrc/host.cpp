@@ -32,7 +32,7 @@ int (*g_fp8_gemm)(const prism_fp8_gemm_args*, void*);
 int64_t (*g_fp8_gemm_ws)(int64_t, int64_t, int64_t);
 int (*g_route)(const prism_moe_route_args*, void*);
 int (*g_experts)(const prism_moe_experts_args*, void*);
-int64_t (*g_experts_ws)(int64_t, int64_t, int64_t);
+int64_t (*g_experts_ws)(int64_t, int64_t, int64_t, int64_t);
 PyObject* g_stream_of;                                        // tensor -> stream handle (raises off the GPU)
 PyObject* g_stream_here;                                      // the same, refusing a device that is not the current one
 PyObject* g_workspace;                                        // (tensor, bytes, stream handle) -> tensor
@@ -488,7 +488,7 @@ int do_experts(PyObject* const* a, Py_ssize_t n) {
     void* stream = stream_of(a[X], true);
     if (h.T == 0) return 0;
     Workspace ws;
-    h.wsp_bytes = g_experts_ws(h.T, h.top, h.I);
+    h.wsp_bytes = g_experts_ws(h.T, h.top, h.H, h.I);
     ws.get(a[X], h.wsp_bytes, stream);
     h.wsp = ws.ptr;
     return g_experts(&h, stream);

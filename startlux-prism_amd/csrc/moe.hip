@@ -5,24 +5,22 @@
 //   experts   out[t] = sum_j w[t][j] down_e (silu(gate_e x_t) * (up_e x_t)),  e = ids[t][j]
 //
 // For a few tokens the experts' weights, read once, are the work: a chunk (16 rows x 128 inputs, 2 KB) is loaded straight
-// into registers, its codes become bf16 (exact) two at a time, and v_mfma_f32_16x16x32_bf16 multiplies them with up to 16
-// tokens' columns, four products per chunk chained from zero, then one fma by the block's scale into the fp32 sum.  Which
-// pairs (token, place) an expert has is found by every wave from the ids with ballots: no sorting launch, and the order of
-// all sums follows from the ids alone.
+// into registers, several ahead, its codes become bf16 (exact) two at a time, and v_mfma_f32_16x16x32_bf16 multiplies them
+// with up to 16 tokens' columns, four products per chunk chained from zero, then one fma by the block's scale into the fp32
+// sum.  Which pairs (token, place) an expert has is found by every workgroup from the ids with ballots: no sorting launch.
 //
-// Two launches.  moe_up_kernel: a workgroup per (expert, 16 hidden rows), its waves splitting the inputs; it leaves the hidden
-// values h = silu(g) u of each pair in the workspace as two bf16 parts (h = hi + lo up to 2^-17 of it: the second product's
-// operand; one part alone would add as much error as the bf16 output's own rounding).  moe_down_kernel: a workgroup per 16
-// outputs of all tokens, its waves taking the experts in turn, each with its own sums of every token in LDS, which are added
-// wave after wave at the end: no atomics, no third launch.
+// Three launches per 128 tokens.  moe_up_kernel leaves the hidden values h = silu(g) u of each pair in the workspace as two
+// bf16 parts (h = hi + lo up to 2^-17 of it: the second product's operand; one part alone would add as much error as the bf16
+// output's own rounding), moe_down_kernel each pair's outputs in fp32, moe_sum_kernel adds a token's in the order of its ids:
+// no atomics, and what a token gets does not depend on the others but for how K is split.
 #include "common.h"
 #include "fp8.h"
 
 namespace prism {
 
-constexpr int kMoeTokens = 128;              // tokens per pass of the experts (their sums lie in LDS)
+constexpr int kMoeTokens = 128;              // tokens per pass of the experts
 constexpr int kMoeTop = 16;
-constexpr int kUpWaves = 4, kDownWaves = 8;
+constexpr int kWaves = 4;
 
 // --------------------------------------------------------------------------------------------------------------- route
 // An order-preserving integer of a number that may be chosen (greater than 0); 0 for NaN and -inf.
@@ -150,25 +148,24 @@ struct ExpertArgs {
     const uint8_t *gate, *up, *down;
     const float *gate_s, *up_s, *down_s;
     uint16_t* h;                             // [pairs][2][128 KBI] bf16: the hidden values' parts
+    float* y;                                // [pairs][H] fp32: the pairs' outputs
     void* out;
     int64_t o_ld;
     const int32_t* n_rows;
     int T, E, top, H, I, KBH, KBI;
     uint32_t div;                            // pair -> token: (pair div) >> 16 (pairs < 2048, top <= 16)
+    int first, room;                         // the pass's tokens: room from first on
     int slots;                               // experts looked at per pass: all, or one per pair where those are fewer
     int vec;
 };
 
-// The pass's tokens [first, first + tokens) and its pairs.
-__device__ __forceinline__ int pass_pairs(const ExpertArgs& a, int first, int& tokens) {
-    tokens = min(min(a.T, __ldg(a.n_rows)) - first, kMoeTokens);
-    return tokens * a.top;
-}
+// The pass's live tokens (0 or less: none).
+__device__ __forceinline__ int pass_tokens(const ExpertArgs& a) { return min(min(a.T, __ldg(a.n_rows)) - a.first, a.room); }
 __device__ __forceinline__ int token_of(const ExpertArgs& a, int pair) { return (int)((uint32_t)pair * a.div >> 16); }
 
-__device__ __forceinline__ int id_of(const ExpertArgs& a, int first, int pair, int pairs) {
-    if (pair >= pairs) return -1;
-    const int t = token_of(a, pair), e = a.ids[(first + t) * a.ids_ld + (pair - t * a.top)];
+// The expert of a pair of the pass; -1: none.
+__device__ __forceinline__ int id_of(const ExpertArgs& a, int pair) {
+    const int t = token_of(a, pair), e = a.ids[(a.first + t) * a.ids_ld + (pair - t * a.top)];
     return (uint32_t)e < (uint32_t)a.E ? e : -1;
 }
 
@@ -197,18 +194,30 @@ __device__ __forceinline__ v4f scaled(v4f t, float s, v4f acc) {
 
 constexpr uint32_t kOut = 0x80000000u;       // an offset past every buffer's range: reads as zeros
 
-// A wave's expert of this slot and its pairs in `list`, in order; the number of pairs (0: none, or an earlier slot's).
-// ids(i): the expert of pair i (-1: none).  by_pair: the slots are pairs, and a pair whose expert an earlier one has is none.
-template <typename F>
-__device__ __forceinline__ int pairs_of(F&& ids, int slot, bool by_pair, int pairs, int lane, uint16_t* list, int& e) {
+// This slot's expert e and its pairs, in order, in `list` (the workgroup's LDS: [pairs] entries, then [pairs] for the ids);
+// the number of pairs, the same in every wave: 0 for an expert without any, for a pair without an expert (slots are pairs
+// where those are fewer than the experts) and for one whose expert an earlier pair has.  Every wave writes the same list.
+__device__ __forceinline__ int pairs_of(const ExpertArgs& a, int slot, int pairs, int lane, uint16_t* list, int& e) {
+    const bool by_pair = a.slots < a.E;
+    if (by_pair && slot >= pairs) return 0;
     e = slot;
-    if (by_pair) {
-        e = __builtin_amdgcn_readfirstlane(ids(slot));
+    if (pairs <= 64) {
+        const int id = lane < pairs ? id_of(a, lane) : -1;
+        if (by_pair) e = __builtin_amdgcn_readlane(id, slot);
         if (e < 0) return 0;
+        const uint64_t m = __ballot(id == e);
+        if (m == 0 || (by_pair && __builtin_ctzll(m) != slot)) return 0;
+        if (id == e) list[__popcll(m & ((1ull << lane) - 1))] = (uint16_t)lane;
+        return __popcll(m);
     }
+    int16_t* ids = reinterpret_cast<int16_t*>(list) + a.room * a.top;
+    for (int i = threadIdx.x; i < pairs; i += 64 * kWaves) ids[i] = (int16_t)id_of(a, i);
+    __syncthreads();
+    if (by_pair) e = __builtin_amdgcn_readfirstlane((int)ids[slot]);
+    if (e < 0) return 0;
     int n = 0;
     for (int at = 0; at < pairs; at += 64) {
-        const bool mine = at + lane < pairs && ids(at + lane) == e;
+        const bool mine = at + lane < pairs && ids[at + lane] == e;
         const uint64_t m = __ballot(mine);
         if (by_pair && n == 0 && m && at + __builtin_ctzll(m) != slot) return 0;
         if (mine) list[n + __popcll(m & ((1ull << lane) - 1))] = (uint16_t)(at + lane);
@@ -217,195 +226,249 @@ __device__ __forceinline__ int pairs_of(F&& ids, int slot, bool by_pair, int pai
     return n;
 }
 
-constexpr int kUpDepth = 4;
-__global__ __launch_bounds__(64 * kUpWaves) void moe_up_kernel(ExpertArgs a) {
+// A workgroup: 4 / KS times N 16-row tiles of the hidden values of one expert; KS waves split the inputs of a tile (wave part
+// q: chunks q, q + KS, ...), each D chunks ahead.
+template <int N, int KS, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void moe_up_kernel(ExpertArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    v4f* red = reinterpret_cast<v4f*>(lds);                                   // [waves][2][64]
+    v4f* red = reinterpret_cast<v4f*>(lds);                                   // [waves][N][2][64] where K is split
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 15, g = lane >> 4;
-    const int first = blockIdx.z * kMoeTokens, tile = blockIdx.x, slot = blockIdx.y;
-    int tokens;
-    const int pairs = pass_pairs(a, first, tokens);
-    const bool by_pair = a.slots < a.E;
-    if (tokens <= 0 || (by_pair && slot >= pairs)) return;
-    uint16_t* list = reinterpret_cast<uint16_t*>(lds + kUpWaves * 2048) + w * kMoeTokens * a.top;
+    const int r = lane & 15, g = lane >> 4, q = w % KS;
+    const int tokens = pass_tokens(a), pairs = tokens * a.top;
+    if (tokens <= 0) return;
+    uint16_t* list = reinterpret_cast<uint16_t*>(lds + (KS > 1 ? kWaves * N * 2048 : 0));
     int e;
-    const int n = pairs_of([&](int i) { return id_of(a, first, i, pairs); }, slot, by_pair, pairs, lane, list, e);
-    if (n == 0) return;                                                       // (the same in all waves)
+    const int n = pairs_of(a, blockIdx.y, pairs, lane, list, e);
+    if (n == 0) return;
 
+    // (tiles past the last are the last once more, chunks past the last the last against zero inputs)
+    const int tiles = a.I / 16, t0 = (blockIdx.x * (kWaves / KS) + w / KS) * N, have = tiles - t0, tc = min(t0, tiles - 1);
     const uint32_t row = (uint32_t)a.KBH * 2048;                              // bytes of a 16-row tile
-    const int64_t at = ((int64_t)e * (a.I / 16) + tile) * row;
-    const __amdgpu_buffer_rsrc_t gr = buf_rsrc_n(a.gate + at, row), ur = buf_rsrc_n(a.up + at, row);
-    const int64_t sat = ((int64_t)e * ((a.I + 127) / 128) + tile / 8) * a.KBH;
-    const float *gs = a.gate_s + sat, *us = a.up_s + sat;
-    const __amdgpu_buffer_rsrc_t xr = buf_rsrc_n(a.x + first * a.x_ld, (uint32_t)((tokens - 1) * a.x_ld + a.H) * 2);
+    const int64_t at = ((int64_t)e * tiles + tc) * row;
+    const __amdgpu_buffer_rsrc_t gr = buf_rsrc(a.gate + at), ur = buf_rsrc(a.up + at);
+    const int64_t sat = ((int64_t)e * ((a.I + 127) / 128) + tc / 8) * a.KBH;
+    const __amdgpu_buffer_rsrc_t gsr = buf_rsrc(a.gate_s + sat), usr = buf_rsrc(a.up_s + sat);
+    const __amdgpu_buffer_rsrc_t xr = buf_rsrc_n(a.x + a.first * a.x_ld, (uint32_t)((tokens - 1) * a.x_ld + a.H) * 2);
     struct Stage {
-        v4i g[2], u[2], x[4];
-    } st[kUpDepth];
+        v4i g[N][2], u[N][2], x[4];
+        float gs, us;
+    } st[D];
     for (int base = 0; base < n; base += 16) {
         const bool there = base + r < n;
         const int pair = there ? list[base + r] : 0;
         const uint32_t xo = there ? (uint32_t)(token_of(a, pair) * a.x_ld + 16 * g) * 2 : kOut;
         auto issue = [&](Stage& s, int b) {
-            const uint32_t past = b < a.KBH ? 0u : kOut;
+            const uint32_t bc = min(b, a.KBH - 1);
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
-                s.g[p] = buf_load16<kBufNT>(gr, (b * 2048u + p * 1024 + lane * 16) | past, 0);
-                s.u[p] = buf_load16<kBufNT>(ur, (b * 2048u + p * 1024 + lane * 16) | past, 0);
-                const uint32_t o = (xo + b * 256u + p * 128) | past | (b * 128 + p * 64 + 16 * g < a.H ? 0u : kOut);
-                s.x[2 * p] = buf_load16(xr, o, 0);
-                s.x[2 * p + 1] = buf_load16(xr, o + 16, 0);
-            }
-        };
-        v4f ga = {0.f, 0.f, 0.f, 0.f}, ua = ga;
-#pragma unroll
-        for (int d = 0; d < kUpDepth; d++) issue(st[d], w + d * kUpWaves);
-        for (int b = w; b < a.KBH; b += kUpDepth * kUpWaves) {
-#pragma unroll
-            for (int d = 0; d < kUpDepth; d++) {
-                const int kb = b + d * kUpWaves, kc = min(kb, a.KBH - 1);
-                v4f tg = {0.f, 0.f, 0.f, 0.f}, tu = tg;
+            for (int i = 0; i < N; i++)
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
-                    v8bf lo, hi;
-                    widen(st[d].g[p], lo, hi);
-                    tg = bf_mfma(hi, st[d].x[2 * p + 1], bf_mfma(lo, st[d].x[2 * p], tg));
-                    widen(st[d].u[p], lo, hi);
-                    tu = bf_mfma(hi, st[d].x[2 * p + 1], bf_mfma(lo, st[d].x[2 * p], tu));
+                    const uint32_t at = min(i, max(have, 1) - 1) * row + bc * 2048;
+                    s.g[i][p] = buf_load16<kBufNT>(gr, lane * 16 + p * 1024, at);
+                    s.u[i][p] = buf_load16<kBufNT>(ur, lane * 16 + p * 1024, at);
                 }
-                ga = scaled(tg, gs[kc], ga);
-                ua = scaled(tu, us[kc], ua);
-                issue(st[d], kb + kUpDepth * kUpWaves);
+            s.gs = __uint_as_float(buf_load4(gsr, 0, bc * 4));
+            s.us = __uint_as_float(buf_load4(usr, 0, bc * 4));
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const uint32_t o = b * 128 + p * 64 + 16 * g < a.H ? xo : kOut;
+                s.x[2 * p] = buf_load16(xr, o + p * 128, bc * 256);
+                s.x[2 * p + 1] = buf_load16(xr, o + p * 128 + 16, bc * 256);
+            }
+        };
+        v4f ga[N], ua[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) ga[i] = ua[i] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < D; d++) issue(st[d], q + d * KS);
+        for (int b = q; b < a.KBH; b += D * KS) {
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    v4f tg = {0.f, 0.f, 0.f, 0.f}, tu = tg;
+#pragma unroll
+                    for (int p = 0; p < 2; p++) {
+                        v8bf lo, hi;
+                        widen(st[d].g[i][p], lo, hi);
+                        tg = bf_mfma(hi, st[d].x[2 * p + 1], bf_mfma(lo, st[d].x[2 * p], tg));
+                        widen(st[d].u[i][p], lo, hi);
+                        tu = bf_mfma(hi, st[d].x[2 * p + 1], bf_mfma(lo, st[d].x[2 * p], tu));
+                    }
+                    ga[i] = scaled(tg, st[d].gs, ga[i]);
+                    ua[i] = scaled(tu, st[d].us, ua[i]);
+                }
+                issue(st[d], b + (d + D) * KS);
             }
         }
-        if (base) __syncthreads();                                            // (the sums before are read)
-        red[(w * 2) * 64 + lane] = ga;
-        red[(w * 2 + 1) * 64 + lane] = ua;
-        __syncthreads();
-        if (w == 0 && there) {
-            for (int i = 1; i < kUpWaves; i++) {
-                const v4f y = red[(i * 2) * 64 + lane], z = red[(i * 2 + 1) * 64 + lane];
+        if (KS > 1) {
+            if (base) __syncthreads();                                        // (the sums before are read)
 #pragma unroll
-                for (int j = 0; j < 4; j++) ga[j] = add_rn(ga[j], y[j]), ua[j] = add_rn(ua[j], z[j]);
+            for (int i = 0; i < N; i++) {
+                red[((w * N + i) * 2) * 64 + lane] = ga[i];
+                red[((w * N + i) * 2 + 1) * 64 + lane] = ua[i];
+            }
+            __syncthreads();
+        }
+        // (of the KS waves of a tile, wave part i finishes tile i, i + KS, ...)
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (i % KS != q || i >= have || !there) continue;
+            v4f gv = ga[i], uv = ua[i];
+            if (KS > 1) {
+                const int w0 = w - q;
+#pragma unroll
+                for (int j = 0; j < KS; j++) {
+                    const v4f y = red[(((w0 + j) * N + i) * 2) * 64 + lane], z = red[(((w0 + j) * N + i) * 2 + 1) * 64 + lane];
+                    if (j == 0) {
+                        gv = y, uv = z;
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) gv[k] = add_rn(gv[k], y[k]), uv[k] = add_rn(uv[k], z[k]);
+                    }
+                }
             }
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float h = mul_rn(div_rn(ga[j], add_rn(1.f, expf(-ga[j]))), ua[j]);
+                const float h = mul_rn(div_rn(gv[j], add_rn(1.f, expf(-gv[j]))), uv[j]);
                 hi[j] = f32_to_bf16(h);
                 const float rest = h - bf16_to_f32(hi[j]);
                 lo[j] = (hi[j] & 0x7f80u) == 0x7f80u ? 0u : f32_to_bf16(rest);
             }
-            uint16_t* o = a.h + ((int64_t)first * a.top + pair) * 2 * a.KBI * 128 + 16 * tile + 4 * g;
+            uint16_t* o = a.h + (int64_t)pair * 2 * a.KBI * 128 + 16 * (t0 + i) + 4 * g;
             *reinterpret_cast<v2u*>(o) = v2u{hi[0] | hi[1] << 16, hi[2] | hi[3] << 16};
             *reinterpret_cast<v2u*>(o + a.KBI * 128) = v2u{lo[0] | lo[1] << 16, lo[2] | lo[3] << 16};
         }
     }
 }
 
-constexpr int kDownDepth = 4;
-template <int EPI>
-__global__ __launch_bounds__(64 * kDownWaves) void moe_down_kernel(ExpertArgs a, int parts) {
+// The same for the outputs of one expert: N tiles share a chunk's hidden values.
+template <int N, int KS, int D>
+__global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    v4f* red = reinterpret_cast<v4f*>(lds);                                   // [waves][N][64] where K is split
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = lane & 15, g = lane >> 4;
-    const int first = blockIdx.y * kMoeTokens, tile = blockIdx.x;
-    int tokens;
-    const int pairs = pass_pairs(a, first, tokens);
+    const int r = lane & 15, g = lane >> 4, q = w % KS;
+    const int tokens = pass_tokens(a), pairs = tokens * a.top;
     if (tokens <= 0) return;
-    const int room = min(a.T, kMoeTokens);                                    // as the host sized LDS
-    v4f* sums = reinterpret_cast<v4f*>(lds) + w * room * 4;                   // [tokens][16 outputs], one per wave
-    int16_t* ids = reinterpret_cast<int16_t*>(lds + kDownWaves * room * 64);
-    uint16_t* list = reinterpret_cast<uint16_t*>(ids) + room * a.top * (1 + w);
-    for (int i = threadIdx.x; i < pairs; i += 64 * kDownWaves) ids[i] = (int16_t)id_of(a, first, i, pairs);
-    for (int i = lane; i < tokens * 4; i += 64) sums[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    __syncthreads();
+    uint16_t* list = reinterpret_cast<uint16_t*>(lds + (KS > 1 ? kWaves * N * 1024 : 0));
+    int e;
+    const int n = pairs_of(a, blockIdx.y, pairs, lane, list, e);
+    if (n == 0) return;
 
-    const bool by_pair = a.slots < a.E;
-    const int units = min(a.slots, by_pair ? pairs : a.E) * parts;
+    const int tiles = a.H / 16, t0 = (blockIdx.x * (kWaves / KS) + w / KS) * N, have = tiles - t0, tc = min(t0, tiles - 1);
     const uint32_t row = (uint32_t)a.KBI * 2048, hrow = (uint32_t)a.KBI * 512;
-    const __amdgpu_buffer_rsrc_t hr = buf_rsrc_n(a.h + (int64_t)first * a.top * 2 * a.KBI * 128, (uint32_t)pairs * hrow);
-    for (int u = w; u < units; u += kDownWaves) {
-        int e;
-        const int n = pairs_of([&](int i) { return (int)ids[i]; }, u / parts, by_pair, pairs, lane, list, e);
-        if (n == 0) continue;
-        const int part = u % parts, b0 = a.KBI * part / parts, b1 = a.KBI * (part + 1) / parts;
-        const __amdgpu_buffer_rsrc_t dr = buf_rsrc_n(a.down + ((int64_t)e * (a.H / 16) + tile) * row, row);
-        const float* ds = a.down_s + ((int64_t)e * ((a.H + 127) / 128) + tile / 8) * a.KBI;
-        struct Stage {
-            v4i d[2], h[2][4];
-        } st[kDownDepth];
-        for (int base = 0; base < n; base += 16) {
-            const bool there = base + r < n;
-            const int pair = there ? list[base + r] : 0;
-            const uint32_t ho = there ? (uint32_t)pair * hrow + 32 * g : kOut;
-            auto issue = [&](Stage& s, int b) {
-                const uint32_t past = b < b1 ? 0u : kOut;
+    const __amdgpu_buffer_rsrc_t dr = buf_rsrc(a.down + ((int64_t)e * tiles + tc) * row);
+    const __amdgpu_buffer_rsrc_t dsr = buf_rsrc(a.down_s + ((int64_t)e * ((a.H + 127) / 128) + tc / 8) * a.KBI);
+    const __amdgpu_buffer_rsrc_t hr = buf_rsrc_n(a.h, (uint32_t)pairs * hrow);
+    struct Stage {
+        v4i d[N][2], h[2][4];
+        float s;
+    } st[D];
+    for (int base = 0; base < n; base += 16) {
+        const bool there = base + r < n;
+        const int pair = there ? list[base + r] : 0;
+        const uint32_t ho = there ? (uint32_t)pair * hrow + 32 * g : kOut;
+        auto issue = [&](Stage& s, int b) {
+            const uint32_t bc = min(b, a.KBI - 1);
 #pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    s.d[p] = buf_load16<kBufNT>(dr, (b * 2048u + p * 1024 + lane * 16) | past, 0);
-                    const uint32_t o = (ho + b * 256u + p * 128) | past | (b * 128 + p * 64 + 16 * g < a.I ? 0u : kOut);
+            for (int i = 0; i < N; i++)
 #pragma unroll
-                    for (int q = 0; q < 2; q++) {
-                        s.h[q][2 * p] = buf_load16(hr, o + q * a.KBI * 256u, 0);
-                        s.h[q][2 * p + 1] = buf_load16(hr, o + q * a.KBI * 256u + 16, 0);
-                    }
+                for (int p = 0; p < 2; p++)
+                    s.d[i][p] = buf_load16<kBufNT>(dr, lane * 16 + p * 1024, min(i, max(have, 1) - 1) * row + bc * 2048);
+            s.s = __uint_as_float(buf_load4(dsr, 0, bc * 4));
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const uint32_t o = b * 128 + p * 64 + 16 * g < a.I ? ho : kOut;
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    s.h[k][2 * p] = buf_load16(hr, o + p * 128, bc * 256 + k * a.KBI * 256);
+                    s.h[k][2 * p + 1] = buf_load16(hr, o + p * 128 + 16, bc * 256 + k * a.KBI * 256);
                 }
-            };
-            v4f y = {0.f, 0.f, 0.f, 0.f};
+            }
+        };
+        v4f y[N];
 #pragma unroll
-            for (int d = 0; d < kDownDepth; d++) issue(st[d], b0 + d);
-            for (int b = b0; b < b1; b += kDownDepth) {
+        for (int i = 0; i < N; i++) y[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int d = 0; d < kDownDepth; d++) {
+        for (int d = 0; d < D; d++) issue(st[d], q + d * KS);
+        for (int b = q; b < a.KBI; b += D * KS) {
+#pragma unroll
+            for (int d = 0; d < D; d++) {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
                     v4f t = {0.f, 0.f, 0.f, 0.f}, l = t;
 #pragma unroll
                     for (int p = 0; p < 2; p++) {
                         v8bf lo, hi;
-                        widen(st[d].d[p], lo, hi);
+                        widen(st[d].d[i][p], lo, hi);
                         t = bf_mfma(hi, st[d].h[0][2 * p + 1], bf_mfma(lo, st[d].h[0][2 * p], t));
                         l = bf_mfma(hi, st[d].h[1][2 * p + 1], bf_mfma(lo, st[d].h[1][2 * p], l));
                     }
-                    const float s = ds[min(b + d, a.KBI - 1)];
-                    y = scaled(l, s, scaled(t, s, y));
-                    issue(st[d], b + d + kDownDepth);
+                    y[i] = scaled(l, st[d].s, scaled(t, st[d].s, y[i]));
+                }
+                issue(st[d], b + (d + D) * KS);
+            }
+        }
+        if (KS > 1) {
+            if (base) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; i++) red[(w * N + i) * 64 + lane] = y[i];
+            __syncthreads();
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (i % KS != q || i >= have || !there) continue;
+            v4f s = y[i];
+            if (KS > 1) {
+                const int w0 = w - q;
+                s = red[(w0 * N + i) * 64 + lane];
+#pragma unroll
+                for (int j = 1; j < KS; j++) {
+                    const v4f z = red[((w0 + j) * N + i) * 64 + lane];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) s[k] = add_rn(s[k], z[k]);
                 }
             }
-            // into this wave's sums; pairs of one token (an expert named twice) one after the other
-            const int t = there ? token_of(a, pair) : -1;
-            const float pw = there ? a.w[(first + t) * a.w_ld + (pair - t * a.top)] : 0.f;
-            const int before = __shfl(t, lane - 1, kWave);
-            const bool twice = __ballot(there && r > 0 && before == t) != 0;
-            for (int j = 0; j < (twice ? a.top : 1); j++)
-                if (there && (!twice || pair - t * a.top == j)) {
-                    const v4f s = sums[t * 4 + g];
-                    sums[t * 4 + g] = scaled(y, pw, s);
-                }
+            *reinterpret_cast<v4f*>(a.y + (int64_t)pair * a.H + 16 * (t0 + i) + 4 * g) = s;
         }
     }
-    __syncthreads();
-    const v4f* all = reinterpret_cast<const v4f*>(lds);
-    for (int i = threadIdx.x; i < tokens * 4; i += 64 * kDownWaves) {
-        v4f y = all[i];
-        for (int j = 1; j < kDownWaves; j++) {
-            const v4f z = all[j * room * 4 + i];
-            y = v4f{add_rn(y.x, z.x), add_rn(y.y, z.y), add_rn(y.z, z.z), add_rn(y.w, z.w)};
-        }
-        const int64_t o = (first + i / 4) * a.o_ld + 16 * tile + 4 * (i & 3);
-        if (EPI == 0) {
-            uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + o;
-            if (a.vec) {
-                *reinterpret_cast<v2u*>(p) = v2u{f32_to_bf16(y.x) | f32_to_bf16(y.y) << 16, f32_to_bf16(y.z) | f32_to_bf16(y.w) << 16};
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) p[j] = (uint16_t)f32_to_bf16(y[j]);
-            }
+}
+
+// A token's pairs, weighted, in the order of its ids: a thread per four outputs.
+template <int EPI>
+__global__ __launch_bounds__(256) void moe_sum_kernel(ExpertArgs a) {
+    const int t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (t >= pass_tokens(a) || c >= a.H) return;
+    v4f y = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < a.top; j++) {
+        const int pair = t * a.top + j;
+        if (id_of(a, pair) < 0) continue;
+        y = scaled(*reinterpret_cast<const v4f*>(a.y + (int64_t)pair * a.H + c), a.w[(a.first + t) * a.w_ld + j], y);
+    }
+    const int64_t o = (a.first + t) * a.o_ld + c;
+    if (EPI == 0) {
+        uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + o;
+        if (a.vec) {
+            *reinterpret_cast<v2u*>(p) = v2u{f32_to_bf16(y.x) | f32_to_bf16(y.y) << 16, f32_to_bf16(y.z) | f32_to_bf16(y.w) << 16};
         } else {
-            float* p = reinterpret_cast<float*>(a.out) + o;
 #pragma unroll
-            for (int j = 0; j < 4; j++) p[j] = add_rn(p[j], y[j]);
+            for (int j = 0; j < 4; j++) p[j] = (uint16_t)f32_to_bf16(y[j]);
         }
+    } else {
+        float* p = reinterpret_cast<float*>(a.out) + o;
+#pragma unroll
+        for (int j = 0; j < 4; j++) p[j] = add_rn(p[j], y[j]);
     }
+}
+
+// The widest split of an expert's tiles over waves that gives two workgroups a CU, else the narrowest: the index of
+// {tiles per workgroup}.
+inline int moe_form(int64_t slots, int64_t tiles, const int* per, int forms) {
+    for (int i = 0; i < forms; i++)
+        if (slots * ((tiles + per[i] - 1) / per[i]) >= 512) return i;
+    return forms - 1;
 }
 
 }  // namespace prism
@@ -439,9 +502,13 @@ extern "C" int prism_moe_route(const prism_moe_route_args* args, void* stream) {
     return PRISM_OK;
 }
 
-extern "C" int64_t prism_moe_experts_workspace_bytes(int64_t T, int64_t top, int64_t I) {
-    if (T < 1 || top < 1 || I < 1) return 0;
-    return T * top * 2 * ((I + 127) / 128 * 128) * 2;
+// The pairs' hidden values and outputs of a pass.
+static int64_t moe_hidden_bytes(int64_t room, int64_t top, int64_t I) { return room * top * 2 * ((I + 127) / 128 * 128) * 2; }
+
+extern "C" int64_t prism_moe_experts_workspace_bytes(int64_t T, int64_t top, int64_t H, int64_t I) {
+    if (T < 1 || top < 1 || H < 1 || I < 1) return 0;
+    const int64_t room = T < kMoeTokens ? T : kMoeTokens;
+    return moe_hidden_bytes(room, top, I) + room * top * H * 4;
 }
 
 extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* stream) {
@@ -450,46 +517,56 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
     if (!h.x || !h.ids || !h.w || !h.gate || !h.gate_s || !h.up || !h.up_s || !h.down || !h.down_s || !h.out || !h.n_rows ||
         (h.epi != 0 && h.epi != 1))
         return PRISM_ERR_ARG;
-    if (h.T < 0 || h.T > 65535 * (int64_t)kMoeTokens || h.E < 1 || h.E > 32767 || h.top < 1 || h.top > kMoeTop) return PRISM_ERR_SHAPE;
+    if (h.T < 0 || h.T > INT32_MAX - kMoeTokens || h.E < 1 || h.E > 32767 || h.top < 1 || h.top > kMoeTop) return PRISM_ERR_SHAPE;
     if (h.H < 16 || h.I < 16 || h.H % 16 || h.I % 16 || h.H > kFp8MaxDim || h.I > kFp8MaxDim) return PRISM_ERR_SHAPE;
     if (h.x_ld < 0 || h.x_ld > kFp8MaxLd || h.ids_ld < 0 || h.w_ld < 0 || h.o_ld < 0) return PRISM_ERR_SHAPE;
     if (h.T > 1 && h.o_ld < h.H) return PRISM_ERR_SHAPE;
+    const int64_t room = h.T < kMoeTokens ? h.T : kMoeTokens;
     // a pass's hidden values are reached by 31-bit offsets
     if ((int64_t)kMoeTokens * h.top * ((h.I + 127) / 128) * 512 > INT32_MAX) return PRISM_ERR_SHAPE;
     if (!PRISM_ALIGNED(h.x, 16) || h.x_ld % 8 || !PRISM_ALIGNED(h.gate, 16) || !PRISM_ALIGNED(h.up, 16) ||
         !PRISM_ALIGNED(h.down, 16) || !PRISM_ALIGNED(h.out, h.epi ? 4 : 2))
         return PRISM_ERR_ALIGN;
     if (h.T == 0) return PRISM_OK;
-    const int64_t need = prism_moe_experts_workspace_bytes(h.T, h.top, h.I);
+    const int64_t need = prism_moe_experts_workspace_bytes(h.T, h.top, h.H, h.I);
     if (!h.wsp || h.wsp_bytes < need) return PRISM_ERR_ARG;
     if (!PRISM_ALIGNED(h.wsp, 16)) return PRISM_ERR_ALIGN;
     ExpertArgs a{};
     a.x = h.x, a.x_ld = h.x_ld, a.ids = h.ids, a.ids_ld = h.ids_ld, a.w = h.w, a.w_ld = h.w_ld;
     a.gate = h.gate, a.up = h.up, a.down = h.down, a.gate_s = h.gate_s, a.up_s = h.up_s, a.down_s = h.down_s;
-    a.h = (uint16_t*)h.wsp, a.out = h.out, a.o_ld = h.o_ld, a.n_rows = h.n_rows;
+    a.h = (uint16_t*)h.wsp, a.y = (float*)((char*)h.wsp + moe_hidden_bytes(room, h.top, h.I));
+    a.out = h.out, a.o_ld = h.o_ld, a.n_rows = h.n_rows;
     a.T = (int)h.T, a.E = (int)h.E, a.top = (int)h.top, a.H = (int)h.H, a.I = (int)h.I;
     a.KBH = (int)((h.H + 127) / 128), a.KBI = (int)((h.I + 127) / 128);
     a.div = 65536u / (uint32_t)h.top + 1;
-    const int room = (int)(h.T < kMoeTokens ? h.T : kMoeTokens);
-    a.slots = room * a.top < a.E ? room * a.top : a.E;
+    a.room = (int)room;
+    a.slots = room * a.top < a.E ? (int)room * a.top : a.E;
     a.vec = h.o_ld % 4 == 0 && PRISM_ALIGNED(h.out, 8);
-    if (a.slots > 65535) return PRISM_ERR_SHAPE;
-    const unsigned passes = (unsigned)((h.T + kMoeTokens - 1) / kMoeTokens);
     const hipStream_t st = (hipStream_t)stream;
-    const size_t up_lds = (size_t)kUpWaves * (2048 + (size_t)kMoeTokens * a.top * 2);
-    hipLaunchKernelGGL(moe_up_kernel, dim3(a.I / 16, a.slots, passes), dim3(64 * kUpWaves), up_lds, st, a);
-    PRISM_LAUNCH_CHECK();
-    const size_t down_lds = (size_t)kDownWaves * room * 64 + (size_t)room * a.top * 2 * (1 + kDownWaves);
-    // few experts: their inputs are split, so that every wave has some
-    int parts = (kDownWaves + a.slots - 1) / a.slots;
-    if (parts > a.KBI) parts = a.KBI;
-    if (h.epi) {
-        allow_lds(moe_down_kernel<1>, down_lds);
-        hipLaunchKernelGGL((moe_down_kernel<1>), dim3(a.H / 16, passes), dim3(64 * kDownWaves), down_lds, st, a, parts);
-    } else {
-        allow_lds(moe_down_kernel<0>, down_lds);
-        hipLaunchKernelGGL((moe_down_kernel<0>), dim3(a.H / 16, passes), dim3(64 * kDownWaves), down_lds, st, a, parts);
+    const size_t ids_lds = (size_t)room * a.top * 4;             // the list and the ids
+    const int up_per[] = {8, 4, 2, 1}, down_per[] = {16, 8, 4, 2};
+    const int up = moe_form(a.slots, a.I / 16, up_per, 4), down = moe_form(a.slots, a.H / 16, down_per, 4);
+    for (a.first = 0; a.first < a.T; a.first += kMoeTokens) {
+#define UP(N, KS, D) do { \
+        const int per = kWaves / KS * N; \
+        hipLaunchKernelGGL((moe_up_kernel<N, KS, D>), dim3((a.I / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
+                           ids_lds + (KS > 1 ? kWaves * N * 2048 : 0), st, a); \
+    } while (0)
+#define DOWN(N, KS, D) do { \
+        const int per = kWaves / KS * N; \
+        hipLaunchKernelGGL((moe_down_kernel<N, KS, D>), dim3((a.H / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
+                           ids_lds + (KS > 1 ? kWaves * N * 1024 : 0), st, a); \
+    } while (0)
+        if (up == 0) UP(2, 1, 4); else if (up == 1) UP(2, 2, 4); else if (up == 2) UP(2, 4, 4); else UP(1, 4, 4);
+        PRISM_LAUNCH_CHECK();
+        if (down == 0) DOWN(4, 1, 3); else if (down == 1) DOWN(4, 2, 3); else if (down == 2) DOWN(2, 2, 3); else DOWN(1, 2, 3);
+        PRISM_LAUNCH_CHECK();
+#undef UP
+#undef DOWN
+        const dim3 grid((a.H / 4 + 255) / 256, (unsigned)room);
+        if (h.epi) hipLaunchKernelGGL((moe_sum_kernel<1>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((moe_sum_kernel<0>), grid, dim3(256), 0, st, a);
+        PRISM_LAUNCH_CHECK();
     }
-    PRISM_LAUNCH_CHECK();
     return PRISM_OK;
 }

@@ -68,7 +68,7 @@ _SIGS = {
     "prism_fp8_gemm_workspace_bytes": (_i64, [_i64] * 3),
     "prism_moe_route": (_int, [_args, _p]),
     "prism_moe_experts": (_int, [_args, _p]),
-    "prism_moe_experts_workspace_bytes": (_i64, [_i64] * 3),
+    "prism_moe_experts_workspace_bytes": (_i64, [_i64] * 4),
 }
 
 _lib = None

@@ -96,8 +96,8 @@ def test_experts_codes(lib):
     assert call(I=2 ** 20, top=16) == SHAPE                      # a pass's hidden values would pass 31-bit offsets
     assert call(x=U) == ALIGN and call(x_ld=68) == ALIGN and call(gate=U) == ALIGN and call(up=U) == ALIGN and call(down=U) == ALIGN
     assert call(out=U) == ALIGN and call(out=P + 2, epi=1) == ALIGN
-    need = lib.prism_moe_experts_workspace_bytes(3, 2, 32)
-    assert need > 0 and lib.prism_moe_experts_workspace_bytes(0, 2, 32) == 0
+    need = lib.prism_moe_experts_workspace_bytes(3, 2, 64, 32)
+    assert need > 0 and lib.prism_moe_experts_workspace_bytes(0, 2, 64, 32) == 0
     assert call(T=3) == ARG and call(T=3, wsp=P, wsp_bytes=need - 1) == ARG and call(T=3, wsp=U, wsp_bytes=need) == ALIGN
 
 
