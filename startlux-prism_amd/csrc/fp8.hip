@@ -33,6 +33,7 @@ template <bool F32, bool VEC, int U>
 __global__ __launch_bounds__(256) void fp8_quant_kernel(const void* __restrict__ x, int64_t x_ld, uint8_t* __restrict__ q,
                                                         int64_t q_ld, float* __restrict__ s, int64_t s_ld,
                                                         const int32_t* __restrict__ n_rows, int T, int k, int KB) {
+    kernel_args_now(x, x_ld, q, q_ld, s, s_ld, n_rows, T, k, KB);
     const int live = min(T, __ldg(n_rows));
     const int64_t units = (int64_t)live * KB, step = (int64_t)gridDim.x * 16;
     const int sub = threadIdx.x & 15;
@@ -184,84 +185,113 @@ __device__ __forceinline__ void store4(const Fp8Gemm& g, int m, int j, v4f y) {
     }
 }
 
-// Few rows (up to 16 MT): a workgroup owns NW2 16-row weight tiles, its 8 waves take the blocks of 128 inputs in turn (wave w
-// block w, w + 8, ...) straight from memory into registers, D blocks ahead, and add their sums through LDS, wave after wave.
-// Rows past the live ones read as zeros (the buffer's range), blocks past the last as the last against zeros, so the loop has
-// no branches.
-constexpr int kStreamWaves = 8;
-template <int MT, int NW2, int D, int EPI>
-__global__ __launch_bounds__(64 * kStreamWaves) void fp8_stream_kernel(Fp8Gemm g) {
+// Few rows (up to 16 MT): a workgroup owns N 16-row weight tiles, its W waves take the blocks of 128 inputs in turn (wave w block
+// w, w + W, ...) straight from memory into registers, D blocks ahead, and add their sums through LDS, wave after wave.  Rows
+// past the live ones and blocks past the last read as zeros: their offsets lie past the buffers' range, which costs no traffic,
+// and the loop has no branches.  Eight neighbouring lanes load an activation row's 128 bytes (a row per lane, as the MFMA
+// wants it, takes the memory pipeline four times as long); the wave turns them in 2 KB of its own LDS per 16 rows: piece c of
+// row r lies at slot c ^ (r % 8), so that the 16 rows of a fragment read lie on distinct banks.
+template <int MT, int N, int D, int W, int EPI>
+__global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Gemm g) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    // (arguments loaded where they are first used come one memory round trip after another)
+    kernel_args_now(g.a, g.a_ld, g.as, g.as_ld, g.w, g.ws, g.out, g.o_ld, g.n_rows, g.T, g.n, g.KB, g.NT, g.vec);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, gr = lane >> 4;
-    const int t0 = blockIdx.x * NW2, m0 = blockIdx.y * 16 * MT;
-    const int live = min(g.T, __ldg(g.n_rows)) - m0;
-    if (live <= 0) return;
+    const int t0 = blockIdx.x * N, m0 = blockIdx.y * 16 * MT;
+    const int n_rows = __ldg(g.n_rows);
     const int tiles = g.NT - t0, KB = g.KB;
     const uint32_t tile = (uint32_t)KB * 2048;
     const __amdgpu_buffer_rsrc_t wr = buf_rsrc(g.w + (int64_t)t0 * tile);
-    const uint32_t rows = min(live, 16 * MT);
-    const __amdgpu_buffer_rsrc_t ar = buf_rsrc_n(g.a + m0 * g.a_ld, (uint32_t)((rows - 1) * g.a_ld + KB * 128));
-    const __amdgpu_buffer_rsrc_t sr = buf_rsrc_n(g.as + m0 * g.as_ld, (uint32_t)((rows - 1) * g.as_ld + KB) * 4);
-    const __amdgpu_buffer_rsrc_t br = buf_rsrc(g.ws + (int64_t)(t0 / 8) * KB);   // (NW2 tiles lie in one block of 128 rows)
+    const __amdgpu_buffer_rsrc_t br = buf_rsrc(g.ws + (int64_t)(t0 >> 3) * KB);    // (N tiles lie in one block of 128 rows)
     constexpr uint32_t kOut = 0x80000000u;
-    uint32_t aoff[MT], soff[MT];
-#pragma unroll
-    for (int c = 0; c < MT; c++) {
-        const int m = 16 * c + r;
-        aoff[c] = m < live ? (uint32_t)(m * g.a_ld + 16 * gr) : kOut;
-        soff[c] = m < live ? (uint32_t)(m * g.as_ld) * 4 : kOut;
-    }
     struct Stage {
-        v4i w[NW2][2], a[MT][2];
+        v4i w[N][2], a[MT][2];
         float s[MT], sw;
     } st[D];
-    auto issue = [&](Stage& x, int b) {
-        const uint32_t bc = min(b, KB - 1), out = b < KB ? 0u : kOut;                  // (wave-uniform)
-        x.sw = __uint_as_float(buf_load4(br, 0, bc * 4));
+    auto issue_w = [&](Stage& x, int b) {
+        const uint32_t bc = min(b, KB - 1), past = b < KB ? 0u : kOut;                 // (wave-uniform)
+        x.sw = __uint_as_float(buf_load4(br, past, bc * 4));
 #pragma unroll
-        for (int t = 0; t < NW2; t++)
+        for (int t = 0; t < N; t++)
 #pragma unroll
-            for (int p = 0; p < 2; p++) x.w[t][p] = buf_load16<kBufNT>(wr, lane * 16 + p * 1024, min(t, tiles - 1) * tile + bc * 2048);
+            for (int p = 0; p < 2; p++) x.w[t][p] = buf_load16<kBufNT>(wr, (lane * 16 | past) + p * 1024, min(t, tiles - 1) * tile + bc * 2048);
+    };
+    // all T rows are read, those not live too: no load waits for the live count
+    const int rows = min(g.T - m0, 16 * MT);
+    const __amdgpu_buffer_rsrc_t ar = buf_rsrc_n(g.a + m0 * g.a_ld, (uint32_t)((rows - 1) * g.a_ld + KB * 128));
+    const __amdgpu_buffer_rsrc_t sr = buf_rsrc_n(g.as + m0 * g.as_ld, (uint32_t)((rows - 1) * g.as_ld + KB) * 4);
+    uint32_t aoff[MT][2], soff[MT];
+#pragma unroll
+    for (int c = 0; c < MT; c++) {
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            const int m = 16 * c + 8 * p + (lane >> 3);
+            aoff[c][p] = m < rows ? (uint32_t)(m * g.a_ld + 16 * (lane & 7)) : kOut;
+        }
+        soff[c] = 16 * c + r < rows ? (uint32_t)((16 * c + r) * g.as_ld) * 4 : kOut;
+    }
+    auto issue_a = [&](Stage& x, int b) {
+        const uint32_t bc = min(b, KB - 1), past = b < KB ? 0u : kOut;
 #pragma unroll
         for (int c = 0; c < MT; c++) {
 #pragma unroll
-            for (int p = 0; p < 2; p++) x.a[c][p] = buf_load16(ar, (aoff[c] | out) + 64 * p, bc * 128);
-            x.s[c] = __uint_as_float(buf_load4(sr, soff[c], bc * 4));
+            for (int p = 0; p < 2; p++) x.a[c][p] = buf_load16(ar, aoff[c][p] | past, bc * 128);
+            x.s[c] = __uint_as_float(buf_load4(sr, soff[c] | past, bc * 4));
         }
     };
-    v4f acc[NW2][MT];
+    uint8_t* turn = lds + w * MT * 2048;
+    const int put = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) * 16);
+    const int get0 = r * 128 + ((gr ^ (r & 7)) * 16), get1 = r * 128 + (((4 + gr) ^ (r & 7)) * 16);
+    v4f acc[N][MT];
 #pragma unroll
-    for (int t = 0; t < NW2; t++)
+    for (int t = 0; t < N; t++)
 #pragma unroll
         for (int c = 0; c < MT; c++) acc[t][c] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int d = 0; d < D; d++) issue(st[d], w + d * kStreamWaves);
-    for (int b = w; b < KB; b += D * kStreamWaves) {
+    for (int d = 0; d < D; d++) {
+        issue_w(st[d], w + d * W);
+        issue_a(st[d], w + d * W);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    const int live = min(g.T, n_rows) - m0;
+    if (live <= 0) return;
+    for (int b = w; b < KB; b += D * W) {
 #pragma unroll
         for (int d = 0; d < D; d++) {
-            const int at = b + d * kStreamWaves;
+            const int at = b + d * W;
+#pragma unroll
+            for (int c = 0; c < MT; c++)
+#pragma unroll
+                for (int p = 0; p < 2; p++) *reinterpret_cast<v4i*>(turn + c * 2048 + p * 1024 + put) = st[d].a[c][p];
 #pragma unroll
             for (int c = 0; c < MT; c++) {
-                const v8i a = join8(st[d].a[c][0], st[d].a[c][1]);
+                const v8i a = join8(*reinterpret_cast<const v4i*>(turn + c * 2048 + get0),
+                                    *reinterpret_cast<const v4i*>(turn + c * 2048 + get1));
                 const float s = mul_rn(st[d].s[c], st[d].sw);
 #pragma unroll
-                for (int t = 0; t < NW2; t++)
+                for (int t = 0; t < N; t++)
                     acc[t][c] = fold(fp8_mfma(join8(st[d].w[t][0], st[d].w[t][1]), a), s, acc[t][c]);
             }
-            issue(st[d], at + D * kStreamWaves);
+            issue_w(st[d], at + D * W);
+            issue_a(st[d], at + D * W);
+            // (else the uses of all stages gather in front and wait for all loads; the loads before the loop are kept in the same
+            // order, as the wait in it has to serve both)
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+    __syncthreads();                                                                   // (the sums lie over the turns)
     v4f* red = reinterpret_cast<v4f*>(lds);
 #pragma unroll
-    for (int t = 0; t < NW2; t++)
+    for (int t = 0; t < N; t++)
 #pragma unroll
-        for (int c = 0; c < MT; c++) red[((t * MT + c) * kStreamWaves + w) * 64 + lane] = acc[t][c];
+        for (int c = 0; c < MT; c++) red[((t * MT + c) * W + w) * 64 + lane] = acc[t][c];
     __syncthreads();
-    for (int i = w; i < NW2 * MT; i += kStreamWaves) {
-        v4f y = red[i * kStreamWaves * 64 + lane];
-        for (int j = 1; j < kStreamWaves; j++) {
-            const v4f z = red[(i * kStreamWaves + j) * 64 + lane];
+    for (int i = w; i < N * MT; i += W) {
+        v4f y = red[i * W * 64 + lane];
+#pragma unroll
+        for (int j = 1; j < W; j++) {
+            const v4f z = red[(i * W + j) * 64 + lane];
             y = v4f{add_rn(y.x, z.x), add_rn(y.y, z.y), add_rn(y.z, z.z), add_rn(y.w, z.w)};
         }
         const int m = 16 * (i % MT) + r, j = (t0 + i / MT) * 16 + 4 * gr;
@@ -484,16 +514,16 @@ extern "C" int prism_fp8_gemm(const prism_fp8_gemm_args* args, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
 #define EP(f) do { if (h.epi) f(1); else f(0); } while (0)
     if (p.kind == 0) {
-#define ST(MT, NW, D, E) do { \
-        const size_t bytes = (size_t)MT * NW * kStreamWaves * 1024; \
-        allow_lds(fp8_stream_kernel<MT, NW, D, E>, bytes); \
-        hipLaunchKernelGGL((fp8_stream_kernel<MT, NW, D, E>), dim3((g.NT + NW - 1) / NW, (unsigned)((h.T + 16 * MT - 1) / (16 * MT))), \
-                           dim3(64 * kStreamWaves), bytes, st, g); \
+#define ST(MT, N, D, W, E) do { \
+        const size_t bytes = (size_t)MT * (N > 2 ? N : 2) * W * 1024; \
+        allow_lds(fp8_stream_kernel<MT, N, D, W, E>, bytes); \
+        hipLaunchKernelGGL((fp8_stream_kernel<MT, N, D, W, E>), dim3((g.NT + N - 1) / N, (unsigned)((h.T + 16 * MT - 1) / (16 * MT))), \
+                           dim3(64 * W), bytes, st, g); \
     } while (0)
-#define S1(E) ST(1, 1, 3, E)
-#define S2(E) ST(2, 2, 2, E)
-#define S3(E) ST(3, 2, 2, E)
-#define S4(E) ST(4, 2, 2, E)
+#define S1(E) ST(1, 1, 5, 8, E)
+#define S2(E) ST(2, 2, 2, 8, E)
+#define S3(E) ST(3, 2, 2, 8, E)
+#define S4(E) ST(4, 2, 2, 8, E)
         if (p.mt == 1) EP(S1); else if (p.mt == 2) EP(S2); else if (p.mt == 3) EP(S3); else EP(S4);
 #undef S1
 #undef S2

@@ -13,6 +13,8 @@
 // bf16 parts (h = hi + lo up to 2^-17 of it: the second product's operand; one part alone would add as much error as the bf16
 // output's own rounding), moe_down_kernel each pair's outputs in fp32, moe_sum_kernel adds a token's in the order of its ids:
 // no atomics, and what a token gets does not depend on the others but for how K is split.
+#include <math.h>
+
 #include "common.h"
 #include "fp8.h"
 
@@ -53,8 +55,10 @@ struct RouteArgs {
 // A wave per token, lane l holding experts l, l + 64, ...; the best of all lanes, top times.
 template <int V, bool F32, bool SIG>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
+    kernel_args_now(a.x, a.x_ld, a.bias, a.ids, a.ids_ld, a.w, a.w_ld, a.n_rows, a.T, a.E, a.top, a.renorm, a.scale);
     const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (t >= min(a.T, __ldg(a.n_rows))) return;
+    if (t >= a.T) return;
+    const int live = __ldg(a.n_rows);
     float x[V];
     double p[SIG ? V : 1];
     uint64_t key[V];
@@ -66,6 +70,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
             x[i] = F32 ? reinterpret_cast<const float*>(a.x)[t * a.x_ld + e]
                        : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.x)[t * a.x_ld + e]);
     }
+    if (t >= live) return;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         if (SIG) {
@@ -157,7 +162,16 @@ struct ExpertArgs {
     int first, room;                         // the pass's tokens: room from first on
     int slots;                               // experts looked at per pass: all, or one per pair where those are fewer
     int vec;
+    int xcd;
 };
+
+// Every argument a kernel goes by in scalar registers at once: loaded where they are first used they come one memory round
+// trip after another, which is most of a decode-size launch.
+__device__ __forceinline__ void experts_now(const ExpertArgs& a) {
+    kernel_args_now(a.x, a.x_ld, a.ids, a.ids_ld, a.w, a.w_ld, a.gate, a.up, a.down, a.gate_s, a.up_s, a.down_s, a.h, a.y, a.out,
+                    a.n_rows);
+    kernel_args_now(a.o_ld, a.T, a.E, a.top, a.H, a.I, a.KBH, a.KBI, a.div, a.first, a.room, a.slots, a.vec);
+}
 
 // The pass's live tokens (0 or less: none).
 __device__ __forceinline__ int pass_tokens(const ExpertArgs& a) { return min(min(a.T, __ldg(a.n_rows)) - a.first, a.room); }
@@ -197,12 +211,15 @@ constexpr uint32_t kOut = 0x80000000u;       // an offset past every buffer's ra
 // This slot's expert e and its pairs, in order, in `list` (the workgroup's LDS: [pairs] entries, then [pairs] for the ids);
 // the number of pairs, the same in every wave: 0 for an expert without any, for a pair without an expert (slots are pairs
 // where those are fewer than the experts) and for one whose expert an earlier pair has.  Every wave writes the same list.
-__device__ __forceinline__ int pairs_of(const ExpertArgs& a, int slot, int pairs, int lane, uint16_t* list, int& e) {
+__device__ __forceinline__ int pairs_of(const ExpertArgs& a, int slot, int lane, uint16_t* list, int& e, int& tokens) {
     const bool by_pair = a.slots < a.E;
-    if (by_pair && slot >= pairs) return 0;
     e = slot;
-    if (pairs <= 64) {
-        const int id = lane < pairs ? id_of(a, lane) : -1;
+    if (a.room * a.top <= 64) {
+        // (the ids of rows that are not live are the caller's buffer as well: loaded beside the live count, not after it)
+        int id = lane < a.room * a.top ? id_of(a, lane) : -1;
+        tokens = pass_tokens(a);
+        asm volatile("" ::"v"(id), "s"(tokens));
+        if (lane >= tokens * a.top) id = -1;
         if (by_pair) e = __builtin_amdgcn_readlane(id, slot);
         if (e < 0) return 0;
         const uint64_t m = __ballot(id == e);
@@ -210,6 +227,9 @@ __device__ __forceinline__ int pairs_of(const ExpertArgs& a, int slot, int pairs
         if (id == e) list[__popcll(m & ((1ull << lane) - 1))] = (uint16_t)lane;
         return __popcll(m);
     }
+    tokens = pass_tokens(a);
+    const int pairs = tokens * a.top;
+    if (tokens <= 0 || (by_pair && slot >= pairs)) return 0;
     int16_t* ids = reinterpret_cast<int16_t*>(list) + a.room * a.top;
     for (int i = threadIdx.x; i < pairs; i += 64 * kWaves) ids[i] = (int16_t)id_of(a, i);
     __syncthreads();
@@ -231,22 +251,21 @@ __device__ __forceinline__ int pairs_of(const ExpertArgs& a, int slot, int pairs
 template <int N, int KS, int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void moe_up_kernel(ExpertArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    experts_now(a);
     v4f* red = reinterpret_cast<v4f*>(lds);                                   // [waves][N][2][64] where K is split
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4, q = w % KS;
-    const int tokens = pass_tokens(a), pairs = tokens * a.top;
-    if (tokens <= 0) return;
     uint16_t* list = reinterpret_cast<uint16_t*>(lds + (KS > 1 ? kWaves * N * 2048 : 0));
-    int e;
-    const int n = pairs_of(a, blockIdx.y, pairs, lane, list, e);
+    int e, tokens;
+    const int n = pairs_of(a, blockIdx.y, lane, list, e, tokens);
     if (n == 0) return;
 
-    // (tiles past the last are the last once more, chunks past the last the last against zero inputs)
-    const int tiles = a.I / 16, t0 = (blockIdx.x * (kWaves / KS) + w / KS) * N, have = tiles - t0, tc = min(t0, tiles - 1);
+    // (tiles past the last are the last once more, chunks past the last read as zeros: an offset past the range costs no traffic)
+    const int tiles = a.I >> 4, t0 = (blockIdx.x * (kWaves / KS) + w / KS) * N, have = tiles - t0, tc = min(t0, tiles - 1);
     const uint32_t row = (uint32_t)a.KBH * 2048;                              // bytes of a 16-row tile
     const int64_t at = ((int64_t)e * tiles + tc) * row;
     const __amdgpu_buffer_rsrc_t gr = buf_rsrc(a.gate + at), ur = buf_rsrc(a.up + at);
-    const int64_t sat = ((int64_t)e * ((a.I + 127) / 128) + tc / 8) * a.KBH;
+    const int64_t sat = ((int64_t)e * ((a.I + 127) >> 7) + (tc >> 3)) * a.KBH;
     const __amdgpu_buffer_rsrc_t gsr = buf_rsrc(a.gate_s + sat), usr = buf_rsrc(a.up_s + sat);
     const __amdgpu_buffer_rsrc_t xr = buf_rsrc_n(a.x + a.first * a.x_ld, (uint32_t)((tokens - 1) * a.x_ld + a.H) * 2);
     struct Stage {
@@ -258,17 +277,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_up_kernel(ExpertArgs a) {
         const int pair = there ? list[base + r] : 0;
         const uint32_t xo = there ? (uint32_t)(token_of(a, pair) * a.x_ld + 16 * g) * 2 : kOut;
         auto issue = [&](Stage& s, int b) {
-            const uint32_t bc = min(b, a.KBH - 1);
+            const uint32_t bc = min(b, a.KBH - 1), past = b < a.KBH ? 0u : kOut;
 #pragma unroll
             for (int i = 0; i < N; i++)
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
                     const uint32_t at = min(i, max(have, 1) - 1) * row + bc * 2048;
-                    s.g[i][p] = buf_load16<kBufNT>(gr, lane * 16 + p * 1024, at);
-                    s.u[i][p] = buf_load16<kBufNT>(ur, lane * 16 + p * 1024, at);
+                    s.g[i][p] = buf_load16<kBufNT>(gr, (lane * 16 | past) + p * 1024, at);
+                    s.u[i][p] = buf_load16<kBufNT>(ur, (lane * 16 | past) + p * 1024, at);
                 }
-            s.gs = __uint_as_float(buf_load4(gsr, 0, bc * 4));
-            s.us = __uint_as_float(buf_load4(usr, 0, bc * 4));
+            s.gs = __uint_as_float(buf_load4(gsr, past, bc * 4));
+            s.us = __uint_as_float(buf_load4(usr, past, bc * 4));
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 const uint32_t o = b * 128 + p * 64 + 16 * g < a.H ? xo : kOut;
@@ -280,7 +299,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_up_kernel(ExpertArgs a) {
 #pragma unroll
         for (int i = 0; i < N; i++) ga[i] = ua[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int d = 0; d < D; d++) issue(st[d], q + d * KS);
+        for (int d = 0; d < D; d++) {
+            issue(st[d], q + d * KS);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         for (int b = q; b < a.KBH; b += D * KS) {
 #pragma unroll
             for (int d = 0; d < D; d++) {
@@ -299,6 +321,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_up_kernel(ExpertArgs a) {
                     ua[i] = scaled(tu, st[d].us, ua[i]);
                 }
                 issue(st[d], b + (d + D) * KS);
+                // (else the uses of all stages gather in front and wait for all loads; the loads before the loop are kept in the
+                // same order, as the wait in it has to serve both)
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (KS > 1) {
@@ -347,21 +372,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_up_kernel(ExpertArgs a) {
 template <int N, int KS, int D>
 __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    experts_now(a);
     v4f* red = reinterpret_cast<v4f*>(lds);                                   // [waves][N][64] where K is split
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4, q = w % KS;
-    const int tokens = pass_tokens(a), pairs = tokens * a.top;
-    if (tokens <= 0) return;
     uint16_t* list = reinterpret_cast<uint16_t*>(lds + (KS > 1 ? kWaves * N * 1024 : 0));
-    int e;
-    const int n = pairs_of(a, blockIdx.y, pairs, lane, list, e);
+    int e, tokens;
+    const int n = pairs_of(a, blockIdx.y, lane, list, e, tokens);
     if (n == 0) return;
 
-    const int tiles = a.H / 16, t0 = (blockIdx.x * (kWaves / KS) + w / KS) * N, have = tiles - t0, tc = min(t0, tiles - 1);
+    const int tiles = a.H >> 4, t0 = (blockIdx.x * (kWaves / KS) + w / KS) * N, have = tiles - t0, tc = min(t0, tiles - 1);
     const uint32_t row = (uint32_t)a.KBI * 2048, hrow = (uint32_t)a.KBI * 512;
     const __amdgpu_buffer_rsrc_t dr = buf_rsrc(a.down + ((int64_t)e * tiles + tc) * row);
-    const __amdgpu_buffer_rsrc_t dsr = buf_rsrc(a.down_s + ((int64_t)e * ((a.H + 127) / 128) + tc / 8) * a.KBI);
-    const __amdgpu_buffer_rsrc_t hr = buf_rsrc_n(a.h, (uint32_t)pairs * hrow);
+    const __amdgpu_buffer_rsrc_t dsr = buf_rsrc(a.down_s + ((int64_t)e * ((a.H + 127) >> 7) + (tc >> 3)) * a.KBI);
+    const __amdgpu_buffer_rsrc_t hr = buf_rsrc_n(a.h, (uint32_t)(tokens * a.top) * hrow);
     struct Stage {
         v4i d[N][2], h[2][4];
         float s;
@@ -371,13 +395,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
         const int pair = there ? list[base + r] : 0;
         const uint32_t ho = there ? (uint32_t)pair * hrow + 32 * g : kOut;
         auto issue = [&](Stage& s, int b) {
-            const uint32_t bc = min(b, a.KBI - 1);
+            const uint32_t bc = min(b, a.KBI - 1), past = b < a.KBI ? 0u : kOut;
 #pragma unroll
             for (int i = 0; i < N; i++)
 #pragma unroll
                 for (int p = 0; p < 2; p++)
-                    s.d[i][p] = buf_load16<kBufNT>(dr, lane * 16 + p * 1024, min(i, max(have, 1) - 1) * row + bc * 2048);
-            s.s = __uint_as_float(buf_load4(dsr, 0, bc * 4));
+                    s.d[i][p] = buf_load16<kBufNT>(dr, (lane * 16 | past) + p * 1024, min(i, max(have, 1) - 1) * row + bc * 2048);
+            s.s = __uint_as_float(buf_load4(dsr, past, bc * 4));
 #pragma unroll
             for (int p = 0; p < 2; p++) {
                 const uint32_t o = b * 128 + p * 64 + 16 * g < a.I ? ho : kOut;
@@ -392,7 +416,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
 #pragma unroll
         for (int i = 0; i < N; i++) y[i] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int d = 0; d < D; d++) issue(st[d], q + d * KS);
+        for (int d = 0; d < D; d++) {
+            issue(st[d], q + d * KS);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         for (int b = q; b < a.KBI; b += D * KS) {
 #pragma unroll
             for (int d = 0; d < D; d++) {
@@ -409,6 +436,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
                     y[i] = scaled(l, st[d].s, scaled(t, st[d].s, y[i]));
                 }
                 issue(st[d], b + (d + D) * KS);
+                // (else the uses of all stages gather in front and wait for all loads; the loads before the loop are kept in the
+                // same order, as the wait in it has to serve both)
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (KS > 1) {
@@ -436,17 +466,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
     }
 }
 
-// A token's pairs, weighted, in the order of its ids: a thread per four outputs.
 template <int EPI>
-__global__ __launch_bounds__(256) void moe_sum_kernel(ExpertArgs a) {
-    const int t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
-    if (t >= pass_tokens(a) || c >= a.H) return;
-    v4f y = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < a.top; j++) {
-        const int pair = t * a.top + j;
-        if (id_of(a, pair) < 0) continue;
-        y = scaled(*reinterpret_cast<const v4f*>(a.y + (int64_t)pair * a.H + c), a.w[(a.first + t) * a.w_ld + j], y);
-    }
+__device__ __forceinline__ void store_out(const ExpertArgs& a, int t, int c, v4f y) {
     const int64_t o = (a.first + t) * a.o_ld + c;
     if (EPI == 0) {
         uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + o;
@@ -463,11 +484,41 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(ExpertArgs a) {
     }
 }
 
-// The widest split of an expert's tiles over waves that gives two workgroups a CU, else the narrowest: the index of
-// {tiles per workgroup}.
-inline int moe_form(int64_t slots, int64_t tiles, const int* per, int forms) {
-    for (int i = 0; i < forms; i++)
-        if (slots * ((tiles + per[i] - 1) / per[i]) >= 512) return i;
+// A token's pairs, weighted, in the order of its ids: a thread per four outputs.  All loads of four pairs go out at once (of
+// pairs without an expert too: their places in the workspace hold anything).
+template <int EPI>
+__global__ __launch_bounds__(64) void moe_sum_kernel(ExpertArgs a) {
+    experts_now(a);
+    const int t = blockIdx.y, c = (blockIdx.x * 64 + threadIdx.x) * 4;
+    if (c >= a.H) return;
+    const int tokens = pass_tokens(a);
+    v4f y = {0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < a.top; j0 += 4) {
+        int id[4];
+        float pw[4];
+        v4f v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int at = min(j0 + j, a.top - 1);
+            id[j] = a.ids[(a.first + t) * a.ids_ld + at];
+            pw[j] = a.w[(a.first + t) * a.w_ld + at];
+            v[j] = *reinterpret_cast<const v4f*>(a.y + (int64_t)(t * a.top + at) * a.H + c);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j0 + j < a.top && (uint32_t)id[j] < (uint32_t)a.E) y = scaled(v[j], pw[j], y);
+    }
+    if (t < tokens) store_out<EPI>(a, t, c, y);
+}
+
+// How many of an expert's 16-row tiles a workgroup takes, of these numbers (descending): the most that leave a workgroup for every
+// CU, counting the experts that as many random ids would reach (us, up with 4 / 2 and down with 16 / 8 / 4: 11 tokens on 2 of 16
+// experts, H 5120, I 1408: 76.9 / 75.1, 67.6 / 61.3 / 64.5; 64 on 8 of 128, 2048, 768: 170 / 181, 149 / 156 / 175; 2 on 2 of 8, 4096,
+// 1792: 35.1 / 29.9, 33.4 / 27.6 / 25.4; the other kernel at one form in each).
+inline int moe_form(int64_t pairs, int64_t E, int64_t tiles, const int* per, int forms) {
+    const double reached = (double)E * (1.0 - pow(1.0 - 1.0 / (double)E, (double)pairs));
+    for (int i = 0; i < forms - 1; i++)
+        if (reached * (double)((tiles + per[i] - 1) / per[i]) >= 300.0) return i;
     return forms - 1;
 }
 
@@ -544,8 +595,8 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
     a.vec = h.o_ld % 4 == 0 && PRISM_ALIGNED(h.out, 8);
     const hipStream_t st = (hipStream_t)stream;
     const size_t ids_lds = (size_t)room * a.top * 4;             // the list and the ids
-    const int up_per[] = {8, 4, 2, 1}, down_per[] = {16, 8, 4, 2};
-    const int up = moe_form(a.slots, a.I / 16, up_per, 4), down = moe_form(a.slots, a.H / 16, down_per, 4);
+    const int up_per[] = {4, 2}, down_per[] = {16, 8, 4};
+    const int up = moe_form(room * a.top, a.E, a.I / 16, up_per, 2), down = moe_form(room * a.top, a.E, a.H / 16, down_per, 3);
     for (a.first = 0; a.first < a.T; a.first += kMoeTokens) {
 #define UP(N, KS, D) do { \
         const int per = kWaves / KS * N; \
@@ -557,15 +608,15 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
         hipLaunchKernelGGL((moe_down_kernel<N, KS, D>), dim3((a.H / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
                            ids_lds + (KS > 1 ? kWaves * N * 1024 : 0), st, a); \
     } while (0)
-        if (up == 0) UP(2, 1, 4); else if (up == 1) UP(2, 2, 4); else if (up == 2) UP(2, 4, 4); else UP(1, 4, 4);
+        if (up == 0) UP(2, 2, 4); else UP(2, 4, 4);
         PRISM_LAUNCH_CHECK();
-        if (down == 0) DOWN(4, 1, 3); else if (down == 1) DOWN(4, 2, 3); else if (down == 2) DOWN(2, 2, 3); else DOWN(1, 2, 3);
+        if (down == 0) DOWN(4, 1, 3); else if (down == 1) DOWN(4, 2, 3); else DOWN(2, 2, 3);
         PRISM_LAUNCH_CHECK();
 #undef UP
 #undef DOWN
-        const dim3 grid((a.H / 4 + 255) / 256, (unsigned)room);
-        if (h.epi) hipLaunchKernelGGL((moe_sum_kernel<1>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((moe_sum_kernel<0>), grid, dim3(256), 0, st, a);
+        const dim3 grid((a.H / 4 + 63) / 64, (unsigned)room);
+        if (h.epi) hipLaunchKernelGGL((moe_sum_kernel<1>), grid, dim3(64), 0, st, a);
+        else hipLaunchKernelGGL((moe_sum_kernel<0>), grid, dim3(64), 0, st, a);
         PRISM_LAUNCH_CHECK();
     }
     return PRISM_OK;
