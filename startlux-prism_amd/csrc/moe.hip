@@ -15,6 +15,8 @@
 // no atomics, and what a token gets does not depend on the others but for how K is split.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "fp8.h"
 
@@ -26,7 +28,7 @@ constexpr int kWaves = 4;
 
 // --------------------------------------------------------------------------------------------------------------- route
 // An order-preserving integer of a number that may be chosen (greater than 0); 0 for NaN and -inf.
-__device__ __forceinline__ uint64_t rank_of(float v) {
+__device__ __forceinline__ uint32_t rank_of(float v) {
     const uint32_t u = __float_as_uint(v);
     if (v != v || u == 0xff800000u) return 0;
     const uint32_t z = u == 0x80000000u ? 0 : u;                              // -0 is 0
@@ -52,63 +54,87 @@ struct RouteArgs {
     float scale;
 };
 
-// A wave per token, lane l holding experts l, l + 64, ...; the best of all lanes, top times.
+// The largest of the wave's values, by row shifts and broadcasts in the vector registers (a shuffle goes through the LDS unit:
+// 18 of them per choice made the choices of 8 of 256 experts 18 of 20 us for 8191 tokens).
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#define PRISM_DPP_MAX(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false))
+    PRISM_DPP_MAX(0x111, 0xf);               // row_shr:1, 2, 4, 8: lane 15 of every 16 has their largest
+    PRISM_DPP_MAX(0x112, 0xf);
+    PRISM_DPP_MAX(0x114, 0xf);
+    PRISM_DPP_MAX(0x118, 0xf);
+    PRISM_DPP_MAX(0x142, 0xa);               // row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3
+    PRISM_DPP_MAX(0x143, 0xc);
+#undef PRISM_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// A wave per token, lane l holding experts l V .. l V + V - 1, so the lowest lane with the largest key, and in it the first, is
+// the lowest number.  top times the largest of all: its high halves first, the low ones only between lanes that share them.
 template <int V, bool F32, bool SIG>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
     kernel_args_now(a.x, a.x_ld, a.bias, a.ids, a.ids_ld, a.w, a.w_ld, a.n_rows, a.T, a.E, a.top, a.renorm, a.scale);
-    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (t >= a.T) return;
     const int live = __ldg(a.n_rows);
-    float x[V];
-    double p[SIG ? V : 1];
-    uint64_t key[V];
+    float x[V], bias[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        const int e = lane + 64 * i;
-        x[i] = __uint_as_float(0xff800000u);
-        if (e < a.E)
-            x[i] = F32 ? reinterpret_cast<const float*>(a.x)[t * a.x_ld + e]
-                       : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.x)[t * a.x_ld + e]);
+        const int e = min(lane * V + i, a.E - 1);
+        x[i] = F32 ? reinterpret_cast<const float*>(a.x)[t * a.x_ld + e]
+                   : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.x)[t * a.x_ld + e]);
+        bias[i] = SIG && a.bias ? a.bias[e] : 0.f;
     }
     if (t >= live) return;
+    typedef typename std::conditional<SIG, uint64_t, uint32_t>::type Key;
+    double p[SIG ? V : 1];
+    Key key[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
         if (SIG) {
-            const int e = lane + 64 * i;
             p[i] = 1.0 / (1.0 + exp(-(double)x[i]));
-            key[i] = rank_of(x[i]) ? rank_of(p[i] + (a.bias && e < a.E ? (double)a.bias[e] : 0.0)) : 0;
+            key[i] = rank_of(x[i]) ? (Key)rank_of(p[i] + (double)bias[i]) : 0;
         } else {
             key[i] = rank_of(x[i]);
         }
+        if (lane * V + i >= a.E) key[i] = 0;
     }
     int id = -1;                                                  // lane j: the j-th choice
     float lx = 0.f;                                               // its logit, or
     double lp = 0.0;                                              // its sigmoid
     for (int j = 0; j < a.top; j++) {
-        uint64_t best = 0;
+        Key best = key[0];
         int at = 0;
 #pragma unroll
-        for (int i = 0; i < V; i++)
+        for (int i = 1; i < V; i++)
             if (key[i] > best) best = key[i], at = i;
-        int e = lane + 64 * at;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t k2 = __shfl_xor((unsigned long long)best, o, kWave);
-            const int e2 = __shfl_xor(e, o, kWave);
-            if (k2 > best || (k2 == best && e2 < e)) best = k2, e = e2;
+        const uint32_t hi = SIG ? (uint32_t)((uint64_t)best >> 32) : (uint32_t)best;
+        const uint32_t most = wave_max_u32(hi);
+        if (most == 0) break;                                     // (none left; a key's high half is not 0)
+        uint64_t m = __ballot(hi == most);
+        if (SIG && (m & (m - 1))) {
+            const uint32_t lo = hi == most ? (uint32_t)best : 0u, low = wave_max_u32(lo);
+            m = __ballot(hi == most && (uint32_t)best == low);
         }
-        if (best == 0) break;                                     // (the same in every lane)
-        float vx = 0.f;
-        double vp = 0.0;
+        const int from = __builtin_ctzll(m);
+        const int i0 = __builtin_amdgcn_readlane(at, from);
+        float vx = x[0];
+        double vp = p[0];
 #pragma unroll
-        for (int i = 0; i < V; i++)
-            if (lane + 64 * i == e) {
-                key[i] = 0, vx = x[i];
+        for (int i = 0; i < V; i++) {
+            if (i == i0) {
+                vx = x[i];
                 if (SIG) vp = p[i];
+                if (lane == from) key[i] = 0;
             }
-        vx = __shfl(vx, e & 63, kWave);
-        if (SIG) vp = __shfl(vp, e & 63, kWave);
-        if (lane == j) id = e, lx = vx, lp = vp;
+        }
+        if (SIG) {
+            const uint64_t u = (uint64_t)__double_as_longlong(vp);
+            const uint32_t l = __builtin_amdgcn_readlane((int)(uint32_t)u, from), h = __builtin_amdgcn_readlane((int)(u >> 32), from);
+            vp = __longlong_as_double((long long)((uint64_t)h << 32 | l));
+        } else {
+            vx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vx), from));
+        }
+        if (lane == j) id = from * V + i0, lx = vx, lp = vp;
     }
     float w = 0.f;
     if (SIG) {
@@ -120,7 +146,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
         }
         w = (float)(lp / sum * (double)a.scale);
     } else {
-        const float m = __shfl(lx, 0, kWave);                     // the largest logit
+        const float m = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(lx)));       // the largest logit
         const float ex = id >= 0 ? expf(lx - m) : 0.f;
         float sum = 0.f;
         if (a.renorm) {
@@ -130,7 +156,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
         } else {
 #pragma unroll
             for (int i = 0; i < V; i++)
-                if (lane + 64 * i < a.E) sum += expf(x[i] - m);
+                if (lane * V + i < a.E) sum += expf(x[i] - m);
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
         }
