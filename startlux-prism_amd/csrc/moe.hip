@@ -68,8 +68,16 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// The number that a rank stands for.
+__device__ __forceinline__ float of_rank(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+
 // A wave per token, lane l holding experts l V .. l V + V - 1, so the lowest lane with the largest key, and in it the first, is
-// the lowest number.  top times the largest of all: its high halves first, the low ones only between lanes that share them.
+// the lowest number; top times the largest of all.
+//
+// Sigmoids with a bias are compared in 64 bits, but first in 32: p and p + bias in fp32 are within 2^-21 (1 + |p + bias|) of their
+// values (expf's and three more roundings), so choices that lie further than 2^-19 (1 + |p + bias|) from the next are the same.
+// Only where two are closer (one token in some thousand, and rows with equal ones) all 64-bit values are made and compared, their
+// high halves first and the low ones between lanes that share them.  8191 tokens, 8 of 256: ROUTEUS us, 13.7 all in 64 bits.
 template <int V, bool F32, bool SIG>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
     kernel_args_now(a.x, a.x_ld, a.bias, a.ids, a.ids_ld, a.w, a.w_ld, a.n_rows, a.T, a.E, a.top, a.renorm, a.scale);
@@ -85,59 +93,82 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
         bias[i] = SIG && a.bias ? a.bias[e] : 0.f;
     }
     if (t >= live) return;
-    typedef typename std::conditional<SIG, uint64_t, uint32_t>::type Key;
-    double p[SIG ? V : 1];
-    Key key[V];
+    uint32_t key[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        if (SIG) {
-            p[i] = 1.0 / (1.0 + exp(-(double)x[i]));
-            key[i] = rank_of(x[i]) ? (Key)rank_of(p[i] + (double)bias[i]) : 0;
-        } else {
-            key[i] = rank_of(x[i]);
-        }
+        key[i] = rank_of(x[i]);
+        if (SIG && key[i]) key[i] = rank_of(add_rn(div_rn(1.f, add_rn(1.f, expf(-x[i]))), bias[i]));
         if (lane * V + i >= a.E) key[i] = 0;
     }
     int id = -1;                                                  // lane j: the j-th choice
-    float lx = 0.f;                                               // its logit, or
-    double lp = 0.0;                                              // its sigmoid
-    for (int j = 0; j < a.top; j++) {
-        Key best = key[0];
+    float lx = 0.f;                                               // and its logit
+    bool sure = true;
+    float last = 0.f, last_x = 0.f;
+    for (int j = 0; j < a.top + (SIG ? 1 : 0); j++) {             // (SIG: the next one too, which the last has to be clear of)
+        uint32_t best = key[0];
         int at = 0;
 #pragma unroll
         for (int i = 1; i < V; i++)
             if (key[i] > best) best = key[i], at = i;
-        const uint32_t hi = SIG ? (uint32_t)((uint64_t)best >> 32) : (uint32_t)best;
-        const uint32_t most = wave_max_u32(hi);
-        if (most == 0) break;                                     // (none left; a key's high half is not 0)
-        uint64_t m = __ballot(hi == most);
-        if (SIG && (m & (m - 1))) {
-            const uint32_t lo = hi == most ? (uint32_t)best : 0u, low = wave_max_u32(lo);
-            m = __ballot(hi == most && (uint32_t)best == low);
-        }
-        const int from = __builtin_ctzll(m);
-        const int i0 = __builtin_amdgcn_readlane(at, from);
+        const uint32_t most = wave_max_u32(best);
+        if (most == 0) break;                                     // (none left)
+        const int from = __builtin_ctzll(__ballot(best == most)), i0 = __builtin_amdgcn_readlane(at, from);
         float vx = x[0];
-        double vp = p[0];
 #pragma unroll
         for (int i = 0; i < V; i++) {
             if (i == i0) {
                 vx = x[i];
-                if (SIG) vp = p[i];
                 if (lane == from) key[i] = 0;
             }
         }
+        vx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vx), from));
         if (SIG) {
-            const uint64_t u = (uint64_t)__double_as_longlong(vp);
-            const uint32_t l = __builtin_amdgcn_readlane((int)(uint32_t)u, from), h = __builtin_amdgcn_readlane((int)(u >> 32), from);
-            vp = __longlong_as_double((long long)((uint64_t)h << 32 | l));
-        } else {
-            vx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vx), from));
+            const float p = of_rank(most);
+            if (j > 0 && !(last - p > 0x1p-19f * (1.f + fabsf(last))) && (a.bias || vx != last_x)) {
+                sure = false;
+                break;
+            }
+            last = p, last_x = vx;
         }
-        if (lane == j) id = from * V + i0, lx = vx, lp = vp;
+        if (lane == j && j < a.top) id = from * V + i0, lx = vx;
+    }
+    if (SIG && !sure) {
+        uint64_t wide[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            wide[i] = rank_of(x[i]) ? rank_of(1.0 / (1.0 + exp(-(double)x[i])) + (double)bias[i]) : 0;
+            if (lane * V + i >= a.E) wide[i] = 0;
+        }
+        id = -1;
+        for (int j = 0; j < a.top; j++) {
+            uint64_t best = wide[0];
+            int at = 0;
+#pragma unroll
+            for (int i = 1; i < V; i++)
+                if (wide[i] > best) best = wide[i], at = i;
+            const uint32_t hi = (uint32_t)(best >> 32), most = wave_max_u32(hi);
+            if (most == 0) break;                                 // (a number's rank has a high half)
+            uint64_t m = __ballot(hi == most);
+            if (m & (m - 1)) {
+                const uint32_t low = wave_max_u32(hi == most ? (uint32_t)best : 0u);
+                m = __ballot(hi == most && (uint32_t)best == low);
+            }
+            const int from = __builtin_ctzll(m), i0 = __builtin_amdgcn_readlane(at, from);
+            float vx = x[0];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                if (i == i0) {
+                    vx = x[i];
+                    if (lane == from) wide[i] = 0;
+                }
+            }
+            vx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vx), from));
+            if (lane == j) id = from * V + i0, lx = vx;
+        }
     }
     float w = 0.f;
     if (SIG) {
+        const double lp = 1.0 / (1.0 + exp(-(double)lx));
         double sum = 1.0;
         if (a.renorm) {
             sum = id >= 0 ? lp : 0.0;
@@ -200,7 +231,9 @@ __device__ __forceinline__ void experts_now(const ExpertArgs& a) {
 }
 
 // The pass's live tokens (0 or less: none).
-__device__ __forceinline__ int pass_tokens(const ExpertArgs& a) { return min(min(a.T, __ldg(a.n_rows)) - a.first, a.room); }
+__device__ __forceinline__ int pass_tokens(const ExpertArgs& a) {
+    return __builtin_amdgcn_readfirstlane(min(min(a.T, __ldg(a.n_rows)) - a.first, a.room));
+}
 __device__ __forceinline__ int token_of(const ExpertArgs& a, int pair) { return (int)((uint32_t)pair * a.div >> 16); }
 
 // The expert of a pair of the pass; -1: none.
