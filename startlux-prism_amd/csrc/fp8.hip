@@ -374,7 +374,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8Gemm g, in
 
     const __amdgpu_buffer_rsrc_t wr = buf_rsrc(g.w + ((int64_t)t0 * KB + b0) * 2048);
     const __amdgpu_buffer_rsrc_t ar = PAN ? buf_rsrc(g.pa + ((int64_t)(m0 / 16) * KB + b0) * 2048)
-                                          : buf_rsrc_n(g.a + m0 * g.a_ld + b0 * 128, (uint32_t)((live - m0 - 1) * g.a_ld + nb * 128));
+                                          : buf_rsrc_n(g.a + m0 * g.a_ld + b0 * 128,
+                                                        (uint32_t)((min(live - m0, 16 * S::TA) - 1) * g.a_ld + nb * 128));
     uint32_t wsoff[S::WD], avoff[S::AD], asoff[S::AD];
     int wdst[S::WD], adst[S::AD];
 #pragma unroll
@@ -568,12 +569,12 @@ inline Fp8Plan fp8_plan(int64_t T, int64_t n, int64_t k) {
     const int64_t rows[] = {32, 64, 128, 256}, tiles[] = {8, 8, 8, 16};
     for (int kind = T <= 32 ? 1 : 2; kind <= 4; kind++) {
         const int64_t wgs = (T + rows[kind - 1] - 1) / rows[kind - 1] * ((NT + tiles[kind - 1] - 1) / tiles[kind - 1]);
-        for (int s = 1; s <= 8 && (s == 1 || KB / s >= 4); s++) {
+        for (int s = 1; s <= 8 && (s == 1 || (KB / s >= 4 && T <= 65535)); s++) {          // (the join's grid)
             const double w = (double)(wgs * s), stages = (double)((KB + s - 1) / s);
             const double x = kind == 1 ? 0.65 * (w > 256 ? w / 256 : 1) : kind == 2 ? 0.7 * (w > 256 ? w / 256 : 1)
                            : kind == 3 ? (w <= 256 ? 0.95 : 1.4 * (w > 512 ? w / 512 : 1)) : 2.0 * ceil(w / 256);
             const double t = 2.5 + fmax(stages * x, read) + (s > 1 ? 3 + 1.1e-6 * s * (double)T * (double)n : 0);
-            if (t < least) least = t, best = {kind, s, (kind == 3 && t > 45) || (kind == 4 && t > 100)};
+            if (t < least) least = t, best = {kind, s, T <= 65535 * 16 && ((kind == 3 && t > 45) || (kind == 4 && t > 100))};
         }
     }
     return best;
@@ -682,6 +683,7 @@ extern "C" int prism_fp8_gemm(const prism_fp8_gemm_args* args, void* stream) {
 #define TL(WM, WN, AR, BR, NS, E, PAN) do { \
         using S = Fp8Tile<WM, WN, AR, BR>; \
         const int tm = (int)((h.T + 16 * S::TA - 1) / (16 * S::TA)), tn = (g.NT + S::TW - 1) / S::TW; \
+        if ((int64_t)tm * tn * p.splits > INT32_MAX) return PRISM_ERR_SHAPE; \
         allow_lds(fp8_tile_kernel<WM, WN, AR, BR, NS, E, PAN>, (size_t)S::BYTES * NS); \
         hipLaunchKernelGGL((fp8_tile_kernel<WM, WN, AR, BR, NS, E, PAN>), dim3((unsigned)(tm * tn * p.splits)), dim3(64 * WM * WN), \
                            (size_t)S::BYTES * NS, st, g, tm, tn, p.splits); \
