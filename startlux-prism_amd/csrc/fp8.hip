@@ -505,10 +505,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8Gemm g, in
 // Activation rows -> panels: a workgroup per chunk of 16 rows x 128 inputs, eight lanes a row's 128 bytes.  In rows a tile's
 // copies are 128 bytes here and there, and its scales 4 bytes of a line each; in panels both are whole.
 __global__ __launch_bounds__(128) void fp8_panel_kernel(Fp8Gemm g, uint8_t* __restrict__ pa, float* __restrict__ ps) {
-    kernel_args_now(g.a, g.a_ld, g.as, g.as_ld, g.n_rows, g.T, g.KB, g.ps_ld, pa, ps);
+    kernel_args_now(g.a, g.a_ld, g.as, g.as_ld, g.T, g.KB, g.ps_ld, pa, ps);
     const int b = blockIdx.x, row = threadIdx.x >> 3, c = threadIdx.x & 7, m = blockIdx.y * 16 + row;
-    const int live = min(g.T, __ldg(g.n_rows));
-    if (m >= live) return;
+    if (m >= g.T) return;                                      // (rows that are not live are copied too: no load before these)
     const v4i v = *reinterpret_cast<const v4i*>(g.a + m * g.a_ld + b * 128 + c * 16);
     *reinterpret_cast<v4i*>(pa + ((int64_t)blockIdx.y * g.KB + b) * 2048 + (c >> 2) * 1024 + ((c & 3) * 16 + row) * 16) = v;
     if (c == 0) ps[(int64_t)b * g.ps_ld + m] = g.as[m * g.as_ld + b];

@@ -550,7 +550,6 @@ __global__ __launch_bounds__(64) void moe_sum_kernel(ExpertArgs a) {
     experts_now(a);
     const int t = blockIdx.y, c = (blockIdx.x * 64 + threadIdx.x) * 4;
     if (c >= a.H) return;
-    const int tokens = pass_tokens(a);
     v4f y = {0.f, 0.f, 0.f, 0.f};
     for (int j0 = 0; j0 < a.top; j0 += 4) {
         int id[4];
@@ -567,18 +566,24 @@ __global__ __launch_bounds__(64) void moe_sum_kernel(ExpertArgs a) {
         for (int j = 0; j < 4; j++)
             if (j0 + j < a.top && (uint32_t)id[j] < (uint32_t)a.E) y = scaled(v[j], pw[j], y);
     }
-    if (t < tokens) store_out<EPI>(a, t, c, y);
+    if (t < pass_tokens(a)) store_out<EPI>(a, t, c, y);
 }
 
-// How many of an expert's 16-row tiles a workgroup takes, of these numbers (descending): the most that leave a workgroup for every
-// CU, counting the experts that as many random ids would reach (us, up with 4 / 2 and down with 16 / 8 / 4: 11 tokens on 2 of 16
-// experts, H 5120, I 1408: 76.9 / 75.1, 67.6 / 61.3 / 64.5; 64 on 8 of 128, 2048, 768: 170 / 181, 149 / 156 / 175; 2 on 2 of 8, 4096,
-// 1792: 35.1 / 29.9, 33.4 / 27.6 / 25.4; the other kernel at one form in each).
-inline int moe_form(int64_t pairs, int64_t E, int64_t tiles, const int* per, int forms) {
+// How many of an expert's 16-row tiles a workgroup takes, of these numbers: the least of (workgroups on the fullest CU) x (tiles
+// + o), for as many experts as that many random ids would reach.  A CU reads at a rate of its own (about 23 GB/s), so the one
+// with the most workgroups ends last; o is a workgroup's own time, in tiles.  Measured (us; up with 4 / 2 / 1, o 0.25, and down
+// with 16 / 8 / 4, o 2, the other kernel at one form in each): 11 tokens on 2 of 16 experts, H 5120, I 1408: 76.9 / 75.1 / 72.8 and
+// 67.6 / 61.3 / 64.5; 64 on 8 of 128, 2048, 768: 170 / 181 / 204 and 149 / 156 / 175; 2 on 2 of 8, 4096, 1792: 35.1 / 29.9 / 30.7
+// and 33.4 / 27.6 / 25.4.
+inline int moe_form(int64_t pairs, int64_t E, int64_t tiles, const int* per, int forms, double o) {
     const double reached = (double)E * (1.0 - pow(1.0 - 1.0 / (double)E, (double)pairs));
-    for (int i = 0; i < forms - 1; i++)
-        if (reached * (double)((tiles + per[i] - 1) / per[i]) >= 300.0) return i;
-    return forms - 1;
+    int best = 0;
+    double least = 1e30;
+    for (int i = 0; i < forms; i++) {
+        const double t = ceil(reached * (double)((tiles + per[i] - 1) / per[i]) / 256.0) * (per[i] + o);
+        if (t < least) least = t, best = i;
+    }
+    return best;
 }
 
 }  // namespace prism
@@ -654,8 +659,8 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
     a.vec = h.o_ld % 4 == 0 && PRISM_ALIGNED(h.out, 8);
     const hipStream_t st = (hipStream_t)stream;
     const size_t ids_lds = (size_t)room * a.top * 4;             // the list and the ids
-    const int up_per[] = {4, 2}, down_per[] = {16, 8, 4};
-    const int up = moe_form(room * a.top, a.E, a.I / 16, up_per, 2), down = moe_form(room * a.top, a.E, a.H / 16, down_per, 3);
+    const int up_per[] = {4, 2, 1}, down_per[] = {16, 8, 4};
+    const int up = moe_form(room * a.top, a.E, a.I / 16, up_per, 3, 0.25), down = moe_form(room * a.top, a.E, a.H / 16, down_per, 3, 2);
     for (a.first = 0; a.first < a.T; a.first += kMoeTokens) {
 #define UP(N, KS, D) do { \
         const int per = kWaves / KS * N; \
@@ -667,7 +672,7 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
         hipLaunchKernelGGL((moe_down_kernel<N, KS, D>), dim3((a.H / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
                            ids_lds + (KS > 1 ? kWaves * N * 1024 : 0), st, a); \
     } while (0)
-        if (up == 0) UP(2, 2, 4); else UP(2, 4, 4);
+        if (up == 0) UP(2, 2, 4); else if (up == 1) UP(2, 4, 4); else UP(1, 4, 4);
         PRISM_LAUNCH_CHECK();
         if (down == 0) DOWN(4, 1, 3); else if (down == 1) DOWN(4, 2, 3); else DOWN(2, 2, 3);
         PRISM_LAUNCH_CHECK();
