@@ -218,10 +218,13 @@ __device__ __forceinline__ void store4(const Fp8Gemm& g, int m, int j, v4f y) {
 
 // Few rows (up to 16 MT): a workgroup owns N 16-row weight tiles, its W waves take the blocks of 128 inputs in turn (wave w block
 // w, w + W, ...) straight from memory into registers, D blocks ahead, and add their sums through LDS, wave after wave.  Rows
-// past the live ones and blocks past the last read as zeros: their offsets lie past the buffers' range, which costs no traffic,
-// and the loop has no branches.  Eight neighbouring lanes load an activation row's 128 bytes (a row per lane, as the MFMA
-// wants it, takes the memory pipeline four times as long); the wave turns them in 2 KB of its own LDS per 16 rows: piece c of
-// row r lies at slot c ^ (r % 8), so that the 16 rows of a fragment read lie on distinct banks.
+// past T and blocks past the last read as zeros: their offsets lie past the buffers' range, which costs no traffic, and the loop
+// has no branches.  Eight neighbouring lanes load an activation row's 128 bytes (a row per lane, as the MFMA wants it, takes
+// the memory pipeline four times as long); the wave turns them in 2 KB of its own LDS per 16 rows: piece c of row r lies at
+// slot c ^ (r % 8), so that the 16 rows of a fragment read lie on distinct banks.
+// One launch, no join: for small weights.  A CU reads at some 23 GB/s whatever it holds, so the CUs with two of the workgroups end
+// last: 1 x 4096 x 17408 (256 workgroups) 14.4 us (5.0 TB/s), 1 x 5120 x 17408 (320) 24; 1 x 5120 x 5120 9.6.  Waves 16 instead of
+// 8: 13.8 (one such workgroup fits a CU, the 320 take two rounds).
 template <int MT, int N, int D, int W, int EPI>
 __global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Gemm g) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -356,7 +359,14 @@ struct Fp8Tile {
 // A stage's first fragments are read before the previous stage's last products: one barrier a stage, right before those, says
 // that the next stage has arrived and that this one has been read, so its place takes the copies of stage b + NS.  Within a
 // stage each 16 rows' fragment is read one step ahead, and a step's results are folded under the next step's products.
-// EPI 2: fp32 partial sums of this part of K to g.part.
+// EPI 2: fp32 partial sums of this part of K to g.part.  PAN: the activations from panels.
+//
+// What bounds it: the copies into LDS.  At 8191 x 27648 x 5120 (256 x 256 tiles, 64 KB a stage from the L2s) the copies alone take
+// 961 us from panels and 1081 from rows, the products alone 934, both 1125 (2.06 PFLOP/s); at 333 x 5120 x 17408 the copies alone
+// take all of the 45 us (605 MB from the L2s, 13 TB/s; 145 MB of it from memory).  Few rows run at the weights' rate (16 x 5120 x
+// 17408: 17.7 us, 5.0 TB/s, and the join).  Measured and dropped: fragments read where they are used (1292), 128 x 256 tiles of 4
+// waves (a third to twice slower: one wave a SIMD), 256 x 128 tiles (333 rows 63, 4096 x 5120 x 5120 149 against 142), six stages for
+// few rows (23.0 against 21.6), the copies through registers (alone 720, but then the products wait for them: 1244 and more).
 template <int WM, int WN, int AR, int BR, int NS, int EPI, bool PAN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8Gemm g, int tiles_m, int tiles_n, int splits) {
     using S = Fp8Tile<WM, WN, AR, BR>;
@@ -503,7 +513,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8Gemm g, in
 }
 
 // Activation rows -> panels: a workgroup per chunk of 16 rows x 128 inputs, eight lanes a row's 128 bytes.  In rows a tile's
-// copies are 128 bytes here and there, and its scales 4 bytes of a line each; in panels both are whole.
+// copies are 128 bytes here and there, and its scales 4 bytes of a line each; in panels both are whole.  8191 x 5120: 21 us.
 __global__ __launch_bounds__(128) void fp8_panel_kernel(Fp8Gemm g, uint8_t* __restrict__ pa, float* __restrict__ ps) {
     kernel_args_now(g.a, g.a_ld, g.as, g.as_ld, g.T, g.KB, g.ps_ld, pa, ps);
     const int b = blockIdx.x, row = threadIdx.x >> 3, c = threadIdx.x & 7, m = blockIdx.y * 16 + row;

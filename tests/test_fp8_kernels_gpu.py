@@ -83,6 +83,19 @@ def test_rows_of_wide_buffers(fp8, dev, K):
     assert torch.equal(out, y[5:6].float().to(torch.bfloat16).expand(M, -1))
 
 
+def test_more_rows_than_a_grid_dimension(fp8, dev):
+    from prism_amd import moe
+    M, N, K = 70000, 40, 300
+    a, sa, w, sw, y = case(M, N, K, dev, 11)
+    out = torch.zeros(M, N, dtype=torch.bfloat16, device=dev)
+    fp8.gemm(a, sa, fp8.from_rows(w, sw), out, None, M)
+    assert torch.equal(out, y.float().to(torch.bfloat16))
+    x = torch.randn(M, 40, device=dev)
+    ids, wt = torch.zeros(M, 2, dtype=torch.int32, device=dev), torch.zeros(M, 2, device=dev)
+    moe.route(x, ids, wt, None, M)
+    assert torch.equal(ids.long(), x.topk(2, 1)[1])
+
+
 def test_two_threads(fp8, dev):
     """Calls that use the workspace, from two threads on their own streams."""
     ins = [case(300, 3300, 9000, dev, i) for i in range(2)]
