@@ -187,7 +187,7 @@ struct Fp8Gemm {
     const float* ps;         // and their scales [KB][ps_ld]
     int ps_ld;
     int T, n, k, KB, NT;     // NT: 16-row weight tiles
-    int vec;                 // the output's rows take whole stores of four
+    int vec;                 // the output's rows take whole stores of four values (2: of eight)
 };
 
 // Four outputs of row m, columns j .. j + 3 (those below n).
@@ -362,7 +362,7 @@ struct Fp8Tile {
 // EPI 2: fp32 partial sums of this part of K to g.part.  PAN: the activations from panels.
 //
 // What bounds it: the copies into LDS.  At 8191 x 27648 x 5120 (256 x 256 tiles, 64 KB a stage from the L2s) the copies alone take
-// 961 us from panels and 1081 from rows, the products alone 934, both 1125 (2.06 PFLOP/s); at 333 x 5120 x 17408 the copies alone
+// 961 us from panels and 1081 from rows, the products alone 934, both 1113 (2.08 PFLOP/s); at 333 x 5120 x 17408 the copies alone
 // take all of the 45 us (605 MB from the L2s, 13 TB/s; 145 MB of it from memory).  Few rows run at the weights' rate (16 x 5120 x
 // 17408: 17.7 us, 5.0 TB/s, and the join).  Measured and dropped: fragments read where they are used (1292), 128 x 256 tiles of 4
 // waves (a third to twice slower: one wave a SIMD), 256 x 128 tiles (333 rows 63, 4096 x 5120 x 5120 149 against 142), six stages for
@@ -495,6 +495,34 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8Gemm g, in
             acc[a][AR - 1] = fold(t[(AR - 1) & 1][a], now, acc[a][AR - 1]);
         }
     }
+    // bf16 rows of 64 outputs a wave, 128 bytes: turned in the wave's own part of the stages' LDS, so that eight neighbouring lanes
+    // store one row (in the products' order a row gets 32 bytes at a time: 1595 x 24704 x 1152 76.9 -> 71.5 us, 8191 x
+    // 27648 x 5120 1125 -> 1113)
+    if constexpr (EPI == 0 && BR == 4) {
+        const int j0 = 16 * (t0 + 4 * wn);
+        if (g.vec == 2 && j0 + 64 <= g.n) {
+            lds_barrier();                                                             // (every wave has read its last fragments)
+            uint8_t* own = lds + w * AR * 2048;
+            static_assert(S::W * AR * 2048 <= NS * S::BYTES, "the waves' outputs lie in the stages");
+#pragma unroll
+            for (int c = 0; c < AR; c++)
+#pragma unroll
+                for (int a = 0; a < 4; a++) {
+                    const v4f y = acc[a][c];
+                    *reinterpret_cast<v2u*>(own + (16 * c + r) * 128 + (((2 * a + (gr >> 1)) ^ (r & 7)) * 16) + (gr & 1) * 8) =
+                        v2u{f32_to_bf16(y.x) | f32_to_bf16(y.y) << 16, f32_to_bf16(y.z) | f32_to_bf16(y.w) << 16};
+                }
+            const int sub = lane >> 3, piece = lane & 7;
+#pragma unroll
+            for (int i = 0; i < AR * 2; i++) {
+                const int m = m0 + 16 * AR * wm + 8 * i + sub;
+                if (m >= live) continue;
+                *reinterpret_cast<v4u*>(reinterpret_cast<uint16_t*>(g.out) + m * g.o_ld + j0 + 8 * piece) =
+                    *reinterpret_cast<const v4u*>(own + (8 * i + sub) * 128 + ((piece ^ sub) * 16));
+            }
+            return;
+        }
+    }
 #pragma unroll
     for (int c = 0; c < AR; c++) {
         const int m = m0 + 16 * (AR * wm + c) + r;
@@ -548,15 +576,16 @@ __global__ __launch_bounds__(64) void fp8_join_kernel(Fp8Gemm g, int splits) {
 
 // Which kernel, into how many parts K is split, and whether the activations go to panels first: the least of each one's time in
 // us by what it measured (random codes, weights from memory; KB blocks of 128 inputs, NT 16-row weight tiles).
-//   stream   3 + a (blocks a CU reads), a = 0.09, 0.11, 0.107, 0.145, 0.19 for 8, 16, 32, 48, 64 rows: 16 x 1024 x 5120 6.7 (measured; a
-//            tile form 8.6), 16 x 5120 x 5120 12.0 (11.4), 16 x 5120 x 17408 30.8 (21.6), 64 x 5120 x 5120 17.5 (14.4)
-//   tiles    2.5 + (stages) x, or the weights at 5.2 TB/s: 32 x 128 (rows x outputs) x = 0.65, 64 x 128 0.7, per 256 workgroups beyond that;
-//            128 x 128 x = 0.95 up to 256, else 1.4 per 512; 256 x 256 x = 2 per whole 256: 333 x 5120 x 17408 on 128 x 128 in 4
-//            parts 59, 256 x 256 in 6 61; 1000 x 5120 x 5120 59 and (3 parts) 50; 2048 x 13824 x 5120 193 and 160; 4096 x 5120 x
-//            5120 144 and 158; 128 x 27648 x 5120 48, on 64 x 128 56
+//   stream   3 + (workgroups on the fullest CU) (a per block, at least 2.2 + 0.03 per block), a = 0.08, 0.105, 0.107, 0.145, 0.19 for
+//            8, 16, 32, 48, 64 rows: 16 x 1024 x 5120 6.7 (measured; a tile form 8.6), 16 x 5120 x 5120 12.0 (11.4), 16 x 5120 x 17408
+//            30.8 (21.6), 64 x 5120 x 5120 17.5 (14.4), 4 x 12544 x 1128 14.9
+//   tiles    2.5 + (stages) x, or the weights at 5.2 TB/s: 32 x 128 (rows x outputs) x = 0.65, 64 x 128 0.7, per 256 workgroups beyond
+//            that; 128 x 128 x = 0.95 up to 256, else 1.4 per round of 512 (a part of a round counts 0.4 more than its share, up to a
+//            round); 256 x 256 x = 2 per whole 256: 333 x 5120 x 17408 on 128 x 128 in 4 parts 59, 256 x 256 in 6 61; 1000 x 5120 x 5120
+//            59 and (3 parts) 50; 2048 x 13824 x 5120 193 and 160; 4096 x 5120 x 5120 144 and 158; 128 x 27648 x 5120 48, on 64 x 128 56
 //   parts    3 + 1.1e-6 per part and output: written, read and added by a second launch
-//   panels   past 45 us on 128 x 128 tiles (333 x 5120 x 17408 60 -> 55, 4096 x 5120 x 5120 144 -> 139; 128 x 5120 x 17408 34 -> 38),
-//            past 100 on 256 x 256 (8191 x 27648 x 5120 1161 -> 1142, the copy included; 2048 x 5120 x 5120 79 -> 81)
+//   panels   from 256 rows, past 45 us on 128 x 128 tiles (333 x 5120 x 17408 60 -> 55, 4096 x 5120 x 5120 144 -> 139; but 128 x 5120 x
+//            17408 34 -> 38), past 100 on 256 x 256 (8191 x 27648 x 5120 1161 -> 1142, the copy included; 2048 x 5120 x 5120 79 -> 81)
 struct Fp8Plan {
     int kind;            // 0 stream; tiles of rows x outputs: 1 32 x 128, 2 64 x 128, 3 128 x 128, 4 256 x 256
     int splits;
@@ -571,8 +600,8 @@ inline Fp8Plan fp8_plan(int64_t T, int64_t n, int64_t k) {
     if (T <= 64) {
         const int mt = (int)((T + 15) / 16);
         const int64_t per = mt == 1 ? 1 : 2, wgs = (NT + per - 1) / per;
-        const double a[] = {T <= 8 ? 0.09 : 0.11, 0.107, 0.145, 0.19};
-        least = 3 + a[mt - 1] * (double)((wgs + 255) / 256 * per * KB);
+        const double a[] = {T <= 8 ? 0.08 : 0.105, 0.107, 0.145, 0.19}, blocks = (double)(per * KB);
+        least = 3 + (double)((wgs + 255) / 256) * fmax(a[mt - 1] * blocks, 2.2 + 0.03 * blocks);
         best = {0, 1, 0};
     }
     const int64_t rows[] = {32, 64, 128, 256}, tiles[] = {8, 8, 8, 16};
@@ -581,9 +610,9 @@ inline Fp8Plan fp8_plan(int64_t T, int64_t n, int64_t k) {
         for (int s = 1; s <= 8 && (s == 1 || (KB / s >= 4 && T <= 65535)); s++) {          // (the join's grid)
             const double w = (double)(wgs * s), stages = (double)((KB + s - 1) / s);
             const double x = kind == 1 ? 0.65 * (w > 256 ? w / 256 : 1) : kind == 2 ? 0.7 * (w > 256 ? w / 256 : 1)
-                           : kind == 3 ? (w <= 256 ? 0.95 : 1.4 * (w > 512 ? w / 512 : 1)) : 2.0 * ceil(w / 256);
+                           : kind == 3 ? (w <= 256 ? 0.95 : 1.4 * fmin(ceil(w / 512), w > 512 ? w / 512 + 0.4 : 1)) : 2.0 * ceil(w / 256);
             const double t = 2.5 + fmax(stages * x, read) + (s > 1 ? 3 + 1.1e-6 * s * (double)T * (double)n : 0);
-            if (t < least) least = t, best = {kind, s, T <= 65535 * 16 && ((kind == 3 && t > 45) || (kind == 4 && t > 100))};
+            if (t < least) least = t, best = {kind, s, T >= 256 && T <= 65535 * 16 && ((kind == 3 && t > 45) || (kind == 4 && t > 100))};
         }
     }
     return best;
@@ -660,6 +689,7 @@ extern "C" int prism_fp8_gemm(const prism_fp8_gemm_args* args, void* stream) {
     Fp8Gemm g{h.a, h.a_ld, h.as, h.as_ld, h.w, h.ws, h.out, h.o_ld, h.n_rows, (float*)h.wsp, nullptr, nullptr, 0, (int)h.T, (int)h.n,
               (int)h.k, (int)KB, (int)((h.n + 15) / 16), 0};
     g.vec = h.o_ld % 4 == 0 && PRISM_ALIGNED(h.out, h.epi ? 16 : 8);
+    if (!h.epi && h.o_ld % 8 == 0 && PRISM_ALIGNED(h.out, 16)) g.vec = 2;
     const Fp8Plan p = fp8_plan(h.T, h.n, h.k);
     const hipStream_t st = (hipStream_t)stream;
     if (p.panels) {

@@ -575,18 +575,18 @@ __global__ __launch_bounds__(64) void moe_sum_kernel(ExpertArgs a) {
     if (t < pass_tokens(a)) store_out<EPI>(a, t, c, y);
 }
 
-// How many of an expert's 16-row tiles a workgroup takes, of these numbers: the least of (workgroups on the fullest CU) x (tiles
-// + o), for as many experts as that many random ids would reach.  A CU reads at a rate of its own (about 23 GB/s), so the one
-// with the most workgroups ends last; o is a workgroup's own time, in tiles.  Measured (us; up with 4 / 2 / 1, o 0.25, and down
-// with 16 / 8 / 4, o 2, the other kernel at one form in each): 11 tokens on 2 of 16 experts, H 5120, I 1408: 76.9 / 75.1 / 72.8 and
-// 67.6 / 61.3 / 64.5; 64 on 8 of 128, 2048, 768: 170 / 181 / 204 and 149 / 156 / 175; 2 on 2 of 8, 4096, 1792: 35.1 / 29.9 / 30.7
-// and 33.4 / 27.6 / 25.4.
-inline int moe_form(int64_t pairs, int64_t E, int64_t tiles, const int* per, int forms, double o) {
+// How many of an expert's 16-row tiles a workgroup takes, of these numbers: the least of (workgroups on the fullest CU) x (its
+// tiles' time + 2 us), for as many experts as that many random ids would reach.  A CU reads at a rate of its own (about 23 GB/s:
+// tile_us), so the one with the most workgroups ends last; 2 us go into a workgroup's start and end.  Measured (us; up with 4 / 2 /
+// 1 tiles and down with 16 / 8 / 4, the other kernel at one form in each): 11 tokens on 2 of 16 experts, H 5120, I 1408: 76.9 / 75.1
+// / 72.8 and 67.6 / 61.3 / 64.5; 64 on 8 of 128, 2048, 768: 170 / 181 / 204 and 149 / 156 / 175; 2 on 2 of 8, 4096, 1792: 35.1 / 29.9
+// / 30.7 and 33.4 / 27.6 / 25.4.
+inline int moe_form(int64_t pairs, int64_t E, int64_t tiles, double tile_us, const int* per, int forms) {
     const double reached = (double)E * (1.0 - pow(1.0 - 1.0 / (double)E, (double)pairs));
     int best = 0;
     double least = 1e30;
     for (int i = 0; i < forms; i++) {
-        const double t = ceil(reached * (double)((tiles + per[i] - 1) / per[i]) / 256.0) * (per[i] + o);
+        const double t = ceil(reached * (double)((tiles + per[i] - 1) / per[i]) / 256.0) * (per[i] * tile_us + 2);
         if (t < least) least = t, best = i;
     }
     return best;
@@ -666,7 +666,8 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
     const hipStream_t st = (hipStream_t)stream;
     const size_t ids_lds = (size_t)room * a.top * 4;             // the list and the ids
     const int up_per[] = {4, 2, 1}, down_per[] = {16, 8, 4};
-    const int up = moe_form(room * a.top, a.E, a.I / 16, up_per, 3, 0.25), down = moe_form(room * a.top, a.E, a.H / 16, down_per, 3, 2);
+    const int up = moe_form(room * a.top, a.E, a.I / 16, 0.178 * a.KBH, up_per, 3);
+    const int down = moe_form(room * a.top, a.E, a.H / 16, 0.089 * a.KBI, down_per, 3);
     for (a.first = 0; a.first < a.T; a.first += kMoeTokens) {
 #define UP(N, KS, D) do { \
         const int per = kWaves / KS * N; \
