@@ -500,8 +500,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void fp8_tile_kernel(Fp8Gemm g, in
     // 27648 x 5120 1125 -> 1113)
     if constexpr (EPI == 0 && BR == 4) {
         const int j0 = 16 * (t0 + 4 * wn);
+        if (g.vec == 2) lds_barrier();                                                 // (every wave has read its last fragments)
         if (g.vec == 2 && j0 + 64 <= g.n) {
-            lds_barrier();                                                             // (every wave has read its last fragments)
             uint8_t* own = lds + w * AR * 2048;
             static_assert(S::W * AR * 2048 <= NS * S::BYTES, "the waves' outputs lie in the stages");
 #pragma unroll
