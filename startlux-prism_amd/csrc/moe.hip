@@ -225,7 +225,6 @@ struct ExpertArgs {
     int first, room;                         // the pass's tokens: room from first on
     int slots;                               // experts looked at per pass: all, or one per pair where those are fewer
     int vec;
-    int xcd;
 };
 
 // Every argument a kernel goes by in scalar registers at once: loaded where they are first used they come one memory round
@@ -660,8 +659,6 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
     a.T = (int)h.T, a.E = (int)h.E, a.top = (int)h.top, a.H = (int)h.H, a.I = (int)h.I;
     a.KBH = (int)((h.H + 127) / 128), a.KBI = (int)((h.I + 127) / 128);
     a.div = 65536u / (uint32_t)h.top + 1;
-    a.room = (int)room;
-    a.slots = room * a.top < a.E ? (int)room * a.top : a.E;
     a.vec = h.o_ld % 4 == 0 && PRISM_ALIGNED(h.out, 8);
     const hipStream_t st = (hipStream_t)stream;
     const size_t ids_lds = (size_t)room * a.top * 4;             // the list and the ids
@@ -669,6 +666,8 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
     const int up = moe_form(room * a.top, a.E, a.I / 16, 0.178 * a.KBH, up_per, 3);
     const int down = moe_form(room * a.top, a.E, a.H / 16, 0.089 * a.KBI, down_per, 3);
     for (a.first = 0; a.first < a.T; a.first += kMoeTokens) {
+        a.room = a.T - a.first < kMoeTokens ? a.T - a.first : kMoeTokens;      // (every row up to there is the caller's)
+        a.slots = a.room * a.top < a.E ? a.room * a.top : a.E;
 #define UP(N, KS, D) do { \
         const int per = kWaves / KS * N; \
         hipLaunchKernelGGL((moe_up_kernel<N, KS, D>), dim3((a.I / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
@@ -685,7 +684,7 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
         PRISM_LAUNCH_CHECK();
 #undef UP
 #undef DOWN
-        const dim3 grid((a.H / 4 + 63) / 64, (unsigned)room);
+        const dim3 grid((a.H / 4 + 63) / 64, (unsigned)a.room);
         if (h.epi) hipLaunchKernelGGL((moe_sum_kernel<1>), grid, dim3(64), 0, st, a);
         else hipLaunchKernelGGL((moe_sum_kernel<0>), grid, dim3(64), 0, st, a);
         PRISM_LAUNCH_CHECK();

@@ -222,6 +222,25 @@ def test_experts_named_twice_or_not_at_all(moe, fp8, dev, T, E, top):
     assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
 
 
+@pytest.mark.parametrize("T,E,top", [(129, 4, 4), (131, 600, 2), (140, 300, 8), (255, 20, 1)])
+def test_experts_last_pass(moe, fp8, dev, T, E, top):
+    """A last pass of few tokens (its pairs found in another way than the first pass's) leaves a token what it gets with other
+    tokens behind it; no tensor has a row past the last."""
+    H, I = 80, 48
+    ws, plain = make(E, H, I, 5, fp8, dev)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn(256, H, generator=g).to(torch.bfloat16)
+    ids = torch.randint(0, E, (256, top), generator=g).int()
+    w = torch.rand(256, top, generator=g)
+    outs = []
+    for rows in (T, 256):
+        out = torch.zeros(rows, H, dtype=torch.bfloat16, device=dev)
+        moe.experts(x[:rows].to(dev), ids[:rows].to(dev), w[:rows].to(dev), *ws, out, None, rows)
+        outs.append(out.cpu())
+    check(outs[0][120:], *plain_experts(x[120:T], ids[120:T], w[120:T], plain))
+    assert torch.equal(outs[0], outs[1][:T])
+
+
 def test_experts_all_tokens_on_one(moe, fp8, dev):
     """More tokens than a tile on one expert, the others idle."""
     E, H, I, T = 20, 128, 64, 100
