@@ -222,11 +222,15 @@ __device__ __forceinline__ void store4(const Fp8Gemm& g, int m, int j, v4f y) {
 // has no branches.  Eight neighbouring lanes load an activation row's 128 bytes (a row per lane, as the MFMA wants it, takes
 // the memory pipeline four times as long); the wave turns them in 2 KB of its own LDS per 16 rows: piece c of row r lies at
 // slot c ^ (r % 8), so that the 16 rows of a fragment read lie on distinct banks.
-// One launch, no join: for small weights.  A CU reads at some 23 GB/s whatever it holds, so the CUs with two of the workgroups end
-// last: 1 x 4096 x 17408 (256 workgroups) 14.4 us (5.0 TB/s), 1 x 5120 x 17408 (320) 24; 1 x 5120 x 5120 9.6.  Waves 16 instead of
-// 8: 13.8 (one such workgroup fits a CU, the 320 take two rounds).
-template <int MT, int N, int D, int W, int EPI>
-__global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Gemm g) {
+// PA 1: up to 8 rows, one load a block instead of two.
+// One launch, no join: for small weights and few rows.  What a load takes to issue counts as much as its bytes: 1 x 5120 x 5120 (320
+// workgroups) took 10.1 us with the last round of a ring asking past the end and two loads of activations a block, 8.8 without
+// the second, 7.4 with neither (8 waves; 4: 6.5-7.3, 3.6-4.1 TB/s; 1 x 13824 x 5120 13.3 and 12.8, 5.5 TB/s; 64 x 12544 x 1128 11.8 and 9.0).
+// More stages than 5 or fewer: 7.6 (4), 7.7 (3), 8.1 (7).
+constexpr int kStreamWaves = 4;
+template <int MT, int N, int D, int PA, int EPI>
+__global__ __launch_bounds__(64 * kStreamWaves) void fp8_stream_kernel(Fp8Gemm g) {
+    constexpr int W = kStreamWaves;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     // (arguments loaded where they are first used come one memory round trip after another)
     kernel_args_now(g.a, g.a_ld, g.as, g.as_ld, g.w, g.ws, g.out, g.o_ld, g.n_rows, g.T, g.n, g.KB, g.NT, g.vec);
@@ -240,7 +244,7 @@ __global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Gemm g) {
     const __amdgpu_buffer_rsrc_t br = buf_rsrc(g.ws + (int64_t)(t0 >> 3) * KB);    // (N tiles lie in one block of 128 rows)
     constexpr uint32_t kOut = 0x80000000u;
     struct Stage {
-        v4i w[N][2], a[MT][2];
+        v4i w[N][2], a[MT][PA];
         float s[MT], sw;
     } st[D];
     auto issue_w = [&](Stage& x, int b) {
@@ -255,11 +259,11 @@ __global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Gemm g) {
     const int rows = min(g.T - m0, 16 * MT);
     const __amdgpu_buffer_rsrc_t ar = buf_rsrc_n(g.a + m0 * g.a_ld, (uint32_t)((rows - 1) * g.a_ld + KB * 128));
     const __amdgpu_buffer_rsrc_t sr = buf_rsrc_n(g.as + m0 * g.as_ld, (uint32_t)((rows - 1) * g.as_ld + KB) * 4);
-    uint32_t aoff[MT][2], soff[MT];
+    uint32_t aoff[MT][PA], soff[MT];
 #pragma unroll
     for (int c = 0; c < MT; c++) {
 #pragma unroll
-        for (int p = 0; p < 2; p++) {
+        for (int p = 0; p < PA; p++) {
             const int m = 16 * c + 8 * p + (lane >> 3);
             aoff[c][p] = m < rows ? (uint32_t)(m * g.a_ld + 16 * (lane & 7)) : kOut;
         }
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Gemm g) {
 #pragma unroll
         for (int c = 0; c < MT; c++) {
 #pragma unroll
-            for (int p = 0; p < 2; p++) x.a[c][p] = buf_load16(ar, aoff[c][p] | past, bc * 128);
+            for (int p = 0; p < PA; p++) x.a[c][p] = buf_load16(ar, aoff[c][p] | past, bc * 128);
             x.s[c] = __uint_as_float(buf_load4(sr, soff[c] | past, bc * 4));
         }
     };
@@ -290,29 +294,35 @@ __global__ __launch_bounds__(64 * W) void fp8_stream_kernel(Fp8Gemm g) {
     }
     const int live = min(g.T, n_rows) - m0;
     if (live <= 0) return;
-    for (int b = w; b < KB; b += D * W) {
+    auto use = [&](const Stage& x) {
+#pragma unroll
+        for (int c = 0; c < MT; c++)
+#pragma unroll
+            for (int p = 0; p < PA; p++) *reinterpret_cast<v4i*>(turn + c * 2048 + p * 1024 + put) = x.a[c][p];
+#pragma unroll
+        for (int c = 0; c < MT; c++) {
+            const v8i a = join8(*reinterpret_cast<const v4i*>(turn + c * 2048 + get0),
+                                *reinterpret_cast<const v4i*>(turn + c * 2048 + get1));
+            const float s = mul_rn(x.s[c], x.sw);
+#pragma unroll
+            for (int t = 0; t < N; t++) acc[t][c] = fold(fp8_mfma(join8(x.w[t][0], x.w[t][1]), a), s, acc[t][c]);
+        }
+    };
+    for (int b = w; b + D * W < KB; b += D * W) {
 #pragma unroll
         for (int d = 0; d < D; d++) {
-            const int at = b + d * W;
-#pragma unroll
-            for (int c = 0; c < MT; c++)
-#pragma unroll
-                for (int p = 0; p < 2; p++) *reinterpret_cast<v4i*>(turn + c * 2048 + p * 1024 + put) = st[d].a[c][p];
-#pragma unroll
-            for (int c = 0; c < MT; c++) {
-                const v8i a = join8(*reinterpret_cast<const v4i*>(turn + c * 2048 + get0),
-                                    *reinterpret_cast<const v4i*>(turn + c * 2048 + get1));
-                const float s = mul_rn(st[d].s[c], st[d].sw);
-#pragma unroll
-                for (int t = 0; t < N; t++)
-                    acc[t][c] = fold(fp8_mfma(join8(st[d].w[t][0], st[d].w[t][1]), a), s, acc[t][c]);
-            }
-            issue_w(st[d], at + D * W);
-            issue_a(st[d], at + D * W);
+            use(st[d]);
+            issue_w(st[d], b + (d + D) * W);
+            issue_a(st[d], b + (d + D) * W);
             // (else the uses of all stages gather in front and wait for all loads; the loads before the loop are kept in the same
             // order, as the wait in it has to serve both)
             __builtin_amdgcn_sched_barrier(0);
         }
+    }
+#pragma unroll
+    for (int d = 0; d < D; d++) {                       // (the last round asks for nothing: loads past the end cost their issue)
+        use(st[d]);
+        __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();                                                                   // (the sums lie over the turns)
     v4f* red = reinterpret_cast<v4f*>(lds);
@@ -576,11 +586,11 @@ __global__ __launch_bounds__(64) void fp8_join_kernel(Fp8Gemm g, int splits) {
 
 // Which kernel, into how many parts K is split, and whether the activations go to panels first: the least of each one's time in
 // us by what it measured (random codes, weights from memory; KB blocks of 128 inputs, NT 16-row weight tiles).
-//   stream   3 + (workgroups on the fullest CU) (a per block, at least 2.2 + 0.03 per block), a = 0.08, 0.105, 0.107, 0.145, 0.19 for
-//            8, 16, 32, 48, 64 rows: 16 x 1024 x 5120 6.7 (measured; a tile form 8.6), 16 x 5120 x 5120 12.0 (11.4), 16 x 5120 x 17408
-//            30.8 (21.6), 64 x 5120 x 5120 17.5 (14.4), 4 x 12544 x 1128 14.9
-//   tiles    2.5 + (stages) x, or the weights at 5.2 TB/s: 32 x 128 (rows x outputs) x = 0.65, 64 x 128 0.7, per 256 workgroups beyond
-//            that; 128 x 128 x = 0.95 up to 256, else 1.4 per round of 512 (a part of a round counts 0.4 more than its share, up to a
+//   stream   2.6 + (workgroups on the fullest CU) a per block, and 0.5 per workgroup after the first; a = 0.06, 0.085, 0.1, 0.127, 0.16
+//            for 8, 16, 32, 48, 64 rows: 8 x 13824 x 5120 14.0 (measured; the best tile form 17.3), 8 x 5120 x 17408 21.2 (20.0), 16 x
+//            1024 x 5120 5.9 (7.7), 16 x 5120 x 5120 9.8 (10.5), 16 x 5120 x 17408 27.2 (20.7), 64 x 5120 x 5120 15.5 (13.9)
+//   tiles    2.5 + (stages) x, or the weights at 5.2 TB/s: 32 x 128 (rows x outputs) x = 0.65 with 256 workgroups, down to half of that
+//            with few (16 x 512 x 17408 in 1 and 8 parts 47.8 and 10.7), 64 x 128 0.7, per 256 workgroups beyond that; 128 x 128 x = 0.95 up to 256, else 1.4 per round of 512 (a part of a round counts 0.4 more than its share, up to a
 //            round); 256 x 256 x = 2 per whole 256: 333 x 5120 x 17408 on 128 x 128 in 4 parts 59, 256 x 256 in 6 61; 1000 x 5120 x 5120
 //            59 and (3 parts) 50; 2048 x 13824 x 5120 193 and 160; 4096 x 5120 x 5120 144 and 158; 128 x 27648 x 5120 48, on 64 x 128 56
 //   parts    3 + 1.1e-6 per part and output: written, read and added by a second launch
@@ -600,8 +610,8 @@ inline Fp8Plan fp8_plan(int64_t T, int64_t n, int64_t k) {
     if (T <= 64) {
         const int mt = (int)((T + 15) / 16);
         const int64_t per = mt == 1 ? 1 : 2, wgs = (NT + per - 1) / per;
-        const double a[] = {T <= 8 ? 0.08 : 0.105, 0.107, 0.145, 0.19}, blocks = (double)(per * KB);
-        least = 3 + (double)((wgs + 255) / 256) * fmax(a[mt - 1] * blocks, 2.2 + 0.03 * blocks);
+        const double a[] = {T <= 8 ? 0.06 : 0.085, 0.1, 0.127, 0.16}, fullest = (double)((wgs + 255) / 256);
+        least = 2.6 + fullest * a[mt - 1] * (double)(per * KB) + 0.5 * (fullest - 1);
         best = {0, 1, 0};
     }
     const int64_t rows[] = {32, 64, 128, 256}, tiles[] = {8, 8, 8, 16};
@@ -609,7 +619,7 @@ inline Fp8Plan fp8_plan(int64_t T, int64_t n, int64_t k) {
         const int64_t wgs = (T + rows[kind - 1] - 1) / rows[kind - 1] * ((NT + tiles[kind - 1] - 1) / tiles[kind - 1]);
         for (int s = 1; s <= 8 && (s == 1 || (KB / s >= 4 && T <= 65535)); s++) {          // (the join's grid)
             const double w = (double)(wgs * s), stages = (double)((KB + s - 1) / s);
-            const double x = kind == 1 ? 0.65 * (w > 256 ? w / 256 : 1) : kind == 2 ? 0.7 * (w > 256 ? w / 256 : 1)
+            const double x = kind == 1 ? 0.65 * (w > 256 ? w / 256 : 0.5 + w / 512) : kind == 2 ? 0.7 * (w > 256 ? w / 256 : 1)
                            : kind == 3 ? (w <= 256 ? 0.95 : 1.4 * fmin(ceil(w / 512), w > 512 ? w / 512 + 0.4 : 1)) : 2.0 * ceil(w / 256);
             const double t = 2.5 + fmax(stages * x, read) + (s > 1 ? 3 + 1.1e-6 * s * (double)T * (double)n : 0);
             if (t < least) least = t, best = {kind, s, T >= 256 && T <= 65535 * 16 && ((kind == 3 && t > 45) || (kind == 4 && t > 100))};
@@ -702,17 +712,16 @@ extern "C" int prism_fp8_gemm(const prism_fp8_gemm_args* args, void* stream) {
     }
 #define EP(f) do { if (h.epi) f(1); else f(0); } while (0)
     if (p.kind == 0) {
-#define ST(MT, N, D, W, E) do { \
-        const size_t bytes = (size_t)MT * (N > 2 ? N : 2) * W * 1024; \
-        allow_lds(fp8_stream_kernel<MT, N, D, W, E>, bytes); \
-        hipLaunchKernelGGL((fp8_stream_kernel<MT, N, D, W, E>), dim3((g.NT + N - 1) / N, (unsigned)((h.T + 16 * MT - 1) / (16 * MT))), \
-                           dim3(64 * W), bytes, st, g); \
-    } while (0)
-#define S1(E) ST(1, 1, 5, 8, E)
-#define S2(E) ST(2, 2, 2, 8, E)
-#define S3(E) ST(3, 2, 2, 8, E)
-#define S4(E) ST(4, 2, 2, 8, E)
-        if (h.T <= 16) EP(S1); else if (h.T <= 32) EP(S2); else if (h.T <= 48) EP(S3); else EP(S4);
+#define ST(MT, N, D, PA, E) \
+        hipLaunchKernelGGL((fp8_stream_kernel<MT, N, D, PA, E>), dim3((g.NT + N - 1) / N, (unsigned)((h.T + 16 * MT - 1) / (16 * MT))), \
+                           dim3(64 * kStreamWaves), (size_t)MT * 2 * kStreamWaves * 1024, st, g)
+#define S0(E) ST(1, 1, 5, 1, E)
+#define S1(E) ST(1, 1, 5, 2, E)
+#define S2(E) ST(2, 2, 2, 2, E)
+#define S3(E) ST(3, 2, 2, 2, E)
+#define S4(E) ST(4, 2, 2, 2, E)
+        if (h.T <= 8) EP(S0); else if (h.T <= 16) EP(S1); else if (h.T <= 32) EP(S2); else if (h.T <= 48) EP(S3); else EP(S4);
+#undef S0
 #undef S1
 #undef S2
 #undef S3

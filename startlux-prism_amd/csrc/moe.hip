@@ -367,28 +367,36 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_up_kernel(ExpertArgs a) {
             issue(st[d], q + d * KS);
             __builtin_amdgcn_sched_barrier(0);
         }
-        for (int b = q; b < a.KBH; b += D * KS) {
+        auto use = [&](const Stage& s) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                v4f tg = {0.f, 0.f, 0.f, 0.f}, tu = tg;
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    v8bf lo, hi;
+                    widen(s.g[i][p], lo, hi);
+                    tg = bf_mfma(hi, s.x[2 * p + 1], bf_mfma(lo, s.x[2 * p], tg));
+                    widen(s.u[i][p], lo, hi);
+                    tu = bf_mfma(hi, s.x[2 * p + 1], bf_mfma(lo, s.x[2 * p], tu));
+                }
+                ga[i] = scaled(tg, s.gs, ga[i]);
+                ua[i] = scaled(tu, s.us, ua[i]);
+            }
+        };
+        for (int b = q; b + D * KS < a.KBH; b += D * KS) {
 #pragma unroll
             for (int d = 0; d < D; d++) {
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    v4f tg = {0.f, 0.f, 0.f, 0.f}, tu = tg;
-#pragma unroll
-                    for (int p = 0; p < 2; p++) {
-                        v8bf lo, hi;
-                        widen(st[d].g[i][p], lo, hi);
-                        tg = bf_mfma(hi, st[d].x[2 * p + 1], bf_mfma(lo, st[d].x[2 * p], tg));
-                        widen(st[d].u[i][p], lo, hi);
-                        tu = bf_mfma(hi, st[d].x[2 * p + 1], bf_mfma(lo, st[d].x[2 * p], tu));
-                    }
-                    ga[i] = scaled(tg, st[d].gs, ga[i]);
-                    ua[i] = scaled(tu, st[d].us, ua[i]);
-                }
+                use(st[d]);
                 issue(st[d], b + (d + D) * KS);
                 // (else the uses of all stages gather in front and wait for all loads; the loads before the loop are kept in the
                 // same order, as the wait in it has to serve both)
                 __builtin_amdgcn_sched_barrier(0);
             }
+        }
+#pragma unroll
+        for (int d = 0; d < D; d++) {                   // (the last round asks for nothing: loads past the end cost their issue)
+            use(st[d]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (KS > 1) {
             if (base) __syncthreads();                                        // (the sums before are read)
@@ -484,26 +492,33 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
             issue(st[d], q + d * KS);
             __builtin_amdgcn_sched_barrier(0);
         }
-        for (int b = q; b < a.KBI; b += D * KS) {
+        auto use = [&](const Stage& s) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                v4f t = {0.f, 0.f, 0.f, 0.f}, l = t;
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    v8bf lo, hi;
+                    widen(s.d[i][p], lo, hi);
+                    t = bf_mfma(hi, s.h[0][2 * p + 1], bf_mfma(lo, s.h[0][2 * p], t));
+                    l = bf_mfma(hi, s.h[1][2 * p + 1], bf_mfma(lo, s.h[1][2 * p], l));
+                }
+                y[i] = scaled(l, s.s, scaled(t, s.s, y[i]));
+            }
+        };
+        for (int b = q; b + D * KS < a.KBI; b += D * KS) {
 #pragma unroll
             for (int d = 0; d < D; d++) {
-#pragma unroll
-                for (int i = 0; i < N; i++) {
-                    v4f t = {0.f, 0.f, 0.f, 0.f}, l = t;
-#pragma unroll
-                    for (int p = 0; p < 2; p++) {
-                        v8bf lo, hi;
-                        widen(st[d].d[i][p], lo, hi);
-                        t = bf_mfma(hi, st[d].h[0][2 * p + 1], bf_mfma(lo, st[d].h[0][2 * p], t));
-                        l = bf_mfma(hi, st[d].h[1][2 * p + 1], bf_mfma(lo, st[d].h[1][2 * p], l));
-                    }
-                    y[i] = scaled(l, st[d].s, scaled(t, st[d].s, y[i]));
-                }
+                use(st[d]);
                 issue(st[d], b + (d + D) * KS);
-                // (else the uses of all stages gather in front and wait for all loads; the loads before the loop are kept in the
-                // same order, as the wait in it has to serve both)
+                // (as in the up kernel)
                 __builtin_amdgcn_sched_barrier(0);
             }
+        }
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            use(st[d]);
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (KS > 1) {
             if (base) __syncthreads();
