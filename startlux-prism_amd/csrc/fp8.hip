@@ -225,8 +225,8 @@ __device__ __forceinline__ void store4(const Fp8Gemm& g, int m, int j, v4f y) {
 // PA 1: up to 8 rows, one load a block instead of two.
 // One launch, no join: for small weights and few rows.  What a load takes to issue counts as much as its bytes: 1 x 5120 x 5120 (320
 // workgroups) took 10.1 us with the last round of a ring asking past the end and two loads of activations a block, 8.8 without
-// the second, 7.4 with neither (8 waves; 4: 6.5-7.3, 3.6-4.1 TB/s; 1 x 13824 x 5120 13.3 and 12.8, 5.5 TB/s; 64 x 12544 x 1128 11.8 and 9.0).
-// More stages than 5 or fewer: 7.6 (4), 7.7 (3), 8.1 (7).
+// the second, 7.4 with neither (8 waves; 4: 6.5-7.3, 3.6-4.1 TB/s; 1 x 13824 x 5120 13.3 and 12.8, 5.5 TB/s; 64 x 12544 x 1128 11.8
+// and 9.0).  More stages than 5 or fewer: 7.6 (4), 7.7 (3), 8.1 (7).
 constexpr int kStreamWaves = 4;
 template <int MT, int N, int D, int PA, int EPI>
 __global__ __launch_bounds__(64 * kStreamWaves) void fp8_stream_kernel(Fp8Gemm g) {
@@ -374,7 +374,7 @@ struct Fp8Tile {
 // What bounds it: the copies into LDS.  At 8191 x 27648 x 5120 (256 x 256 tiles, 64 KB a stage from the L2s) the copies alone take
 // 961 us from panels and 1081 from rows, the products alone 934, both 1113 (2.08 PFLOP/s); at 333 x 5120 x 17408 the copies alone
 // take all of the 45 us (605 MB from the L2s, 13 TB/s; 145 MB of it from memory).  Few rows run at the weights' rate (16 x 5120 x
-// 17408: 17.7 us, 5.0 TB/s, and the join).  Measured and dropped: fragments read where they are used (1292), 128 x 256 tiles of 4
+// 17408: 15.9 us, 5.6 TB/s, and the join).  Measured and dropped: fragments read where they are used (1292), 128 x 256 tiles of 4
 // waves (a third to twice slower: one wave a SIMD), 256 x 128 tiles (333 rows 63, 4096 x 5120 x 5120 149 against 142), six stages for
 // few rows (23.0 against 21.6), the copies through registers (alone 720, but then the products wait for them: 1244 and more).
 template <int WM, int WN, int AR, int BR, int NS, int EPI, bool PAN>
@@ -589,10 +589,13 @@ __global__ __launch_bounds__(64) void fp8_join_kernel(Fp8Gemm g, int splits) {
 //   stream   2.6 + (workgroups on the fullest CU) a per block, and 0.5 per workgroup after the first; a = 0.06, 0.085, 0.1, 0.127, 0.16
 //            for 8, 16, 32, 48, 64 rows: 8 x 13824 x 5120 14.0 (measured; the best tile form 17.3), 8 x 5120 x 17408 21.2 (20.0), 16 x
 //            1024 x 5120 5.9 (7.7), 16 x 5120 x 5120 9.8 (10.5), 16 x 5120 x 17408 27.2 (20.7), 64 x 5120 x 5120 15.5 (13.9)
-//   tiles    2.5 + (stages) x, or the weights at 5.2 TB/s: 32 x 128 (rows x outputs) x = 0.65 with 256 workgroups, down to half of that
-//            with few (16 x 512 x 17408 in 1 and 8 parts 47.8 and 10.7), 64 x 128 0.7, per 256 workgroups beyond that; 128 x 128 x = 0.95 up to 256, else 1.4 per round of 512 (a part of a round counts 0.4 more than its share, up to a
-//            round); 256 x 256 x = 2 per whole 256: 333 x 5120 x 17408 on 128 x 128 in 4 parts 59, 256 x 256 in 6 61; 1000 x 5120 x 5120
-//            59 and (3 parts) 50; 2048 x 13824 x 5120 193 and 160; 4096 x 5120 x 5120 144 and 158; 128 x 27648 x 5120 48, on 64 x 128 56
+//   tiles    2.5 + (stages) x, or the weights at 5.2 TB/s, less with under 256 workgroups (16 x 5120 x 17408 in 5 and 6 parts, 200 and
+//            240 workgroups: 19.2 and 18.7): 32 x 128 (rows x outputs) x = 0.65 with 256 workgroups, down to half of that with few (16 x
+//            512 x 17408 in 1 and 8 parts 47.8 and 10.7), 64 x 128 0.7, both per round of 256 (48 x 13824 x 5120 in 2 and 3 parts, 216
+//            and 324 workgroups: 21.7 and 27.5); 128 x 128 x = 0.95 up to 256, else 1.4 per round of 512 (a part of a round counts
+//            0.4 more than its share, up to a round); 256 x 256 x = 2 per whole 256: 333 x 5120 x 17408 on 128 x 128 in 4 parts 59,
+//            256 x 256 in 6 61; 1000 x 5120 x 5120 59 and (3 parts) 50; 2048 x 13824 x 5120 193 and 160; 4096 x 5120 x 5120 144 and
+//            158; 128 x 27648 x 5120 48, on 64 x 128 56
 //   parts    3 + 1.1e-6 per part and output: written, read and added by a second launch
 //   panels   from 256 rows, past 45 us on 128 x 128 tiles (333 x 5120 x 17408 60 -> 55, 4096 x 5120 x 5120 144 -> 139; but 128 x 5120 x
 //            17408 34 -> 38), past 100 on 256 x 256 (8191 x 27648 x 5120 1161 -> 1142, the copy included; 2048 x 5120 x 5120 79 -> 81)
@@ -619,9 +622,9 @@ inline Fp8Plan fp8_plan(int64_t T, int64_t n, int64_t k) {
         const int64_t wgs = (T + rows[kind - 1] - 1) / rows[kind - 1] * ((NT + tiles[kind - 1] - 1) / tiles[kind - 1]);
         for (int s = 1; s <= 8 && (s == 1 || (KB / s >= 4 && T <= 65535)); s++) {          // (the join's grid)
             const double w = (double)(wgs * s), stages = (double)((KB + s - 1) / s);
-            const double x = kind == 1 ? 0.65 * (w > 256 ? w / 256 : 0.5 + w / 512) : kind == 2 ? 0.7 * (w > 256 ? w / 256 : 1)
+            const double x = kind == 1 ? 0.65 * (w > 256 ? ceil(w / 256) : 0.5 + w / 512) : kind == 2 ? 0.7 * ceil(w / 256)
                            : kind == 3 ? (w <= 256 ? 0.95 : 1.4 * fmin(ceil(w / 512), w > 512 ? w / 512 + 0.4 : 1)) : 2.0 * ceil(w / 256);
-            const double t = 2.5 + fmax(stages * x, read) + (s > 1 ? 3 + 1.1e-6 * s * (double)T * (double)n : 0);
+            const double t = 2.5 + fmax(stages * x, read * (w < 256 ? 1.25 - w / 1024 : 1)) + (s > 1 ? 3 + 1.1e-6 * s * (double)T * (double)n : 0);
             if (t < least) least = t, best = {kind, s, T >= 256 && T <= 65535 * 16 && ((kind == 3 && t > 45) || (kind == 4 && t > 100))};
         }
     }

@@ -14,11 +14,12 @@
 // output's own rounding), moe_down_kernel each pair's outputs in fp32, moe_sum_kernel adds a token's in the order of its ids:
 // no atomics, and what a token gets does not depend on the others but for how K is split.
 //
-// The weights' bytes bound it: 64 tokens on 8 of 128 experts (H 2048, I 768; 594 MB) up 74, down 47, sum 4.5 us, 116 in all (5.1
-// TB/s; memory read alone runs at 6.0); 11 tokens on 2 of 16 (5120, 1408; 265 MB) 43, 22 and 4.5, 64 in all; one token on 8 of 128
-// (38 MB) 8.5, 5 and 2.5, 17.4 in all: three launches and their first loads.  Measured and dropped: the outputs of all experts
-// summed by one workgroup per 16 outputs (64 tokens: down 160 us), or for one token a wave per pair (12 us against 5 + 2.5: each CU then
-// goes to eight experts' pages); experts dealt out over the XCDs (no change, 11 tokens 75 against 62).
+// The weights' bytes bound it: 64 tokens on 8 of 128 experts (H 2048, I 768; 594 MB) up 67, down 40, sum 4.7 us, 109 in all (5.5
+// TB/s; memory read alone runs at 6.0); 11 tokens on 2 of 16 (5120, 1408; 265 MB) 33, 15 and 4.6, 53 in all; one token on 8 of 128
+// (38 MB) 7.4, 4.1 and 2.9, 15.3 in all: three launches and their first loads.  Loads count by their number too: a ring's last round
+// that asked past the end made these 115, 64 and 17.2.  Measured and dropped: the outputs of all experts summed by one workgroup per
+// 16 outputs (64 tokens: down 160 us), or for one token a wave per pair (12 us against 5 + 2.5: each CU then goes to eight experts'
+// pages); experts dealt out over the XCDs (no change, 11 tokens 75 against 62).
 #include <math.h>
 
 #include <type_traits>
@@ -440,8 +441,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_up_kernel(ExpertArgs a) {
     }
 }
 
-// The same for the outputs of one expert: N tiles share a chunk's hidden values.
-template <int N, int KS, int D>
+// The same for the outputs of one expert: N tiles share a chunk's hidden values, C pairs at a time.  C 8: the 16 columns are eight
+// pairs' first parts and their second parts, half the loads and products of C 16, where they are two operands; an expert of
+// more pairs reads its weights again for each C.
+template <int N, int KS, int D, int C>
 __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     experts_now(a);
@@ -458,14 +461,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
     const __amdgpu_buffer_rsrc_t dr = buf_rsrc(a.down + ((int64_t)e * tiles + tc) * row);
     const __amdgpu_buffer_rsrc_t dsr = buf_rsrc(a.down_s + ((int64_t)e * ((a.H + 127) >> 7) + (tc >> 3)) * a.KBI);
     const __amdgpu_buffer_rsrc_t hr = buf_rsrc_n(a.h, (uint32_t)(tokens * a.top) * hrow);
+    constexpr int P = C == 8 ? 1 : 2;                                         // operands of hidden values
     struct Stage {
-        v4i d[N][2], h[2][4];
+        v4i d[N][2], h[P][4];
         float s;
     } st[D];
-    for (int base = 0; base < n; base += 16) {
-        const bool there = base + r < n;
-        const int pair = there ? list[base + r] : 0;
-        const uint32_t ho = there ? (uint32_t)pair * hrow + 32 * g : kOut;
+    for (int base = 0; base < n; base += C) {
+        const int col = r % C;
+        const bool there = base + col < n;
+        const int pair = there ? list[base + col] : 0;
+        const uint32_t ho = there ? (uint32_t)pair * hrow + 32 * g + (r / C) * (hrow / 2) : kOut;
         auto issue = [&](Stage& s, int b) {
             const uint32_t bc = min(b, a.KBI - 1), past = b < a.KBI ? 0u : kOut;
 #pragma unroll
@@ -478,7 +483,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
             for (int p = 0; p < 2; p++) {
                 const uint32_t o = b * 128 + p * 64 + 16 * g < a.I ? ho : kOut;
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
+                for (int k = 0; k < P; k++) {
                     s.h[k][2 * p] = buf_load16(hr, o + p * 128, bc * 256 + k * a.KBI * 256);
                     s.h[k][2 * p + 1] = buf_load16(hr, o + p * 128 + 16, bc * 256 + k * a.KBI * 256);
                 }
@@ -501,9 +506,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
                     v8bf lo, hi;
                     widen(s.d[i][p], lo, hi);
                     t = bf_mfma(hi, s.h[0][2 * p + 1], bf_mfma(lo, s.h[0][2 * p], t));
-                    l = bf_mfma(hi, s.h[1][2 * p + 1], bf_mfma(lo, s.h[1][2 * p], l));
+                    if (P == 2) l = bf_mfma(hi, s.h[P - 1][2 * p + 1], bf_mfma(lo, s.h[P - 1][2 * p], l));
                 }
-                y[i] = scaled(l, s.s, scaled(t, s.s, y[i]));
+                y[i] = scaled(t, s.s, y[i]);
+                if (P == 2) y[i] = scaled(l, s.s, y[i]);
             }
         };
         for (int b = q; b + D * KS < a.KBI; b += D * KS) {
@@ -528,7 +534,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
         }
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            if (i % KS != q || i >= have || !there) continue;
+            if (i % KS != q || i >= have) continue;
             v4f s = y[i];
             if (KS > 1) {
                 const int w0 = w - q;
@@ -540,7 +546,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void moe_down_kernel(ExpertArgs a) 
                     for (int k = 0; k < 4; k++) s[k] = add_rn(s[k], z[k]);
                 }
             }
-            *reinterpret_cast<v4f*>(a.y + (int64_t)pair * a.H + 16 * (t0 + i) + 4 * g) = s;
+            if (C == 8) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) s[k] = add_rn(s[k], __shfl_xor(s[k], 8, kWave));
+            }
+            if (there && r < C) *reinterpret_cast<v4f*>(a.y + (int64_t)pair * a.H + 16 * (t0 + i) + 4 * g) = s;
         }
     }
 }
@@ -589,6 +599,9 @@ __global__ __launch_bounds__(64) void moe_sum_kernel(ExpertArgs a) {
     if (t < pass_tokens(a)) store_out<EPI>(a, t, c, y);
 }
 
+// The experts that as many random ids would reach.
+inline double moe_reached(int64_t pairs, int64_t E) { return (double)E * (1.0 - pow(1.0 - 1.0 / (double)E, (double)pairs)); }
+
 // How many of an expert's 16-row tiles a workgroup takes, of these numbers: the least of (workgroups on the fullest CU) x (its
 // tiles' time + 2 us), for as many experts as that many random ids would reach.  A CU reads at a rate of its own (about 23 GB/s:
 // tile_us), so the one with the most workgroups ends last; 2 us go into a workgroup's start and end.  Measured (us; up with 4 / 2 /
@@ -596,7 +609,7 @@ __global__ __launch_bounds__(64) void moe_sum_kernel(ExpertArgs a) {
 // / 72.8 and 67.6 / 61.3 / 64.5; 64 on 8 of 128, 2048, 768: 170 / 181 / 204 and 149 / 156 / 175; 2 on 2 of 8, 4096, 1792: 35.1 / 29.9
 // / 30.7 and 33.4 / 27.6 / 25.4.
 inline int moe_form(int64_t pairs, int64_t E, int64_t tiles, double tile_us, const int* per, int forms) {
-    const double reached = (double)E * (1.0 - pow(1.0 - 1.0 / (double)E, (double)pairs));
+    const double reached = moe_reached(pairs, E);
     int best = 0;
     double least = 1e30;
     for (int i = 0; i < forms; i++) {
@@ -680,6 +693,9 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
     const int up_per[] = {4, 2, 1}, down_per[] = {16, 8, 4};
     const int up = moe_form(room * a.top, a.E, a.I / 16, 0.178 * a.KBH, up_per, 3);
     const int down = moe_form(room * a.top, a.E, a.H / 16, 0.089 * a.KBI, down_per, 3);
+    // eight pairs at a time in the down kernel where three or fewer are expected on an expert (2 tokens on 3 of 8, H 2752, I 1824 30.8
+    // -> 28.5 us, one on 6 of 128, 1264, 336 15.0 -> 13.4; but 63 on 6 of 64, 640, 1760 69.8 -> 72.5, 64 on 8 of 128 109 -> 111)
+    const bool eight = (double)(room * a.top) <= 3.0 * moe_reached(room * a.top, a.E);
     for (a.first = 0; a.first < a.T; a.first += kMoeTokens) {
         a.room = a.T - a.first < kMoeTokens ? a.T - a.first : kMoeTokens;      // (every row up to there is the caller's)
         a.slots = a.room * a.top < a.E ? a.room * a.top : a.E;
@@ -688,14 +704,18 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
         hipLaunchKernelGGL((moe_up_kernel<N, KS, D>), dim3((a.I / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
                            ids_lds + (KS > 1 ? kWaves * N * 2048 : 0), st, a); \
     } while (0)
-#define DOWN(N, KS, D) do { \
+#define DOWN(N, KS, D, C) do { \
         const int per = kWaves / KS * N; \
-        hipLaunchKernelGGL((moe_down_kernel<N, KS, D>), dim3((a.H / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
+        hipLaunchKernelGGL((moe_down_kernel<N, KS, D, C>), dim3((a.H / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
                            ids_lds + (KS > 1 ? kWaves * N * 1024 : 0), st, a); \
     } while (0)
         if (up == 0) UP(2, 2, 4); else if (up == 1) UP(2, 4, 4); else UP(1, 4, 4);
         PRISM_LAUNCH_CHECK();
-        if (down == 0) DOWN(4, 1, 3); else if (down == 1) DOWN(4, 2, 3); else DOWN(2, 2, 3);
+        if (eight) {
+            if (down == 0) DOWN(4, 1, 3, 8); else if (down == 1) DOWN(4, 2, 3, 8); else DOWN(2, 2, 3, 8);
+        } else {
+            if (down == 0) DOWN(4, 1, 3, 16); else if (down == 1) DOWN(4, 2, 3, 16); else DOWN(2, 2, 3, 16);
+        }
         PRISM_LAUNCH_CHECK();
 #undef UP
 #undef DOWN

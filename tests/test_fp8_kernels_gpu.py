@@ -37,7 +37,8 @@ def case(M, N, K, dev, seed):
 
 FORMS = [(3, 5000, 130), (20, 8200, 130), (20, 40, 5000), (32, 1300, 9000), (70, 40, 130), (64, 40, 2050), (50, 5000, 9000), (520, 5000, 130),
          (300, 3300, 9000), (130, 8200, 9000), (1030, 5000, 5000), (2060, 3300, 2050), (4100, 40, 5000), (4100, 515, 9000), (4100, 8200, 1000),
-         (4100, 3300, 130), (4100, 3300, 9000), (4100, 1000, 17000)]
+         (4100, 3300, 130), (4100, 3300, 9000), (4100, 1000, 17000), (1, 40, 13000), (7, 5000, 5000),
+         (12, 3300, 2050), (30, 4100, 2600), (47, 2000, 1300), (64, 3300, 2050)]
 
 
 @pytest.mark.parametrize("M,N,K", FORMS)
