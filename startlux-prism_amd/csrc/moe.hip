@@ -602,18 +602,21 @@ __global__ __launch_bounds__(64) void moe_sum_kernel(ExpertArgs a) {
 // The experts that as many random ids would reach.
 inline double moe_reached(int64_t pairs, int64_t E) { return (double)E * (1.0 - pow(1.0 - 1.0 / (double)E, (double)pairs)); }
 
-// How many of an expert's 16-row tiles a workgroup takes, of these numbers: the least of (workgroups on the fullest CU) x (its
-// tiles' time + 2 us), for as many experts as that many random ids would reach.  A CU reads at a rate of its own (about 23 GB/s:
-// tile_us), so the one with the most workgroups ends last; 2 us go into a workgroup's start and end.  Measured (us; up with 4 / 2 /
-// 1 tiles and down with 16 / 8 / 4, the other kernel at one form in each): 11 tokens on 2 of 16 experts, H 5120, I 1408: 76.9 / 75.1
-// / 72.8 and 67.6 / 61.3 / 64.5; 64 on 8 of 128, 2048, 768: 170 / 181 / 204 and 149 / 156 / 175; 2 on 2 of 8, 4096, 1792: 35.1 / 29.9
-// / 30.7 and 33.4 / 27.6 / 25.4.
+// How many of an expert's 16-row tiles a workgroup takes, of these numbers: the least time of the fullest CU, for as many experts as
+// that many random ids would reach.  Its workgroups read at the CU's rate (tile_us a tile, about 23 GB/s), one alone at 5 / 8 of it,
+// and each costs 0.8 us more.  Measured (us, all three launches; up with 4 / 2 / 1 tiles and down with 16 / 8 / 4, the other kernel at
+// one form in each): 11 tokens on 2 of 16 experts, H 5120, I 1408: 59.0 / 53.4 / 50.1 and 59.1 / 55.8 / 53.3; 64 on 8 of 128, 2048, 768:
+// 106 / 107 / 112 and 106 / 113 / 122; 2 on 3 of 8, 2752, 1824: 25.6 / 25.4 / 24.2 and 31.6 / 26.6 / 26.7; 5 on 8 of 40, 4560, 208:
+// 31.6 / 32.0 / 26.8 and 32.5 / 32.1 / 35.3.
+// Two stages in registers, so that three and more workgroups share a CU: with four (up) and three (down), two workgroups a CU, these
+// were 54.6, 107, 28.3 and 37.6 and 63 tokens on 6 of 64 (640, 1760) 66 against 60.
 inline int moe_form(int64_t pairs, int64_t E, int64_t tiles, double tile_us, const int* per, int forms) {
     const double reached = moe_reached(pairs, E);
     int best = 0;
     double least = 1e30;
     for (int i = 0; i < forms; i++) {
-        const double t = ceil(reached * (double)((tiles + per[i] - 1) / per[i]) / 256.0) * (per[i] * tile_us + 2);
+        const double rounds = ceil(reached * (double)((tiles + per[i] - 1) / per[i]) / 256.0);
+        const double t = fmax(rounds, 1.6) * per[i] * tile_us + 0.8 * rounds;
         if (t < least) least = t, best = i;
     }
     return best;
@@ -704,21 +707,24 @@ extern "C" int prism_moe_experts(const prism_moe_experts_args* args, void* strea
         hipLaunchKernelGGL((moe_up_kernel<N, KS, D>), dim3((a.I / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
                            ids_lds + (KS > 1 ? kWaves * N * 2048 : 0), st, a); \
     } while (0)
+        // (down with 8 tiles: short sums are not split, 5 tokens on 8 of 40, I 208: 35.0 -> 32.1; from 7 blocks on they are, I 1760 67.5 ->
+        // 65.2)
 #define DOWN(N, KS, D, C) do { \
         const int per = kWaves / KS * N; \
         hipLaunchKernelGGL((moe_down_kernel<N, KS, D, C>), dim3((a.H / 16 + per - 1) / per, a.slots), dim3(64 * kWaves), \
                            ids_lds + (KS > 1 ? kWaves * N * 1024 : 0), st, a); \
     } while (0)
-        if (up == 0) UP(2, 2, 4); else if (up == 1) UP(2, 4, 4); else UP(1, 4, 4);
+        if (up == 0) UP(2, 2, 2); else if (up == 1) UP(2, 4, 2); else UP(1, 4, 2);
         PRISM_LAUNCH_CHECK();
-        if (eight) {
-            if (down == 0) DOWN(4, 1, 3, 8); else if (down == 1) DOWN(4, 2, 3, 8); else DOWN(2, 2, 3, 8);
-        } else {
-            if (down == 0) DOWN(4, 1, 3, 16); else if (down == 1) DOWN(4, 2, 3, 16); else DOWN(2, 2, 3, 16);
-        }
+#define DOWNS(C) do { \
+        if (down == 0) DOWN(4, 1, 2, C); else if (down == 2) DOWN(2, 2, 2, C); \
+        else if (a.KBI <= 6) DOWN(2, 1, 2, C); else DOWN(4, 2, 2, C); \
+    } while (0)
+        if (eight) DOWNS(8); else DOWNS(16);
         PRISM_LAUNCH_CHECK();
 #undef UP
 #undef DOWN
+#undef DOWNS
         const dim3 grid((a.H / 4 + 63) / 64, (unsigned)a.room);
         if (h.epi) hipLaunchKernelGGL((moe_sum_kernel<1>), grid, dim3(64), 0, st, a);
         else hipLaunchKernelGGL((moe_sum_kernel<0>), grid, dim3(64), 0, st, a);
