@@ -568,7 +568,7 @@ PRISM_API int64_t prism_fp8_gemm_workspace_bytes(int64_t T, int64_t n, int64_t k
  * once to bf16 (epi 0) or added to out in fp32 (epi 1); an id outside 0 .. E - 1 takes no part (a row without experts: zeros).
  * x bf16 [T, H]; gate, up [E] weights [I, H] and down [E] weights [H, I], each the E weights' chunks one after the other and
  * their scales likewise.  Sums in fp32; a hidden value goes into the second product as two bf16 parts (16 bits).  Needs
- * H, I % 16 == 0, 16-byte aligned x and weights, x_ld % 8 == 0, top <= 16.  wsp as above (prism_moe_experts_workspace_bytes).
+ * H, I % 16 == 0, 16-byte aligned x and weights, x_ld % 8 == 0, top <= 16, E <= 32767, top ceil(I / 128) < 2^15.  wsp as above (prism_moe_experts_workspace_bytes).
  */
 typedef struct {
     const void* x;

@@ -14,9 +14,9 @@
 // output's own rounding), moe_down_kernel each pair's outputs in fp32, moe_sum_kernel adds a token's in the order of its ids:
 // no atomics, and what a token gets does not depend on the others but for how K is split.
 //
-// The weights' bytes bound it: 64 tokens on 8 of 128 experts (H 2048, I 768; 594 MB) up 67, down 40, sum 4.7 us, 109 in all (5.5
-// TB/s; memory read alone runs at 6.0); 11 tokens on 2 of 16 (5120, 1408; 265 MB) 33, 15 and 4.6, 53 in all; one token on 8 of 128
-// (38 MB) 7.4, 4.1 and 2.9, 15.3 in all: three launches and their first loads.  Loads count by their number too: a ring's last round
+// The weights' bytes bound it: 64 tokens on 8 of 128 experts (H 2048, I 768; 594 MB) up 66, down 40, sum 4.6 us, 109 in all (5.5
+// TB/s; memory read alone runs at 6.0); 11 tokens on 2 of 16 (5120, 1408; 265 MB) 29, 15 and 4.6, 45-49 in all; one token on 8 of 128
+// (38 MB) 7.2, 4.7 and 2.9, 15.1 in all: three launches and their first loads.  Loads count by their number too: a ring's last round
 // that asked past the end made these 115, 64 and 17.2.  Measured and dropped: the outputs of all experts summed by one workgroup per
 // 16 outputs (64 tokens: down 160 us), or for one token a wave per pair (12 us against 5 + 2.5: each CU then goes to eight experts'
 // pages); experts dealt out over the XCDs (no change, 11 tokens 75 against 62).

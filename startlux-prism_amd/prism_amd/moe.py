@@ -31,7 +31,7 @@ def route(logits, ids, weights, n, T, score="softmax", bias=None, renorm=True, s
 def experts(x, ids, weights, gate, up, down, out, n, T, epi=0):
     """x bf16 [>= T, H] through the experts that ids names (numbers outside 0 .. experts - 1 take no part; a row with none
     gets zeros; one named twice counts twice).  gate, up: fp8.F8 of [experts, I, H], down of [experts, H, I]; H and I multiples
-    of 16.  epi=0 writes bf16 `out` [>= T, H], rounded once; epi=1 adds into the fp32 residual `out`.
+    of 16, up to 32767 experts.  epi=0 writes bf16 `out` [>= T, H], rounded once; epi=1 adds into the fp32 residual `out`.
 
     Weights are multiplied as they stand for and activations as they are, sums in fp32; the hidden values enter the second
     product with 16 bits.  Made for up to 128 tokens at a time: more go through in passes that each read their experts."""
