@@ -84,9 +84,10 @@ def to_rows(w: F8):
 
 
 def quantize_act(x, q, s, n, T):
-    """x bf16 or fp32 [>= T, k] -> q, s (module comment): per row and 128 inputs the scale max(amax, 1e-10) / 448 (IEEE
-    division) and codes nearest x / scale (ties to even); q's columns from k on become zeros.  A NaN stays one; an infinity
-    gives its 128 inputs the scale infinity, and so a NaN product."""
+    """x bf16 or fp32 [>= T, k] -> q, s (module comment): per row and 128 inputs the scale max(amax, 1e-10) / 448 and
+    codes nearest x / scale (ties to even), both divisions rounded to fp32 as IEEE has it: bf16 inputs often lie just between
+    two codes, and a scale multiplied by 1 / 448 takes the other one there.  q's columns from k on become zeros.  A NaN stays
+    one; an infinity gives its 128 inputs the scale infinity, and so a NaN product."""
     if n is None:
         n = _live(n, T, x.device)
     rc = (L._host or L.host()).fp8_quant(x, q, s, n, T)
