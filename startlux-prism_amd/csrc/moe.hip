@@ -78,13 +78,20 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 // The number that a rank stands for.
 __device__ __forceinline__ float of_rank(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
 
+// Whether no other fp32 number has x's sigmoid in 64 bits, so that logits order theirs beside x's: the next number's is at least
+// (1 - p) 2^-24 |x| p away, 2^-49 p at 20 and 2^-45 p at +-2^-20, where exp (1 ulp), the sum and the division leave each within
+// 2^-51 p; from -700 on exp(-x) does not overflow.
+__device__ __forceinline__ bool sigmoids_apart(float x) { return x <= 20.f && x >= -700.f && fabsf(x) >= 0x1p-20f; }
+
 // A wave per token, lane l holding experts l V .. l V + V - 1, so the lowest lane with the largest key, and in it the first, is
 // the lowest number; top times the largest of all.
 //
-// Sigmoids with a bias are compared in 64 bits, but first in 32: p and p + bias in fp32 are within 2^-21 (1 + |p + bias|) of their
+// Sigmoids are compared in 64 bits, but first in 32.  With a bias: p and p + bias in fp32 are within 2^-21 (1 + |p + bias|) of their
 // values (expf's and three more roundings), so choices that lie further than 2^-19 (1 + |p + bias|) from the next are the same.
-// Only where two are closer (one token in some thousand, and rows with equal ones) all 64-bit values are made and compared, their
-// high halves first and the low ones between lanes that share them.  8191 tokens, 8 of 256: 12.7 us, 13.7 all in 64 bits.
+// Without one the logits are compared: they order the sigmoids unless a chosen one shares its 64-bit sigmoid with another logit
+// (not sigmoids_apart).  Only where two sums are that close (one token in some thousand, and rows with equal ones) or a chosen
+// logit is not apart, all 64-bit values are made and compared, their high halves first and the low ones between lanes that share
+// them.  8191 tokens, 8 of 256: with a bias 12.7-13.2 us (13.7 all in 64 bits), without 9.5, softmax 7.2.
 template <int V, bool F32, bool SIG>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
     kernel_args_now(a.x, a.x_ld, a.bias, a.ids, a.ids_ld, a.w, a.w_ld, a.n_rows, a.T, a.E, a.top, a.renorm, a.scale);
@@ -104,14 +111,15 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
         key[i] = rank_of(x[i]);
-        if (SIG && key[i]) key[i] = rank_of(add_rn(div_rn(1.f, add_rn(1.f, expf(-x[i]))), bias[i]));
+        if (SIG && a.bias && key[i]) key[i] = rank_of(add_rn(div_rn(1.f, add_rn(1.f, expf(-x[i]))), bias[i]));
         if (lane * V + i >= a.E) key[i] = 0;
     }
     int id = -1;                                                  // lane j: the j-th choice
     float lx = 0.f;                                               // and its logit
     bool sure = true;
-    float last = 0.f, last_x = 0.f;
-    for (int j = 0; j < a.top + (SIG ? 1 : 0); j++) {             // (SIG: the next one too, which the last has to be clear of)
+    float last = 0.f;
+    const int looks = a.top + (SIG && a.bias ? 1 : 0);            // (a bias: the next one too, which the last has to be clear of)
+    for (int j = 0; j < looks; j++) {
         uint32_t best = key[0];
         int at = 0;
 #pragma unroll
@@ -131,11 +139,11 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
         vx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vx), from));
         if (SIG) {
             const float p = of_rank(most);
-            if (j > 0 && !(last - p > 0x1p-19f * (1.f + fabsf(last))) && (a.bias || vx != last_x)) {
+            if (a.bias ? j > 0 && !(last - p > 0x1p-19f * (1.f + fabsf(last))) : !sigmoids_apart(vx)) {
                 sure = false;
                 break;
             }
-            last = p, last_x = vx;
+            last = p;
         }
         if (lane == j && j < a.top) id = from * V + i0, lx = vx;
     }

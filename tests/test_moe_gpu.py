@@ -334,3 +334,51 @@ def test_layer_captured(moe, fp8, dev):
         check(h.cpu()[:live], y[:live], tol[:live], 1, h0[:live])
         assert torch.equal(h.cpu()[live:], h0[live:])
         check(h2.cpu(), y[:3], tol[:3], 1, torch.zeros(3, H))
+
+
+# -------------------------------------------------------------------------------- route by sigmoids that lie close or coincide
+TIED = [  # logits, top, the choice by the 64-bit sigmoids
+    ([14, 14, 14.0625], 1, [2]), ([16, 16, 16.125], 1, [2]), ([20, 20, 20.125], 1, [2]), ([1, 1, 1 + 2 ** -23], 1, [2]),
+    ([18, 18, 18, 18, 18.125, 19], 3, [5, 4, 0]),                  # as many equal ones as are looked at, a larger one behind
+    ([2, 1, 1, 1, 1, 1.0078125], 2, [0, 5]), ([-9, -9, -9, -8.9375], 2, [3, 0]), ([-30, -30, -30, -29.875], 1, [3]),
+    ([40, 50, 50], 1, [0]), ([50, 40, 60, 39], 3, [0, 1, 2]),      # sigmoids that are 1 in 64 bits: the lower number
+    ([-800, -750, -750, -760], 2, [0, 1]), ([-800, 3, -750], 2, [1, 0]),       # ... that are 0
+    ([1e-20, 3e-20, 0, -1e-20, 1], 3, [4, 0, 1]), ([-0.0, 0, 1e-30], 1, [0]),  # ... that are 1 / 2
+    ([math.inf, 45, math.inf, 44], 3, [0, 1, 2]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E", [0, 70, 130, 257, 700])
+def test_route_close_sigmoids_without_a_bias(moe, dev, dtype, E):
+    """Equal logits in front of a larger one that fp32 sigmoids cannot tell from them, and different logits whose 64-bit sigmoids
+    are one number; alone and among experts far below (E: spread over so many)."""
+    for x, top, want in TIED:
+        v = torch.tensor(x, dtype=torch.float32)
+        if not torch.equal(v.to(dtype).float(), v) and 1 + 2 ** -23 in x:
+            continue                                               # (no bf16 number)
+        at = torch.arange(len(x))
+        if E:
+            at = (at * (E // len(x))) + 1
+            v = torch.full((E,), -math.inf).index_copy(0, at, v)
+        rows = v.to(dtype).repeat(5, 1)
+        ids, w = run_route(moe, rows, top, dev, score="sigmoid", renorm=False)
+        assert torch.equal(ids, at[want].int().repeat(5, 1)), (x, top)
+        assert torch.equal(ids, plain_route(rows[:1].float(), top, "sigmoid", None, False, 1.0)[0].repeat(5, 1)), (x, top)
+        p = 1 / (1 + torch.exp(-rows.double()))
+        want_w = torch.gather(p, 1, ids.long())
+        assert ((w.double() - want_w).abs() <= W_REL * want_w + 2.0 ** -149).all(), (x, top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("top", [1, 3, 8])
+@pytest.mark.parametrize("E", [8, 64, 100, 256])
+def test_route_rows_full_of_ties(moe, dev, dtype, top, E):
+    """Logits of a few neighbouring values, so that every choice is between equal ones and the next."""
+    g = torch.Generator().manual_seed(E * top)
+    base = torch.tensor([0.5, 3.0, 9.0, 14.0, 17.0, 19.0, -1.0, -12.0, -40.0])
+    bits = base.view(torch.int32)[:, None] + torch.randint(0, 3, (9, E), generator=g, dtype=torch.int32) * (
+        65536 if dtype == torch.bfloat16 else 1)
+    x = bits.view(torch.float32)
+    ids, _ = run_route(moe, x.to(dtype), top, dev, score="sigmoid")
+    assert torch.equal(ids, plain_route(x, top, "sigmoid", None, True, 1.0)[0])
