@@ -244,9 +244,10 @@ __device__ __forceinline__ void experts_now(const ExpertArgs& a) {
     kernel_args_now(a.o_ld, a.T, a.E, a.top, a.H, a.I, a.KBH, a.KBI, a.div, a.first, a.room, a.slots, a.vec);
 }
 
-// The pass's live tokens (0 or less: none).
+// The pass's live tokens (0 or less: none).  (A live count below zero is made zero first: less the pass's first token, the lowest
+// ones would wrap to a full pass.)
 __device__ __forceinline__ int pass_tokens(const ExpertArgs& a) {
-    return __builtin_amdgcn_readfirstlane(min(min(a.T, __ldg(a.n_rows)) - a.first, a.room));
+    return __builtin_amdgcn_readfirstlane(min(max(min(a.T, __ldg(a.n_rows)), 0) - a.first, a.room));
 }
 __device__ __forceinline__ int token_of(const ExpertArgs& a, int pair) { return (int)((uint32_t)pair * a.div >> 16); }
 

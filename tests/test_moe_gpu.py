@@ -382,3 +382,21 @@ def test_route_rows_full_of_ties(moe, dev, dtype, top, E):
     x = bits.view(torch.float32)
     ids, _ = run_route(moe, x.to(dtype), top, dev, score="sigmoid")
     assert torch.equal(ids, plain_route(x, top, "sigmoid", None, True, 1.0)[0])
+
+
+@pytest.mark.parametrize("live", [0, -1, -1000, -2 ** 31, -2 ** 31 + 200, 400, 2 ** 31 - 1])
+def test_any_live_count(moe, fp8, dev, live):
+    """Live counts below zero are none and above T are T, in every pass of a long call."""
+    T, E, top, H, I = 300, 6, 2, 48, 32
+    ws, plain = make(E, H, I, 13, fp8, dev)
+    g = torch.Generator().manual_seed(14)
+    x, logits = torch.randn(T, H, generator=g).to(torch.bfloat16), torch.randn(T, E, generator=g)
+    ids, w = run_route(moe, logits, top, dev, live=live)
+    out = torch.full((T, H), 9.0, dtype=torch.bfloat16, device=dev)
+    want_ids, want_w = plain_route(logits, top, "softmax", None, True, 1.0)
+    moe.experts(x.to(dev), want_ids.to(dev), want_w.float().to(dev), *ws, out, n_of(live, dev), T)
+    if live <= 0:
+        assert (ids == -7).all() and (w == -7).all() and (out == 9).all()
+    else:
+        assert torch.equal(ids, want_ids)
+        check(out.cpu(), *plain_experts(x, want_ids, want_w.float(), plain))
