@@ -562,7 +562,9 @@ PRISM_API int64_t prism_fp8_gemm_workspace_bytes(int64_t T, int64_t n, int64_t k
  * strides ids_ld, w_ld), best first.  sigmoid = 0: the experts with the largest logits, w = softmax over all E; 1: those with
  * the largest sigmoid(logit) + bias[e] (bias fp32 [E] or null; compared in 64 bits), w = sigmoid(logit).  Equal ones: the
  * lower number first.  An expert whose logit or sum is NaN or -inf is not chosen; where fewer than top are left the rest are
- * id -1, w 0.  renorm = 1: w divided by the chosen ones' sum; then times scale.  E <= 1024, top <= min(E, 16).
+ * id -1, w 0.  renorm = 1: w divided by the chosen ones' sum; then times scale.  E <= 1024, top <= min(E, 16).  A finite logit
+ * masks nothing: sigmoids of logits below -709.8 are 0 in 64 bits, and where all the chosen ones are, renorm = 1 divides 0 by 0 (ids stay,
+ * w NaN).  A logit of +inf, and with sigmoid = 0 and renorm = 0 a NaN one, makes its row's softmax weights NaN.
  *
  * prism_moe_experts: out[t] = sum_j w[t][j] down_e (silu(gate_e x_t) * (up_e x_t)) over the valid e = ids[t][j], rounded
  * once to bf16 (epi 0) or added to out in fp32 (epi 1); an id outside 0 .. E - 1 takes no part (a row without experts: zeros).

@@ -20,7 +20,10 @@ def route(logits, ids, weights, n, T, score="softmax", bias=None, renorm=True, s
     lower number comes first.  renorm: the weights divided by the chosen ones' sum; then all times scale.
 
     An expert whose logit (or its sum with the bias) is -inf or NaN is not chosen; if fewer than top are left, the rest of the
-    row is id -1 with weight 0, which `experts` passes over."""
+    row is id -1 with weight 0, which `experts` passes over.  So -inf is the mask; a large negative number is a logit as others:
+    sigmoids of logits below -709.8 are 0 in 64 bits, and a row whose chosen ones all are has weights 0 / 0 = NaN with renorm (score="softmax"
+    has the chosen ones' softmax there).  A logit of +inf makes its row's softmax weights NaN, as does a NaN one with
+    renorm=False, where the weights are softmax over all experts."""
     if n is None:
         n = _live(n, T, logits.device)
     rc = (L._host or L.host()).moe_route(logits, ids, weights, n, T, score, bias, renorm, scale)

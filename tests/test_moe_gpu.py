@@ -400,3 +400,20 @@ def test_any_live_count(moe, fp8, dev, live):
     else:
         assert torch.equal(ids, want_ids)
         check(out.cpu(), *plain_experts(x, want_ids, want_w.float(), plain))
+
+
+def test_route_weights_that_vanish_or_are_not_finite(moe, dev):
+    """What finite logits whose sigmoids are 0 in 64 bits, infinite logits and NaN ones leave, beside -inf, the mask."""
+    nan, inf, low = float("nan"), math.inf, torch.finfo(torch.float32).min
+    x = torch.tensor([[low, low, low, low], [-1e9, -800, -710, low], [-1e9, 0.5, low, -800], [-inf, -inf, 1, -inf], [1, nan, 2, 3],
+                      [1, inf, 2, 3]])
+    ids, w = run_route(moe, x, 2, dev, score="sigmoid")
+    assert ids.tolist() == [[0, 1], [0, 1], [1, 0], [2, -1], [3, 2], [1, 3]]
+    assert w[:2].isnan().all() and w[2].tolist() == [1, 0] and w[3].tolist() == [1, 0] and w[4:].isfinite().all()
+    ids, w = run_route(moe, x, 2, dev, score="sigmoid", renorm=False)
+    assert (w[:2] == 0).all() and w.isfinite().all()
+    ids, w = run_route(moe, x, 2, dev)
+    assert ids.tolist() == [[0, 1], [2, 1], [1, 3], [2, -1], [3, 2], [1, 3]]
+    assert w[0].tolist() == [0.5, 0.5] and w[:5].isfinite().all() and w[5].isnan().all()
+    ids, w = run_route(moe, x, 2, dev, renorm=False)
+    assert w[0].tolist() == [0.25, 0.25] and w[:4].isfinite().all() and w[4:].isnan().all()
