@@ -91,8 +91,9 @@ __device__ __forceinline__ bool sigmoids_apart(float x) { return x <= 20.f && x 
 // Without one the logits are compared: they order the sigmoids unless a chosen one shares its 64-bit sigmoid with another logit
 // (not sigmoids_apart).  Only where two sums are that close (one token in some thousand, and rows with equal ones) or a chosen
 // logit is not apart, all 64-bit values are made and compared, their high halves first and the low ones between lanes that share
-// them.  8191 tokens, 8 of 256: with a bias 12.7-13.2 us (13.7 all in 64 bits), without 9.5, softmax 7.2.
-template <int V, bool F32, bool SIG>
+// them.  8191 tokens, 8 of 256: with a bias 12.7 us (13.7 all in 64 bits), without 8.4 (BIAS: 13.2 and 9.4 with one kernel for both),
+// softmax 7.3.
+template <int V, bool F32, bool SIG, bool BIAS>
 __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
     kernel_args_now(a.x, a.x_ld, a.bias, a.ids, a.ids_ld, a.w, a.w_ld, a.n_rows, a.T, a.E, a.top, a.renorm, a.scale);
     const int t = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -104,21 +105,21 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
         const int e = min(lane * V + i, a.E - 1);
         x[i] = F32 ? reinterpret_cast<const float*>(a.x)[t * a.x_ld + e]
                    : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.x)[t * a.x_ld + e]);
-        bias[i] = SIG && a.bias ? a.bias[e] : 0.f;
+        bias[i] = BIAS ? a.bias[e] : 0.f;
     }
     if (t >= live) return;
     uint32_t key[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
         key[i] = rank_of(x[i]);
-        if (SIG && a.bias && key[i]) key[i] = rank_of(add_rn(div_rn(1.f, add_rn(1.f, expf(-x[i]))), bias[i]));
+        if (BIAS && key[i]) key[i] = rank_of(add_rn(div_rn(1.f, add_rn(1.f, expf(-x[i]))), bias[i]));
         if (lane * V + i >= a.E) key[i] = 0;
     }
     int id = -1;                                                  // lane j: the j-th choice
     float lx = 0.f;                                               // and its logit
     bool sure = true;
     float last = 0.f;
-    const int looks = a.top + (SIG && a.bias ? 1 : 0);            // (a bias: the next one too, which the last has to be clear of)
+    const int looks = a.top + (BIAS ? 1 : 0);            // (a bias: the next one too, which the last has to be clear of)
     for (int j = 0; j < looks; j++) {
         uint32_t best = key[0];
         int at = 0;
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
         vx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vx), from));
         if (SIG) {
             const float p = of_rank(most);
-            if (a.bias ? j > 0 && !(last - p > 0x1p-19f * (1.f + fabsf(last))) : !sigmoids_apart(vx)) {
+            if (BIAS ? j > 0 && !(last - p > 0x1p-19f * (1.f + fabsf(last))) : !sigmoids_apart(vx)) {
                 sure = false;
                 break;
             }
@@ -650,14 +651,15 @@ extern "C" int prism_moe_route(const prism_moe_route_args* args, void* stream) {
                       (float)h.scale};
     const dim3 grid((unsigned)((h.T + 3) / 4));
     const hipStream_t st = (hipStream_t)stream;
-#define RT(V) do { \
-        if (h.f32 && h.sigmoid) hipLaunchKernelGGL((moe_route_kernel<V, true, true>), grid, dim3(256), 0, st, a); \
-        else if (h.f32) hipLaunchKernelGGL((moe_route_kernel<V, true, false>), grid, dim3(256), 0, st, a); \
-        else if (h.sigmoid) hipLaunchKernelGGL((moe_route_kernel<V, false, true>), grid, dim3(256), 0, st, a); \
-        else hipLaunchKernelGGL((moe_route_kernel<V, false, false>), grid, dim3(256), 0, st, a); \
+#define RF(V, F) do { \
+        if (h.bias) hipLaunchKernelGGL((moe_route_kernel<V, F, true, true>), grid, dim3(256), 0, st, a); \
+        else if (h.sigmoid) hipLaunchKernelGGL((moe_route_kernel<V, F, true, false>), grid, dim3(256), 0, st, a); \
+        else hipLaunchKernelGGL((moe_route_kernel<V, F, false, false>), grid, dim3(256), 0, st, a); \
     } while (0)
+#define RT(V) do { if (h.f32) RF(V, true); else RF(V, false); } while (0)
     if (h.E <= 64) RT(1); else if (h.E <= 128) RT(2); else if (h.E <= 256) RT(4); else if (h.E <= 512) RT(8); else RT(16);
 #undef RT
+#undef RF
     PRISM_LAUNCH_CHECK();
     return PRISM_OK;
 }
