@@ -372,8 +372,8 @@ struct Fp8Tile {
 // EPI 2: fp32 partial sums of this part of K to g.part.  PAN: the activations from panels.
 //
 // What bounds it: the copies into LDS.  At 8191 x 27648 x 5120 (256 x 256 tiles, 64 KB a stage from the L2s) the copies alone take
-// 961 us from panels and 1081 from rows, the products alone 934, both 1113 (2.08 PFLOP/s); at 333 x 5120 x 17408 the copies alone
-// take all of the 45 us (605 MB from the L2s, 13 TB/s; 145 MB of it from memory).  Few rows run at the weights' rate (16 x 5120 x
+// 961 us from panels and 1081 from rows, the products alone 934, both 1113-1164 from card to card (1.99-2.08 PFLOP/s); at 333 x 5120 x 17408 the copies
+// alone take all of the 45 us (605 MB from the L2s, 13 TB/s; 145 MB of it from memory).  Few rows run at the weights' rate (16 x 5120 x
 // 17408: 15.9 us, 5.6 TB/s, and the join).  Measured and dropped: fragments read where they are used (1292), 128 x 256 tiles of 4
 // waves (a third to twice slower: one wave a SIMD), 256 x 128 tiles (333 rows 63, 4096 x 5120 x 5120 149 against 142), six stages for
 // few rows (23.0 against 21.6), the copies through registers (alone 720, but then the products wait for them: 1244 and more).
@@ -584,8 +584,12 @@ __global__ __launch_bounds__(64) void fp8_join_kernel(Fp8Gemm g, int splits) {
     if (m < n_rows) store4<EPI>(g, m, j, y);
 }
 
-// Which kernel, into how many parts K is split, and whether the activations go to panels first: the least of each one's time in
-// us by what it measured (random codes, weights from memory; KB blocks of 128 inputs, NT 16-row weight tiles).
+// Which kernel, into how many parts K is split, and whether the activations go to panels first: the least of the times in us that
+// a model gives each (random codes, weights from memory; KB blocks of 128 inputs, NT 16-row weight tiles).  The model's constants come
+// from the measurements named here, and at the chosen form it is within 15% of the time (1 x 5120 x 5120 7.9 and 7.1, 16 x 5120 x 17408
+// 23.4 and 20.8, 48 x 13824 x 5120 21.1 and 21.7, 128 x 27648 x 5120 40.5 and 46.2, 1000 x 5120 x 5120 50.4 and 49, 4096 x 5120 x 5120 162
+// and 155): forms nearer each other are told apart by the constants, not by a measurement of both.  Weights that the 256 MB
+// memory-side cache holds take less than it says: three in turn 6.8, 18.8 and 17.0.
 //   stream   2.6 + (workgroups on the fullest CU) a per block, and 0.5 per workgroup after the first; a = 0.06, 0.085, 0.1, 0.127, 0.16
 //            for 8, 16, 32, 48, 64 rows: 8 x 13824 x 5120 14.0 (measured; the best tile form 17.3), 8 x 5120 x 17408 21.2 (20.0), 16 x
 //            1024 x 5120 5.9 (7.7), 16 x 5120 x 5120 9.8 (10.5), 16 x 5120 x 17408 27.2 (20.7), 64 x 5120 x 5120 15.5 (13.9)
@@ -597,8 +601,9 @@ __global__ __launch_bounds__(64) void fp8_join_kernel(Fp8Gemm g, int splits) {
 //            256 x 256 in 6 61; 1000 x 5120 x 5120 59 and (3 parts) 50; 2048 x 13824 x 5120 193 and 160; 4096 x 5120 x 5120 144 and
 //            158; 128 x 27648 x 5120 48, on 64 x 128 56
 //   parts    3 + 1.1e-6 per part and output: written, read and added by a second launch
-//   panels   from 256 rows, past 45 us on 128 x 128 tiles (333 x 5120 x 17408 60 -> 55, 4096 x 5120 x 5120 144 -> 139; but 128 x 5120 x
-//            17408 34 -> 38), past 100 on 256 x 256 (8191 x 27648 x 5120 1161 -> 1142, the copy included; 2048 x 5120 x 5120 79 -> 81)
+//   panels   from 256 rows, past 45 us on 128 x 128 tiles (333 x 5120 x 17408 60 -> 55; 4096 x 5120 x 5120 144 -> 139, for which the model
+//            takes 256 x 256, 155; but 128 x 5120 x 17408 34 -> 38), past 100 on 256 x 256 (8191 x 27648 x 5120 1161 -> 1142, the copy
+//            included; 2048 x 5120 x 5120 79 -> 81)
 struct Fp8Plan {
     int kind;            // 0 stream; tiles of rows x outputs: 1 32 x 128, 2 64 x 128, 3 128 x 128, 4 256 x 256
     int splits;

@@ -12,10 +12,11 @@
 // Three launches per 128 tokens.  moe_up_kernel leaves the hidden values h = silu(g) u of each pair in the workspace as two
 // bf16 parts (h = hi + lo up to 2^-17 of it: the second product's operand; one part alone would add as much error as the bf16
 // output's own rounding), moe_down_kernel each pair's outputs in fp32, moe_sum_kernel adds a token's in the order of its ids:
-// no atomics, and what a token gets does not depend on the others but for how K is split.
+// no atomics, and what a token gets depends on the others only in the order of its fp32 sums, by T and the sizes (how K is split,
+// and whether a hidden value's two parts are summed apart).
 //
 // The weights' bytes bound it: 64 tokens on 8 of 128 experts (H 2048, I 768; 594 MB) up 66, down 40, sum 4.6 us, 109 in all (5.5
-// TB/s; memory read alone runs at 6.0); 11 tokens on 2 of 16 (5120, 1408; 265 MB) 29, 15 and 4.6, 45-49 in all; one token on 8 of 128
+// TB/s; memory read alone runs at 6.0); 11 tokens on 2 of 16 (5120, 1408; 265 MB) 29, 15 and 4.6, 45-51 in all; one token on 8 of 128
 // (38 MB) 7.2, 4.7 and 2.9, 15.1 in all: three launches and their first loads.  Loads count by their number too: a ring's last round
 // that asked past the end made these 115, 64 and 17.2.  Measured and dropped: the outputs of all experts summed by one workgroup per
 // 16 outputs (64 tokens: down 160 us), or for one token a wave per pair (12 us against 5 + 2.5: each CU then goes to eight experts'

@@ -100,7 +100,8 @@ def gemm(a_q, a_s, w: F8, out, n, T, epi=0):
 
     A block's 128 products go through the fp8 matrix cores, which align each 8 on the largest of them with 13 bits kept below
     it: a product counts up to 2^-13 of the largest of its 8 (1.5e-5 of the result on normal values, 2-norm; bf16's rounding
-    is 1.7e-3).  Blocks are added in fp32, in an order that depends on T and the sizes."""
+    is 1.7e-3; in the fp32 residual it is what remains).  Blocks are added in fp32, in an order that depends on T and the sizes.
+    a_q's rows lie on whole 16 bytes, they and a_s's at most 2^22 values apart; up to 2^22 - 1 rows."""
     if n is None:
         n = _live(n, T, a_q.device)
     rc = (L._host or L.host()).fp8_gemm(a_q, a_s, w, out, n, T, epi)

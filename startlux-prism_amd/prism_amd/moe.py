@@ -21,8 +21,8 @@ def route(logits, ids, weights, n, T, score="softmax", bias=None, renorm=True, s
 
     An expert whose logit (or its sum with the bias) is -inf or NaN is not chosen; if fewer than top are left, the rest of the
     row is id -1 with weight 0, which `experts` passes over.  So -inf is the mask; a large negative number is a logit as others:
-    sigmoids of logits below -709.8 are 0 in 64 bits, and a row whose chosen ones all are has weights 0 / 0 = NaN with renorm (score="softmax"
-    has the chosen ones' softmax there).  A logit of +inf makes its row's softmax weights NaN, as does a NaN one with
+    sigmoids of logits below -709.8 are 0 in 64 bits, and a row whose chosen ones all are has weights 0 / 0 = NaN with renorm
+    (score="softmax" has the chosen ones' softmax there).  A logit of +inf makes its row's softmax weights NaN, as does a NaN one with
     renorm=False, where the weights are softmax over all experts."""
     if n is None:
         n = _live(n, T, logits.device)
@@ -34,10 +34,11 @@ def route(logits, ids, weights, n, T, score="softmax", bias=None, renorm=True, s
 def experts(x, ids, weights, gate, up, down, out, n, T, epi=0):
     """x bf16 [>= T, H] through the experts that ids names (numbers outside 0 .. experts - 1 take no part; a row with none
     gets zeros; one named twice counts twice).  gate, up: fp8.F8 of [experts, I, H], down of [experts, H, I]; H and I multiples
-    of 16, up to 32767 experts.  epi=0 writes bf16 `out` [>= T, H], rounded once; epi=1 adds into the fp32 residual `out`.
+    of 16, up to 32767 experts; x's rows on whole 16 bytes, at most 2^22 values apart.  epi=0 writes bf16 `out` [>= T, H], rounded once; epi=1 adds into the fp32 residual `out`.
 
     Weights are multiplied as they stand for and activations as they are, sums in fp32; the hidden values enter the second
-    product with 16 bits.  Made for up to 128 tokens at a time: more go through in passes that each read their experts."""
+    product with 16 bits; the order of the sums depends on T and the sizes.  Made for up to 128 tokens at a time: more go through
+    in passes that each read their experts (512 tokens on 8 of 128 experts take 4.6 times as long as 64)."""
     if n is None:
         n = _live(n, T, x.device)
     rc = (L._host or L.host()).moe_experts(x, ids, weights, gate, up, down, out, n, T, epi)
